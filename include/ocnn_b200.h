@@ -650,6 +650,74 @@ int ocnn_batch_norm_backward(const float* x_dev, const float* gy_dev, const floa
                              int channels, int rows, const float* weight_dev, const float* save_mean_dev,
                              const float* save_invstd_dev, float* g_weight_dev, float* g_bias_dev, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * An attention layer over octree nodes (no counterpart among the reference's operators).  A level's nodes
+ * lie shape by shape in Morton order, so consecutive nodes are neighbours in space; a batch is packed, sequence b
+ * holding the nodes offsets[b] .. offsets[b + 1] - 1.  Data: rows of heads, [n][heads][dim], the last dimension
+ * contiguous, strides of the first two in elements.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Rotary positions with several axes: pair t of every head's channels turns by positions[i][axis of t] * freqs[t],
+ * pairs as (t, t + dim/2) or (2t, 2t + 1); sections[a] pairs per axis (1 to 8 axes), the pairs behind the last
+ * axis' pass through.  positions: [rows][axes] int32 or float; freqs: one double per pair; inverse turns back
+ * (the gradient).  y: contiguous [rows][heads][dim], not x unless x is contiguous too. */
+int ocnn_octree_rotary(const void* x_dev, const int64_t x_stride[2], void* y_dev, const void* positions_dev,
+                       int float_positions, const double* freqs_dev, int axes, const int* sections_host,
+                       int64_t rows, int heads, int dim, int interleaved, int inverse, int dtype, void* stream);
+
+/* sum = x + residual (residual NULL: x alone; sum_dev NULL: not stored), y = sum * rsqrt(mean(sum^2) + eps) * weight
+ * over rows of `channels`; row strides of x and residual in elements, sum and y contiguous.  weight_dtype: OCNN_F32 or
+ * dtype.  Backward: grad_x = grad_sum + the norm's share (either gradient may be NULL), the gradient of x and of
+ * residual; grad_weight in weight_dtype, NULL if not wanted (then no workspace). */
+int ocnn_add_rms_norm(const void* x_dev, int64_t x_row, const void* residual_dev, int64_t residual_row,
+                      const void* weight_dev, int weight_dtype, void* sum_dev, void* y_dev, int64_t rows, int channels,
+                      float eps, int dtype, void* stream);
+size_t ocnn_add_rms_norm_backward_workspace_bytes(int channels);
+int ocnn_add_rms_norm_backward(const void* sum_dev, int64_t sum_row, const void* weight_dev, int weight_dtype,
+                               const void* grad_y_dev, int64_t grad_y_row, const void* grad_sum_dev,
+                               int64_t grad_sum_row, void* grad_x_dev, void* grad_weight_dev, int64_t rows,
+                               int channels, float eps, int dtype, void* workspace_dev, size_t workspace_bytes,
+                               void* stream);
+
+/* Attention over a window of a sequence's nodes and its first `sinks` ones.  Node i sees key j of its sequence when
+ *   causal:  j <= i and (i - j < window or j - start < sinks);   else:  |i - j| < window or j - start < sinks
+ * (window 0: every key) and mask[j] != 0 (mask NULL: all).  out_i = sum_j softmax_j(scale * q_i . k_j) v_j, zeros for a
+ * node that sees nothing and for nodes outside of every sequence.  q: heads, k and v: kv_heads (a divisor of heads),
+ * dim up to 128, sinks up to 64.  out: contiguous; lse: [heads][n] fp32 for the backward pass, or NULL.
+ * The backward pass takes the same structure, out and lse of the forward pass and the gradient of out; dq, dk, dv:
+ * contiguous.  status_dev: as in ocnn_octree_conv_tc. */
+typedef struct ocnn_attention {
+  const void *q_dev, *k_dev, *v_dev;
+  int64_t q_stride[2], k_stride[2], v_stride[2];    /* node, head */
+  const int32_t* offsets_dev;                       /* batch + 1, ascending */
+  const uint8_t* mask_dev;                          /* n, or NULL */
+  int32_t batch, n, heads, kv_heads, dim, window, sinks, causal, dtype;
+  float scale;
+} ocnn_attention;
+int ocnn_octree_attention(const ocnn_attention* attention, void* out_dev, float* lse_dev, int32_t* status_dev,
+                          void* stream);
+size_t ocnn_octree_attention_backward_workspace_bytes(const ocnn_attention* attention);
+int ocnn_octree_attention_backward(const ocnn_attention* attention, const void* out_dev, const float* lse_dev,
+                                   const void* grad_dev, const int64_t grad_stride[2], void* dq_dev, void* dk_dev,
+                                   void* dv_dev, void* workspace_dev, size_t workspace_bytes, int32_t* status_dev,
+                                   void* stream);
+
+/* The same (causal) for one new node per sequence against a cache.  Sequence b stands at position lengths[b]: k and v of
+ * the new node are written there, and its queries see it and the nodes before it.  Place of position x in the cache:
+ * x, or, where window + sinks <= capacity (and window > 0), sinks + (x - sinks) mod (capacity - sinks) from x = capacity on, so
+ * the sequence may grow without end; else a sequence without room is left as it is and its output is NaN.  A negative
+ * length: the sequence is passed over, its output zero.  Rows start on 16-byte boundaries.  out: contiguous. */
+typedef struct ocnn_attention_cache {
+  void *k_dev, *v_dev;
+  int64_t k_stride[3], v_stride[3];                 /* sequence, place, head */
+  const int32_t* lengths_dev;
+  int32_t batch, capacity, kv_heads, dim, dtype;
+} ocnn_attention_cache;
+int ocnn_octree_attention_step(const ocnn_attention_cache* cache, const void* q_dev, const int64_t q_stride[2],
+                               const void* k_dev, const int64_t k_stride[2], const void* v_dev,
+                               const int64_t v_stride[2], void* out_dev, int heads, int window, int sinks,
+                               float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -63,21 +63,32 @@ def build_ext(force=False):
   import sysconfig
   import torch
   from torch.utils import cpp_extension
-  src = os.path.join(HERE, 'torch_ext', 'ocnn_nn.cpp')
+  ext = os.path.join(HERE, 'torch_ext')
+  srcs = sorted(os.path.join(ext, f) for f in os.listdir(ext) if f.endswith('.cpp'))
   suffix = sysconfig.get_config_var('EXT_SUFFIX')
   out = os.path.join(HERE, 'ocnn', 'nn' + suffix)
-  deps = [src, os.path.join(HERE, '..', 'include', 'ocnn_b200.h'), LIB]
-  if not force and not _newer(out, deps):
+  header = os.path.join(HERE, '..', 'include', 'ocnn_b200.h')
+  if not force and not _newer(out, srcs + [header, LIB]):
     return out
   inc = ['-I' + p for p in cpp_extension.include_paths()]
   inc += ['-I' + sysconfig.get_paths()['include'], '-I' + os.path.join(HERE, '..', 'include')]
   tlib = os.path.join(os.path.dirname(torch.__file__), 'lib')
   cuda_inc = '/usr/local/cuda/include'
-  cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-DTORCH_EXTENSION_NAME=nn',
-         '-DTORCH_API_INCLUDE_EXTENSION_H', '-D_GLIBCXX_USE_CXX11_ABI=%d' % int(torch._C._GLIBCXX_USE_CXX11_ABI),
-         '-I' + cuda_inc] + inc + [src, '-o', out, '-L' + HERE, '-locnn_b200',
-         '-L' + tlib, '-ltorch', '-ltorch_cpu', '-ltorch_python', '-lc10', '-lc10_cuda', '-ltorch_cuda',
-         '-Wl,-rpath,$ORIGIN/..', '-Wl,-rpath,' + tlib]
+  def compiled(src):
+    obj = os.path.join(OBJ, os.path.basename(src) + '.o')
+    if force or _newer(obj, [src, header]):
+      subprocess.check_call(['g++', '-O2', '-std=c++17', '-fPIC', '-DTORCH_EXTENSION_NAME=nn',
+                             '-DTORCH_API_INCLUDE_EXTENSION_H',
+                             '-D_GLIBCXX_USE_CXX11_ABI=%d' % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+                             '-I' + cuda_inc] + inc + ['-c', src, '-o', obj])
+    return obj
+
+  os.makedirs(OBJ, exist_ok=True)
+  with concurrent.futures.ThreadPoolExecutor(max_workers=4) as ex:
+    objs = list(ex.map(compiled, srcs))
+  cmd = ['g++', '-shared', '-o', out] + objs + [
+      '-L' + HERE, '-locnn_b200', '-L' + tlib, '-ltorch', '-ltorch_cpu', '-ltorch_python', '-lc10', '-lc10_cuda',
+      '-ltorch_cuda', '-Wl,-rpath,$ORIGIN/..', '-Wl,-rpath,' + tlib]
   subprocess.check_call(cmd)
   return out
 

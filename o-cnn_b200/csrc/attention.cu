@@ -1,0 +1,95 @@
+// Entry points of the attention over a window of nodes: checks, and which kernels take a call.
+#include "attention.cuh"
+
+namespace ocnn {
+namespace {
+
+int size_of(int dtype) { return dtype == OCNN_F32 ? 4 : 2; }
+
+int check(const ocnn_attention* a, const char* who) {
+  OCNN_REQUIRE(a != nullptr, "%s: null pointer", who);
+  OCNN_REQUIRE(a->n >= 0 && a->batch >= 0 && a->heads >= 1 && a->kv_heads >= 1 && a->dim >= 1, "%s: bad sizes", who);
+  OCNN_REQUIRE(a->dtype >= OCNN_F32 && a->dtype <= OCNN_F16, "%s: bad dtype %d", who, a->dtype);
+  OCNN_REQUIRE(a->heads % a->kv_heads == 0, "%s: %d heads over %d key heads", who, a->heads, a->kv_heads);
+  OCNN_REQUIRE(a->window >= 0 && a->sinks >= 0, "%s: window and sinks must not be negative", who);
+  if (a->dim > kMaxHeadDim || a->sinks > kMaxSinks || a->heads > 65535)
+    return fail(OCNN_ERR_UNSUPPORTED, "%s: heads of %d channels with %d first nodes (up to %d and %d)", who, a->dim,
+                a->sinks, kMaxHeadDim, kMaxSinks);
+  OCNN_REQUIRE(a->n == 0 || (a->q_dev && a->k_dev && a->v_dev && a->offsets_dev), "%s: null pointer", who);
+  return OCNN_OK;
+}
+
+AttnArgs args_of(const ocnn_attention* p) {
+  AttnArgs a = {};
+  a.q = p->q_dev, a.q_row = p->q_stride[0], a.q_head = p->q_stride[1];
+  a.k = p->k_dev, a.k_row = p->k_stride[0], a.k_head = p->k_stride[1];
+  a.v = p->v_dev, a.v_row = p->v_stride[0], a.v_head = p->v_stride[1];
+  a.offsets = p->offsets_dev, a.mask = p->mask_dev;
+  a.batch = p->batch, a.n = p->n, a.heads = p->heads, a.kv_heads = p->kv_heads, a.dim = p->dim;
+  // a window as long as the batch is none
+  a.window = p->window == 0 || p->window > p->n ? p->n : p->window;
+  a.sinks = a.window == p->n ? 0 : p->sinks;
+  a.causal = p->causal != 0;
+  a.scale = p->scale;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  return a;
+}
+
+// Whether rows of `elements` values can be read from p at these strides in one access each.
+bool on_boundary(const void* p, const int64_t stride[2], int dim, int elements, int size) {
+  return reinterpret_cast<uintptr_t>(p) % (elements * size) == 0 && stride[0] % elements == 0 &&
+         stride[1] % elements == 0 && dim % elements == 0;
+}
+bool all_on_boundary(const ocnn_attention* a, int elements) {
+  const int size = size_of(a->dtype);
+  return on_boundary(a->q_dev, a->q_stride, a->dim, elements, size) &&
+         on_boundary(a->k_dev, a->k_stride, a->dim, elements, size) &&
+         on_boundary(a->v_dev, a->v_stride, a->dim, elements, size);
+}
+
+size_t delta_floats(const ocnn_attention* a) { return ((size_t)a->heads * a->n + 31) / 32 * 32; }
+
+}  // namespace
+}  // namespace ocnn
+
+using namespace ocnn;
+
+extern "C" {
+
+int ocnn_octree_attention(const ocnn_attention* p, void* out_dev, float* lse_dev, int32_t* status_dev, void* stream) {
+  const int status = check(p, "ocnn_octree_attention");
+  if (status != OCNN_OK || p->n == 0) return status;
+  OCNN_REQUIRE(out_dev && status_dev, "ocnn_octree_attention: null pointer");
+  return attn_simt_forward(args_of(p), p->dtype, out_dev, lse_dev, all_on_boundary(p, 4), (cudaStream_t)stream);
+}
+
+size_t ocnn_octree_attention_backward_workspace_bytes(const ocnn_attention* p) {
+  if (check(p, "ocnn_octree_attention_backward_workspace_bytes") != OCNN_OK || p->n == 0) return 0;
+  const AttnArgs a = args_of(p);
+  return (delta_floats(p) + (size_t)far_slots(a.n, a.batch) * a.kv_heads * a.sinks * 2 * a.dim) * sizeof(float);
+}
+
+int ocnn_octree_attention_backward(const ocnn_attention* p, const void* out_dev, const float* lse_dev,
+                                   const void* grad_dev, const int64_t grad_stride[2], void* dq_dev, void* dk_dev,
+                                   void* dv_dev, void* workspace_dev, size_t workspace_bytes, int32_t* status_dev,
+                                   void* stream) {
+  const int status = check(p, "ocnn_octree_attention_backward");
+  if (status != OCNN_OK || p->n == 0) return status;
+  OCNN_REQUIRE(out_dev && lse_dev && grad_dev && grad_stride && dq_dev && dk_dev && dv_dev && status_dev,
+               "ocnn_octree_attention_backward: null pointer");
+  const size_t need = ocnn_octree_attention_backward_workspace_bytes(p);
+  if (workspace_dev == nullptr || workspace_bytes < need)
+    return fail(OCNN_ERR_CAPACITY, "ocnn_octree_attention_backward: %zu bytes of workspace are needed", need);
+  const AttnArgs a = args_of(p);
+  AttnGrad g = {};
+  g.out = out_dev, g.grad = grad_dev, g.grad_row = grad_stride[0], g.grad_head = grad_stride[1];
+  g.lse = lse_dev;
+  g.delta = (float*)workspace_dev;
+  g.far = g.delta + delta_floats(p);
+  g.dq = dq_dev, g.dk = dk_dev, g.dv = dv_dev;
+  const bool vec = all_on_boundary(p, 4) && on_boundary(grad_dev, grad_stride, p->dim, 4, size_of(p->dtype)) &&
+                   reinterpret_cast<uintptr_t>(out_dev) % (4 * size_of(p->dtype)) == 0;
+  return attn_simt_backward(a, g, p->dtype, vec, (cudaStream_t)stream);
+}
+
+}  // extern "C"

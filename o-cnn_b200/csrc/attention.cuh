@@ -1,0 +1,201 @@
+// What the attention kernels share: which keys a node sees, and which nodes see a key.
+//
+// The batch is packed: node i belongs to the sequence b with offsets[b] <= i < offsets[b + 1] (a shape's nodes of a
+// level, in Morton order).  It sees key j of its own sequence when
+//     causal:      j <= i  and  (i - j < window  or  j - start < sinks)
+//     both ways:   |i - j| < window  or  j - start < sinks
+// and the mask (if any) keeps j.  So a node's keys are a window [lo, hi) and the sequence's first nodes
+// [start, first); seen from a key, its nodes are an interval too, and, for a first node, those far behind it.
+#pragma once
+
+#include <climits>
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace ocnn {
+
+constexpr int kMaxSinks = 64;                 // first nodes that stay visible: "a few" (the far pass keeps their sums)
+constexpr int kMaxHeadDim = 128;
+
+// The operands as the kernels take them; strides in elements.
+struct AttnArgs {
+  const void *q, *k, *v;
+  long long q_row, q_head, k_row, k_head, v_row, v_head;
+  const int* offsets;
+  const unsigned char* mask;                  // of keys, or NULL
+  int batch, n, heads, kv_heads, dim, window, sinks, causal;
+  float scale_log2;                           // scale * log2(e): scores are kept in powers of two
+  float scale;
+};
+
+// What the backward pass has besides.  out, dq, dk, dv: contiguous; lse (in powers of two, +inf for a row that sees
+// nothing) and delta: [heads][n].
+struct AttnGrad {
+  const void *out, *grad;
+  long long grad_row, grad_head;
+  const float* lse;
+  float *delta, *far;
+  void *dq, *dk, *dv;
+};
+
+int attn_simt_forward(const AttnArgs& a, int dtype, void* out, float* lse, bool vec, cudaStream_t st);
+int attn_simt_backward(const AttnArgs& a, const AttnGrad& g, int dtype, bool vec, cudaStream_t st);
+
+// Sequence of node i: [start, end), empty for a node outside of every sequence.  Offsets are clamped to [0, n], so
+// that no offset makes a kernel leave its tensors.
+struct Span { int start, end, seq; };
+__device__ __forceinline__ int attn_offset(const AttnArgs& a, int b) { return min(max(a.offsets[b], 0), a.n); }
+__device__ __forceinline__ Span attn_span(const AttnArgs& a, int i) {
+  int lo = 0, hi = a.batch;                   // the last b with offsets[b] <= i
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (attn_offset(a, mid) <= i) lo = mid;
+    else hi = mid - 1;
+  }
+  Span s = {0, 0, lo};
+  if (i >= a.n || lo >= a.batch) return s;
+  const int start = attn_offset(a, lo), end = attn_offset(a, lo + 1);
+  if (i < start || i >= end) return s;
+  s.start = start;
+  s.end = end;
+  return s;
+}
+
+// What node i sees: [lo, hi) and [start, first).
+struct RowKeys { int lo, hi, start, first; };
+__device__ __forceinline__ RowKeys attn_row_keys(const AttnArgs& a, int i, const Span& s) {
+  RowKeys r = {0, 0, 0, 0};
+  if (s.end <= s.start) return r;
+  r.lo = max(s.start, i - a.window + 1);
+  r.hi = a.causal ? i + 1 : i + min(s.end - i, a.window);
+  r.start = s.start;
+  r.first = s.start + min(a.sinks, (a.causal ? i + 1 : s.end) - s.start);
+  return r;
+}
+__device__ __forceinline__ bool attn_sees(const RowKeys& r, int j) {
+  return (j >= r.lo && j < r.hi) || (j >= r.start && j < r.first);
+}
+
+// The nodes that see key j from within the window: [lo, hi).  A first node is seen by every node before it too (both
+// ways); the nodes from j + window on, which see it as a first node only, are left to the far pass.
+struct KeyRows { int lo, hi; };
+__device__ __forceinline__ KeyRows attn_key_rows(const AttnArgs& a, int j, const Span& s) {
+  KeyRows r = {0, 0};
+  if (s.end <= s.start || (a.mask != nullptr && a.mask[j] == 0)) return r;
+  r.lo = a.causal ? j : (j - s.start < a.sinks ? s.start : max(s.start, j - a.window + 1));
+  r.hi = j + min(s.end - j, a.window);
+  return r;
+}
+
+// The keys that the nodes [r0, r1) see between them: the first nodes of r0's sequence where they lie before the windows,
+// then one interval.  (Only r0's: the first nodes of a sequence that starts behind r0 lie in the interval.)
+struct TileKeys {
+  int first, n_first;                         // [first, first + n_first)
+  int lo, n;                                  // then [lo, lo + n - n_first); n keys in all
+  __device__ __forceinline__ int key(int t) const { return t < n_first ? first + t : lo + (t - n_first); }
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T x) { return (float)x; }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x) { return (T)x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16(x); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half(x); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) <= 3.402823466e38f); }
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
+  return x;
+}
+
+// ---- rows key by key ----------------------------------------------------------------------------------------
+// A tile multiplies a hidden pair's probability, 0, by whatever the hidden value is: 0 x inf is not 0.  A row whose
+// result is not finite is therefore formed once more by its warp, from the keys that it sees only (where one of those
+// is not finite the result stays what it is).
+template <typename T>
+__device__ void attn_forward_row(const AttnArgs& a, int i, int h, T* out, float* lse) {
+  const int lane = threadIdx.x & 31;
+  const RowKeys r = attn_row_keys(a, i, attn_span(a, i));
+  const int hk = h / (a.heads / a.kv_heads);
+  const T* q = (const T*)a.q + i * a.q_row + h * a.q_head;
+  float qv[4], acc[4] = {};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) qv[c] = lane + 32 * c < a.dim ? to_f32(q[lane + 32 * c]) : 0.f;
+  float top = -INFINITY, total = 0.f;
+  const int n_first = max(0, min(r.first, r.lo) - r.start), behind = max(r.hi, r.first);
+  for (int t = 0; t < n_first + behind - r.lo; ++t) {
+    const int j = t < n_first ? r.start + t : r.lo + t - n_first;
+    if (!attn_sees(r, j) || (a.mask != nullptr && a.mask[j] == 0)) continue;
+    const T* k = (const T*)a.k + j * a.k_row + hk * a.k_head;
+    const T* v = (const T*)a.v + j * a.v_row + hk * a.v_head;
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (lane + 32 * c < a.dim) s += qv[c] * to_f32(k[lane + 32 * c]);
+    s = warp_sum(s) * a.scale_log2;
+    const float m = fmaxf(top, s), keep = m == -INFINITY ? 1.f : exp2f(top - m);
+    const float p = m == -INFINITY ? 0.f : exp2f(s - m);
+    total = total * keep + p;
+    top = m;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (lane + 32 * c < a.dim) acc[c] = acc[c] * keep + (p == 0.f ? 0.f : p * to_f32(v[lane + 32 * c]));
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (lane + 32 * c < a.dim)
+      out[((long long)i * a.heads + h) * a.dim + lane + 32 * c] = from_f32<T>(total == 0.f ? 0.f : acc[c] / total);
+  if (lse != nullptr && lane == 0)
+    lse[(long long)h * a.n + i] = total == 0.f ? INFINITY : top + log2f(total);
+}
+
+// ---- first nodes seen from far behind -----------------------------------------------------------------------
+// What the nodes behind the window add to the gradients of their sequence's first nodes comes from all over the
+// sequence.  It is summed in blocks of kFarRows nodes, each block's share of a sequence in a slot of its own, and the
+// kernel that writes the keys' gradients adds the slots in order: no atomics, the same bits every time.  Slot = block +
+// sequence: along the packed batch either the block or the sequence moves on, so no two pairs share one.
+constexpr int kFarRows = 512;
+inline int far_slots(int n, int batch) { return ceil_div(n, kFarRows) + batch; }
+__device__ __forceinline__ float* far_slot(const AttnArgs& a, const AttnGrad& g, int slot, int hk, int sink) {
+  return g.far + (((long long)slot * a.kv_heads + hk) * a.sinks + sink) * (2 * a.dim);
+}
+// The slots of key j: first, step between slots and their number (0 for a key that nobody sees from far).
+struct FarSums {
+  const float* at;
+  long long step;
+  int count, dim;
+  __device__ __forceinline__ void add(int d, float& dk, float& dv) const {
+    for (int s = 0; s < count; ++s) {
+      dk += at[s * step + d];
+      dv += at[s * step + dim + d];
+    }
+  }
+};
+__device__ __forceinline__ FarSums far_sums(const AttnArgs& a, const AttnGrad& g, int j, int hk) {
+  FarSums f = {nullptr, 0, 0, a.dim};
+  if (a.sinks == 0) return f;
+  const Span s = attn_span(a, j);
+  if (j - s.start >= a.sinks || s.end - j <= a.window || (a.mask != nullptr && a.mask[j] == 0)) return f;
+  const int first = (j + a.window) / kFarRows;
+  f.at = far_slot(a, g, first + s.seq, hk, j - s.start);
+  f.step = (long long)a.kv_heads * a.sinks * 2 * a.dim;
+  f.count = (s.end - 1) / kFarRows - first + 1;
+  return f;
+}
+
+}  // namespace ocnn

@@ -1,0 +1,525 @@
+// Attention over a window of nodes on the CUDA cores: fp32 data, and 16-bit data in shapes or alignments that the
+// tensor-core kernels do not take.
+#include "attention.cuh"
+
+namespace ocnn {
+namespace {
+
+constexpr int kB = 64;                        // queries and keys per tile
+constexpr int kThreads = 256;                 // 16 x 16: thread (ty, tx) has rows 4 ty .. 4 ty + 3, columns tx + 16 c
+constexpr int kPad = 4;                       // a row of DP + 4 floats: 16 rows 16 bytes each hit distinct banks
+
+// Rows of a [n, heads, dim] tensor as floats, zeros for row < 0 and behind dim.  `index` gives the row for 0 .. kB - 1.
+template <typename T, int DP, typename Index>
+__device__ __forceinline__ void load_rows(float* dst, const void* base, long long row, long long head_offset, int dim,
+                                          bool vec, Index index) {
+  const T* src = (const T*)base + head_offset;
+  for (int e = threadIdx.x; e < kB * (DP / 4); e += kThreads) {
+    const int r = e / (DP / 4), d = (e % (DP / 4)) * 4, i = index(r);
+    float x[4] = {};
+    if (i >= 0 && d < dim) {
+      const T* p = src + i * row + d;
+      if (vec) {
+        if constexpr (sizeof(T) == 4) {
+          const float4 w = *reinterpret_cast<const float4*>(p);
+          x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(p);
+          const T* t = reinterpret_cast<const T*>(&w);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) x[c] = to_f32(t[c]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (d + c < dim) x[c] = to_f32(p[c]);
+      }
+    }
+    *reinterpret_cast<float4*>(dst + r * (DP + kPad) + d) = make_float4(x[0], x[1], x[2], x[3]);
+  }
+}
+
+// acc[r][c] = A row (4 ty + r) . B row (tx + 16 c)
+template <int DP>
+__device__ __forceinline__ void tile_dot(const float* A, const float* B, float (&acc)[4][4]) {
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[r][c] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < DP; d += 4) {
+    float4 x[4], y[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const float4*>(A + (4 * ty + r) * (DP + kPad) + d);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) y[c] = *reinterpret_cast<const float4*>(B + (tx + 16 * c) * (DP + kPad) + d);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        acc[r][c] = fmaf(x[r].x, y[c].x, acc[r][c]);
+        acc[r][c] = fmaf(x[r].y, y[c].y, acc[r][c]);
+        acc[r][c] = fmaf(x[r].z, y[c].z, acc[r][c]);
+        acc[r][c] = fmaf(x[r].w, y[c].w, acc[r][c]);
+      }
+  }
+}
+
+constexpr int kPRow = kB + 4;
+// A thread's columns of a [kB][DP] tile: pairs 2 tx + 32 c (two adjacent floats a lane).
+template <int DP>
+__device__ __forceinline__ int out_col(int c) { return 2 * (threadIdx.x & 15) + 32 * (c >> 1) + (c & 1); }
+
+// acc[r][c] += sum over the kB columns of P row (4 ty + r) * B row: out = P B
+template <int DP>
+__device__ __forceinline__ void tile_mul(const float* P, const float* B, float (&acc)[4][DP / 16]) {
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+#pragma unroll 2
+  for (int j = 0; j < kB; j += 4) {
+    float4 p[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[r] = *reinterpret_cast<const float4*>(P + (4 * ty + r) * kPRow + j);
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+#pragma unroll
+      for (int c = 0; c < DP / 16; c += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(B + (j + jj) * (DP + kPad) + 2 * tx + 16 * c);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float x = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
+          acc[r][c] = fmaf(x, v.x, acc[r][c]);
+          acc[r][c + 1] = fmaf(x, v.y, acc[r][c + 1]);
+        }
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float row_max(float x) {
+#pragma unroll
+  for (int m = 8; m > 0; m >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
+  return x;
+}
+__device__ __forceinline__ float row_sum(float x) {
+#pragma unroll
+  for (int m = 8; m > 0; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
+  return x;
+}
+
+template <int DP>
+constexpr size_t smem_bytes(int tiles, int p_tiles) {
+  return (size_t)(tiles * kB * (DP + kPad) + p_tiles * kB * kPRow) * 4;
+}
+
+// The keys of the query tile at r0 and each row's (rows[] in shared memory), by all threads of the block.
+__device__ __forceinline__ TileKeys query_tile(const AttnArgs& a, int r0, RowKeys* rows, int* ext) {
+  if (threadIdx.x == 0) {
+    ext[0] = INT_MAX;
+    ext[1] = 0;
+  }
+  __syncthreads();
+  if (threadIdx.x < kB) {
+    const int i = r0 + threadIdx.x;
+    const RowKeys r = attn_row_keys(a, i, attn_span(a, i));
+    rows[threadIdx.x] = r;
+    if (r.hi > r.lo) {
+      atomicMin(&ext[0], r.lo);
+      atomicMax(&ext[1], max(r.hi, r.first));
+    }
+    // (the first nodes of the first row's sequence; an empty row's are none)
+    if (threadIdx.x == 0) {
+      ext[2] = r.start;
+      ext[3] = r.start;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < kB) {
+    const RowKeys r = rows[threadIdx.x];
+    if (r.start == ext[2] && r.hi > r.lo) atomicMax(&ext[3], r.first);
+  }
+  __syncthreads();
+  TileKeys t;
+  t.lo = ext[0];
+  t.first = ext[2];
+  t.n_first = ext[1] > ext[0] ? max(0, min(ext[3], t.lo) - t.first) : 0;
+  t.n = t.n_first + max(0, ext[1] - (ext[1] > 0 ? t.lo : 0));
+  return t;
+}
+
+// One tile of 64 queries of one head: a pass over the keys that they see, with a running maximum and sum per row.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) attn_simt_kernel(const AttnArgs a, T* out, float* lse, bool vec) {
+  extern __shared__ float smem[];
+  float* sq = smem;
+  float* sk = sq + kB * (DP + kPad);
+  float* sv = sk + kB * (DP + kPad);
+  float* sp = sv + kB * (DP + kPad);
+  __shared__ RowKeys rows[kB];
+  __shared__ int ext[4], redo[kB];
+  const int r0 = blockIdx.x * kB, h = blockIdx.y, hk = h / (a.heads / a.kv_heads);
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const TileKeys keys = query_tile(a, r0, rows, ext);
+  load_rows<T, DP>(sq, a.q, a.q_row, h * a.q_head, a.dim, vec, [&](int r) { return r0 + r < a.n ? r0 + r : -1; });
+
+  float acc[4][DP / 16] = {}, top[4], total[4] = {};
+#pragma unroll
+  for (int r = 0; r < 4; ++r) top[r] = -INFINITY;
+  for (int t0 = 0; t0 < keys.n; t0 += kB) {
+    // a hidden key's row reads as zeros: what lies there has no say
+    auto row_of = [&](int t) {
+      if (t0 + t >= keys.n) return -1;
+      const int j = keys.key(t0 + t);
+      return a.mask != nullptr && a.mask[j] == 0 ? -1 : j;
+    };
+    __syncthreads();
+    load_rows<T, DP>(sk, a.k, a.k_row, hk * a.k_head, a.dim, vec, row_of);
+    load_rows<T, DP>(sv, a.v, a.v_row, hk * a.v_head, a.dim, vec, row_of);
+    int j[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) j[c] = row_of(tx + 16 * c);
+    __syncthreads();
+    float s[4][4];
+    tile_dot<DP>(sq, sk, s);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const RowKeys rk = rows[4 * ty + r];
+      float m = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        s[r][c] = j[c] >= 0 && attn_sees(rk, j[c]) ? s[r][c] * a.scale_log2 : -INFINITY;
+        m = fmaxf(m, s[r][c]);
+      }
+      m = fmaxf(top[r], row_max(m));
+      const float base = m == -INFINITY ? 0.f : m;          // a row that has seen nothing yet
+      const float keep = exp2f(top[r] - base);
+      top[r] = m;
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float p = exp2f(s[r][c] - base);
+        sp[(4 * ty + r) * kPRow + tx + 16 * c] = p;
+        sum += p;
+      }
+      total[r] = total[r] * keep + sum;
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) acc[r][c] *= keep;
+    }
+    __syncwarp();                                            // (a row of P is written and read by one half warp)
+    tile_mul<DP>(sp, sv, acc);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = r0 + 4 * ty + r;
+    const float sum = row_sum(total[r]), inv = sum == 0.f ? 0.f : 1.f / sum;
+    bool bad = not_finite(sum);
+    if (i < a.n) {
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) {
+        bad |= not_finite(acc[r][c]);
+        const int d = out_col<DP>(c);
+        if (d < a.dim) out[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(sum == 0.f ? 0.f : acc[r][c] * inv);
+      }
+      if (tx == 0 && lse != nullptr) lse[(long long)h * a.n + i] = sum == 0.f ? INFINITY : top[r] + log2f(sum);
+    }
+    const unsigned any = __ballot_sync(0xffffffffu, bad);
+    if (tx == 0) redo[4 * ty + r] = (any >> (tid & 16)) & 0xffffu;
+  }
+  __syncthreads();
+  for (int r = tid >> 5; r < kB; r += kThreads / 32)
+    if (redo[r] != 0 && r0 + r < a.n) attn_forward_row<T>(a, r0 + r, h, out, lse);
+}
+
+// Gradient of the queries of one tile, and delta_i = dO_i . o_i for the keys' gradients.
+//     p = exp2(s - lse), ds = p (dO . v - delta), dq = scale sum_j ds k_j
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const AttnArgs a, const AttnGrad g, bool vec) {
+  extern __shared__ float smem[];
+  float* sq = smem;
+  float* sg = sq + kB * (DP + kPad);
+  float* sk = sg + kB * (DP + kPad);
+  float* sv = sk + kB * (DP + kPad);
+  float* sp = sv + kB * (DP + kPad);
+  __shared__ RowKeys rows[kB];
+  __shared__ int ext[4];
+  const int r0 = blockIdx.x * kB, h = blockIdx.y, hk = h / (a.heads / a.kv_heads);
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const TileKeys keys = query_tile(a, r0, rows, ext);
+  auto query = [&](int r) { return r0 + r < a.n ? r0 + r : -1; };
+  load_rows<T, DP>(sq, a.q, a.q_row, h * a.q_head, a.dim, vec, query);
+  load_rows<T, DP>(sg, g.grad, g.grad_row, h * g.grad_head, a.dim, vec, query);
+  load_rows<T, DP>(sk, g.out, (long long)a.heads * a.dim, (long long)h * a.dim, a.dim, vec, query);
+  __syncthreads();
+  float lse[4], delta[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = r0 + 4 * ty + r;
+    lse[r] = i < a.n ? g.lse[(long long)h * a.n + i] : INFINITY;
+    float x = 0.f;
+    for (int d = tx; d < DP; d += 16) x = fmaf(sg[(4 * ty + r) * (DP + kPad) + d], sk[(4 * ty + r) * (DP + kPad) + d], x);
+    delta[r] = row_sum(x);
+    if (tx == 0 && i < a.n) g.delta[(long long)h * a.n + i] = delta[r];
+  }
+  float acc[4][DP / 16] = {};
+  for (int t0 = 0; t0 < keys.n; t0 += kB) {
+    auto row_of = [&](int t) {
+      if (t0 + t >= keys.n) return -1;
+      const int j = keys.key(t0 + t);
+      return a.mask != nullptr && a.mask[j] == 0 ? -1 : j;
+    };
+    __syncthreads();
+    load_rows<T, DP>(sk, a.k, a.k_row, hk * a.k_head, a.dim, vec, row_of);
+    load_rows<T, DP>(sv, a.v, a.v_row, hk * a.v_head, a.dim, vec, row_of);
+    int j[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) j[c] = row_of(tx + 16 * c);
+    __syncthreads();
+    float s[4][4], dp[4][4];
+    tile_dot<DP>(sq, sk, s);
+    tile_dot<DP>(sg, sv, dp);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const RowKeys rk = rows[4 * ty + r];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bool seen = j[c] >= 0 && attn_sees(rk, j[c]);
+        sp[(4 * ty + r) * kPRow + tx + 16 * c] =
+            seen ? exp2f(s[r][c] * a.scale_log2 - lse[r]) * (dp[r][c] - delta[r]) : 0.f;
+      }
+    }
+    __syncwarp();
+    tile_mul<DP>(sp, sk, acc);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = r0 + 4 * ty + r;
+    if (i >= a.n) continue;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      const int d = out_col<DP>(c);
+      if (d < a.dim) ((T*)g.dq)[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(acc[r][c] * a.scale);
+    }
+  }
+}
+
+// Gradients of the keys and values of one tile of 64 keys: over the nodes that see them from within the window, head
+// by head of the group; what the far pass has summed for first nodes is added at the end.
+//     dv_j = sum_i p_ij dO_i, dk_j = scale sum_i ds_ij q_i
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs a, const AttnGrad g, bool vec) {
+  extern __shared__ float smem[];
+  float* sk = smem;
+  float* sv = sk + kB * (DP + kPad);
+  float* sq = sv + kB * (DP + kPad);
+  float* sg = sq + kB * (DP + kPad);
+  float* sp = sg + kB * (DP + kPad);
+  float* sd = sp + kB * kPRow;
+  __shared__ KeyRows rows[kB];
+  __shared__ int ext[2];
+  const int k0 = blockIdx.x * kB, hk = blockIdx.y, group = a.heads / a.kv_heads;
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  if (tid == 0) {
+    ext[0] = INT_MAX;
+    ext[1] = 0;
+  }
+  __syncthreads();
+  if (tid < kB) {
+    const int j = k0 + tid;
+    const KeyRows r = j < a.n ? attn_key_rows(a, j, attn_span(a, j)) : KeyRows{0, 0};
+    rows[tid] = r;
+    if (r.hi > r.lo) {
+      atomicMin(&ext[0], r.lo);
+      atomicMax(&ext[1], r.hi);
+    }
+  }
+  __syncthreads();
+  auto key = [&](int t) { return rows[t].hi > rows[t].lo ? k0 + t : -1; };
+  load_rows<T, DP>(sk, a.k, a.k_row, hk * a.k_head, a.dim, vec, key);
+  load_rows<T, DP>(sv, a.v, a.v_row, hk * a.v_head, a.dim, vec, key);
+  float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
+  for (int hg = 0; hg < group; ++hg) {
+    const int h = hk * group + hg;
+    for (int i0 = ext[0]; i0 < ext[1]; i0 += kB) {
+      auto query = [&](int t) { return i0 + t < ext[1] ? i0 + t : -1; };
+      __syncthreads();
+      load_rows<T, DP>(sq, a.q, a.q_row, h * a.q_head, a.dim, vec, query);
+      load_rows<T, DP>(sg, g.grad, g.grad_row, h * g.grad_head, a.dim, vec, query);
+      float lse[4], delta[4];
+      int i[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        i[c] = query(tx + 16 * c);
+        lse[c] = i[c] >= 0 ? g.lse[(long long)h * a.n + i[c]] : 0.f;
+        delta[c] = i[c] >= 0 ? g.delta[(long long)h * a.n + i[c]] : 0.f;
+      }
+      __syncthreads();
+      float s[4][4], dp[4][4];
+      tile_dot<DP>(sk, sq, s);
+      tile_dot<DP>(sv, sg, dp);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const KeyRows kr = rows[4 * ty + r];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float p = i[c] >= kr.lo && i[c] < kr.hi ? exp2f(s[r][c] * a.scale_log2 - lse[c]) : 0.f;
+          sp[(4 * ty + r) * kPRow + tx + 16 * c] = p;
+          sd[(4 * ty + r) * kPRow + tx + 16 * c] = p == 0.f ? 0.f : p * (dp[r][c] - delta[c]);
+        }
+      }
+      __syncwarp();
+      tile_mul<DP>(sp, sg, dv);
+      tile_mul<DP>(sd, sq, dk);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int j = k0 + 4 * ty + r;
+    if (j >= a.n) continue;
+    const FarSums far = far_sums(a, g, j, hk);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      const int d = out_col<DP>(c);
+      if (d >= a.dim) continue;
+      float x = dk[r][c], y = dv[r][c];
+      far.add(d, x, y);
+      ((T*)g.dk)[((long long)j * a.kv_heads + hk) * a.dim + d] = from_f32<T>(x * a.scale);
+      ((T*)g.dv)[((long long)j * a.kv_heads + hk) * a.dim + d] = from_f32<T>(y);
+    }
+  }
+}
+
+// The far pass: what the nodes beyond the window add to the gradients of their sequence's first nodes.  A block takes
+// kFarRows nodes of one key head, every warp its share of them; a lane holds four channels of the sums (dim <= 128).
+// Partial sums go to slot block + sequence, which no other pair of block and sequence has: along the packed batch
+// either the block or the sequence moves on.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_far_kernel(const AttnArgs a, const AttnGrad g) {
+  const int hk = blockIdx.y, group = a.heads / a.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r0 = blockIdx.x * kFarRows, r1 = min(a.n, r0 + kFarRows);
+  __shared__ float part[8][2][kMaxHeadDim];
+  for (int i0 = r0; i0 < r1;) {
+    Span s = attn_span(a, i0);
+    if (s.end <= s.start) {                        // outside of every sequence: on to the next one's first node
+      const int next = s.seq < a.batch ? (s.seq == 0 && i0 < attn_offset(a, 0) ? attn_offset(a, 0) : a.n) : a.n;
+      i0 = max(i0 + 1, next);
+      continue;
+    }
+    const int end = min(r1, s.end);
+    for (int t = 0; t < a.sinks && s.start + t < s.end; ++t) {
+      const int j = s.start + t;
+      float k[4], v[4], dk[4] = {}, dv[4] = {};
+      const bool kept = a.mask == nullptr || a.mask[j] != 0;
+      const bool any = kept && end > j + (long long)a.window;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int d = lane + 32 * c;
+        k[c] = any && d < a.dim ? to_f32(((const T*)a.k)[j * a.k_row + hk * a.k_head + d]) : 0.f;
+        v[c] = any && d < a.dim ? to_f32(((const T*)a.v)[j * a.v_row + hk * a.v_head + d]) : 0.f;
+      }
+      if (any) {
+        for (int i = max(i0, j + a.window) + warp; i < end; i += 8) {
+          for (int hg = 0; hg < group; ++hg) {
+            const int h = hk * group + hg;
+            float q[4], o[4], x = 0.f, y = 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int d = lane + 32 * c;
+              q[c] = d < a.dim ? to_f32(((const T*)a.q)[i * a.q_row + h * a.q_head + d]) : 0.f;
+              o[c] = d < a.dim ? to_f32(((const T*)g.grad)[i * g.grad_row + h * g.grad_head + d]) : 0.f;
+              x = fmaf(q[c], k[c], x);
+              y = fmaf(o[c], v[c], y);
+            }
+            x = warp_sum(x);
+            y = warp_sum(y);
+            const float p = exp2f(x * a.scale_log2 - g.lse[(long long)h * a.n + i]);
+            const float ds = p * (y - g.delta[(long long)h * a.n + i]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              dk[c] = fmaf(ds, q[c], dk[c]);
+              dv[c] = fmaf(p, o[c], dv[c]);
+            }
+          }
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        part[warp][0][lane + 32 * c] = dk[c];
+        part[warp][1][lane + 32 * c] = dv[c];
+      }
+      __syncthreads();
+      float* dst = far_slot(a, g, blockIdx.x + s.seq, hk, t);
+      for (int e = threadIdx.x; e < 2 * kMaxHeadDim; e += 256) {
+        const int which = e / kMaxHeadDim, d = e % kMaxHeadDim;
+        if (d >= a.dim) continue;
+        float x = 0.f;
+        for (int w = 0; w < 8; ++w) x += part[w][which][d];
+        dst[which * a.dim + d] = x;
+      }
+    }
+    i0 = s.end;
+  }
+}
+
+template <typename T, int DP>
+int forward_launch(const AttnArgs& a, void* out, float* lse, bool vec, cudaStream_t st) {
+  static PerDeviceOnce once;
+  const size_t bytes = smem_bytes<DP>(3, 1);
+  const int status = once.run([&]() -> int {
+    OCNN_CUDA_OK(cudaFuncSetAttribute(attn_simt_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    return OCNN_OK;
+  });
+  if (status != OCNN_OK) return status;
+  attn_simt_kernel<T, DP><<<dim3(ceil_div(a.n, kB), a.heads), kThreads, bytes, st>>>(a, (T*)out, lse, vec);
+  OCNN_LAUNCH_OK("attn_simt_kernel");
+  return OCNN_OK;
+}
+
+template <typename T, int DP>
+int backward_launch(const AttnArgs& a, const AttnGrad& g, bool vec, cudaStream_t st) {
+  static PerDeviceOnce once;
+  const size_t dq_bytes = smem_bytes<DP>(4, 1), dkv_bytes = smem_bytes<DP>(4, 2);
+  const int status = once.run([&]() -> int {
+    OCNN_CUDA_OK(cudaFuncSetAttribute(attn_simt_dq_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dq_bytes));
+    OCNN_CUDA_OK(cudaFuncSetAttribute(attn_simt_dkv_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dkv_bytes));
+    return OCNN_OK;
+  });
+  if (status != OCNN_OK) return status;
+  attn_simt_dq_kernel<T, DP><<<dim3(ceil_div(a.n, kB), a.heads), kThreads, dq_bytes, st>>>(a, g, vec);
+  OCNN_LAUNCH_OK("attn_simt_dq_kernel");
+  if (a.sinks > 0) {
+    attn_far_kernel<T><<<dim3(ceil_div(a.n, kFarRows), a.kv_heads), 256, 0, st>>>(a, g);
+    OCNN_LAUNCH_OK("attn_far_kernel");
+  }
+  attn_simt_dkv_kernel<T, DP><<<dim3(ceil_div(a.n, kB), a.kv_heads), kThreads, dkv_bytes, st>>>(a, g, vec);
+  OCNN_LAUNCH_OK("attn_simt_dkv_kernel");
+  return OCNN_OK;
+}
+
+template <typename F>
+int by_type(int dtype, int dim, F f) {
+  auto width = [&](auto t) {
+    using T = decltype(t);
+    if (dim <= 32) return f(t, std::integral_constant<int, 32>());
+    if (dim <= 64) return f(t, std::integral_constant<int, 64>());
+    return f(T(), std::integral_constant<int, 128>());
+  };
+  if (dtype == OCNN_F32) return width(float());
+  if (dtype == OCNN_BF16) return width(__nv_bfloat16());
+  return width(__half());
+}
+
+}  // namespace
+
+int attn_simt_forward(const AttnArgs& a, int dtype, void* out, float* lse, bool vec, cudaStream_t st) {
+  return by_type(dtype, a.dim, [&](auto t, auto dp) {
+    return forward_launch<decltype(t), decltype(dp)::value>(a, out, lse, vec, st);
+  });
+}
+int attn_simt_backward(const AttnArgs& a, const AttnGrad& g, int dtype, bool vec, cudaStream_t st) {
+  return by_type(dtype, a.dim, [&](auto t, auto dp) {
+    return backward_launch<decltype(t), decltype(dp)::value>(a, g, vec, st);
+  });
+}
+
+}  // namespace ocnn

@@ -41,6 +41,9 @@ from .modules import (OctreeConvBn, OctreeConvBnRelu, OctreeDeConvBnRelu, FcBnRe
                       OctreeConv1x1Bn, OctreeConv1x1BnRelu, OctreeResBlock, OctreeResBlock2,
                       OctreeResBlocks, octree_trilinear_pts, octree_trilinear, octree_nearest_pts,
                       OctreeTrilinear, OctreeInterp, octree_feature, create_full_octree)
+from .octree_attention import (octree_sequence, OctreeSequence, rotary_freqs, octree_rotary, add_rms_norm,
+                               octree_attention, octree_attention_step, AddRMSNorm, AttentionCache,
+                               OctreeAttention, OctreeAttentionBlock)
 from .lenet import LeNet
 from .resnet import ResNet
 from .unet import UNet

@@ -2982,6 +2982,10 @@ Tensor not_built(const char* name) {
 
 }  // namespace
 
+// For attention.cpp, whose operators are bound beside these.
+Tensor ocnn_tc_status(c10::Device device) { return tc_status(device); }
+void bind_attention(pybind11::module_& m);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   namespace py = pybind11;
   m.doc() = "ocnn.nn on libocnn_b200 (CUDA sm_100a)";
@@ -3152,6 +3156,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def("trace_ms", &NetExecutor::trace_ms)
       .def("op_names", &NetExecutor::op_names)
       .def("status", &NetExecutor::status);
+  bind_attention(m);
   m.def("last_error", []() { return string(ocnn_last_error()); });
   m.def("launch_count", []() { return (int64_t)ocnn_launch_count(); });
 }
