@@ -673,7 +673,8 @@ int ocnn_add_rms_norm(const void* x_dev, int64_t x_row, const void* residual_dev
                       const void* weight_dev, int weight_dtype, void* sum_dev, void* y_dev, int64_t rows, int channels,
                       float eps, int dtype, void* stream);
 size_t ocnn_add_rms_norm_backward_workspace_bytes(int channels);
-int ocnn_add_rms_norm_backward(const void* sum_dev, int64_t sum_row, const void* weight_dev, int weight_dtype,
+int ocnn_add_rms_norm_backward(const void* x_dev, int64_t x_row, const void* residual_dev, int64_t residual_row,
+                               const void* weight_dev, int weight_dtype,
                                const void* grad_y_dev, int64_t grad_y_row, const void* grad_sum_dev,
                                int64_t grad_sum_row, void* grad_x_dev, void* grad_weight_dev, int64_t rows,
                                int channels, float eps, int dtype, void* workspace_dev, size_t workspace_bytes,

@@ -1,4 +1,6 @@
 // Entry points of the attention over a window of nodes: checks, and which kernels take a call.
+#include <cmath>
+
 #include "attention.cuh"
 
 namespace ocnn {
@@ -8,7 +10,7 @@ int size_of(int dtype) { return dtype == OCNN_F32 ? 4 : 2; }
 
 int check(const ocnn_attention* a, const char* who) {
   OCNN_REQUIRE(a != nullptr, "%s: null pointer", who);
-  OCNN_REQUIRE(a->n >= 0 && a->batch >= 0 && a->heads >= 1 && a->kv_heads >= 1 && a->dim >= 1, "%s: bad sizes", who);
+  OCNN_REQUIRE(a->n >= 0 && a->n <= INT_MAX - 1024 && a->batch >= 0 && a->heads >= 1 && a->kv_heads >= 1 && a->dim >= 1, "%s: bad sizes", who);
   OCNN_REQUIRE(a->dtype >= OCNN_F32 && a->dtype <= OCNN_F16, "%s: bad dtype %d", who, a->dtype);
   OCNN_REQUIRE(a->heads % a->kv_heads == 0, "%s: %d heads over %d key heads", who, a->heads, a->kv_heads);
   OCNN_REQUIRE(a->window >= 0 && a->sinks >= 0, "%s: window and sinks must not be negative", who);
@@ -47,6 +49,11 @@ bool all_on_boundary(const ocnn_attention* a, int elements) {
          on_boundary(a->v_dev, a->v_stride, a->dim, elements, size);
 }
 
+// 16-bit rows in whole pieces of 16 bytes, and a positive scale (a tile's maximum is taken before it).
+bool on_tensor_cores(const ocnn_attention* a) {
+  return a->dtype != OCNN_F32 && all_on_boundary(a, 8) && a->scale > 0.f && a->scale < INFINITY;
+}
+
 size_t delta_floats(const ocnn_attention* a) { return ((size_t)a->heads * a->n + 31) / 32 * 32; }
 
 }  // namespace
@@ -60,7 +67,10 @@ int ocnn_octree_attention(const ocnn_attention* p, void* out_dev, float* lse_dev
   const int status = check(p, "ocnn_octree_attention");
   if (status != OCNN_OK || p->n == 0) return status;
   OCNN_REQUIRE(out_dev && status_dev, "ocnn_octree_attention: null pointer");
-  return attn_simt_forward(args_of(p), p->dtype, out_dev, lse_dev, all_on_boundary(p, 4), (cudaStream_t)stream);
+  const AttnArgs a = args_of(p);
+  if (on_tensor_cores(p) && reinterpret_cast<uintptr_t>(out_dev) % 16 == 0)
+    return attn_tc_forward(a, p->dtype, out_dev, lse_dev, status_dev, (cudaStream_t)stream);
+  return attn_simt_forward(a, p->dtype, out_dev, lse_dev, all_on_boundary(p, 4), (cudaStream_t)stream);
 }
 
 size_t ocnn_octree_attention_backward_workspace_bytes(const ocnn_attention* p) {

@@ -39,6 +39,13 @@ struct AttnGrad {
   void *dq, *dk, *dv;
 };
 
+// Heads of a node that stand side by side in a tensor-core tile: the largest power of two in the group.
+inline int attn_pack(const AttnArgs& a) {
+  const int group = a.heads / a.kv_heads, pack = group & -group;
+  return pack < 32 ? pack : 32;
+}
+
+int attn_tc_forward(const AttnArgs& a, int dtype, void* out, float* lse, int* status, cudaStream_t st);
 int attn_simt_forward(const AttnArgs& a, int dtype, void* out, float* lse, bool vec, cudaStream_t st);
 int attn_simt_backward(const AttnArgs& a, const AttnGrad& g, int dtype, bool vec, cudaStream_t st);
 

@@ -512,12 +512,12 @@ int by_type(int dtype, int dim, F f) {
 }  // namespace
 
 int attn_simt_forward(const AttnArgs& a, int dtype, void* out, float* lse, bool vec, cudaStream_t st) {
-  return by_type(dtype, a.dim, [&](auto t, auto dp) {
+  return by_type(dtype, a.dim, [&](auto t, auto dp) -> int {
     return forward_launch<decltype(t), decltype(dp)::value>(a, out, lse, vec, st);
   });
 }
 int attn_simt_backward(const AttnArgs& a, const AttnGrad& g, int dtype, bool vec, cudaStream_t st) {
-  return by_type(dtype, a.dim, [&](auto t, auto dp) {
+  return by_type(dtype, a.dim, [&](auto t, auto dp) -> int {
     return backward_launch<decltype(t), decltype(dp)::value>(a, g, vec, st);
   });
 }

@@ -2,11 +2,12 @@
 //     s = x + r,   y = s * rsqrt(mean(s^2) + eps) * w
 // and the gradient, with u = s * rsqrt(...), from gy and gs:
 //     g = gs + rsqrt(...) * (w gy - u mean(w gy u)),   gw = sum over rows of gy u
-// (g is the gradient of both x and r).  Sums are held in fp32.  The forward pass norms s before it is rounded to the
-// data's type; the backward pass reads the rounded s and forms its statistics anew, in the same pass over the row as the
-// mean of w gy u, so nothing but s is kept.
+// (g is the gradient of both x and r).  Sums are held in fp32, and s is never rounded before it is used: the backward pass
+// reads x and r again, not the s that was stored (one row more; from a bf16 s the weight's gradient, which is fp32,
+// was off by 1.9e-3).  It forms the statistics anew, in the same pass over the row as the mean of w gy u, so nothing is
+// kept between the two.
 //
-// Bound: HBM.  Forward 2 rows read and 2 written, backward 3 read and 1 written.  A row is taken by as few lanes as hold
+// Bound: HBM.  Forward 2 rows read and 2 written, backward 4 read and 1 written.  A row is taken by as few lanes as hold
 // it in two to four vectors each (8 channels of 16 bits or 4 of 32), so that a warp has several rows in flight and the
 // statistics are a few shuffles; a row of more than 4 vectors x 32 lanes takes a block, and one that even a block cannot
 // keep in registers is read twice (the second time from L2).  gw: every thread keeps the sums of its own channels over
@@ -19,7 +20,7 @@ namespace {
 constexpr int kNormThreads = 256, kNormVectors = 4;
 
 struct NormArgs {
-  const void *x, *r, *w, *gy, *gs, *s;
+  const void *x, *r, *w, *gy, *gs;
   void *sum, *y, *g;
   long long rows, x_row, r_row, gy_row, gs_row;
   float* partial;
@@ -54,6 +55,17 @@ __device__ __forceinline__ void norm_weight(const NormArgs& a, int c, float (&f)
 #pragma unroll
   for (int i = 0; i < V; ++i)
     f[i] = a.w_f32 ? ((const float*)a.w)[c + i] : norm_f32(((const T*)a.w)[c + i]);
+}
+
+// x + r (x alone without r) of row i from channel c on
+template <typename T, int V>
+__device__ __forceinline__ void norm_sum(const NormArgs& a, long long i, int c, float (&s)[V]) {
+  norm_load<T, V>(a.x, i * a.x_row + c, s);
+  if (a.r == nullptr) return;
+  float r[V];
+  norm_load<T, V>(a.r, i * a.r_row + c, r);
+#pragma unroll
+  for (int e = 0; e < V; ++e) s[e] += r[e];
 }
 
 // Sums over the LANES threads of a row, to all of them.  LANES = kNormThreads: the whole block.
@@ -106,13 +118,7 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_kernel(const NormArgs a
 #pragma unroll
         for (int e = 0; e < V; ++e) s[k][e] = 0.f;
         if (!in) continue;
-        norm_load<T, V>(a.x, i * a.x_row + c, s[k]);
-        if (a.r != nullptr) {
-          float r[V];
-          norm_load<T, V>(a.r, i * a.r_row + c, r);
-#pragma unroll
-          for (int e = 0; e < V; ++e) s[k][e] += r[e];
-        }
+        norm_sum<T, V>(a, i, c, s[k]);
 #pragma unroll
         for (int e = 0; e < V; ++e) total[0] = fmaf(s[k][e], s[k][e], total[0]);
       }
@@ -128,18 +134,9 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_kernel(const NormArgs a
         norm_store<T, V>(a.y, i * a.channels + c, s[k]);
       }
     } else {
-      auto row = [&](int c, float (&s)[V]) {
-        norm_load<T, V>(a.x, i * a.x_row + c, s);
-        if (a.r != nullptr) {
-          float r[V];
-          norm_load<T, V>(a.r, i * a.r_row + c, r);
-#pragma unroll
-          for (int e = 0; e < V; ++e) s[e] += r[e];
-        }
-      };
       for (int c = lane * V; live && c < a.channels; c += LANES * V) {
         float s[V];
-        row(c, s);
+        norm_sum<T, V>(a, i, c, s);
 #pragma unroll
         for (int e = 0; e < V; ++e) total[0] = fmaf(s[e], s[e], total[0]);
       }
@@ -147,7 +144,7 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_kernel(const NormArgs a
       const float inv = rsqrtf(total[0] * inv_c + a.eps);
       for (int c = lane * V; live && c < a.channels; c += LANES * V) {
         float s[V], w[V];
-        row(c, s);
+        norm_sum<T, V>(a, i, c, s);
         if (a.sum != nullptr) norm_store<T, V>(a.sum, i * a.channels + c, s);
         norm_weight<T, V>(a, c, w);
 #pragma unroll
@@ -185,7 +182,7 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_backward_kernel(const N
 #pragma unroll
         for (int e = 0; e < V; ++e) s[k][e] = gy[k][e] = gs[k][e] = 0.f;
         if (!live || c >= a.channels) continue;
-        norm_load<T, V>(a.s, i * a.r_row + c, s[k]);
+        norm_sum<T, V>(a, i, c, s[k]);
         if (a.gy != nullptr) norm_load<T, V>(a.gy, i * a.gy_row + c, gy[k]);
         if (a.gs != nullptr) norm_load<T, V>(a.gs, i * a.gs_row + c, gs[k]);
 #pragma unroll
@@ -232,7 +229,7 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_backward_kernel(const N
       float total[2] = {0.f, 0.f};
       for (int c = lane * V; c < a.channels; c += LANES * V) {
         float s[V], gy[V] = {}, w[V];
-        norm_load<T, V>(a.s, i * a.r_row + c, s);
+        norm_sum<T, V>(a, i, c, s);
         if (a.gy != nullptr) norm_load<T, V>(a.gy, i * a.gy_row + c, gy);
         norm_weight<T, V>(a, c, w);
 #pragma unroll
@@ -245,7 +242,7 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_backward_kernel(const N
       const float inv = rsqrtf(total[0] * inv_c + a.eps), along = total[1] * inv * inv_c;
       for (int c = lane * V; c < a.channels; c += LANES * V) {
         float s[V], gy[V] = {}, gs[V] = {}, w[V];
-        norm_load<T, V>(a.s, i * a.r_row + c, s);
+        norm_sum<T, V>(a, i, c, s);
         if (a.gy != nullptr) norm_load<T, V>(a.gy, i * a.gy_row + c, gy);
         if (a.gs != nullptr) norm_load<T, V>(a.gs, i * a.gs_row + c, gs);
         norm_weight<T, V>(a, c, w);
@@ -330,7 +327,7 @@ int norm_by_width(const NormArgs& a, int* blocks, cudaStream_t st) {
 template <typename T>
 int norm_by_vector(const NormArgs& a, int* blocks, cudaStream_t st) {
   constexpr int kMost = 16 / sizeof(T);
-  uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.r | (uintptr_t)a.gy | (uintptr_t)a.gs | (uintptr_t)a.s |
+  uintptr_t bits = (uintptr_t)a.x | (uintptr_t)a.r | (uintptr_t)a.gy | (uintptr_t)a.gs |
                    (uintptr_t)a.sum | (uintptr_t)a.y | (uintptr_t)a.g;
   for (long long stride : {a.x_row, a.r_row, a.gy_row, a.gs_row, (long long)a.channels})
     bits |= (uintptr_t)(stride * (long long)sizeof(T));
@@ -371,7 +368,8 @@ size_t ocnn_add_rms_norm_backward_workspace_bytes(int channels) {
   return channels > 0 ? (size_t)4 * sm_count() * channels * sizeof(float) : 0;
 }
 
-int ocnn_add_rms_norm_backward(const void* sum_dev, int64_t sum_row, const void* weight_dev, int weight_dtype,
+int ocnn_add_rms_norm_backward(const void* x_dev, int64_t x_row, const void* residual_dev, int64_t residual_row,
+                               const void* weight_dev, int weight_dtype,
                                const void* grad_y_dev, int64_t grad_y_row, const void* grad_sum_dev,
                                int64_t grad_sum_row, void* grad_x_dev, void* grad_weight_dev, int64_t rows,
                                int channels, float eps, int dtype, void* workspace_dev, size_t workspace_bytes,
@@ -385,18 +383,18 @@ int ocnn_add_rms_norm_backward(const void* sum_dev, int64_t sum_row, const void*
       OCNN_CUDA_OK(cudaMemsetAsync(grad_weight_dev, 0, (size_t)channels * (weight_dtype == OCNN_F32 ? 4 : 2), st));
     return OCNN_OK;
   }
-  OCNN_REQUIRE(sum_dev && weight_dev, "ocnn_add_rms_norm_backward: null pointer");
+  OCNN_REQUIRE(x_dev && weight_dev, "ocnn_add_rms_norm_backward: null pointer");
   if (grad_weight_dev != nullptr &&
       (workspace_dev == nullptr || workspace_bytes < ocnn_add_rms_norm_backward_workspace_bytes(channels)))
     return fail(OCNN_ERR_CAPACITY, "ocnn_add_rms_norm_backward: %zu bytes of workspace are needed",
                 ocnn_add_rms_norm_backward_workspace_bytes(channels));
   NormArgs a = {};
-  a.s = sum_dev, a.r_row = sum_row, a.w = weight_dev, a.w_f32 = weight_dtype == OCNN_F32;
-  a.gy = grad_y_dev, a.gy_row = grad_y_dev ? grad_y_row : sum_row;
-  a.gs = grad_sum_dev, a.gs_row = grad_sum_dev ? grad_sum_row : sum_row;
+  a.x = x_dev, a.x_row = x_row, a.r = residual_dev, a.r_row = residual_dev ? residual_row : x_row;
+  a.w = weight_dev, a.w_f32 = weight_dtype == OCNN_F32;
+  a.gy = grad_y_dev, a.gy_row = grad_y_dev ? grad_y_row : x_row;
+  a.gs = grad_sum_dev, a.gs_row = grad_sum_dev ? grad_sum_row : x_row;
   a.g = grad_x_dev, a.rows = rows, a.channels = channels, a.eps = eps;
   a.partial = grad_weight_dev != nullptr ? (float*)workspace_dev : nullptr;
-  a.x_row = sum_row;
   int blocks = 0;
   const int status = norm_by_type(a, dtype, &blocks, st);
   if (status != OCNN_OK || grad_weight_dev == nullptr) return status;

@@ -148,7 +148,7 @@ struct AddRmsNorm : public torch::autograd::Function<AddRmsNorm> {
     at::AutoDispatchBelowADInplaceOrView guard;
     vector<Tensor> out = norm_call(data, residual, weight, eps);
     const bool has = out[1].defined();
-    ctx->save_for_backward({has ? out[1] : data, weight});
+    ctx->save_for_backward({data, weight, has ? *residual : Tensor()});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["has"] = has;
     ctx->set_materialize_grads(false);
@@ -168,14 +168,14 @@ struct AddRmsNorm : public torch::autograd::Function<AddRmsNorm> {
     const Tensor gy = grads[0], gs = has ? grads[1] : Tensor();
     if ((!gy.defined() && !gs.defined()) || (!need_x && !need_w)) return res;
     c10::cuda::CUDAGuard guard(weight.device());
-    const Tensor s = flat_rows(saved[0]), w = weight.contiguous();
+    const Tensor s = flat_rows(saved[0]), r = has ? flat_rows(saved[2]) : Tensor(), w = weight.contiguous();
     const int64_t rows = s.size(0), channels = s.size(1);
     const Tensor fy = gy.defined() ? flat_rows(gy) : Tensor(), fs = gs.defined() ? flat_rows(gs) : Tensor();
     Tensor g = need_x ? empty_rows(saved[0]) : Tensor(), gw = need_w ? torch::empty_like(w) : Tensor(), ws;
     const size_t bytes = need_w ? ocnn_add_rms_norm_backward_workspace_bytes((int)channels) : 0;
     if (bytes > 0) ws = torch::empty({(int64_t)bytes}, s.options().dtype(torch::kUInt8));
     OCNN_CALL(ocnn_add_rms_norm_backward(
-        s.data_ptr(), s.stride(0), w.data_ptr(), dtype_of(w, who), fy.defined() ? fy.data_ptr() : nullptr,
+        s.data_ptr(), s.stride(0), has ? r.data_ptr() : nullptr, has ? r.stride(0) : 0, w.data_ptr(), dtype_of(w, who), fy.defined() ? fy.data_ptr() : nullptr,
         fy.defined() ? fy.stride(0) : 0, fs.defined() ? fs.data_ptr() : nullptr, fs.defined() ? fs.stride(0) : 0,
         need_x ? g.data_ptr() : nullptr, need_w ? gw.data_ptr() : nullptr, rows, (int)channels,
         (float)ctx->saved_data["eps"].toDouble(), dtype_of(s, who), bytes > 0 ? ws.data_ptr() : nullptr, bytes,

@@ -84,7 +84,7 @@ def test_rotary_and_norm():
                                ctypes.c_float(1e-6), dtype, None)
   assert [norm(channels=0), norm(weight_dtype=2), norm(dtype=9), norm(rows=-1), norm(x=None)] == [INVALID] * 5
   assert norm(rows=0) == OK
-  assert L.ocnn_add_rms_norm_backward(P(64), I64(16), P(64), 0, None, I64(0), None, I64(0), P(64), P(64), I64(5), 16,
+  assert L.ocnn_add_rms_norm_backward(P(64), I64(16), None, I64(0), P(64), 0, None, I64(0), None, I64(0), P(64), P(64), I64(5), 16,
                                       ctypes.c_float(1e-6), 1, None, ctypes.c_size_t(0), None) == CAPACITY
 
 
