@@ -97,6 +97,10 @@ int ocnn_octree_attention_backward(const ocnn_attention* p, const void* out_dev,
   g.delta = (float*)workspace_dev;
   g.far = g.delta + delta_floats(p);
   g.dq = dq_dev, g.dk = dk_dev, g.dv = dv_dev;
+  if (on_tensor_cores(p) && on_boundary(grad_dev, grad_stride, p->dim, 8, 2) &&
+      (reinterpret_cast<uintptr_t>(out_dev) | reinterpret_cast<uintptr_t>(dq_dev) | reinterpret_cast<uintptr_t>(dk_dev) |
+       reinterpret_cast<uintptr_t>(dv_dev)) % 16 == 0)
+    return attn_tc_backward(a, g, p->dtype, status_dev, (cudaStream_t)stream);
   const bool vec = all_on_boundary(p, 4) && on_boundary(grad_dev, grad_stride, p->dim, 4, size_of(p->dtype)) &&
                    reinterpret_cast<uintptr_t>(out_dev) % (4 * size_of(p->dtype)) == 0;
   return attn_simt_backward(a, g, p->dtype, vec, (cudaStream_t)stream);

@@ -46,6 +46,8 @@ inline int attn_pack(const AttnArgs& a) {
 }
 
 int attn_tc_forward(const AttnArgs& a, int dtype, void* out, float* lse, int* status, cudaStream_t st);
+int attn_tc_backward(const AttnArgs& a, const AttnGrad& g, int dtype, int* status, cudaStream_t st);
+int attn_far_sums(const AttnArgs& a, const AttnGrad& g, int dtype, cudaStream_t st);
 int attn_simt_forward(const AttnArgs& a, int dtype, void* out, float* lse, bool vec, cudaStream_t st);
 int attn_simt_backward(const AttnArgs& a, const AttnGrad& g, int dtype, bool vec, cudaStream_t st);
 

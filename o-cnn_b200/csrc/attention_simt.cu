@@ -461,6 +461,13 @@ __global__ void __launch_bounds__(256) attn_far_kernel(const AttnArgs a, const A
   }
 }
 
+template <typename T>
+int far_launch(const AttnArgs& a, const AttnGrad& g, cudaStream_t st) {
+  attn_far_kernel<T><<<dim3(ceil_div(a.n, kFarRows), a.kv_heads), 256, 0, st>>>(a, g);
+  OCNN_LAUNCH_OK("attn_far_kernel");
+  return OCNN_OK;
+}
+
 template <typename T, int DP>
 int forward_launch(const AttnArgs& a, void* out, float* lse, bool vec, cudaStream_t st) {
   static PerDeviceOnce once;
@@ -488,8 +495,8 @@ int backward_launch(const AttnArgs& a, const AttnGrad& g, bool vec, cudaStream_t
   attn_simt_dq_kernel<T, DP><<<dim3(ceil_div(a.n, kB), a.heads), kThreads, dq_bytes, st>>>(a, g, vec);
   OCNN_LAUNCH_OK("attn_simt_dq_kernel");
   if (a.sinks > 0) {
-    attn_far_kernel<T><<<dim3(ceil_div(a.n, kFarRows), a.kv_heads), 256, 0, st>>>(a, g);
-    OCNN_LAUNCH_OK("attn_far_kernel");
+    const int far = far_launch<T>(a, g, st);
+    if (far != OCNN_OK) return far;
   }
   attn_simt_dkv_kernel<T, DP><<<dim3(ceil_div(a.n, kB), a.kv_heads), kThreads, dkv_bytes, st>>>(a, g, vec);
   OCNN_LAUNCH_OK("attn_simt_dkv_kernel");
@@ -511,6 +518,10 @@ int by_type(int dtype, int dim, F f) {
 
 }  // namespace
 
+int attn_far_sums(const AttnArgs& a, const AttnGrad& g, int dtype, cudaStream_t st) {
+  return dtype == OCNN_F32 ? far_launch<float>(a, g, st)
+         : dtype == OCNN_BF16 ? far_launch<__nv_bfloat16>(a, g, st) : far_launch<__half>(a, g, st);
+}
 int attn_simt_forward(const AttnArgs& a, int dtype, void* out, float* lse, bool vec, cudaStream_t st) {
   return by_type(dtype, a.dim, [&](auto t, auto dp) -> int {
     return forward_launch<decltype(t), decltype(dp)::value>(a, out, lse, vec, st);

@@ -1,0 +1,623 @@
+// Gradients of the attention over a window of nodes on the tensor cores, 16-bit data.
+//
+//     p = exp2(scale s - lse),  ds = p (dO . v - delta),  delta_i = dO_i . o_i
+//     dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij dO_i
+//
+// Two kernels, one over tiles of queries and one over tiles of keys, each forming s, dO . v and p for itself: seven
+// products instead of five, but every sum stays in tensor memory, in one order, and is written once; one kernel would
+// have to add dq into fp32 in global memory, with atomics whose order changes the result.
+//   queries: S = Q K^T, dP = dO V^T -> dS (tensor memory, in S's place) -> dQ += dS K
+//   keys:    S' = K Q^T, dP' = V dO^T -> P', dS' (in place) -> dV += P' dO, dK += dS' Q
+// P and dS are rounded to the data's type, which is what the products take.  Roles and tiles as in attention_tc.cu.
+#include "attention_tc.cuh"
+
+namespace ocnn {
+namespace {
+
+enum : int { kErrGradLoad = 21, kErrGradSlot = 22, kErrGradS = 23, kErrGradP = 24, kErrGradDone = 25, kErrGradTile = 26 };
+
+constexpr int kBN = 64;                        // columns of a block: keys, or rows of queries
+constexpr int kMaxStages = 6;
+
+struct GradArgs {
+  AttnArgs a;
+  AttnGrad g;
+  int* status;
+  int pack, stages;
+};
+
+constexpr int tmem_columns(int need) { return need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512; }
+
+template <int DP, int W>
+struct DqShape {
+  static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
+  static constexpr int kTile = 128 * kRowBytes * kPieces;                // Q, then dO
+  static constexpr int kBlock = kBN * kRowBytes * kPieces;               // K, then V
+  static constexpr int kAcc = 2 * kBN + DP;
+  static constexpr int kCols = tmem_columns(W * kAcc);
+  static constexpr size_t smem(int stages) { return (size_t)W * 2 * kTile + (size_t)stages * 2 * kBlock + 1024 + 256; }
+};
+
+// scores of one operand pair: D[128 x kBN] = A B^T over the channels
+template <bool HALF, int ROWS_A>
+__device__ __forceinline__ void product_channels(uint32_t d, uint32_t a, uint32_t b, int ksteps, uint32_t idesc) {
+  for (int k = 0; k < ksteps; ++k) {
+    const uint32_t in = (k & 3) * 32, piece = k >> 2;
+    umma_bf16(d, smem_desc_sw128(a + piece * (ROWS_A * kRowBytes) + in), smem_desc_sw128(b + piece * (kBN * kRowBytes) + in),
+              idesc, k > 0 ? 1u : 0u);
+  }
+}
+// D[128 x channels] += P[128 x kBN] B over the block's rows
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, bool first) {
+#pragma unroll
+  for (int k = 0; k < kBN / 16; ++k)
+    umma_ts(d, p + 8 * k, smem_desc_mn128(b + k * (16 * kRowBytes), kBN * kRowBytes), idesc, !first || k > 0 ? 1u : 0u);
+}
+
+template <int DP, int W, bool HALF, int CTAS>
+__global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_dq_kernel(const GradArgs p) {
+  using Shape = DqShape<DP, W>;
+  using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
+  const AttnArgs& a = p.a;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* stq = smem;
+  uint8_t* skv = stq + W * 2 * Shape::kTile;
+  uint64_t* full = reinterpret_cast<uint64_t*>(skv + p.stages * 2 * Shape::kBlock);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* qfull = empty + kMaxStages;
+  uint64_t* sfull = qfull + 1;
+  uint64_t* dsfull = sfull + W;
+  uint64_t* dqdone = dsfull + W;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dqdone + W);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  int* ranges = reinterpret_cast<int*>(tmem_holder + 2);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nodes = 128 / p.pack, r0 = blockIdx.x * (W * nodes);
+  const int group = a.heads / a.kv_heads, per_kv = group / p.pack;
+  const int hk = blockIdx.y / per_kv, h0 = hk * group + (blockIdx.y % per_kv) * p.pack;
+  if (tid == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(smem_u32(&full[s]), 32);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(qfull), 128 * W);
+    for (int t = 0; t < W; ++t) {
+      mbar_init(smem_u32(&sfull[t]), 1);
+      mbar_init(smem_u32(&dsfull[t]), 128);
+      mbar_init(smem_u32(&dqdone[t]), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4 * W) tmem_alloc(tmem_holder, Shape::kCols);
+  const TileKeys keys = attn_tile_keys(a, r0, r0 + W * nodes);
+  const int blocks = (keys.n + kBN - 1) / kBN;
+  if (W > 1 && tid < W) {
+    const TileKeys k = attn_tile_keys(a, r0 + tid * nodes, r0 + (tid + 1) * nodes);
+    const int at = k.lo - keys.lo + keys.n_first, end = at + k.n - k.n_first;
+    ranges[3 * tid] = k.n > 0 ? at / kBN : 0;
+    ranges[3 * tid + 1] = k.n > 0 ? (end + kBN - 1) / kBN : 0;
+    ranges[3 * tid + 2] = k.n > 0 && keys.n_first > 0 && k.first == keys.first;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  auto active = [&](int t, int b) {
+    if (W == 1) return true;
+    return (b >= ranges[3 * t] && b < ranges[3 * t + 1]) || (b == 0 && ranges[3 * t + 2] != 0);
+  };
+  const int ksteps = (a.dim + 15) / 16;
+
+  if (warp < 4 * W) {
+    // ---------------- rows ----------------
+    const int t = warp >> 2, row = tid & 127;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * Shape::kAcc, acc = lanes + 2 * kBN;
+    if (blocks > 0) {
+      const uint32_t dst = smem_u32(stq + t * 2 * Shape::kTile);
+      copy_tile<DP, 128, 128>(dst, row, a.dim, a.q, [&](int r) -> const void* {
+        const int i = r0 + t * nodes + r / p.pack;
+        return i < a.n ? (const T*)a.q + i * a.q_row + (h0 + r % p.pack) * a.q_head : nullptr;
+      });
+      copy_tile<DP, 128, 128>(dst + Shape::kTile, row, a.dim, a.q, [&](int r) -> const void* {
+        const int i = r0 + t * nodes + r / p.pack;
+        return i < a.n ? (const T*)p.g.grad + i * p.g.grad_row + (h0 + r % p.pack) * p.g.grad_head : nullptr;
+      });
+      cp_async_arrive(smem_u32(qfull));
+    }
+    const int i = r0 + t * nodes + row / p.pack, h = h0 + row % p.pack;
+    const bool in = i < a.n;
+    const RowKeys r = in ? attn_row_keys(a, i, attn_span(a, i)) : RowKeys{0, 0, 0, 0};
+    const float lse = in ? p.g.lse[(long long)h * a.n + i] : INFINITY;
+    float delta = 0.f;
+    if (in) {
+      const T* go = (const T*)p.g.grad + i * p.g.grad_row + h * p.g.grad_head;
+      const T* o = (const T*)p.g.out + ((long long)i * a.heads + h) * a.dim;
+      for (int d = 0; d < a.dim; d += 8) {
+        const uint4 x = *reinterpret_cast<const uint4*>(go + d), y = *reinterpret_cast<const uint4*>(o + d);
+        const uint32_t *xs = &x.x, *ys = &y.x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 u = unpack2(xs[e], HALF), v = unpack2(ys[e], HALF);
+          delta = fmaf(u.x, v.x, delta);
+          delta = fmaf(u.y, v.y, delta);
+        }
+      }
+      p.g.delta[(long long)h * a.n + i] = delta;
+    }
+    const float c = a.scale_log2;
+    int done = 0;
+    bool alive = true;
+    for (int b = 0; b < blocks && alive; ++b) {
+      if (!active(t, b)) continue;
+      uint32_t bits[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        bits[k] = seen_bits(a, keys, r, b * kBN + 32 * k);
+        if (a.mask != nullptr) {
+          const int at = b * kBN + 32 * k + lane;
+          bits[k] &= __ballot_sync(0xffffffffu, at < keys.n && a.mask[keys.key(at)] != 0);
+        }
+      }
+      alive = mbar_wait(smem_u32(&sfull[t]), done & 1, abort_flag, p.status, kErrGradS);
+      alive = __all_sync(0xffffffffu, alive);
+      if (!alive) break;
+      tc_fence_after();
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t w[16];
+        if (__any_sync(0xffffffffu, bits[k] != 0)) {
+          uint32_t s[32], dp[32];
+          tmem_ld32(lanes + 32 * k, s);
+          tmem_ld32(lanes + kBN + 32 * k, dp);
+          tmem_wait_ld();
+          const bool all = __all_sync(0xffffffffu, bits[k] == 0xffffffffu);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float x = exp2_approx(fmaf(__uint_as_float(s[e]), c, -lse)) * (__uint_as_float(dp[e]) - delta);
+            s[e] = __float_as_uint(all || ((bits[k] >> e) & 1) ? x : 0.f);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = pack16<HALF>(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = 0;
+        }
+        tmem_st16(lanes + 16 * k, w);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&dsfull[t]));
+      ++done;
+    }
+    if (done > 0 && alive) {
+      alive = mbar_wait(smem_u32(&dqdone[t]), (done - 1) & 1, abort_flag, p.status, kErrGradDone);
+      alive = __all_sync(0xffffffffu, alive);
+      tc_fence_after();
+    }
+    if (alive) {
+      T* dst = (T*)p.g.dq + ((long long)i * a.heads + h) * a.dim;
+#pragma unroll 1
+      for (int d = 0; d < a.dim; d += 16) {
+        uint32_t o[16], w[8];
+        if (done > 0) {
+          tmem_ld16(acc + d, o);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          w[e] = done > 0 ? pack16<HALF>(__uint_as_float(o[2 * e]) * a.scale, __uint_as_float(o[2 * e + 1]) * a.scale) : 0u;
+        if (in) {
+          *reinterpret_cast<uint4*>(dst + d) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (d + 8 < a.dim) *reinterpret_cast<uint4*>(dst + d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+      }
+    }
+  } else if (warp == 4 * W) {
+    // ---------------- products ----------------
+    if (lane == 0 && blocks > 0) {
+      const uint32_t idesc_s = attn_idesc<HALF>(kBN, false), idesc_o = attn_idesc<HALF>(16 * ksteps, true);
+      int n[W] = {};
+      bool alive = mbar_wait(smem_u32(qfull), 0, abort_flag, p.status, kErrGradTile);
+      int stage = 0;
+      uint32_t phase = 0;
+      auto wait_stage = [&](int s, uint32_t ph) {
+        if (alive) alive = mbar_wait(smem_u32(&full[s]), ph, abort_flag, p.status, kErrGradLoad);
+        if (alive) proxy_fence();
+      };
+      auto scores = [&](int t, int s) {
+        const uint32_t q = smem_u32(stq + t * 2 * Shape::kTile), k = smem_u32(skv + s * 2 * Shape::kBlock);
+        const uint32_t d = tmem + t * Shape::kAcc;
+        product_channels<HALF, 128>(d, q, k, ksteps, idesc_s);
+        product_channels<HALF, 128>(d + kBN, q + Shape::kTile, k + Shape::kBlock, ksteps, idesc_s);
+        umma_commit(smem_u32(&sfull[t]));
+      };
+      wait_stage(0, 0);
+      if (alive) tc_fence_after();
+      for (int t = 0; t < W && alive; ++t)
+        if (active(t, 0)) scores(t, 0);
+      for (int b = 0; b < blocks && alive; ++b) {
+        const int next = stage + 1 == p.stages ? 0 : stage + 1;
+        const uint32_t next_phase = next == 0 ? phase ^ 1u : phase;
+        if (b + 1 < blocks) wait_stage(next, next_phase);
+        for (int t = 0; t < W && alive; ++t) {
+          if (active(t, b)) {
+            alive = mbar_wait(smem_u32(&dsfull[t]), n[t] & 1, abort_flag, p.status, kErrGradP);
+            if (!alive) break;
+            tc_fence_after();
+            product_rows(tmem + t * Shape::kAcc + 2 * kBN, tmem + t * Shape::kAcc,
+                         smem_u32(skv + stage * 2 * Shape::kBlock), idesc_o, n[t] == 0);
+            umma_commit(smem_u32(&dqdone[t]));
+            ++n[t];
+          }
+          if (t == W - 1 && b + p.stages < blocks) umma_commit(smem_u32(&empty[stage]));
+          if (b + 1 < blocks && active(t, b + 1)) {
+            // (S lies where dS does: the product that reads dS has to be through)
+            if (n[t] > 0) alive = mbar_wait(smem_u32(&dqdone[t]), (n[t] - 1) & 1, abort_flag, p.status, kErrGradDone);
+            if (!alive) break;
+            tc_fence_after();
+            scores(t, next);
+          }
+        }
+        stage = next;
+        phase = next_phase;
+      }
+      if (!alive)
+        for (int it = 0; it < 64; ++it) __nanosleep(1000);       // (products under way end before tensor memory is freed)
+    }
+  } else {
+    // ---------------- copies of K and V ----------------
+    int stage = 0;
+    uint32_t phase = 0;
+    bool alive = true;
+    for (int b = 0; b < blocks && alive; ++b) {
+      uint32_t kept[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int at = b * kBN + 32 * k + lane;
+        kept[k] = __ballot_sync(0xffffffffu, at < keys.n && (a.mask == nullptr || a.mask[keys.key(at)] != 0));
+      }
+      if (b >= p.stages) {
+        alive = mbar_wait(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.status, kErrGradSlot);
+        alive = __all_sync(0xffffffffu, alive);
+        if (!alive) break;
+      }
+      const uint32_t dst = smem_u32(skv + stage * 2 * Shape::kBlock);
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {
+        const T* src = kv == 0 ? (const T*)a.k + hk * a.k_head : (const T*)a.v + hk * a.v_head;
+        const long long stride = kv == 0 ? a.k_row : a.v_row;
+        copy_tile<DP, kBN, 32>(dst + kv * Shape::kBlock, lane, a.dim, src, [&](int r) -> const void* {
+          return ((r < 32 ? kept[0] : kept[1]) >> (r & 31)) & 1 ? src + keys.key(b * kBN + r) * stride : nullptr;
+        });
+      }
+      cp_async_arrive(smem_u32(&full[stage]));
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4 * W)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Shape::kCols) : "memory");
+}
+
+// The nodes that see the keys [k0, k1) from within the window, whatever the mask says.
+__device__ __forceinline__ KeyRows attn_tile_rows(AttnArgs a, int k0, int k1) {
+  a.mask = nullptr;
+  const int f = max(k0, attn_offset(a, 0)), l = min(min(k1, a.n), attn_offset(a, a.batch)) - 1;
+  if (f > l) return KeyRows{0, 0};
+  const KeyRows x = attn_key_rows(a, f, attn_span(a, f)), y = attn_key_rows(a, l, attn_span(a, l));
+  return KeyRows{x.lo, y.hi};
+}
+
+template <int DP, int G>
+struct DkvShape {
+  static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
+  static constexpr int kTile = 128 * kRowBytes * kPieces;                // K, then V
+  static constexpr int kBlock = kBN * kRowBytes * kPieces;               // Q, then dO
+  static constexpr int kCols = tmem_columns(G * 2 * kBN + 2 * DP);       // S' and dP' of G blocks, dK, dV
+  static constexpr size_t smem(int stages) {
+    return (size_t)2 * kTile + (size_t)stages * 2 * kBlock + G * 2 * kBN * sizeof(float2) + 1024 + 256;
+  }
+};
+
+// One tile of 128 keys.  A block is kBN rows of queries: kBN / pack nodes, pack heads each; G groups of four warps take
+// the blocks in turn, each with S' and dP' of its own.
+template <int DP, int G, bool HALF, int CTAS>
+__global__ void __launch_bounds__(128 * G + 64, CTAS) attn_tc_dkv_kernel(const GradArgs p) {
+  using Shape = DkvShape<DP, G>;
+  using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
+  const AttnArgs& a = p.a;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* skv = smem;
+  uint8_t* sqg = skv + 2 * Shape::kTile;
+  float2* stats = reinterpret_cast<float2*>(sqg + p.stages * 2 * Shape::kBlock);     // [G][2][kBN]: lse, delta
+  uint64_t* full = reinterpret_cast<uint64_t*>(stats + G * 2 * kBN);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* kvfull = empty + kMaxStages;
+  uint64_t* sfull = kvfull + 1;
+  uint64_t* pfull = sfull + G;
+  uint64_t* done = pfull + G;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + G);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int k0 = blockIdx.x * 128, hk = blockIdx.y, group = a.heads / a.kv_heads;
+  if (tid == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(smem_u32(&full[s]), 32);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(kvfull), 128 * G);
+    for (int t = 0; t < G; ++t) {
+      mbar_init(smem_u32(&sfull[t]), 1);
+      mbar_init(smem_u32(&pfull[t]), 128);
+      mbar_init(smem_u32(&done[t]), 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4 * G) tmem_alloc(tmem_holder, Shape::kCols);
+  const KeyRows span = attn_tile_rows(a, k0, k0 + 128);
+  const int nodes = kBN / p.pack;                                          // of a block
+  const int per_head = (max(0, span.hi - span.lo) + nodes - 1) / nodes;    // blocks of `pack` heads
+  const int blocks = per_head * (group / p.pack);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  constexpr int kAcc = G * 2 * kBN;                                        // dK, then dV
+  const int ksteps = (a.dim + 15) / 16;
+  auto first_node = [&](int b) { return span.lo + (b % per_head) * nodes; };
+  auto first_head = [&](int b) { return hk * group + (b / per_head) * p.pack; };
+
+  if (warp < 4 * G) {
+    // ---------------- rows: keys ----------------
+    const int t = warp >> 2, row = tid & 127, j = k0 + row;
+    const uint32_t quarter = tmem + ((uint32_t)((warp & 3) * 32) << 16), lanes = quarter + t * 2 * kBN;
+    if (blocks > 0) {
+      auto kept = [&](int r) { return k0 + r < a.n && (a.mask == nullptr || a.mask[k0 + r] != 0); };
+      copy_tile<DP, 128, 128 * G>(smem_u32(skv), tid, a.dim, a.k, [&](int r) -> const void* {
+        return kept(r) ? (const T*)a.k + (k0 + r) * a.k_row + hk * a.k_head : nullptr;
+      });
+      copy_tile<DP, 128, 128 * G>(smem_u32(skv + Shape::kTile), tid, a.dim, a.k, [&](int r) -> const void* {
+        return kept(r) ? (const T*)a.v + (k0 + r) * a.v_row + hk * a.v_head : nullptr;
+      });
+      cp_async_arrive(smem_u32(kvfull));
+    }
+    const KeyRows kr = j < a.n ? attn_key_rows(a, j, attn_span(a, j)) : KeyRows{0, 0};
+    const float c = a.scale_log2;
+    // lse and delta of a block's rows: two threads a row fetch them a block ahead
+    auto fetch = [&](int b) {
+      const int r = row & (kBN - 1), i = first_node(b) + r / p.pack;
+      if (b >= blocks || i >= span.hi) return row < kBN ? INFINITY : 0.f;
+      const long long at = (long long)(first_head(b) + r % p.pack) * a.n + i;
+      return row < kBN ? p.g.lse[at] : p.g.delta[at];
+    };
+    float ahead = t < blocks ? fetch(t) : 0.f;
+    int n = 0;
+    bool alive = true;
+    // (a group's warps meet at the barrier in every block, one that has given up too)
+    for (int b = t; b < blocks; b += G, ++n) {
+      float2* st = stats + (t * 2 + (n & 1)) * kBN;
+      (row < kBN ? st[row].x : st[row - kBN].y) = ahead;
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+      ahead = fetch(b + G);
+      const int i0 = first_node(b);
+      const int lo = (max(kr.lo, i0) - i0) * p.pack, hi = (max(min(kr.hi, i0 + nodes), i0) - i0) * p.pack;
+      if (alive) alive = mbar_wait(smem_u32(&sfull[t]), n & 1, abort_flag, p.status, kErrGradS);
+      alive = __all_sync(0xffffffffu, alive);
+      if (alive) {
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t bits = bit_run(lo - 32 * k, hi - 32 * k);
+          uint32_t w[16], v[16];
+          if (__any_sync(0xffffffffu, bits != 0)) {
+            uint32_t s[32], dp[32];
+            tmem_ld32(lanes + 32 * k, s);
+            tmem_ld32(lanes + kBN + 32 * k, dp);
+            tmem_wait_ld();
+            const bool all = __all_sync(0xffffffffu, bits == 0xffffffffu);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float4 ld = *reinterpret_cast<const float4*>(st + 32 * k + e);
+              float x = exp2_approx(fmaf(__uint_as_float(s[e]), c, -ld.x));
+              float y = exp2_approx(fmaf(__uint_as_float(s[e + 1]), c, -ld.z));
+              float dx = x * (__uint_as_float(dp[e]) - ld.y), dy = y * (__uint_as_float(dp[e + 1]) - ld.w);
+              if (!all) {
+                if (!((bits >> e) & 1)) x = dx = 0.f;
+                if (!((bits >> (e + 1)) & 1)) y = dy = 0.f;
+              }
+              w[e / 2] = pack16<HALF>(x, y);
+              v[e / 2] = pack16<HALF>(dx, dy);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] = v[e] = 0;
+          }
+          tmem_st16(lanes + 16 * k, w);
+          tmem_st16(lanes + kBN + 16 * k, v);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&pfull[t]));
+      }
+    }
+    // The accumulators are through with the last block of every group of warps.  (Its own first: behind that, every other
+    // group's barrier is in the phase of its last block, or past it.)
+    for (int k = 0; k < G && alive; ++k) {
+      const int u = (t + k) % G, count = blocks > u ? (blocks - u + G - 1) / G : 0;
+      if (count > 0) alive = mbar_wait(smem_u32(&done[u]), (count - 1) & 1, abort_flag, p.status, kErrGradDone);
+    }
+    alive = __all_sync(0xffffffffu, alive);
+    tc_fence_after();
+    if (alive) {
+      const bool in = j < a.n;
+      const FarSums far = in ? far_sums(a, p.g, j, hk) : FarSums{nullptr, 0, 0, 0};
+      // group 0 writes dK, the last one dV (both, where there is one)
+#pragma unroll 1
+      for (int which = t == 0 ? 0 : 1; which <= (t == G - 1 ? 1 : 0); ++which) {
+        const float f = which == 0 ? a.scale : 1.f;
+        T* dst = (T*)(which == 0 ? p.g.dk : p.g.dv) + ((long long)j * a.kv_heads + hk) * a.dim;
+#pragma unroll 1
+        for (int d = 0; d < a.dim; d += 16) {
+          uint32_t o[16], w[8];
+          if (blocks > 0) {
+            tmem_ld16(quarter + kAcc + which * DP + d, o);
+            tmem_wait_ld();
+          }
+          if (in) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float x = blocks > 0 ? __uint_as_float(o[e]) : 0.f;
+              if (far.count > 0 && d + e < a.dim) {
+                float y = 0.f;
+                if (which == 0) far.add(d + e, x, y);
+                else far.add(d + e, y, x);
+              }
+              o[e] = __float_as_uint(x * f);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = pack16<HALF>(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+            *reinterpret_cast<uint4*>(dst + d) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (d + 8 < a.dim) *reinterpret_cast<uint4*>(dst + d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        }
+      }
+    }
+  } else if (warp == 4 * G) {
+    // ---------------- products ----------------
+    if (lane == 0 && blocks > 0) {
+      const uint32_t idesc_s = attn_idesc<HALF>(kBN, false), idesc_o = attn_idesc<HALF>(16 * ksteps, true);
+      bool alive = mbar_wait(smem_u32(kvfull), 0, abort_flag, p.status, kErrGradTile);
+      int ahead = 0, ahead_stage = 0;
+      uint32_t ahead_phase = 0;
+      auto scores = [&]() {                            // of the next block that has none yet
+        const int t = ahead % G, n = ahead / G;
+        if (alive) alive = mbar_wait(smem_u32(&full[ahead_stage]), ahead_phase, abort_flag, p.status, kErrGradLoad);
+        // (S' and dP' lie where P' and dS' do: the products that read those have to be through)
+        if (alive && n > 0) alive = mbar_wait(smem_u32(&done[t]), (n - 1) & 1, abort_flag, p.status, kErrGradDone);
+        if (!alive) return;
+        proxy_fence();
+        tc_fence_after();
+        const uint32_t q = smem_u32(sqg + ahead_stage * 2 * Shape::kBlock), k = smem_u32(skv), d = tmem + t * 2 * kBN;
+        product_channels<HALF, 128>(d, k, q, ksteps, idesc_s);
+        product_channels<HALF, 128>(d + kBN, k + Shape::kTile, q + Shape::kBlock, ksteps, idesc_s);
+        umma_commit(smem_u32(&sfull[t]));
+        ++ahead;
+        if (++ahead_stage == p.stages) {
+          ahead_stage = 0;
+          ahead_phase ^= 1u;
+        }
+      };
+      while (alive && ahead < blocks && ahead < G) scores();
+      int stage = 0;
+      for (int b = 0; b < blocks && alive; ++b) {
+        const int t = b % G;
+        alive = mbar_wait(smem_u32(&pfull[t]), (b / G) & 1, abort_flag, p.status, kErrGradP);
+        if (!alive) break;
+        tc_fence_after();
+        const uint32_t q = smem_u32(sqg + stage * 2 * Shape::kBlock), d = tmem + t * 2 * kBN;
+        product_rows(tmem + kAcc + DP, d, q + Shape::kBlock, idesc_o, b == 0);         // dV += P' dO
+        product_rows(tmem + kAcc, d + kBN, q, idesc_o, b == 0);                        // dK += dS' Q
+        umma_commit(smem_u32(&done[t]));
+        if (b + p.stages < blocks) umma_commit(smem_u32(&empty[stage]));
+        if (++stage == p.stages) stage = 0;
+        if (ahead < blocks) scores();
+      }
+      if (!alive)
+        for (int it = 0; it < 64; ++it) __nanosleep(1000);       // (products under way end before tensor memory is freed)
+    }
+  } else {
+    // ---------------- copies of Q and dO ----------------
+    int stage = 0;
+    uint32_t phase = 0;
+    bool alive = true;
+    for (int b = 0; b < blocks && alive; ++b) {
+      if (b >= p.stages) {
+        alive = mbar_wait(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.status, kErrGradSlot);
+        alive = __all_sync(0xffffffffu, alive);
+        if (!alive) break;
+      }
+      const uint32_t dst = smem_u32(sqg + stage * 2 * Shape::kBlock);
+      const int i0 = first_node(b), h0 = first_head(b);
+      copy_tile<DP, kBN, 32>(dst, lane, a.dim, a.q, [&](int r) -> const void* {
+        const int i = i0 + r / p.pack;
+        return i < span.hi ? (const T*)a.q + i * a.q_row + (h0 + r % p.pack) * a.q_head : nullptr;
+      });
+      copy_tile<DP, kBN, 32>(dst + Shape::kBlock, lane, a.dim, a.q, [&](int r) -> const void* {
+        const int i = i0 + r / p.pack;
+        return i < span.hi ? (const T*)p.g.grad + i * p.g.grad_row + (h0 + r % p.pack) * p.g.grad_head : nullptr;
+      });
+      cp_async_arrive(smem_u32(&full[stage]));
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4 * G)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Shape::kCols) : "memory");
+}
+
+template <typename Shape, int CTAS>
+int stages_for() {
+  constexpr size_t kMost = (227 * 1024) / CTAS - 1024;
+  int stages = kMaxStages;
+  while (stages > 2 && Shape::smem(stages) > kMost) --stages;
+  return stages;
+}
+
+template <int DP, int W, int G, bool HALF, int CTAS_Q, int CTAS_K>
+int grad_launch(GradArgs& p, cudaStream_t st) {
+  using Dq = DqShape<DP, W>;
+  using Dkv = DkvShape<DP, G>;
+  auto dq = attn_tc_dq_kernel<DP, W, HALF, CTAS_Q>;
+  auto dkv = attn_tc_dkv_kernel<DP, G, HALF, CTAS_K>;
+  const int stages_q = stages_for<Dq, CTAS_Q>(), stages_k = stages_for<Dkv, CTAS_K>();
+  static PerDeviceOnce once;
+  const int status = once.run([&]() -> int {
+    OCNN_CUDA_OK(cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Dq::smem(stages_q)));
+    OCNN_CUDA_OK(cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Dkv::smem(stages_k)));
+    return OCNN_OK;
+  });
+  if (status != OCNN_OK) return status;
+  p.stages = stages_q;
+  dq<<<dim3(ceil_div(p.a.n, W * 128 / p.pack), p.a.heads / p.pack), 128 * W + 64, Dq::smem(stages_q), st>>>(p);
+  OCNN_LAUNCH_OK("attn_tc_dq_kernel");
+  if (p.a.sinks > 0) {
+    const int far = attn_far_sums(p.a, p.g, HALF ? OCNN_F16 : OCNN_BF16, st);
+    if (far != OCNN_OK) return far;
+  }
+  p.stages = stages_k;
+  dkv<<<dim3(ceil_div(p.a.n, 128), p.a.kv_heads), 128 * G + 64, Dkv::smem(stages_k), st>>>(p);
+  OCNN_LAUNCH_OK("attn_tc_dkv_kernel");
+  return OCNN_OK;
+}
+
+template <bool HALF>
+int grad_by_width(GradArgs& p, cudaStream_t st) {
+  if (p.a.dim <= 32) return grad_launch<32, 1, 1, HALF, 2, 2>(p, st);
+  if (p.a.dim <= 64) return grad_launch<64, 1, 1, HALF, 2, 2>(p, st);
+  return grad_launch<128, 2, 2, HALF, 1, 1>(p, st);
+}
+
+}  // namespace
+
+int attn_tc_backward(const AttnArgs& a, const AttnGrad& g, int dtype, int* status, cudaStream_t st) {
+  GradArgs p = {a, g, status, attn_pack(a), 0};
+  return dtype == OCNN_F16 ? grad_by_width<true>(p, st) : grad_by_width<false>(p, st);
+}
+
+}  // namespace ocnn
