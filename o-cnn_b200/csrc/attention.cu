@@ -49,9 +49,12 @@ bool all_on_boundary(const ocnn_attention* a, int elements) {
          on_boundary(a->v_dev, a->v_stride, a->dim, elements, size);
 }
 
-// 16-bit rows in whole pieces of 16 bytes, and a positive scale (a tile's maximum is taken before it).
+// 16-bit rows in whole pieces of 16 bytes, less than 2^31 bytes apart (the kernels form addresses as base + node * int),
+// and a positive scale (a tile's maximum is taken before it).
+bool near_rows(const int64_t stride[2]) { return stride[0] < (1 << 30) && stride[0] > -(1 << 30); }
 bool on_tensor_cores(const ocnn_attention* a) {
-  return a->dtype != OCNN_F32 && all_on_boundary(a, 8) && a->scale > 0.f && a->scale < INFINITY;
+  return a->dtype != OCNN_F32 && all_on_boundary(a, 8) && a->scale > 0.f && a->scale < INFINITY &&
+         near_rows(a->q_stride) && near_rows(a->k_stride) && near_rows(a->v_stride);
 }
 
 size_t delta_floats(const ocnn_attention* a) { return ((size_t)a->heads * a->n + 31) / 32 * 32; }
@@ -97,7 +100,7 @@ int ocnn_octree_attention_backward(const ocnn_attention* p, const void* out_dev,
   g.delta = (float*)workspace_dev;
   g.far = g.delta + delta_floats(p);
   g.dq = dq_dev, g.dk = dk_dev, g.dv = dv_dev;
-  if (on_tensor_cores(p) && on_boundary(grad_dev, grad_stride, p->dim, 8, 2) &&
+  if (on_tensor_cores(p) && near_rows(grad_stride) && on_boundary(grad_dev, grad_stride, p->dim, 8, 2) &&
       (reinterpret_cast<uintptr_t>(out_dev) | reinterpret_cast<uintptr_t>(dq_dev) | reinterpret_cast<uintptr_t>(dk_dev) |
        reinterpret_cast<uintptr_t>(dv_dev)) % 16 == 0)
     return attn_tc_backward(a, g, p->dtype, status_dev, (cudaStream_t)stream);

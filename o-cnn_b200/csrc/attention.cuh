@@ -40,9 +40,11 @@ struct AttnGrad {
 };
 
 // Heads of a node that stand side by side in a tensor-core tile: the largest power of two in the group.
-inline int attn_pack(const AttnArgs& a) {
-  const int group = a.heads / a.kv_heads, pack = group & -group;
-  return pack < 32 ? pack : 32;
+inline int attn_pack_log(const AttnArgs& a) {
+  const int group = a.heads / a.kv_heads;
+  int log = 0;
+  while (log < 5 && (group >> log) % 2 == 0) ++log;
+  return log;
 }
 
 int attn_tc_forward(const AttnArgs& a, int dtype, void* out, float* lse, int* status, cudaStream_t st);

@@ -21,14 +21,15 @@ struct AttnFwdArgs {
   void* out;
   float* lse;
   int* status;
-  int pack, slots;
+  int pack_log, slots;
 };
 
 enum : int { kErrAttnQ = 11, kErrAttnLoad = 12, kErrAttnSlot = 13, kErrAttnP = 14, kErrAttnS = 15, kErrAttnO = 16 };
 
 template <int DP, int W, int BN>
 struct FwdShape {
-  static constexpr int kThreads = 128 * W + 64;
+  static constexpr int kLoad = DP > 64 ? 2 : 1;                            // warps that copy
+  static constexpr int kThreads = 128 * W + 32 + 32 * kLoad;
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTileQ = 128 * kRowBytes * kPieces;
   static constexpr int kSlot = BN * kRowBytes * kPieces;
@@ -38,7 +39,7 @@ struct FwdShape {
 };
 
 template <int DP, int W, int BN, bool HALF, int CTAS>
-__global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_kernel(const AttnFwdArgs p) {
+__global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS) attn_tc_kernel(const AttnFwdArgs p) {
   using Shape = FwdShape<DP, W, BN>;
   using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
   constexpr int kMaxSlots = 8;
@@ -58,14 +59,14 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_kernel(const AttnF
   int* ranges = reinterpret_cast<int*>(tmem_holder + 2);                   // per tile: first and last block, first nodes
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int nodes = 128 / p.pack;                                          // of a tile
+  const int nodes = 128 >> p.pack_log, pack = 1 << p.pack_log;             // of a tile
   const int r0 = blockIdx.x * (W * nodes);
-  const int group = a.heads / a.kv_heads, per_kv = group / p.pack;
-  const int hk = blockIdx.y / per_kv, h0 = hk * group + (blockIdx.y % per_kv) * p.pack;
+  const int group = a.heads / a.kv_heads, per_kv = group >> p.pack_log;
+  const int hk = blockIdx.y / per_kv, h0 = hk * group + (blockIdx.y % per_kv) * pack;
 
   if (tid == 0) {
     for (int s = 0; s < p.slots; ++s) {
-      mbar_init(smem_u32(&full[s]), 32);
+      mbar_init(smem_u32(&full[s]), 32 * Shape::kLoad);
       mbar_init(smem_u32(&empty[s]), 1);
     }
     mbar_init(smem_u32(qfull), 128 * W);
@@ -103,13 +104,13 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_kernel(const AttnF
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * Shape::kAcc, acc = lanes + BN;
     if (blocks > 0) {
-      copy_tile<DP, 128, 128>(smem_u32(sq + t * Shape::kTileQ), row, a.dim, a.q, [&](int r) -> const void* {
-        const int i = r0 + t * nodes + r / p.pack;
-        return i < a.n ? (const T*)a.q + i * a.q_row + (h0 + r % p.pack) * a.q_head : nullptr;
-      });
+      const int node = r0 + t * nodes;
+      const PackedRows q = {(const uint8_t*)((const T*)a.q + h0 * a.q_head), (int)(a.q_row * 2), p.pack_log, a.q_head * 2};
+      copy_tile<DP, 128, 128>(smem_u32(sq + t * Shape::kTileQ), row, a.dim, a.q, [&](int r) { return q(node, r); },
+                              [&](int r) { return node + (r >> p.pack_log) < a.n; });
       cp_async_arrive(smem_u32(qfull));
     }
-    const int i = r0 + t * nodes + row / p.pack, h = h0 + row % p.pack;
+    const int i = r0 + t * nodes + (row >> p.pack_log), h = h0 + (row & (pack - 1));
     const RowKeys r = i < a.n ? attn_row_keys(a, i, attn_span(a, i)) : RowKeys{0, 0, 0, 0};
     const float c = a.scale_log2;
     float ref = -INFINITY, total = 0.f;                                    // the reference, in powers of two
@@ -130,22 +131,23 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_kernel(const AttnF
       alive = __all_sync(0xffffffffu, alive);
       if (!alive) break;
       tc_fence_after();
-      float top = -INFINITY;
+      float s[BN];
+      tmem_load<BN>(lanes, s);
+      bool all = true;
 #pragma unroll
-      for (int k = 0; k < BN / 32; ++k) {
-        if (!__any_sync(0xffffffffu, bits[k] != 0)) continue;
-        uint32_t s[32];
-        tmem_ld32(lanes + 32 * k, s);
-        tmem_wait_ld();
-        if (__all_sync(0xffffffffu, bits[k] == 0xffffffffu)) {
+      for (int k = 0; k < BN / 32; ++k) all = all && bits[k] == 0xffffffffu;
+      all = __all_sync(0xffffffffu, all);
+      tmem_wait_ld();
+      if (!all) {
+        // (a hidden score is -inf, c > 0: its p is 0)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(s[e]));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) top = fmaxf(top, (bits[k] >> e) & 1 ? __uint_as_float(s[e]) : -INFINITY);
-        }
+        for (int e = 0; e < BN; ++e)
+          if (!((bits[e / 32] >> (e & 31)) & 1)) s[e] = -INFINITY;
       }
-      top *= c;
+      float tops[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int e = 4; e < BN; e += 2) tops[(e / 2) & 3] = max3(tops[(e / 2) & 3], s[e], s[e + 1]);
+      const float top = max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]) * c;
       const bool move = top > ref + 8.f;                                   // (from -inf too)
       if (__any_sync(0xffffffffu, move)) {
         const float keep = move ? exp2_approx(ref - top) : 1.f;
@@ -166,33 +168,22 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_kernel(const AttnF
         }
       }
       const float base = ref == -INFINITY ? 0.f : ref;
+      const uint64_t c2 = pair(c, c), base2 = pair(-base, -base);
+      uint64_t sums[2] = {pair(total, 0.f), 0};
 #pragma unroll
       for (int k = 0; k < BN / 32; ++k) {
         uint32_t w[16];
-        if (__any_sync(0xffffffffu, bits[k] != 0)) {
-          uint32_t s[32];
-          tmem_ld32(lanes + 32 * k, s);
-          tmem_wait_ld();
-          if (!__all_sync(0xffffffffu, bits[k] == 0xffffffffu)) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((bits[k] >> e) & 1)) s[e] = __float_as_uint(-INFINITY);
-          }
-          // (a hidden score is -inf, c > 0: its p is 0)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float x = exp2_approx(fmaf(__uint_as_float(s[2 * e]), c, -base));
-            const float y = exp2_approx(fmaf(__uint_as_float(s[2 * e + 1]), c, -base));
-            total += x + y;
-            w[e] = pack16<HALF>(x, y);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = 0;
+        for (int e = 0; e < 16; ++e) {
+          const float2 x = unpair(fma2(pair(s[32 * k + 2 * e], s[32 * k + 2 * e + 1]), c2, base2));
+          const float px = exp2_approx(x.x), py = exp2_approx(x.y);
+          sums[e & 1] = add2(sums[e & 1], pair(px, py));
+          w[e] = pack16<HALF>(px, py);
         }
-        // columns 16 k .. of P lie where scores 16 k .. lay: read by now
-        tmem_st16(lanes + 16 * k, w);
+        tmem_st16(lanes + 16 * k, w);                                      // (where the scores lay: all read)
       }
+      const float2 sum = unpair(add2(sums[0], sums[1]));
+      total = sum.x + sum.y;
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(smem_u32(&pfull[t]));
@@ -308,6 +299,10 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_kernel(const AttnF
     }
   } else {
     // ---------------- copies of K and V ----------------
+    const int thread = tid - 128 * W - 32;
+    const uint8_t* const base[2] = {(const uint8_t*)((const T*)a.k + hk * a.k_head),
+                                    (const uint8_t*)((const T*)a.v + hk * a.v_head)};
+    const int stride[2] = {(int)(a.k_row * 2), (int)(a.v_row * 2)};
     int slot = 0;
     uint32_t empty_phase = 0;
     bool alive = true;
@@ -318,6 +313,7 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_kernel(const AttnF
         const int at = b * BN + 32 * k + lane;
         kept[k] = __ballot_sync(0xffffffffu, at < keys.n && (a.mask == nullptr || a.mask[keys.key(at)] != 0));
       }
+      const int j0 = keys.lo - keys.n_first + b * BN, nf = keys.n_first - b * BN, early = keys.first - j0;
 #pragma unroll 1
       for (int kv = 0; kv < 2 && alive; ++kv) {
         if (2 * b + kv >= p.slots) {
@@ -326,15 +322,10 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_kernel(const AttnF
           empty_phase ^= 1u << slot;
           if (!alive) break;
         }
-        const T* src = kv == 0 ? (const T*)a.k + hk * a.k_head : (const T*)a.v + hk * a.v_head;
-        const long long stride = kv == 0 ? a.k_row : a.v_row;
-        copy_tile<DP, BN, 32>(smem_u32(skv + slot * Shape::kSlot), lane, a.dim, src, [&](int r) -> const void* {
-          uint32_t w = kept[0];
-#pragma unroll
-          for (int k = 1; k < BN / 32; ++k)
-            if (r >= 32 * k) w = kept[k];
-          return (w >> (r & 31)) & 1 ? src + keys.key(b * BN + r) * stride : nullptr;
-        });
+        copy_tile<DP, BN, 32 * Shape::kLoad>(
+            smem_u32(skv + slot * Shape::kSlot), thread, a.dim, base[0],
+            [&](int r) { return base[kv] + (long long)(j0 + r + (r < nf ? early : 0)) * stride[kv]; },
+            [&](int r) { return ((r < 32 ? kept[0] : r < 64 ? kept[1] : r < 96 ? kept[BN / 32 - 2] : kept[BN / 32 - 1]) >> (r & 31)) & 1; });
         cp_async_arrive(smem_u32(&full[slot]));
         slot = slot + 1 == p.slots ? 0 : slot + 1;
       }
@@ -362,23 +353,23 @@ int fwd_launch(AttnFwdArgs& p, cudaStream_t st) {
     return OCNN_OK;
   });
   if (status != OCNN_OK) return status;
-  const int nodes = W * 128 / p.pack;
-  attn_tc_kernel<DP, W, BN, HALF, CTAS><<<dim3(ceil_div(p.a.n, nodes), p.a.heads / p.pack), Shape::kThreads, bytes, st>>>(p);
+  const int nodes = W * 128 >> p.pack_log;
+  attn_tc_kernel<DP, W, BN, HALF, CTAS><<<dim3(ceil_div(p.a.n, nodes), p.a.heads >> p.pack_log), Shape::kThreads, bytes, st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_kernel");
   return OCNN_OK;
 }
 
 template <bool HALF>
 int fwd_by_width(AttnFwdArgs& p, cudaStream_t st) {
-  if (p.a.dim <= 32) return fwd_launch<32, 1, 64, HALF, 4>(p, st);
-  if (p.a.dim <= 64) return fwd_launch<64, 1, 64, HALF, 4>(p, st);
+  if (p.a.dim <= 32) return fwd_launch<32, 1, 64, HALF, 3>(p, st);
+  if (p.a.dim <= 64) return fwd_launch<64, 1, 64, HALF, 3>(p, st);
   return fwd_launch<128, 2, 128, HALF, 1>(p, st);
 }
 
 }  // namespace
 
 int attn_tc_forward(const AttnArgs& a, int dtype, void* out, float* lse, int* status, cudaStream_t st) {
-  AttnFwdArgs p = {a, out, lse, status, attn_pack(a), 0};
+  AttnFwdArgs p = {a, out, lse, status, attn_pack_log(a), 0};
   return dtype == OCNN_F16 ? fwd_by_width<true>(p, st) : fwd_by_width<false>(p, st);
 }
 

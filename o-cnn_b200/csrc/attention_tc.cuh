@@ -61,21 +61,36 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// Copies of ROWS rows of `dim` channels (zeros up to the next multiple of 16, and for rows where src gives NULL).
-template <int DP, int ROWS, int LANES, typename Src>
-__device__ __forceinline__ void copy_tile(uint32_t dst, int lane, int dim, const void* any, Src src) {
-  constexpr int kChunks = DP / 8;
-  const int full = dim >> 3, chunks = (dim + 15) / 16 * 2;
-#pragma unroll 4
-  for (int e = lane; e < ROWS * kChunks; e += LANES) {
-    const int r = e / kChunks, c = e % kChunks;
-    if (c >= chunks) continue;
-    const uint8_t* row = (const uint8_t*)src(r);
-    const bool live = row != nullptr && c < full;
-    cp_async16(dst + (c >> 3) * (ROWS * kRowBytes) + r * kRowBytes + (((c & 7) ^ (r & 7)) << 4),
-               live ? row + c * 16 : any, live ? 16u : 0u);
+// Copies of ROWS rows of `dim` channels by LANES threads, zeros up to the next multiple of 16 and for rows that are not
+// live.  row(r): where row r starts.  A lane has one piece of every kStep-th row, so that all but the row's address is known
+// before the loop (one warp per CTA makes all its copies: with a division and 64-bit products per piece it was the copies'
+// instructions that bounded every kernel here).
+template <int DP, int ROWS, int LANES, typename Row, typename Live>
+__device__ __forceinline__ void copy_tile(uint32_t dst, int lane, int dim, const void* any, Row row, Live live) {
+  constexpr int kChunks = DP / 8, kStep = LANES / kChunks;
+  static_assert(LANES % kChunks == 0 && ROWS % kStep == 0, "every lane has whole pieces");
+  const int c = lane % kChunks, sub = lane / kChunks;
+  if (c >= (dim + 15) / 16 * 2) return;
+  const bool in = c < (dim >> 3);
+  const uint32_t base = dst + (c >> 3) * (ROWS * kRowBytes) + sub * kRowBytes, x = (c & 7) ^ (sub & 7);
+#pragma unroll 8
+  for (int it = 0; it < ROWS / kStep; ++it) {
+    const int r = it * kStep + sub;
+    const bool ok = in && live(r);
+    cp_async16(base + it * (kStep * kRowBytes) + ((x ^ ((it * kStep) & 7)) << 4), ok ? row(r) + c * 16 : any,
+               ok ? 16u : 0u);
   }
 }
+
+// The rows of a tile that are (node, head) pairs, 1 << pack_log heads of each node side by side.
+struct PackedRows {
+  const uint8_t* base;               // node 0, first head
+  int row, pack_log;                 // bytes from node to node
+  long long head;
+  __device__ __forceinline__ const uint8_t* operator()(int node, int r) const {
+    return base + (long long)(node + (r >> pack_log)) * row + (r & ((1 << pack_log) - 1)) * head;
+  }
+};
 
 // The keys that the nodes [r0, r1) see between them.  Windows move on with the nodes, so the first and the last node
 // that are in a sequence say it all.
@@ -118,6 +133,50 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   if constexpr (HALF) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
   else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
   return w;
+}
+
+// ---- two fp32 values per instruction (sm_100) -------------------------------------------------------------------
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// N columns of tensor memory, all under way at once.
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[N]) {
+#pragma unroll
+  for (int k = 0; k < N / 32; ++k) tmem_ld32(addr + 32 * k, reinterpret_cast<uint32_t(&)[32]>(v[32 * k]));
+}
+template <int N>
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&v)[N]) {
+#pragma unroll
+  for (int k = 0; k < N / 16; ++k) tmem_st16(addr + 16 * k, reinterpret_cast<const uint32_t(&)[16]>(v[16 * k]));
 }
 
 // An instruction descriptor: fp32 accumulator, 128 rows, n columns; B K-major or MN-major.

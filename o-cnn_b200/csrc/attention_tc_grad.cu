@@ -23,13 +23,17 @@ struct GradArgs {
   AttnArgs a;
   AttnGrad g;
   int* status;
-  int pack, stages;
+  int pack_log, stages;
 };
 
 constexpr int tmem_columns(int need) { return need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512; }
 
+template <int DP>
+constexpr int kLoadWarps = DP > 64 ? 2 : 1;      // warps that copy
+
 template <int DP, int W>
 struct DqShape {
+  static constexpr int kThreads = 128 * W + 32 + 32 * kLoadWarps<DP>;
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTile = 128 * kRowBytes * kPieces;                // Q, then dO
   static constexpr int kBlock = kBN * kRowBytes * kPieces;               // K, then V
@@ -55,7 +59,7 @@ __device__ __forceinline__ void product_rows(uint32_t d, uint32_t p, uint32_t b,
 }
 
 template <int DP, int W, bool HALF, int CTAS>
-__global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_dq_kernel(const GradArgs p) {
+__global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_kernel(const GradArgs p) {
   using Shape = DqShape<DP, W>;
   using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
   const AttnArgs& a = p.a;
@@ -74,12 +78,12 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_dq_kernel(const Gr
   int* ranges = reinterpret_cast<int*>(tmem_holder + 2);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int nodes = 128 / p.pack, r0 = blockIdx.x * (W * nodes);
-  const int group = a.heads / a.kv_heads, per_kv = group / p.pack;
-  const int hk = blockIdx.y / per_kv, h0 = hk * group + (blockIdx.y % per_kv) * p.pack;
+  const int nodes = 128 >> p.pack_log, pack = 1 << p.pack_log, r0 = blockIdx.x * (W * nodes);
+  const int group = a.heads / a.kv_heads, per_kv = group >> p.pack_log;
+  const int hk = blockIdx.y / per_kv, h0 = hk * group + (blockIdx.y % per_kv) * pack;
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(smem_u32(&full[s]), 32);
+      mbar_init(smem_u32(&full[s]), 32 * kLoadWarps<DP>);
       mbar_init(smem_u32(&empty[s]), 1);
     }
     mbar_init(smem_u32(qfull), 128 * W);
@@ -117,17 +121,16 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_dq_kernel(const Gr
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * Shape::kAcc, acc = lanes + 2 * kBN;
     if (blocks > 0) {
       const uint32_t dst = smem_u32(stq + t * 2 * Shape::kTile);
-      copy_tile<DP, 128, 128>(dst, row, a.dim, a.q, [&](int r) -> const void* {
-        const int i = r0 + t * nodes + r / p.pack;
-        return i < a.n ? (const T*)a.q + i * a.q_row + (h0 + r % p.pack) * a.q_head : nullptr;
-      });
-      copy_tile<DP, 128, 128>(dst + Shape::kTile, row, a.dim, a.q, [&](int r) -> const void* {
-        const int i = r0 + t * nodes + r / p.pack;
-        return i < a.n ? (const T*)p.g.grad + i * p.g.grad_row + (h0 + r % p.pack) * p.g.grad_head : nullptr;
-      });
+      const int node = r0 + t * nodes;
+      const PackedRows q = {(const uint8_t*)((const T*)a.q + h0 * a.q_head), (int)(a.q_row * 2), p.pack_log, a.q_head * 2};
+      const PackedRows g = {(const uint8_t*)((const T*)p.g.grad + h0 * p.g.grad_head), (int)(p.g.grad_row * 2), p.pack_log,
+                            p.g.grad_head * 2};
+      auto live = [&](int r) { return node + (r >> p.pack_log) < a.n; };
+      copy_tile<DP, 128, 128>(dst, row, a.dim, a.q, [&](int r) { return q(node, r); }, live);
+      copy_tile<DP, 128, 128>(dst + Shape::kTile, row, a.dim, a.q, [&](int r) { return g(node, r); }, live);
       cp_async_arrive(smem_u32(qfull));
     }
-    const int i = r0 + t * nodes + row / p.pack, h = h0 + row % p.pack;
+    const int i = r0 + t * nodes + (row >> p.pack_log), h = h0 + (row & (pack - 1));
     const bool in = i < a.n;
     const RowKeys r = in ? attn_row_keys(a, i, attn_span(a, i)) : RowKeys{0, 0, 0, 0};
     const float lse = in ? p.g.lse[(long long)h * a.n + i] : INFINITY;
@@ -147,7 +150,7 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_dq_kernel(const Gr
       }
       p.g.delta[(long long)h * a.n + i] = delta;
     }
-    const float c = a.scale_log2;
+    const uint64_t c2 = pair(a.scale_log2, a.scale_log2), lse2 = pair(-lse, -lse), delta2 = pair(-delta, -delta);
     int done = 0;
     bool alive = true;
     for (int b = 0; b < blocks && alive; ++b) {
@@ -165,28 +168,28 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_dq_kernel(const Gr
       alive = __all_sync(0xffffffffu, alive);
       if (!alive) break;
       tc_fence_after();
+      float s[kBN], dp[kBN];
+      tmem_load<kBN>(lanes, s);
+      tmem_load<kBN>(lanes + kBN, dp);
+      const bool all = __all_sync(0xffffffffu, (bits[0] & bits[1]) == 0xffffffffu);
+      tmem_wait_ld();
+      uint32_t w[kBN / 2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint32_t w[16];
-        if (__any_sync(0xffffffffu, bits[k] != 0)) {
-          uint32_t s[32], dp[32];
-          tmem_ld32(lanes + 32 * k, s);
-          tmem_ld32(lanes + kBN + 32 * k, dp);
-          tmem_wait_ld();
-          const bool all = __all_sync(0xffffffffu, bits[k] == 0xffffffffu);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float x = exp2_approx(fmaf(__uint_as_float(s[e]), c, -lse)) * (__uint_as_float(dp[e]) - delta);
-            s[e] = __float_as_uint(all || ((bits[k] >> e) & 1) ? x : 0.f);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = pack16<HALF>(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = 0;
-        }
-        tmem_st16(lanes + 16 * k, w);
+      for (int e = 0; e < kBN / 2; ++e) {
+        const float2 x = unpair(fma2(pair(s[2 * e], s[2 * e + 1]), c2, lse2));
+        const uint64_t ds = mul2(pair(exp2_approx(x.x), exp2_approx(x.y)), add2(pair(dp[2 * e], dp[2 * e + 1]), delta2));
+        const float2 y = unpair(ds);
+        s[2 * e] = y.x;
+        s[2 * e + 1] = y.y;
       }
+      if (!all) {
+#pragma unroll
+        for (int e = 0; e < kBN; ++e)
+          if (!((bits[e / 32] >> (e & 31)) & 1)) s[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < kBN / 2; ++e) w[e] = pack16<HALF>(s[2 * e], s[2 * e + 1]);
+      tmem_store<kBN / 2>(lanes, w);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(smem_u32(&dsfull[t]));
@@ -269,6 +272,10 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_dq_kernel(const Gr
     }
   } else {
     // ---------------- copies of K and V ----------------
+    const int thread = tid - 128 * W - 32;
+    const uint8_t* const base[2] = {(const uint8_t*)((const T*)a.k + hk * a.k_head),
+                                    (const uint8_t*)((const T*)a.v + hk * a.v_head)};
+    const int stride[2] = {(int)(a.k_row * 2), (int)(a.v_row * 2)};
     int stage = 0;
     uint32_t phase = 0;
     bool alive = true;
@@ -285,14 +292,13 @@ __global__ void __launch_bounds__(128 * W + 64, CTAS) attn_tc_dq_kernel(const Gr
         if (!alive) break;
       }
       const uint32_t dst = smem_u32(skv + stage * 2 * Shape::kBlock);
+      const int j0 = keys.lo - keys.n_first + b * kBN, nf = keys.n_first - b * kBN, early = keys.first - j0;
 #pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv) {
-        const T* src = kv == 0 ? (const T*)a.k + hk * a.k_head : (const T*)a.v + hk * a.v_head;
-        const long long stride = kv == 0 ? a.k_row : a.v_row;
-        copy_tile<DP, kBN, 32>(dst + kv * Shape::kBlock, lane, a.dim, src, [&](int r) -> const void* {
-          return ((r < 32 ? kept[0] : kept[1]) >> (r & 31)) & 1 ? src + keys.key(b * kBN + r) * stride : nullptr;
-        });
-      }
+      for (int kv = 0; kv < 2; ++kv)
+        copy_tile<DP, kBN, 32 * kLoadWarps<DP>>(
+            dst + kv * Shape::kBlock, thread, a.dim, base[0],
+            [&](int r) { return base[kv] + (long long)(j0 + r + (r < nf ? early : 0)) * stride[kv]; },
+            [&](int r) { return ((r < 32 ? kept[0] : kept[1]) >> (r & 31)) & 1; });
       cp_async_arrive(smem_u32(&full[stage]));
       if (++stage == p.stages) {
         stage = 0;
@@ -318,19 +324,20 @@ __device__ __forceinline__ KeyRows attn_tile_rows(AttnArgs a, int k0, int k1) {
 
 template <int DP, int G>
 struct DkvShape {
+  static constexpr int kThreads = 128 * G + 32 + 32 * kLoadWarps<DP>;
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTile = 128 * kRowBytes * kPieces;                // K, then V
   static constexpr int kBlock = kBN * kRowBytes * kPieces;               // Q, then dO
   static constexpr int kCols = tmem_columns(G * 2 * kBN + 2 * DP);       // S' and dP' of G blocks, dK, dV
   static constexpr size_t smem(int stages) {
-    return (size_t)2 * kTile + (size_t)stages * 2 * kBlock + G * 2 * kBN * sizeof(float2) + 1024 + 256;
+    return (size_t)2 * kTile + (size_t)stages * 2 * kBlock + G * 4 * kBN * sizeof(float) + 1024 + 256;
   }
 };
 
 // One tile of 128 keys.  A block is kBN rows of queries: kBN / pack nodes, pack heads each; G groups of four warps take
 // the blocks in turn, each with S' and dP' of its own.
 template <int DP, int G, bool HALF, int CTAS>
-__global__ void __launch_bounds__(128 * G + 64, CTAS) attn_tc_dkv_kernel(const GradArgs p) {
+__global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_kernel(const GradArgs p) {
   using Shape = DkvShape<DP, G>;
   using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
   const AttnArgs& a = p.a;
@@ -338,8 +345,8 @@ __global__ void __launch_bounds__(128 * G + 64, CTAS) attn_tc_dkv_kernel(const G
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* skv = smem;
   uint8_t* sqg = skv + 2 * Shape::kTile;
-  float2* stats = reinterpret_cast<float2*>(sqg + p.stages * 2 * Shape::kBlock);     // [G][2][kBN]: lse, delta
-  uint64_t* full = reinterpret_cast<uint64_t*>(stats + G * 2 * kBN);
+  float* stats = reinterpret_cast<float*>(sqg + p.stages * 2 * Shape::kBlock);       // [G][2][-lse, -delta][kBN]
+  uint64_t* full = reinterpret_cast<uint64_t*>(stats + G * 4 * kBN);
   uint64_t* empty = full + kMaxStages;
   uint64_t* kvfull = empty + kMaxStages;
   uint64_t* sfull = kvfull + 1;
@@ -352,7 +359,7 @@ __global__ void __launch_bounds__(128 * G + 64, CTAS) attn_tc_dkv_kernel(const G
   const int k0 = blockIdx.x * 128, hk = blockIdx.y, group = a.heads / a.kv_heads;
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(smem_u32(&full[s]), 32);
+      mbar_init(smem_u32(&full[s]), 32 * kLoadWarps<DP>);
       mbar_init(smem_u32(&empty[s]), 1);
     }
     mbar_init(smem_u32(kvfull), 128 * G);
@@ -366,17 +373,19 @@ __global__ void __launch_bounds__(128 * G + 64, CTAS) attn_tc_dkv_kernel(const G
   }
   if (warp == 4 * G) tmem_alloc(tmem_holder, Shape::kCols);
   const KeyRows span = attn_tile_rows(a, k0, k0 + 128);
-  const int nodes = kBN / p.pack;                                          // of a block
-  const int per_head = (max(0, span.hi - span.lo) + nodes - 1) / nodes;    // blocks of `pack` heads
-  const int blocks = per_head * (group / p.pack);
+  const int pack = 1 << p.pack_log, nodes = kBN >> p.pack_log;             // nodes of a block
+  const int per_head = (max(0, span.hi - span.lo) + nodes - 1) >> (6 - p.pack_log);   // blocks of `pack` heads
+  const int blocks = per_head * (group >> p.pack_log);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   constexpr int kAcc = G * 2 * kBN;                                        // dK, then dV
   const int ksteps = (a.dim + 15) / 16;
-  auto first_node = [&](int b) { return span.lo + (b % per_head) * nodes; };
-  auto first_head = [&](int b) { return hk * group + (b / per_head) * p.pack; };
+  // (blocks go head by head: no division where there is only one run of them)
+  auto run_of = [&](int b) { return b < per_head ? 0 : b / per_head; };
+  auto first_node = [&](int b) { return span.lo + (b - run_of(b) * per_head) * nodes; };
+  auto first_head = [&](int b) { return hk * group + run_of(b) * pack; };
 
   if (warp < 4 * G) {
     // ---------------- rows: keys ----------------
@@ -384,65 +393,66 @@ __global__ void __launch_bounds__(128 * G + 64, CTAS) attn_tc_dkv_kernel(const G
     const uint32_t quarter = tmem + ((uint32_t)((warp & 3) * 32) << 16), lanes = quarter + t * 2 * kBN;
     if (blocks > 0) {
       auto kept = [&](int r) { return k0 + r < a.n && (a.mask == nullptr || a.mask[k0 + r] != 0); };
-      copy_tile<DP, 128, 128 * G>(smem_u32(skv), tid, a.dim, a.k, [&](int r) -> const void* {
-        return kept(r) ? (const T*)a.k + (k0 + r) * a.k_row + hk * a.k_head : nullptr;
-      });
-      copy_tile<DP, 128, 128 * G>(smem_u32(skv + Shape::kTile), tid, a.dim, a.k, [&](int r) -> const void* {
-        return kept(r) ? (const T*)a.v + (k0 + r) * a.v_row + hk * a.v_head : nullptr;
-      });
+      const T *k = (const T*)a.k + hk * a.k_head, *v = (const T*)a.v + hk * a.v_head;
+      copy_tile<DP, 128, 128 * G>(smem_u32(skv), tid, a.dim, a.k,
+                                  [&](int r) { return (const uint8_t*)(k + (k0 + r) * a.k_row); }, kept);
+      copy_tile<DP, 128, 128 * G>(smem_u32(skv + Shape::kTile), tid, a.dim, a.k,
+                                  [&](int r) { return (const uint8_t*)(v + (k0 + r) * a.v_row); }, kept);
       cp_async_arrive(smem_u32(kvfull));
     }
     const KeyRows kr = j < a.n ? attn_key_rows(a, j, attn_span(a, j)) : KeyRows{0, 0};
-    const float c = a.scale_log2;
+    const uint64_t c2 = pair(a.scale_log2, a.scale_log2);
     // lse and delta of a block's rows: two threads a row fetch them a block ahead
     auto fetch = [&](int b) {
-      const int r = row & (kBN - 1), i = first_node(b) + r / p.pack;
-      if (b >= blocks || i >= span.hi) return row < kBN ? INFINITY : 0.f;
-      const long long at = (long long)(first_head(b) + r % p.pack) * a.n + i;
-      return row < kBN ? p.g.lse[at] : p.g.delta[at];
+      const int r = row & (kBN - 1), i = first_node(b) + (r >> p.pack_log);
+      if (b >= blocks || i >= span.hi) return row < kBN ? -INFINITY : 0.f;
+      const long long at = (long long)(first_head(b) + (r & (pack - 1))) * a.n + i;
+      return row < kBN ? -p.g.lse[at] : -p.g.delta[at];
     };
     float ahead = t < blocks ? fetch(t) : 0.f;
     int n = 0;
     bool alive = true;
     // (a group's warps meet at the barrier in every block, one that has given up too)
     for (int b = t; b < blocks; b += G, ++n) {
-      float2* st = stats + (t * 2 + (n & 1)) * kBN;
-      (row < kBN ? st[row].x : st[row - kBN].y) = ahead;
+      float* st = stats + (t * 2 + (n & 1)) * (2 * kBN);
+      st[row] = ahead;
       asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
       ahead = fetch(b + G);
       const int i0 = first_node(b);
-      const int lo = (max(kr.lo, i0) - i0) * p.pack, hi = (max(min(kr.hi, i0 + nodes), i0) - i0) * p.pack;
+      const int lo = (max(kr.lo, i0) - i0) << p.pack_log, hi = (max(min(kr.hi, i0 + nodes), i0) - i0) << p.pack_log;
       if (alive) alive = mbar_wait(smem_u32(&sfull[t]), n & 1, abort_flag, p.status, kErrGradS);
       alive = __all_sync(0xffffffffu, alive);
       if (alive) {
         tc_fence_after();
+        const uint32_t bits[2] = {bit_run(lo, hi), bit_run(lo - 32, hi - 32)};
+        const bool all = __all_sync(0xffffffffu, (bits[0] & bits[1]) == 0xffffffffu);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const uint32_t bits = bit_run(lo - 32 * k, hi - 32 * k);
+          float s[32], dp[32];
+          tmem_load<32>(lanes + 32 * k, s);
+          tmem_load<32>(lanes + kBN + 32 * k, dp);
+          tmem_wait_ld();
           uint32_t w[16], v[16];
-          if (__any_sync(0xffffffffu, bits != 0)) {
-            uint32_t s[32], dp[32];
-            tmem_ld32(lanes + 32 * k, s);
-            tmem_ld32(lanes + kBN + 32 * k, dp);
-            tmem_wait_ld();
-            const bool all = __all_sync(0xffffffffu, bits == 0xffffffffu);
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float4 ld = *reinterpret_cast<const float4*>(st + 32 * k + e);
-              float x = exp2_approx(fmaf(__uint_as_float(s[e]), c, -ld.x));
-              float y = exp2_approx(fmaf(__uint_as_float(s[e + 1]), c, -ld.z));
-              float dx = x * (__uint_as_float(dp[e]) - ld.y), dy = y * (__uint_as_float(dp[e + 1]) - ld.w);
-              if (!all) {
-                if (!((bits >> e) & 1)) x = dx = 0.f;
-                if (!((bits >> (e + 1)) & 1)) y = dy = 0.f;
-              }
-              w[e / 2] = pack16<HALF>(x, y);
-              v[e / 2] = pack16<HALF>(dx, dy);
+          for (int e = 0; e < 32; e += 2) {
+            const uint64_t lse = *reinterpret_cast<const uint64_t*>(st + 32 * k + e);
+            const uint64_t delta = *reinterpret_cast<const uint64_t*>(st + kBN + 32 * k + e);
+            const float2 x = unpair(fma2(pair(s[e], s[e + 1]), c2, lse));
+            float px = exp2_approx(x.x), py = exp2_approx(x.y);
+            if (!all) {
+              if (!((bits[k] >> e) & 1)) px = 0.f;
+              if (!((bits[k] >> (e + 1)) & 1)) py = 0.f;
             }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) w[e] = v[e] = 0;
+            float2 ds = unpair(mul2(pair(px, py), add2(pair(dp[e], dp[e + 1]), delta)));
+            if (!all) {
+              // (a hidden row's dP may be anything)
+              if (px == 0.f) ds.x = 0.f;
+              if (py == 0.f) ds.y = 0.f;
+            }
+            w[e / 2] = pack16<HALF>(px, py);
+            v[e / 2] = pack16<HALF>(ds.x, ds.y);
           }
+          // P' lies where the scores of the first 32 columns lay, dS' likewise: all read by now
           tmem_st16(lanes + 16 * k, w);
           tmem_st16(lanes + kBN + 16 * k, v);
         }
@@ -538,6 +548,7 @@ __global__ void __launch_bounds__(128 * G + 64, CTAS) attn_tc_dkv_kernel(const G
     }
   } else {
     // ---------------- copies of Q and dO ----------------
+    const int thread = tid - 128 * G - 32;
     int stage = 0;
     uint32_t phase = 0;
     bool alive = true;
@@ -549,14 +560,12 @@ __global__ void __launch_bounds__(128 * G + 64, CTAS) attn_tc_dkv_kernel(const G
       }
       const uint32_t dst = smem_u32(sqg + stage * 2 * Shape::kBlock);
       const int i0 = first_node(b), h0 = first_head(b);
-      copy_tile<DP, kBN, 32>(dst, lane, a.dim, a.q, [&](int r) -> const void* {
-        const int i = i0 + r / p.pack;
-        return i < span.hi ? (const T*)a.q + i * a.q_row + (h0 + r % p.pack) * a.q_head : nullptr;
-      });
-      copy_tile<DP, kBN, 32>(dst + Shape::kBlock, lane, a.dim, a.q, [&](int r) -> const void* {
-        const int i = i0 + r / p.pack;
-        return i < span.hi ? (const T*)p.g.grad + i * p.g.grad_row + (h0 + r % p.pack) * p.g.grad_head : nullptr;
-      });
+      const PackedRows q = {(const uint8_t*)((const T*)a.q + h0 * a.q_head), (int)(a.q_row * 2), p.pack_log, a.q_head * 2};
+      const PackedRows g = {(const uint8_t*)((const T*)p.g.grad + h0 * p.g.grad_head), (int)(p.g.grad_row * 2), p.pack_log,
+                            p.g.grad_head * 2};
+      auto live = [&](int r) { return i0 + (r >> p.pack_log) < span.hi; };
+      copy_tile<DP, kBN, 32 * kLoadWarps<DP>>(dst, thread, a.dim, a.q, [&](int r) { return q(i0, r); }, live);
+      copy_tile<DP, kBN, 32 * kLoadWarps<DP>>(dst + Shape::kBlock, thread, a.dim, a.q, [&](int r) { return g(i0, r); }, live);
       cp_async_arrive(smem_u32(&full[stage]));
       if (++stage == p.stages) {
         stage = 0;
@@ -594,14 +603,14 @@ int grad_launch(GradArgs& p, cudaStream_t st) {
   });
   if (status != OCNN_OK) return status;
   p.stages = stages_q;
-  dq<<<dim3(ceil_div(p.a.n, W * 128 / p.pack), p.a.heads / p.pack), 128 * W + 64, Dq::smem(stages_q), st>>>(p);
+  dq<<<dim3(ceil_div(p.a.n, W * 128 >> p.pack_log), p.a.heads >> p.pack_log), Dq::kThreads, Dq::smem(stages_q), st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_dq_kernel");
   if (p.a.sinks > 0) {
     const int far = attn_far_sums(p.a, p.g, HALF ? OCNN_F16 : OCNN_BF16, st);
     if (far != OCNN_OK) return far;
   }
   p.stages = stages_k;
-  dkv<<<dim3(ceil_div(p.a.n, 128), p.a.kv_heads), 128 * G + 64, Dkv::smem(stages_k), st>>>(p);
+  dkv<<<dim3(ceil_div(p.a.n, 128), p.a.kv_heads), Dkv::kThreads, Dkv::smem(stages_k), st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_dkv_kernel");
   return OCNN_OK;
 }
@@ -616,7 +625,7 @@ int grad_by_width(GradArgs& p, cudaStream_t st) {
 }  // namespace
 
 int attn_tc_backward(const AttnArgs& a, const AttnGrad& g, int dtype, int* status, cudaStream_t st) {
-  GradArgs p = {a, g, status, attn_pack(a), 0};
+  GradArgs p = {a, g, status, attn_pack_log(a), 0};
   return dtype == OCNN_F16 ? grad_by_width<true>(p, st) : grad_by_width<false>(p, st);
 }
 
