@@ -29,7 +29,7 @@ enum : int { kErrAttnQ = 11, kErrAttnLoad = 12, kErrAttnSlot = 13, kErrAttnP = 1
 template <int DP, int W, int BN>
 struct FwdShape {
   static constexpr int kLoad = DP > 64 ? 2 : 1;                            // warps that copy
-  static constexpr int kThreads = 128 * W + 32 + 32 * kLoad;
+  static constexpr int kThreads = 128 * W + 32 * W + 32 * kLoad;         // rows, products, copies
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTileQ = 128 * kRowBytes * kPieces;
   static constexpr int kSlot = BN * kRowBytes * kPieces;
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS) attn_tc_k
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   int* ranges = reinterpret_cast<int*>(tmem_holder + 2);                   // per tile: first and last block, first nodes
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int nodes = 128 >> p.pack_log, pack = 1 << p.pack_log;             // of a tile
   const int r0 = blockIdx.x * (W * nodes);
   const int group = a.heads / a.kv_heads, per_kv = group >> p.pack_log;
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS) attn_tc_k
   if (tid == 0) {
     for (int s = 0; s < p.slots; ++s) {
       mbar_init(smem_u32(&full[s]), 32 * Shape::kLoad);
-      mbar_init(smem_u32(&empty[s]), 1);
+      mbar_init(smem_u32(&empty[s]), W);
     }
     mbar_init(smem_u32(qfull), 128 * W);
     for (int t = 0; t < W; ++t) {
@@ -230,76 +230,64 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS) attn_tc_k
         attn_forward_row<T>(a, __shfl_sync(0xffffffffu, i, at), __shfl_sync(0xffffffffu, h, at), (T*)p.out, p.lse);
       }
     }
-  } else if (warp == 4 * W) {
-    // ---------------- products ----------------
-    if (lane == 0 && blocks > 0) {
+  } else if (warp < 5 * W) {
+    // ---------------- products: a warp per tile ----------------
+    // (The whole warp walks the loop, so that descriptors are formed in uniform registers; one thread of it issues.)
+    if (blocks > 0) {
+      const int t = warp - 4 * W;
+      const bool leader = elect_one();
       const uint32_t idesc_s = attn_idesc<HALF>(BN, false), idesc_o = attn_idesc<HALF>(16 * ksteps, true);
+      const uint32_t q = smem_u32(sq + t * Shape::kTileQ), kv = smem_u32(skv), d = tmem + t * Shape::kAcc;
       uint32_t full_phase = 0;                                             // per slot
-      int n_s[W] = {}, n_p[W] = {};
+      int n = 0;
       bool alive = mbar_wait(smem_u32(qfull), 0, abort_flag, p.status, kErrAttnQ);
       auto wait_slot = [&](int s) {
         if (alive) alive = mbar_wait(smem_u32(&full[s]), (full_phase >> s) & 1, abort_flag, p.status, kErrAttnLoad);
         full_phase ^= 1u << s;
-        if (alive) proxy_fence();
+        proxy_fence();
       };
-      auto scores = [&](int t, int slot) {
-        const uint32_t qa = smem_u32(sq + t * Shape::kTileQ), kb = smem_u32(skv + slot * Shape::kSlot);
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t in = (k & 3) * 32, piece = k >> 2;
-          umma_bf16(tmem + t * Shape::kAcc, smem_desc_sw128(qa + piece * (128 * kRowBytes) + in),
-                    smem_desc_sw128(kb + piece * (BN * kRowBytes) + in), idesc_s, k > 0 ? 1u : 0u);
-        }
-        umma_commit(smem_u32(&sfull[t]));
-        ++n_s[t];
-      };
-      auto last_product = [&](int t) {
-        if (alive && n_p[t] > 0)
-          alive = mbar_wait(smem_u32(&pvdone[t]), (n_p[t] - 1) & 1, abort_flag, p.status, kErrAttnO);
-        if (alive) tc_fence_after();
-      };
-      auto values = [&](int t, int slot) {
-        const uint32_t vb = smem_u32(skv + slot * Shape::kSlot);
-        if (alive) alive = mbar_wait(smem_u32(&pfull[t]), n_p[t] & 1, abort_flag, p.status, kErrAttnP);
-        if (!alive) return;
+      auto scores = [&](int slot) {
         tc_fence_after();
-        for (int k = 0; k < BN / 16; ++k)
-          umma_ts(tmem + t * Shape::kAcc + BN, tmem + t * Shape::kAcc + 8 * k,
-                  smem_desc_mn128(vb + k * (16 * kRowBytes), BN * kRowBytes), idesc_o, n_p[t] > 0 || k > 0 ? 1u : 0u);
-        umma_commit(smem_u32(&pvdone[t]));
-        ++n_p[t];
+        if (leader) {
+          product_channels<DP / 16, 128, BN>(d, q, kv + slot * Shape::kSlot, ksteps, idesc_s);
+          umma_commit(smem_u32(&sfull[t]));
+        }
       };
       int slot = 0;
       auto next = [&](int s) { return s + 1 == p.slots ? 0 : s + 1; };
-      if (alive) wait_slot(slot);
-      if (alive) tc_fence_after();
-      for (int t = 0; t < W && alive; ++t)
-        if (active(t, 0)) scores(t, slot);
-      if (alive) umma_commit(smem_u32(&empty[slot]));
+      wait_slot(slot);
+      if (alive && active(t, 0)) scores(slot);
+      if (alive && leader) umma_commit(smem_u32(&empty[slot]));
       for (int b = 0; b < blocks && alive; ++b) {
         const int vs = next(slot), ks = next(vs);
+        const bool more = b + 1 < blocks;
         wait_slot(vs);
-        if (alive && b + 1 < blocks) wait_slot(ks);
-        for (int t = 0; t < W && alive; ++t) {
-          if (active(t, b)) values(t, vs);
-          if (alive && t == W - 1 && b + 1 < blocks) umma_commit(smem_u32(&empty[vs]));
-          // (S lies where P does: the product that reads P has to be through)
-          if (alive && b + 1 < blocks && active(t, b + 1)) {
-            last_product(t);
-            if (alive) scores(t, ks);
+        if (more) wait_slot(ks);
+        if (alive && active(t, b)) {
+          alive = mbar_wait(smem_u32(&pfull[t]), n & 1, abort_flag, p.status, kErrAttnP);
+          if (!alive) break;
+          tc_fence_after();
+          if (leader) {
+            product_rows<BN>(d + BN, d, kv + vs * Shape::kSlot, idesc_o, n == 0);
+            umma_commit(smem_u32(&pvdone[t]));
           }
+          ++n;
         }
-        if (alive && b + 1 < blocks) umma_commit(smem_u32(&empty[ks]));
+        if (alive && more && leader) umma_commit(smem_u32(&empty[vs]));
+        // (S lies where P does: the product that reads P has to be through)
+        if (alive && more && active(t, b + 1)) {
+          if (n > 0) alive = mbar_wait(smem_u32(&pvdone[t]), (n - 1) & 1, abort_flag, p.status, kErrAttnO);
+          if (alive) scores(ks);
+        }
+        if (alive && more && leader) umma_commit(smem_u32(&empty[ks]));
         slot = ks;
       }
-      if (!alive) {
-        // gave up: the products that are under way have to be through before tensor memory is freed
-        umma_commit(smem_u32(qfull));
-        for (int it = 0; it < 64; ++it) __nanosleep(1000);
-      }
+      if (!alive)
+        for (int it = 0; it < 64; ++it) __nanosleep(1000);       // (products under way end before tensor memory is freed)
     }
   } else {
     // ---------------- copies of K and V ----------------
-    const int thread = tid - 128 * W - 32;
+    const int thread = tid - 160 * W;
     const uint8_t* const base[2] = {(const uint8_t*)((const T*)a.k + hk * a.k_head),
                                     (const uint8_t*)((const T*)a.v + hk * a.v_head)};
     const int stride[2] = {(int)(a.k_row * 2), (int)(a.v_row * 2)};

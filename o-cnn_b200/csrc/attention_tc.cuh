@@ -20,6 +20,13 @@ __device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t addr, uint32_t piec
          (1ull << 46) | (2ull << 61);
 }
 
+// One thread of the warp, the same every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // D[tmem] (+)= A[tmem] B[smem]
 __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accumulate) {
@@ -133,6 +140,25 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   if constexpr (HALF) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
   else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
   return w;
+}
+
+// Products over the channels (KS steps of 16 at most, `ksteps` of them): D[128 x n] = A B^T, both tiles as copied.
+template <int KS, int ROWS_A, int ROWS_B>
+__device__ __forceinline__ void product_channels(uint32_t d, uint32_t a, uint32_t b, int ksteps, uint32_t idesc) {
+  const uint64_t da = smem_desc_sw128(a), db = smem_desc_sw128(b);
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    if (k >= ksteps) break;
+    umma_bf16(d, da + (k >> 2) * (ROWS_A * kRowBytes >> 4) + (k & 3) * 2, db + (k >> 2) * (ROWS_B * kRowBytes >> 4) + (k & 3) * 2,
+              idesc, k > 0 ? 1u : 0u);
+  }
+}
+// Products over a block's rows: D[128 x channels] (+)= P[128 x ROWS] B, P in tensor memory.
+template <int ROWS>
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, bool first) {
+  const uint64_t db = smem_desc_mn128(b, ROWS * kRowBytes);
+#pragma unroll
+  for (int k = 0; k < ROWS / 16; ++k) umma_ts(d, p + 8 * k, db + k * (16 * kRowBytes >> 4), idesc, !first || k > 0 ? 1u : 0u);
 }
 
 // ---- two fp32 values per instruction (sm_100) -------------------------------------------------------------------

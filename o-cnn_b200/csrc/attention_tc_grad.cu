@@ -33,7 +33,7 @@ constexpr int kLoadWarps = DP > 64 ? 2 : 1;      // warps that copy
 
 template <int DP, int W>
 struct DqShape {
-  static constexpr int kThreads = 128 * W + 32 + 32 * kLoadWarps<DP>;
+  static constexpr int kThreads = 160 * W + 32 * kLoadWarps<DP>;
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTile = 128 * kRowBytes * kPieces;                // Q, then dO
   static constexpr int kBlock = kBN * kRowBytes * kPieces;               // K, then V
@@ -41,22 +41,6 @@ struct DqShape {
   static constexpr int kCols = tmem_columns(W * kAcc);
   static constexpr size_t smem(int stages) { return (size_t)W * 2 * kTile + (size_t)stages * 2 * kBlock + 1024 + 256; }
 };
-
-// scores of one operand pair: D[128 x kBN] = A B^T over the channels
-template <bool HALF, int ROWS_A>
-__device__ __forceinline__ void product_channels(uint32_t d, uint32_t a, uint32_t b, int ksteps, uint32_t idesc) {
-  for (int k = 0; k < ksteps; ++k) {
-    const uint32_t in = (k & 3) * 32, piece = k >> 2;
-    umma_bf16(d, smem_desc_sw128(a + piece * (ROWS_A * kRowBytes) + in), smem_desc_sw128(b + piece * (kBN * kRowBytes) + in),
-              idesc, k > 0 ? 1u : 0u);
-  }
-}
-// D[128 x channels] += P[128 x kBN] B over the block's rows
-__device__ __forceinline__ void product_rows(uint32_t d, uint32_t p, uint32_t b, uint32_t idesc, bool first) {
-#pragma unroll
-  for (int k = 0; k < kBN / 16; ++k)
-    umma_ts(d, p + 8 * k, smem_desc_mn128(b + k * (16 * kRowBytes), kBN * kRowBytes), idesc, !first || k > 0 ? 1u : 0u);
-}
 
 template <int DP, int W, bool HALF, int CTAS>
 __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_kernel(const GradArgs p) {
@@ -77,14 +61,14 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   int* ranges = reinterpret_cast<int*>(tmem_holder + 2);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int nodes = 128 >> p.pack_log, pack = 1 << p.pack_log, r0 = blockIdx.x * (W * nodes);
   const int group = a.heads / a.kv_heads, per_kv = group >> p.pack_log;
   const int hk = blockIdx.y / per_kv, h0 = hk * group + (blockIdx.y % per_kv) * pack;
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(smem_u32(&full[s]), 32 * kLoadWarps<DP>);
-      mbar_init(smem_u32(&empty[s]), 1);
+      mbar_init(smem_u32(&empty[s]), W);
     }
     mbar_init(smem_u32(qfull), 128 * W);
     for (int t = 0; t < W; ++t) {
@@ -218,51 +202,50 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
         }
       }
     }
-  } else if (warp == 4 * W) {
-    // ---------------- products ----------------
-    if (lane == 0 && blocks > 0) {
+  } else if (warp < 5 * W) {
+    // ---------------- products: a warp per tile, one thread of it issues ----------------
+    if (blocks > 0) {
+      const int t = warp - 4 * W;
+      const bool leader = elect_one();
       const uint32_t idesc_s = attn_idesc<HALF>(kBN, false), idesc_o = attn_idesc<HALF>(16 * ksteps, true);
-      int n[W] = {};
-      bool alive = mbar_wait(smem_u32(qfull), 0, abort_flag, p.status, kErrGradTile);
-      int stage = 0;
+      const uint32_t q = smem_u32(stq + t * 2 * Shape::kTile), kv = smem_u32(skv), d = tmem + t * Shape::kAcc;
+      int n = 0, stage = 0;
       uint32_t phase = 0;
+      bool alive = mbar_wait(smem_u32(qfull), 0, abort_flag, p.status, kErrGradTile);
       auto wait_stage = [&](int s, uint32_t ph) {
         if (alive) alive = mbar_wait(smem_u32(&full[s]), ph, abort_flag, p.status, kErrGradLoad);
-        if (alive) proxy_fence();
+        proxy_fence();
       };
-      auto scores = [&](int t, int s) {
-        const uint32_t q = smem_u32(stq + t * 2 * Shape::kTile), k = smem_u32(skv + s * 2 * Shape::kBlock);
-        const uint32_t d = tmem + t * Shape::kAcc;
-        product_channels<HALF, 128>(d, q, k, ksteps, idesc_s);
-        product_channels<HALF, 128>(d + kBN, q + Shape::kTile, k + Shape::kBlock, ksteps, idesc_s);
-        umma_commit(smem_u32(&sfull[t]));
+      auto scores = [&](int s) {
+        tc_fence_after();
+        if (leader) {
+          const uint32_t k = kv + s * 2 * Shape::kBlock;
+          product_channels<DP / 16, 128, kBN>(d, q, k, ksteps, idesc_s);
+          product_channels<DP / 16, 128, kBN>(d + kBN, q + Shape::kTile, k + Shape::kBlock, ksteps, idesc_s);
+          umma_commit(smem_u32(&sfull[t]));
+        }
       };
       wait_stage(0, 0);
-      if (alive) tc_fence_after();
-      for (int t = 0; t < W && alive; ++t)
-        if (active(t, 0)) scores(t, 0);
+      if (alive && active(t, 0)) scores(0);
       for (int b = 0; b < blocks && alive; ++b) {
         const int next = stage + 1 == p.stages ? 0 : stage + 1;
         const uint32_t next_phase = next == 0 ? phase ^ 1u : phase;
         if (b + 1 < blocks) wait_stage(next, next_phase);
-        for (int t = 0; t < W && alive; ++t) {
-          if (active(t, b)) {
-            alive = mbar_wait(smem_u32(&dsfull[t]), n[t] & 1, abort_flag, p.status, kErrGradP);
-            if (!alive) break;
-            tc_fence_after();
-            product_rows(tmem + t * Shape::kAcc + 2 * kBN, tmem + t * Shape::kAcc,
-                         smem_u32(skv + stage * 2 * Shape::kBlock), idesc_o, n[t] == 0);
+        if (alive && active(t, b)) {
+          alive = mbar_wait(smem_u32(&dsfull[t]), n & 1, abort_flag, p.status, kErrGradP);
+          if (!alive) break;
+          tc_fence_after();
+          if (leader) {
+            product_rows<kBN>(d + 2 * kBN, d, kv + stage * 2 * Shape::kBlock, idesc_o, n == 0);
             umma_commit(smem_u32(&dqdone[t]));
-            ++n[t];
           }
-          if (t == W - 1 && b + p.stages < blocks) umma_commit(smem_u32(&empty[stage]));
-          if (b + 1 < blocks && active(t, b + 1)) {
-            // (S lies where dS does: the product that reads dS has to be through)
-            if (n[t] > 0) alive = mbar_wait(smem_u32(&dqdone[t]), (n[t] - 1) & 1, abort_flag, p.status, kErrGradDone);
-            if (!alive) break;
-            tc_fence_after();
-            scores(t, next);
-          }
+          ++n;
+        }
+        if (alive && leader && b + p.stages < blocks) umma_commit(smem_u32(&empty[stage]));
+        if (alive && b + 1 < blocks && active(t, b + 1)) {
+          // (S lies where dS does: the product that reads dS has to be through)
+          if (n > 0) alive = mbar_wait(smem_u32(&dqdone[t]), (n - 1) & 1, abort_flag, p.status, kErrGradDone);
+          if (alive) scores(next);
         }
         stage = next;
         phase = next_phase;
@@ -272,7 +255,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     }
   } else {
     // ---------------- copies of K and V ----------------
-    const int thread = tid - 128 * W - 32;
+    const int thread = tid - 160 * W;
     const uint8_t* const base[2] = {(const uint8_t*)((const T*)a.k + hk * a.k_head),
                                     (const uint8_t*)((const T*)a.v + hk * a.v_head)};
     const int stride[2] = {(int)(a.k_row * 2), (int)(a.v_row * 2)};
@@ -355,7 +338,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + G);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int k0 = blockIdx.x * 128, hk = blockIdx.y, group = a.heads / a.kv_heads;
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -426,36 +409,41 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
         tc_fence_after();
         const uint32_t bits[2] = {bit_run(lo, hi), bit_run(lo - 32, hi - 32)};
         const bool all = __all_sync(0xffffffffu, (bits[0] & bits[1]) == 0xffffffffu);
+        auto form = [&](auto every) {
+          constexpr bool ALL = decltype(every)::value;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float s[32], dp[32];
-          tmem_load<32>(lanes + 32 * k, s);
-          tmem_load<32>(lanes + kBN + 32 * k, dp);
-          tmem_wait_ld();
-          uint32_t w[16], v[16];
+          for (int k = 0; k < 2; ++k) {
+            float s[32], dp[32];
+            tmem_load<32>(lanes + 32 * k, s);
+            tmem_load<32>(lanes + kBN + 32 * k, dp);
+            tmem_wait_ld();
+            uint32_t w[16], v[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const uint64_t lse = *reinterpret_cast<const uint64_t*>(st + 32 * k + e);
-            const uint64_t delta = *reinterpret_cast<const uint64_t*>(st + kBN + 32 * k + e);
-            const float2 x = unpair(fma2(pair(s[e], s[e + 1]), c2, lse));
-            float px = exp2_approx(x.x), py = exp2_approx(x.y);
-            if (!all) {
-              if (!((bits[k] >> e) & 1)) px = 0.f;
-              if (!((bits[k] >> (e + 1)) & 1)) py = 0.f;
+            for (int e = 0; e < 32; e += 2) {
+              const uint64_t lse = *reinterpret_cast<const uint64_t*>(st + 32 * k + e);
+              const uint64_t delta = *reinterpret_cast<const uint64_t*>(st + kBN + 32 * k + e);
+              const float2 x = unpair(fma2(pair(s[e], s[e + 1]), c2, lse));
+              float px = exp2_approx(x.x), py = exp2_approx(x.y);
+              if (!ALL) {
+                if (!((bits[k] >> e) & 1)) px = 0.f;
+                if (!((bits[k] >> (e + 1)) & 1)) py = 0.f;
+              }
+              float2 ds = unpair(mul2(pair(px, py), add2(pair(dp[e], dp[e + 1]), delta)));
+              if (!ALL) {
+                // (a hidden row's dP may be anything)
+                if (px == 0.f) ds.x = 0.f;
+                if (py == 0.f) ds.y = 0.f;
+              }
+              w[e / 2] = pack16<HALF>(px, py);
+              v[e / 2] = pack16<HALF>(ds.x, ds.y);
             }
-            float2 ds = unpair(mul2(pair(px, py), add2(pair(dp[e], dp[e + 1]), delta)));
-            if (!all) {
-              // (a hidden row's dP may be anything)
-              if (px == 0.f) ds.x = 0.f;
-              if (py == 0.f) ds.y = 0.f;
-            }
-            w[e / 2] = pack16<HALF>(px, py);
-            v[e / 2] = pack16<HALF>(ds.x, ds.y);
+            // P' lies where the scores of the first 32 columns lay, dS' likewise: all read by now
+            tmem_st16(lanes + 16 * k, w);
+            tmem_st16(lanes + kBN + 16 * k, v);
           }
-          // P' lies where the scores of the first 32 columns lay, dS' likewise: all read by now
-          tmem_st16(lanes + 16 * k, w);
-          tmem_st16(lanes + kBN + 16 * k, v);
-        }
+        };
+        if (all) form(std::true_type());
+        else form(std::false_type());
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(smem_u32(&pfull[t]));
@@ -504,10 +492,12 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
       }
     }
   } else if (warp == 4 * G) {
-    // ---------------- products ----------------
-    if (lane == 0 && blocks > 0) {
+    // ---------------- products: one thread of the warp issues ----------------
+    if (blocks > 0) {
+      const bool leader = elect_one();
       const uint32_t idesc_s = attn_idesc<HALF>(kBN, false), idesc_o = attn_idesc<HALF>(16 * ksteps, true);
       bool alive = mbar_wait(smem_u32(kvfull), 0, abort_flag, p.status, kErrGradTile);
+      const uint32_t qg = smem_u32(sqg), k = smem_u32(skv);
       int ahead = 0, ahead_stage = 0;
       uint32_t ahead_phase = 0;
       auto scores = [&]() {                            // of the next block that has none yet
@@ -518,10 +508,12 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
         if (!alive) return;
         proxy_fence();
         tc_fence_after();
-        const uint32_t q = smem_u32(sqg + ahead_stage * 2 * Shape::kBlock), k = smem_u32(skv), d = tmem + t * 2 * kBN;
-        product_channels<HALF, 128>(d, k, q, ksteps, idesc_s);
-        product_channels<HALF, 128>(d + kBN, k + Shape::kTile, q + Shape::kBlock, ksteps, idesc_s);
-        umma_commit(smem_u32(&sfull[t]));
+        if (leader) {
+          const uint32_t q = qg + ahead_stage * 2 * Shape::kBlock, d = tmem + t * 2 * kBN;
+          product_channels<DP / 16, 128, kBN>(d, k, q, ksteps, idesc_s);
+          product_channels<DP / 16, 128, kBN>(d + kBN, k + Shape::kTile, q + Shape::kBlock, ksteps, idesc_s);
+          umma_commit(smem_u32(&sfull[t]));
+        }
         ++ahead;
         if (++ahead_stage == p.stages) {
           ahead_stage = 0;
@@ -535,11 +527,13 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
         alive = mbar_wait(smem_u32(&pfull[t]), (b / G) & 1, abort_flag, p.status, kErrGradP);
         if (!alive) break;
         tc_fence_after();
-        const uint32_t q = smem_u32(sqg + stage * 2 * Shape::kBlock), d = tmem + t * 2 * kBN;
-        product_rows(tmem + kAcc + DP, d, q + Shape::kBlock, idesc_o, b == 0);         // dV += P' dO
-        product_rows(tmem + kAcc, d + kBN, q, idesc_o, b == 0);                        // dK += dS' Q
-        umma_commit(smem_u32(&done[t]));
-        if (b + p.stages < blocks) umma_commit(smem_u32(&empty[stage]));
+        if (leader) {
+          const uint32_t q = qg + stage * 2 * Shape::kBlock, d = tmem + t * 2 * kBN;
+          product_rows<kBN>(tmem + kAcc + DP, d, q + Shape::kBlock, idesc_o, b == 0);    // dV += P' dO
+          product_rows<kBN>(tmem + kAcc, d + kBN, q, idesc_o, b == 0);                   // dK += dS' Q
+          umma_commit(smem_u32(&done[t]));
+          if (b + p.stages < blocks) umma_commit(smem_u32(&empty[stage]));
+        }
         if (++stage == p.stages) stage = 0;
         if (ahead < blocks) scores();
       }
