@@ -73,6 +73,34 @@ __device__ __forceinline__ Span attn_span(const AttnArgs& a, int i) {
   return s;
 }
 
+// The same by a whole warp, which looks at 32 offsets at a time (a search node by node is a chain of loads).
+__device__ __forceinline__ Span attn_span_warp(const AttnArgs& a, int i) {
+  const int lane = threadIdx.x & 31;
+  int first = 0, step = 1, left = a.batch + 1;            // candidates first, first + step, ...
+  while (step * 32 < left) step *= 32;
+  int last = 0;
+  for (;; step /= 32) {
+    const int b = first + lane * step;
+    const unsigned under = __ballot_sync(0xffffffffu, b <= a.batch && attn_offset(a, min(b, a.batch)) <= i);
+    last = under == 0 ? first : first + (31 - __clz(under)) * step;
+    if (step == 1) break;
+    first = last;
+  }
+  Span s = {0, 0, last};
+  if (i >= a.n || last >= a.batch) return s;
+  const int start = attn_offset(a, last), end = attn_offset(a, last + 1);
+  if (i < start || i >= end) return s;
+  s.start = start;
+  s.end = end;
+  return s;
+}
+// Node i's, where the nodes of a tile are known to lie between those of spans f and l.
+__device__ __forceinline__ Span attn_span_near(const AttnArgs& a, int i, const Span& f, const Span& l) {
+  if (i >= f.start && i < f.end) return f;
+  if (i >= l.start && i < l.end) return l;
+  return attn_span(a, i);
+}
+
 // What node i sees: [lo, hi) and [start, first).
 struct RowKeys { int lo, hi, start, first; };
 __device__ __forceinline__ RowKeys attn_row_keys(const AttnArgs& a, int i, const Span& s) {
@@ -91,12 +119,15 @@ __device__ __forceinline__ bool attn_sees(const RowKeys& r, int j) {
 // The nodes that see key j from within the window: [lo, hi).  A first node is seen by every node before it too (both
 // ways); the nodes from j + window on, which see it as a first node only, are left to the far pass.
 struct KeyRows { int lo, hi; };
-__device__ __forceinline__ KeyRows attn_key_rows(const AttnArgs& a, int j, const Span& s) {
+__device__ __forceinline__ KeyRows attn_rows_of_key(const AttnArgs& a, int j, const Span& s) {
   KeyRows r = {0, 0};
-  if (s.end <= s.start || (a.mask != nullptr && a.mask[j] == 0)) return r;
+  if (s.end <= s.start) return r;
   r.lo = a.causal ? j : (j - s.start < a.sinks ? s.start : max(s.start, j - a.window + 1));
   r.hi = j + min(s.end - j, a.window);
   return r;
+}
+__device__ __forceinline__ KeyRows attn_key_rows(const AttnArgs& a, int j, const Span& s) {
+  return a.mask != nullptr && a.mask[j] == 0 ? KeyRows{0, 0} : attn_rows_of_key(a, j, s);
 }
 
 // The keys that the nodes [r0, r1) see between them: the first nodes of r0's sequence where they lie before the windows,
@@ -175,6 +206,73 @@ __device__ void attn_forward_row(const AttnArgs& a, int i, int h, T* out, float*
     lse[(long long)h * a.n + i] = total == 0.f ? INFINITY : top + log2f(total);
 }
 
+// Gradient of query i of head h from the keys that it sees, and of key j from the queries that see it: as
+// attn_forward_row, for rows whose result in a tile is not finite.
+template <typename T>
+__device__ __forceinline__ void attn_row(const void* base, long long at, int dim, float (&x)[4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) x[c] = lane + 32 * c < dim ? to_f32(((const T*)base)[at + lane + 32 * c]) : 0.f;
+}
+__device__ __forceinline__ float attn_dot(const float (&x)[4], const float (&y)[4]) {
+  return warp_sum(x[0] * y[0] + x[1] * y[1] + x[2] * y[2] + x[3] * y[3]);
+}
+template <typename T>
+__device__ void attn_dq_row(const AttnArgs& a, const AttnGrad& g, int i, int h) {
+  const int lane = threadIdx.x & 31, hk = h / (a.heads / a.kv_heads);
+  const RowKeys r = attn_row_keys(a, i, attn_span(a, i));
+  const float lse = g.lse[(long long)h * a.n + i], delta = g.delta[(long long)h * a.n + i];
+  float q[4], go[4], acc[4] = {};
+  attn_row<T>(a.q, i * a.q_row + h * a.q_head, a.dim, q);
+  attn_row<T>(g.grad, i * g.grad_row + h * g.grad_head, a.dim, go);
+  const int n_first = max(0, min(r.first, r.lo) - r.start), behind = max(r.hi, r.first);
+  for (int t = 0; t < n_first + behind - r.lo; ++t) {
+    const int j = t < n_first ? r.start + t : r.lo + t - n_first;
+    if (!attn_sees(r, j) || (a.mask != nullptr && a.mask[j] == 0)) continue;
+    float k[4], v[4];
+    attn_row<T>(a.k, j * a.k_row + hk * a.k_head, a.dim, k);
+    attn_row<T>(a.v, j * a.v_row + hk * a.v_head, a.dim, v);
+    const float p = exp2f(attn_dot(q, k) * a.scale_log2 - lse), ds = p == 0.f ? 0.f : p * (attn_dot(go, v) - delta);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] += ds == 0.f ? 0.f : ds * k[c];
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (lane + 32 * c < a.dim)
+      ((T*)g.dq)[((long long)i * a.heads + h) * a.dim + lane + 32 * c] = from_f32<T>(acc[c] * a.scale);
+}
+template <typename T>
+__device__ void attn_dkv_row(const AttnArgs& a, const AttnGrad& g, int j, int hk, bool write_dk, bool write_dv) {
+  const int lane = threadIdx.x & 31, group = a.heads / a.kv_heads;
+  const Span s = attn_span(a, j);
+  const KeyRows r = attn_key_rows(a, j, s);
+  const int end = r.hi > r.lo && j - s.start < a.sinks ? s.end : r.hi;        // (a first node: to the sequence's end)
+  float k[4], v[4], dk[4] = {}, dv[4] = {};
+  attn_row<T>(a.k, j * a.k_row + hk * a.k_head, a.dim, k);
+  attn_row<T>(a.v, j * a.v_row + hk * a.v_head, a.dim, v);
+  for (int h = hk * group; h < (hk + 1) * group; ++h) {
+    for (int i = r.lo; i < end; ++i) {
+      float q[4], go[4];
+      attn_row<T>(a.q, i * a.q_row + h * a.q_head, a.dim, q);
+      attn_row<T>(g.grad, i * g.grad_row + h * g.grad_head, a.dim, go);
+      const float p = exp2f(attn_dot(q, k) * a.scale_log2 - g.lse[(long long)h * a.n + i]);
+      const float ds = p == 0.f ? 0.f : p * (attn_dot(go, v) - g.delta[(long long)h * a.n + i]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        dk[c] += ds == 0.f ? 0.f : ds * q[c];
+        dv[c] += p == 0.f ? 0.f : p * go[c];
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const long long at = ((long long)j * a.kv_heads + hk) * a.dim + lane + 32 * c;
+    if (lane + 32 * c >= a.dim) continue;
+    if (write_dk) ((T*)g.dk)[at] = from_f32<T>(dk[c] * a.scale);
+    if (write_dv) ((T*)g.dv)[at] = from_f32<T>(dv[c]);
+  }
+}
+
 // ---- first nodes seen from far behind -----------------------------------------------------------------------
 // What the nodes behind the window add to the gradients of their sequence's first nodes comes from all over the
 // sequence.  It is summed in blocks of kFarRows nodes, each block's share of a sequence in a slot of its own, and the
@@ -189,16 +287,16 @@ __device__ __forceinline__ float* far_slot(const AttnArgs& a, const AttnGrad& g,
 struct FarSums {
   const float* at;
   long long step;
-  int count, dim;
-  __device__ __forceinline__ void add(int d, float& dk, float& dv) const {
-    for (int s = 0; s < count; ++s) {
-      dk += at[s * step + d];
-      dv += at[s * step + dim + d];
-    }
+  int count;
+  // of dK's channel d, and of dV's at dim + d
+  __device__ __forceinline__ float sum(int d) const {
+    float x = 0.f;
+    for (int s = 0; s < count; ++s) x += at[s * step + d];
+    return x;
   }
 };
 __device__ __forceinline__ FarSums far_sums(const AttnArgs& a, const AttnGrad& g, int j, int hk) {
-  FarSums f = {nullptr, 0, 0, a.dim};
+  FarSums f = {nullptr, 0, 0};
   if (a.sinks == 0) return f;
   const Span s = attn_span(a, j);
   if (j - s.start >= a.sinks || s.end - j <= a.window || (a.mask != nullptr && a.mask[j] == 0)) return f;

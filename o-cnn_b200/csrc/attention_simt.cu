@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const AttnArgs a
   float* sv = sk + kB * (DP + kPad);
   float* sp = sv + kB * (DP + kPad);
   __shared__ RowKeys rows[kB];
-  __shared__ int ext[4];
+  __shared__ int ext[4], redo[kB];
   const int r0 = blockIdx.x * kB, h = blockIdx.y, hk = h / (a.heads / a.kv_heads);
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const TileKeys keys = query_tile(a, r0, rows, ext);
@@ -293,13 +293,19 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const AttnArgs a
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int i = r0 + 4 * ty + r;
-    if (i >= a.n) continue;
+    bool bad = false;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const int d = out_col<DP>(c);
-      if (d < a.dim) ((T*)g.dq)[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(acc[r][c] * a.scale);
+      bad |= not_finite(acc[r][c]);
+      if (i < a.n && d < a.dim) ((T*)g.dq)[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(acc[r][c] * a.scale);
     }
+    const unsigned any = __ballot_sync(0xffffffffu, bad);
+    if (tx == 0) redo[4 * ty + r] = (any >> (tid & 16)) & 0xffffu;
   }
+  __syncthreads();
+  for (int r = tid >> 5; r < kB; r += kThreads / 32)
+    if (redo[r] != 0 && r0 + r < a.n) attn_dq_row<T>(a, g, r0 + r, h);
 }
 
 // Gradients of the keys and values of one tile of 64 keys: over the nodes that see them from within the window, head
@@ -315,7 +321,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
   float* sp = sg + kB * (DP + kPad);
   float* sd = sp + kB * kPRow;
   __shared__ KeyRows rows[kB];
-  __shared__ int ext[2];
+  __shared__ int ext[2], redo[kB];
   const int k0 = blockIdx.x * kB, hk = blockIdx.y, group = a.heads / a.kv_heads;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   if (tid == 0) {
@@ -374,18 +380,23 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int j = k0 + 4 * ty + r;
-    if (j >= a.n) continue;
-    const FarSums far = far_sums(a, g, j, hk);
+    const FarSums far = j < a.n ? far_sums(a, g, j, hk) : FarSums{nullptr, 0, 0};
+    bool bad = false;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const int d = out_col<DP>(c);
-      if (d >= a.dim) continue;
-      float x = dk[r][c], y = dv[r][c];
-      far.add(d, x, y);
+      bad |= not_finite(dk[r][c]) | not_finite(dv[r][c]);
+      if (j >= a.n || d >= a.dim) continue;
+      const float x = dk[r][c] + far.sum(d), y = dv[r][c] + far.sum(a.dim + d);
       ((T*)g.dk)[((long long)j * a.kv_heads + hk) * a.dim + d] = from_f32<T>(x * a.scale);
       ((T*)g.dv)[((long long)j * a.kv_heads + hk) * a.dim + d] = from_f32<T>(y);
     }
+    const unsigned any = __ballot_sync(0xffffffffu, bad);
+    if (tx == 0) redo[4 * ty + r] = (any >> (tid & 16)) & 0xffffu;
   }
+  __syncthreads();
+  for (int r = tid >> 5; r < kB; r += kThreads / 32)
+    if (redo[r] != 0 && k0 + r < a.n) attn_dkv_row<T>(a, g, k0 + r, hk, true, true);
 }
 
 // The far pass: what the nodes beyond the window add to the gradients of their sequence's first nodes.  A block takes

@@ -7,42 +7,44 @@
 // with 128 threads per tile, one row each, between the two products.  m is the row's reference: its running maximum, but
 // moved only when a block exceeds it by more than 8 (any reference gives the same quotient as long as nothing overflows,
 // and 2^8 is far from that), so O is hardly ever scaled.  P is rounded to the data's type, which is what the product takes;
-// its sum is of the unrounded values.
+// its sum is of the unrounded values.  Scores have two places, so that a block's are ready when its rows come to it.
 //
-// Roles: 4 W warps of rows (they load Q, form P and write O), one warp that copies K and V blocks into a ring of slots
-// (16 bytes per cp.async: any strides, zeros for keys that the mask hides), one thread that issues the products.
+// Roles: 4 W warps of rows, W warps that issue products (one thread of each), one warp that brings Q and the blocks of K
+// and V by TMA into a ring of slots (and clears the rows that the mask hides: see clear_rows).
 #include "attention_tc.cuh"
 
 namespace ocnn {
 namespace {
 
 struct AttnFwdArgs {
+  CUtensorMap q, k, v;
   AttnArgs a;
   void* out;
   float* lse;
   int* status;
-  int pack_log, slots;
+  int pack_log, slots, wide;
 };
 
 enum : int { kErrAttnQ = 11, kErrAttnLoad = 12, kErrAttnSlot = 13, kErrAttnP = 14, kErrAttnS = 15, kErrAttnO = 16 };
 
+constexpr int kMaxSlots = 8;
+
 template <int DP, int W, int BN>
 struct FwdShape {
-  static constexpr int kLoad = DP > 64 ? 2 : 1;                            // warps that copy
-  static constexpr int kThreads = 128 * W + 32 * W + 32 * kLoad;         // rows, products, copies
+  static constexpr int kThreads = 160 * W + 32;                          // rows, products, copies
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTileQ = 128 * kRowBytes * kPieces;
   static constexpr int kSlot = BN * kRowBytes * kPieces;
-  static constexpr int kAcc = BN + DP;                                   // S and O of a tile
-  static constexpr int kCols = W * kAcc <= 64 ? 64 : W * kAcc <= 128 ? 128 : W * kAcc <= 256 ? 256 : 512;
+  static constexpr int kAcc = 2 * BN + DP;                               // two places for S, and O
+  static constexpr int kCols = W * kAcc <= 128 ? 128 : W * kAcc <= 256 ? 256 : 512;
   static constexpr size_t smem(int slots) { return (size_t)W * kTileQ + (size_t)slots * kSlot + 1024 + 512; }
 };
 
 template <int DP, int W, int BN, bool HALF, int CTAS>
-__global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS) attn_tc_kernel(const AttnFwdArgs p) {
+__global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
+    attn_tc_kernel(const __grid_constant__ AttnFwdArgs p) {
   using Shape = FwdShape<DP, W, BN>;
   using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
-  constexpr int kMaxSlots = 8;
   const AttnArgs& a = p.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -50,13 +52,15 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS) attn_tc_k
   uint8_t* skv = sq + W * Shape::kTileQ;
   uint64_t* full = reinterpret_cast<uint64_t*>(skv + p.slots * Shape::kSlot);
   uint64_t* empty = full + kMaxSlots;
-  uint64_t* qfull = empty + kMaxSlots;
-  uint64_t* sfull = qfull + 1;
-  uint64_t* pfull = sfull + W;
-  uint64_t* pvdone = pfull + W;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(pvdone + W);
+  uint64_t* clean = empty + kMaxSlots;                                     // (the slot's rows are cleared)
+  uint64_t* qfull = clean + kMaxSlots;
+  uint64_t* sfull = qfull + 1;                                             // [tile][place]
+  uint64_t* pfull = sfull + 2 * W;
+  uint64_t* pvdone = pfull + 2 * W;
+  uint64_t* ofull = pvdone + W;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(ofull + W);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  int* ranges = reinterpret_cast<int*>(tmem_holder + 2);                   // per tile: first and last block, first nodes
+  BlockRange* ranges = reinterpret_cast<BlockRange*>(tmem_holder + 2);
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int nodes = 128 >> p.pack_log, pack = 1 << p.pack_log;             // of a tile
@@ -66,83 +70,75 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS) attn_tc_k
 
   if (tid == 0) {
     for (int s = 0; s < p.slots; ++s) {
-      mbar_init(smem_u32(&full[s]), 32 * Shape::kLoad);
+      mbar_init(smem_u32(&full[s]), 1);
       mbar_init(smem_u32(&empty[s]), W);
+      mbar_init(smem_u32(&clean[s]), 1);
     }
-    mbar_init(smem_u32(qfull), 128 * W);
+    mbar_init(smem_u32(qfull), 1);
     for (int t = 0; t < W; ++t) {
-      mbar_init(smem_u32(&sfull[t]), 1);
-      mbar_init(smem_u32(&pfull[t]), 128);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(smem_u32(&sfull[2 * t + k]), 1);
+        mbar_init(smem_u32(&pfull[2 * t + k]), 128);
+      }
       mbar_init(smem_u32(&pvdone[t]), 1);
+      mbar_init(smem_u32(&ofull[t]), 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 4 * W) tmem_alloc(tmem_holder, Shape::kCols);
-  const TileKeys keys = attn_tile_keys(a, r0, r0 + W * nodes);
-  const int blocks = (keys.n + BN - 1) / BN;
-  if (W > 1 && tid < W) {
-    // the blocks that tile t needs: an interval, and the first block where it holds first nodes that the tile sees
-    const TileKeys k = attn_tile_keys(a, r0 + tid * nodes, r0 + (tid + 1) * nodes);
-    const int at = k.lo - keys.lo + keys.n_first, end = at + k.n - k.n_first;
-    ranges[3 * tid] = k.n > 0 ? at / BN : 0;
-    ranges[3 * tid + 1] = k.n > 0 ? (end + BN - 1) / BN : 0;
-    ranges[3 * tid + 2] = k.n > 0 && keys.n_first > 0 && k.first == keys.first;
+  Span f, l;
+  const TileKeys tile_keys = attn_tile_keys(a, r0, r0 + W * nodes, f, l);
+  const KeyBlocks<BN> keys(tile_keys);
+  const int blocks = keys.count;
+  if (W > 1 && warp < W) {
+    Span x, y;
+    const BlockRange r = block_range<BN>(keys, attn_tile_keys(a, r0 + warp * nodes, r0 + (warp + 1) * nodes, x, y));
+    if (lane == 0) ranges[warp] = r;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  auto active = [&](int t, int b) {
-    if (W == 1) return true;
-    return (b >= ranges[3 * t] && b < ranges[3 * t + 1]) || (b == 0 && ranges[3 * t + 2] != 0);
-  };
-  const int ksteps = (a.dim + 15) / 16;
+  auto active = [&](int t, int b) { return W == 1 || in_range(ranges[t], b); };
+  const int ksteps = (a.dim + 15) / 16, end = batch_end(a);
+  const bool cleared = a.mask != nullptr || (end < a.n && keys.reaches(end));   // (see clear_rows)
 
   if (warp < 4 * W) {
     // ---------------- rows ----------------
     const int t = warp >> 2, row = tid & 127;
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * Shape::kAcc, acc = lanes + BN;
-    if (blocks > 0) {
-      const int node = r0 + t * nodes;
-      const PackedRows q = {(const uint8_t*)((const T*)a.q + h0 * a.q_head), (int)(a.q_row * 2), p.pack_log, a.q_head * 2};
-      copy_tile<DP, 128, 128>(smem_u32(sq + t * Shape::kTileQ), row, a.dim, a.q, [&](int r) { return q(node, r); },
-                              [&](int r) { return node + (r >> p.pack_log) < a.n; });
-      cp_async_arrive(smem_u32(qfull));
-    }
+    const uint32_t quarter = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * Shape::kAcc, acc = quarter + 2 * BN;
     const int i = r0 + t * nodes + (row >> p.pack_log), h = h0 + (row & (pack - 1));
-    const RowKeys r = i < a.n ? attn_row_keys(a, i, attn_span(a, i)) : RowKeys{0, 0, 0, 0};
+    const RowKeys r = i < a.n ? attn_row_keys(a, i, attn_span_near(a, i, f, l)) : RowKeys{0, 0, 0, 0};
     const float c = a.scale_log2;
+    const uint64_t c2 = pair(c, c);
     float ref = -INFINITY, total = 0.f;                                    // the reference, in powers of two
     int done = 0;
     bool alive = true;
     for (int b = 0; b < blocks && alive; ++b) {
       if (!active(t, b)) continue;
-      uint32_t bits[BN / 32];
-#pragma unroll
-      for (int k = 0; k < BN / 32; ++k) {
-        bits[k] = seen_bits(a, keys, r, b * BN + 32 * k);
-        if (a.mask != nullptr) {
-          const int at = b * BN + 32 * k + lane;
-          bits[k] &= __ballot_sync(0xffffffffu, at < keys.n && a.mask[keys.key(at)] != 0);
-        }
-      }
-      alive = mbar_wait(smem_u32(&sfull[t]), done & 1, abort_flag, p.status, kErrAttnS);
+      const int place = done & 1, j = keys.key(b);
+      const uint32_t lanes = quarter + place * BN;
+      // does every row of the warp see every key?
+      const bool first = keys.is_first(b);
+      const bool all = a.mask == nullptr && !first && __all_sync(0xffffffffu, r.lo <= j && j + BN <= r.hi);
+      alive = mbar_wait(smem_u32(&sfull[2 * t + place]), (done >> 1) & 1, abort_flag, p.status, kErrAttnS);
       alive = __all_sync(0xffffffffu, alive);
       if (!alive) break;
       tc_fence_after();
       float s[BN];
       tmem_load<BN>(lanes, s);
-      bool all = true;
-#pragma unroll
-      for (int k = 0; k < BN / 32; ++k) all = all && bits[k] == 0xffffffffu;
-      all = __all_sync(0xffffffffu, all);
       tmem_wait_ld();
       if (!all) {
         // (a hidden score is -inf, c > 0: its p is 0)
 #pragma unroll
-        for (int e = 0; e < BN; ++e)
-          if (!((bits[e / 32] >> (e & 31)) & 1)) s[e] = -INFINITY;
+        for (int k = 0; k < BN / 32; ++k) {
+          uint32_t bits = first ? seen_first(keys, r, 32 * k) : seen_bits(a, r, j + 32 * k);
+          if (a.mask != nullptr) bits &= kept_bits(a, j + 32 * k, a.n);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((bits >> e) & 1)) s[32 * k + e] = -INFINITY;
+        }
       }
       float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -156,6 +152,11 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS) attn_tc_k
           total *= keep;
         }
         if (done > 0) {
+          // (the last block's product may still be adding to O)
+          alive = mbar_wait(smem_u32(&pvdone[t]), (done - 1) & 1, abort_flag, p.status, kErrAttnO);
+          alive = __all_sync(0xffffffffu, alive);
+          if (!alive) break;
+          tc_fence_after();
 #pragma unroll 1
           for (int d = 0; d < a.dim; d += 16) {
             uint32_t o[16];
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS) attn_tc_k
         }
       }
       const float base = ref == -INFINITY ? 0.f : ref;
-      const uint64_t c2 = pair(c, c), base2 = pair(-base, -base);
+      const uint64_t base2 = pair(-base, -base);
       uint64_t sums[2] = {pair(total, 0.f), 0};
 #pragma unroll
       for (int k = 0; k < BN / 32; ++k) {
@@ -186,43 +187,33 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS) attn_tc_k
       total = sum.x + sum.y;
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(smem_u32(&pfull[t]));
+      mbar_arrive(smem_u32(&pfull[2 * t + place]));
       ++done;
     }
     // ---------------- O / sum ----------------
-    bool bad = false;
-    if (done > 0 && alive) {
-      alive = mbar_wait(smem_u32(&pvdone[t]), (done - 1) & 1, abort_flag, p.status, kErrAttnO);
-      alive = __all_sync(0xffffffffu, alive);
-      tc_fence_after();
-    }
+    if (done > 0 && alive) alive = mbar_wait(smem_u32(&ofull[t]), 0, abort_flag, p.status, kErrAttnO);
+    alive = __all_sync(0xffffffffu, alive);
+    tc_fence_after();
     if (alive) {
-      const bool empty_row = total == 0.f;
-      const float inv = empty_row ? 0.f : 1.f / total;
-      bad = not_finite(total);
+      const bool none = total == 0.f;
+      const float inv = none ? 0.f : 1.f / total;
+      bool bad = not_finite(total);
       T* dst = (T*)p.out + ((long long)i * a.heads + h) * a.dim;
-#pragma unroll 1
+#pragma unroll 2
       for (int d = 0; d < a.dim; d += 16) {
-        uint32_t o[16];
+        float x[16] = {};
         if (done > 0) {
-          tmem_ld16(acc + d, o);
+          tmem_ld16(acc + d, reinterpret_cast<uint32_t(&)[16]>(x));
           tmem_wait_ld();
         }
-        uint32_t w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = empty_row ? 0.f : __uint_as_float(o[2 * e]) * inv;
-          const float y = empty_row ? 0.f : __uint_as_float(o[2 * e + 1]) * inv;
-          bad |= not_finite(x) | (d + 2 * e + 1 < a.dim && not_finite(y));
-          w[e] = pack16<HALF>(x, y);
+        for (int e = 0; e < 16; ++e) {
+          x[e] = none ? 0.f : x[e] * inv;
+          bad |= not_finite(x[e]);
         }
-        if (i < a.n) {
-          // (dim is a multiple of 8, rows start on 16-byte boundaries)
-          *reinterpret_cast<uint4*>(dst + d) = make_uint4(w[0], w[1], w[2], w[3]);
-          if (d + 8 < a.dim) *reinterpret_cast<uint4*>(dst + d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-        }
+        if (i < a.n) store_row<HALF>(dst, d, a.dim, p.wide, x);
       }
-      if (i < a.n && p.lse != nullptr) p.lse[(long long)h * a.n + i] = empty_row ? INFINITY : ref + log2f(total);
+      if (i < a.n && p.lse != nullptr) p.lse[(long long)h * a.n + i] = none ? INFINITY : ref + log2f(total);
       unsigned redo = __ballot_sync(0xffffffffu, bad && i < a.n);
       while (redo != 0) {
         const int at = __ffs(redo) - 1;
@@ -238,87 +229,98 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS) attn_tc_k
       const bool leader = elect_one();
       const uint32_t idesc_s = attn_idesc<HALF>(BN, false), idesc_o = attn_idesc<HALF>(16 * ksteps, true);
       const uint32_t q = smem_u32(sq + t * Shape::kTileQ), kv = smem_u32(skv), d = tmem + t * Shape::kAcc;
-      uint32_t full_phase = 0;                                             // per slot
-      int n = 0;
-      bool alive = mbar_wait(smem_u32(qfull), 0, abort_flag, p.status, kErrAttnQ);
-      auto wait_slot = [&](int s) {
-        if (alive) alive = mbar_wait(smem_u32(&full[s]), (full_phase >> s) & 1, abort_flag, p.status, kErrAttnLoad);
-        full_phase ^= 1u << s;
-        proxy_fence();
-      };
-      auto scores = [&](int slot) {
-        tc_fence_after();
-        if (leader) {
-          product_channels<DP / 16, 128, BN>(d, q, kv + slot * Shape::kSlot, ksteps, idesc_s);
-          umma_commit(smem_u32(&sfull[t]));
+      uint64_t* ready = cleared ? clean : full;
+      // K of block b lies in slot 2 b, V in slot 2 b + 1, modulo the ring
+      int ks = 0, vs = 1, scored = 0, n = 0;
+      uint32_t kp = 0, vp = 0;
+      auto on = [&](int& slot, uint32_t& phase) {
+        slot += 2;
+        if (slot >= p.slots) {
+          slot -= p.slots;
+          phase ^= 1u;
         }
       };
-      int slot = 0;
-      auto next = [&](int s) { return s + 1 == p.slots ? 0 : s + 1; };
-      wait_slot(slot);
-      if (alive && active(t, 0)) scores(slot);
-      if (alive && leader) umma_commit(smem_u32(&empty[slot]));
-      for (int b = 0; b < blocks && alive; ++b) {
-        const int vs = next(slot), ks = next(vs);
-        const bool more = b + 1 < blocks;
-        wait_slot(vs);
-        if (more) wait_slot(ks);
+      bool alive = mbar_wait(smem_u32(qfull), 0, abort_flag, p.status, kErrAttnQ);
+      auto scores = [&](int b) {
+        if (alive) alive = mbar_wait(smem_u32(&ready[ks]), kp, abort_flag, p.status, kErrAttnLoad);
         if (alive && active(t, b)) {
-          alive = mbar_wait(smem_u32(&pfull[t]), n & 1, abort_flag, p.status, kErrAttnP);
+          // (the place's last P has to be through)
+          if (scored > 1) alive = mbar_wait(smem_u32(&pvdone[t]), (scored - 2) & 1, abort_flag, p.status, kErrAttnO);
+          if (alive) {
+            tc_fence_after();
+            if (leader) {
+              product_channels<DP / 16, 128, BN>(d + (scored & 1) * BN, q, kv + ks * Shape::kSlot, ksteps, idesc_s);
+              umma_commit(smem_u32(&sfull[2 * t + (scored & 1)]));
+            }
+            ++scored;
+          }
+        }
+        if (alive && leader && 2 * b + p.slots < 2 * blocks) umma_commit(smem_u32(&empty[ks]));
+        on(ks, kp);
+      };
+      scores(0);
+      for (int b = 0; b < blocks && alive; ++b) {
+        if (b + 1 < blocks) scores(b + 1);
+        if (alive) alive = mbar_wait(smem_u32(&ready[vs]), vp, abort_flag, p.status, kErrAttnLoad);
+        if (alive && active(t, b)) {
+          alive = mbar_wait(smem_u32(&pfull[2 * t + (n & 1)]), (n >> 1) & 1, abort_flag, p.status, kErrAttnP);
           if (!alive) break;
           tc_fence_after();
           if (leader) {
-            product_rows<BN>(d + BN, d, kv + vs * Shape::kSlot, idesc_o, n == 0);
+            product_rows<BN>(d + 2 * BN, d + (n & 1) * BN, kv + vs * Shape::kSlot, idesc_o, n == 0);
             umma_commit(smem_u32(&pvdone[t]));
           }
           ++n;
         }
-        if (alive && more && leader) umma_commit(smem_u32(&empty[vs]));
-        // (S lies where P does: the product that reads P has to be through)
-        if (alive && more && active(t, b + 1)) {
-          if (n > 0) alive = mbar_wait(smem_u32(&pvdone[t]), (n - 1) & 1, abort_flag, p.status, kErrAttnO);
-          if (alive) scores(ks);
-        }
-        if (alive && more && leader) umma_commit(smem_u32(&empty[ks]));
-        slot = ks;
+        if (alive && leader && 2 * b + 1 + p.slots < 2 * blocks) umma_commit(smem_u32(&empty[vs]));
+        on(vs, vp);
       }
+      if (leader) umma_commit(smem_u32(&ofull[t]));              // (a barrier of its own: rows cannot tell pvdone's phases apart)
       if (!alive)
         for (int it = 0; it < 64; ++it) __nanosleep(1000);       // (products under way end before tensor memory is freed)
     }
-  } else {
-    // ---------------- copies of K and V ----------------
-    const int thread = tid - 160 * W;
-    const uint8_t* const base[2] = {(const uint8_t*)((const T*)a.k + hk * a.k_head),
-                                    (const uint8_t*)((const T*)a.v + hk * a.v_head)};
-    const int stride[2] = {(int)(a.k_row * 2), (int)(a.v_row * 2)};
-    int slot = 0;
-    uint32_t empty_phase = 0;
+  } else if (blocks > 0) {
+    // ---------------- copies ----------------
+    if (lane == 0) {
+      mbar_arrive_expect_tx(smem_u32(qfull), W * tile_bytes<128>(a.dim));
+      for (int t = 0; t < W; ++t)
+        tma_tile<Shape::kPieces, 128>(smem_u32(sq + t * Shape::kTileQ), &p.q, a.dim, h0, r0 + t * nodes, smem_u32(qfull));
+    }
+    int slot = 0, cslot = 0;
+    uint32_t phase = 1, cphase = 0;
     bool alive = true;
-    for (int b = 0; b < blocks && alive; ++b) {
-      uint32_t kept[BN / 32];
-#pragma unroll
-      for (int k = 0; k < BN / 32; ++k) {
-        const int at = b * BN + 32 * k + lane;
-        kept[k] = __ballot_sync(0xffffffffu, at < keys.n && (a.mask == nullptr || a.mask[keys.key(at)] != 0));
-      }
-      const int j0 = keys.lo - keys.n_first + b * BN, nf = keys.n_first - b * BN, early = keys.first - j0;
-#pragma unroll 1
-      for (int kv = 0; kv < 2 && alive; ++kv) {
-        if (2 * b + kv >= p.slots) {
-          alive = mbar_wait(smem_u32(&empty[slot]), (empty_phase >> slot) & 1, abort_flag, p.status, kErrAttnSlot);
-          alive = __all_sync(0xffffffffu, alive);
-          empty_phase ^= 1u << slot;
-          if (!alive) break;
+    for (int c = 0; c < 2 * blocks + (cleared ? 1 : 0) && alive; ++c) {
+      if (c < 2 * blocks) {
+        if (c >= p.slots) alive = mbar_wait(smem_u32(&empty[slot]), phase, abort_flag, p.status, kErrAttnSlot);
+        if (!alive) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(smem_u32(&full[slot]), tile_bytes<BN>(a.dim));
+          tma_tile<Shape::kPieces, BN>(smem_u32(skv + slot * Shape::kSlot), (c & 1) == 0 ? &p.k : &p.v, a.dim, hk,
+                                       keys.key(c >> 1), smem_u32(&full[slot]));
         }
-        copy_tile<DP, BN, 32 * Shape::kLoad>(
-            smem_u32(skv + slot * Shape::kSlot), thread, a.dim, base[0],
-            [&](int r) { return base[kv] + (long long)(j0 + r + (r < nf ? early : 0)) * stride[kv]; },
-            [&](int r) { return ((r < 32 ? kept[0] : r < 64 ? kept[1] : r < 96 ? kept[BN / 32 - 2] : kept[BN / 32 - 1]) >> (r & 31)) & 1; });
-        cp_async_arrive(smem_u32(&full[slot]));
-        slot = slot + 1 == p.slots ? 0 : slot + 1;
+        if (++slot == p.slots) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      }
+      // the slot before has landed or is about to
+      if (cleared && c > 0) {
+        alive = mbar_wait(smem_u32(&full[cslot]), cphase, abort_flag, p.status, kErrAttnLoad);
+        alive = __all_sync(0xffffffffu, alive);
+        if (!alive) break;
+        const int j = keys.key((c - 1) >> 1);
+        clear_rows<Shape::kPieces, BN>(skv + cslot * Shape::kSlot, [&](int k) { return kept_bits(a, j + 32 * k, end); });
+        proxy_fence();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&clean[cslot]));
+        if (++cslot == p.slots) {
+          cslot = 0;
+          cphase ^= 1u;
+        }
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!alive)
+      for (int it = 0; it < 64; ++it) __nanosleep(1000);         // (copies under way end before the CTA does)
   }
   tc_fence_before();
   __syncthreads();
@@ -330,34 +332,47 @@ template <int DP, int W, int BN, bool HALF, int CTAS>
 int fwd_launch(AttnFwdArgs& p, cudaStream_t st) {
   using Shape = FwdShape<DP, W, BN>;
   constexpr size_t kMost = (227 * 1024) / CTAS - 1024;
-  int slots = 8;
-  while (slots > 3 && Shape::smem(slots) > kMost) --slots;
+  constexpr int dtype = HALF ? OCNN_F16 : OCNN_BF16;
+  int slots = kMaxSlots;
+  static_assert(Shape::smem(3) <= kMost, "with a mask, three slots at least: one is cleared while two are read");
+  while (Shape::smem(slots) > kMost) --slots;
   p.slots = slots;
   const size_t bytes = Shape::smem(slots);
+  const AttnArgs& a = p.a;
+  int status = attn_map(&p.q, a.q, dtype, a.dim, a.heads, a.n, a.q_row, a.q_head, 1 << p.pack_log, 128 >> p.pack_log);
+  if (status == OCNN_OK) status = attn_map(&p.k, a.k, dtype, a.dim, a.kv_heads, a.n, a.k_row, a.k_head, 1, BN);
+  if (status == OCNN_OK) status = attn_map(&p.v, a.v, dtype, a.dim, a.kv_heads, a.n, a.v_row, a.v_head, 1, BN);
+  if (status != OCNN_OK) return status;
   static PerDeviceOnce once;
-  const int status = once.run([&]() -> int {
+  status = once.run([&]() -> int {
     OCNN_CUDA_OK(cudaFuncSetAttribute(attn_tc_kernel<DP, W, BN, HALF, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)bytes));
     return OCNN_OK;
   });
   if (status != OCNN_OK) return status;
   const int nodes = W * 128 >> p.pack_log;
-  attn_tc_kernel<DP, W, BN, HALF, CTAS><<<dim3(ceil_div(p.a.n, nodes), p.a.heads >> p.pack_log), Shape::kThreads, bytes, st>>>(p);
+  attn_tc_kernel<DP, W, BN, HALF, CTAS><<<dim3(ceil_div(a.n, nodes), a.heads >> p.pack_log), Shape::kThreads, bytes, st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_kernel");
   return OCNN_OK;
 }
 
 template <bool HALF>
 int fwd_by_width(AttnFwdArgs& p, cudaStream_t st) {
-  if (p.a.dim <= 32) return fwd_launch<32, 1, 64, HALF, 3>(p, st);
-  if (p.a.dim <= 64) return fwd_launch<64, 1, 64, HALF, 3>(p, st);
-  return fwd_launch<128, 2, 128, HALF, 1>(p, st);
+  if (p.a.dim <= 32) return fwd_launch<32, 1, 64, HALF, 2>(p, st);
+  if (p.a.dim <= 64) return fwd_launch<64, 1, 64, HALF, 2>(p, st);
+  return fwd_launch<128, 2, 64, HALF, 1>(p, st);
 }
 
 }  // namespace
 
 int attn_tc_forward(const AttnArgs& a, int dtype, void* out, float* lse, int* status, cudaStream_t st) {
-  AttnFwdArgs p = {a, out, lse, status, attn_pack_log(a), 0};
+  AttnFwdArgs p;
+  p.a = a;
+  p.out = out;
+  p.lse = lse;
+  p.status = status;
+  p.pack_log = attn_pack_log(a);
+  p.wide = wide_rows(out, a.dim);
   return dtype == OCNN_F16 ? fwd_by_width<true>(p, st) : fwd_by_width<false>(p, st);
 }
 

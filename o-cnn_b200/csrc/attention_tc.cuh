@@ -5,6 +5,8 @@
 // rows (probabilities times values).  So one copy of K, V, Q or dO serves both of its products.
 #pragma once
 
+#include <cuda.h>
+
 #include "attention.cuh"
 #include "tc.cuh"
 
@@ -69,9 +71,7 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
 }
 
 // Copies of ROWS rows of `dim` channels by LANES threads, zeros up to the next multiple of 16 and for rows that are not
-// live.  row(r): where row r starts.  A lane has one piece of every kStep-th row, so that all but the row's address is known
-// before the loop (one warp per CTA makes all its copies: with a division and 64-bit products per piece it was the copies'
-// instructions that bounded every kernel here).
+// live.  row(r): where row r starts.
 template <int DP, int ROWS, int LANES, typename Row, typename Live>
 __device__ __forceinline__ void copy_tile(uint32_t dst, int lane, int dim, const void* any, Row row, Live live) {
   constexpr int kChunks = DP / 8, kStep = LANES / kChunks;
@@ -89,48 +89,144 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, int lane, int dim, const
   }
 }
 
-// The rows of a tile that are (node, head) pairs, 1 << pack_log heads of each node side by side.
-struct PackedRows {
-  const uint8_t* base;               // node 0, first head
-  int row, pack_log;                 // bytes from node to node
-  long long head;
-  __device__ __forceinline__ const uint8_t* operator()(int node, int r) const {
-    return base + (long long)(node + (r >> pack_log)) * row + (r & ((1 << pack_log) - 1)) * head;
-  }
-};
+// ---- tiles by TMA ---------------------------------------------------------------------------------------------
+// A box of 64 channels x `heads` heads x `nodes` nodes of a [n, heads, dim] tensor: (node, head) rows, swizzled as above;
+// what lies outside of the tensor reads as zeros.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int channel, int head, int node, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(channel), "r"(head), "r"(node), "r"(bar)
+      : "memory");
+}
+template <int PIECES, int ROWS>
+__device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, int dim, int head, int node, uint32_t bar) {
+#pragma unroll
+  for (int c = 0; c < PIECES; ++c)
+    if (c == 0 || 64 * c < dim) tma_box(dst + c * (ROWS * kRowBytes), map, 64 * c, head, node, bar);
+}
+// Bytes that a tile's boxes bring.
+template <int ROWS>
+__device__ __forceinline__ uint32_t tile_bytes(int dim) { return (uint32_t)(dim > 64 ? 2 : 1) * ROWS * kRowBytes; }
 
-// The keys that the nodes [r0, r1) see between them.  Windows move on with the nodes, so the first and the last node
-// that are in a sequence say it all.
-__device__ __forceinline__ TileKeys attn_tile_keys(const AttnArgs& a, int r0, int r1) {
+inline int attn_map(CUtensorMap* map, const void* base, int dtype, int dim, int heads, int n, long long row, long long head,
+                    int box_heads, int box_nodes) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess) fn = nullptr;
+    return (Encode)fn;
+  }();
+  if (encode == nullptr) return fail(OCNN_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)n};
+  // (the stride of a dimension of one is whatever its tensor says: any will do)
+  const cuuint64_t strides[2] = {heads == 1 ? 16 : (cuuint64_t)head * 2, n == 1 ? 16 : (cuuint64_t)row * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_nodes}, steps[3] = {1, 1, 1};
+  const CUresult rc = encode(map, dtype == OCNN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                             const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(OCNN_ERR_CUDA, "cuTensorMapEncodeTiled: error %d", (int)rc);
+  return OCNN_OK;
+}
+
+// ---- the keys of a tile of queries ------------------------------------------------------------------------------
+// The keys that the nodes [r0, r1) see between them (TileKeys), by a whole warp.  Windows move on with the nodes, so the
+// first and the last node that are in a sequence say it all; their sequences go to f and l.
+__device__ __forceinline__ TileKeys attn_tile_keys(const AttnArgs& a, int r0, int r1, Span& f, Span& l) {
   TileKeys t = {0, 0, 0, 0};
-  const int f = max(r0, attn_offset(a, 0)), l = min(min(r1, a.n), attn_offset(a, a.batch)) - 1;
-  if (f > l) return t;
-  const Span sf = attn_span(a, f);
-  const RowKeys rf = attn_row_keys(a, f, sf), rl = attn_row_keys(a, l, attn_span(a, l));
-  t.lo = rf.lo;
+  const int x = max(r0, attn_offset(a, 0)), y = min(min(r1, a.n), attn_offset(a, a.batch)) - 1;
+  f = l = Span{0, 0, 0};
+  if (x > y) return t;
+  f = attn_span_warp(a, x);
+  l = y < f.end ? f : attn_span_warp(a, y);
+  const RowKeys rx = attn_row_keys(a, x, f), ry = attn_row_keys(a, y, l);
+  t.lo = rx.lo;
   if (a.sinks > 0) {
-    const int i = min(l, sf.end - 1);          // the last node of the first one's sequence
-    t.first = sf.start;
-    t.n_first = max(0, min(attn_row_keys(a, i, sf).first, t.lo) - sf.start);
+    t.first = f.start;                         // (the last of the tile's nodes in the first one's sequence sees most of them)
+    t.n_first = max(0, min(attn_row_keys(a, min(y, f.end - 1), f).first, t.lo) - f.start);
   }
-  t.n = t.n_first + max(0, max(rl.hi, rl.first) - t.lo);
+  t.n = t.n_first + max(0, max(ry.hi, ry.first) - t.lo);
   return t;
 }
+// They are taken in blocks of BN consecutive keys: one for the first nodes, where they lie before the windows, and the
+// windows' interval cut from its begin.
+template <int BN>
+struct KeyBlocks {
+  int first, n_first, lo, count;
+  __device__ __forceinline__ explicit KeyBlocks(const TileKeys& t)
+      : first(t.first), n_first(t.n_first), lo(t.lo), count((t.n_first > 0) + (t.n - t.n_first + BN - 1) / BN) {}
+  __device__ __forceinline__ bool is_first(int b) const { return b == 0 && n_first > 0; }
+  __device__ __forceinline__ bool reaches(int end) const { return count > 0 && key(count - 1) + BN > end; }
+  __device__ __forceinline__ int key(int b) const { return is_first(b) ? first : lo + (b - (n_first > 0)) * BN; }
+};
 
 __device__ __forceinline__ uint32_t bit_run(int lo, int hi) {      // bits [lo, hi), within 0 .. 32
   lo = max(lo, 0);
   hi = min(hi, 32);
   return hi > lo ? (0xffffffffu >> (32 - (hi - lo))) << lo : 0u;
 }
-// Which of the keys with list indices t .. t + 31 row r sees.
-__device__ __forceinline__ uint32_t seen_bits(const AttnArgs& a, const TileKeys& k, const RowKeys& r, int t) {
-  const int base = k.lo - k.n_first + t;       // the key of column 0, behind the first nodes
-  uint32_t w = bit_run(r.lo - base, r.hi - base);
-  if (a.sinks > 0 && r.first > r.start) {
-    w |= bit_run(max(r.start - base, k.n_first - t), r.first - base);
-    if (r.start == k.first) w |= bit_run(-t, min(k.n_first, r.first - r.start) - t);
-  }
+// Which of the 32 keys from j on row r sees, in a block of the windows' interval; in the block of first nodes, from column c on.
+__device__ __forceinline__ uint32_t seen_bits(const AttnArgs& a, const RowKeys& r, int j) {
+  uint32_t w = bit_run(r.lo - j, r.hi - j);
+  if (a.sinks > 0) w |= bit_run(r.start - j, r.first - j);
   return w;
+}
+template <int BN>
+__device__ __forceinline__ uint32_t seen_first(const KeyBlocks<BN>& k, const RowKeys& r, int c) {
+  return r.first > r.start && r.start == k.first ? bit_run(-c, min(k.n_first, r.first - r.start) - c) : 0u;
+}
+// Which of the 32 keys from j on the mask keeps, if they lie before node `end`.
+__device__ __forceinline__ uint32_t kept_bits(const AttnArgs& a, int j, int end) {
+  const int at = j + (threadIdx.x & 31);
+  return __ballot_sync(0xffffffffu, at < end && (a.mask == nullptr || a.mask[at] != 0));
+}
+
+// Zeros in the rows of a tile that `kept` (32 rows from 32 k on) leaves out, by a whole warp: what lies there, behind the
+// mask or behind the last sequence, may not be a number, and a product with a probability of 0 would be none.
+template <int PIECES, int BN, typename Kept>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, Kept kept) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = 0; k < BN / 32; ++k) {
+    const uint32_t bits = kept(k);
+    for (int r = lane >> 3; r < 32; r += 4) {
+      if ((bits >> r) & 1) continue;
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c)
+        *reinterpret_cast<uint4*>(tile + c * (BN * kRowBytes) + (32 * k + r) * kRowBytes + (lane & 7) * 16) =
+            make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+// Where the last sequence ends; what lies behind is nobody's.
+__device__ __forceinline__ int batch_end(const AttnArgs& a) { return min(a.n, attn_offset(a, a.batch)); }
+
+// Which blocks a tile of several that share their copies needs: an interval, those of first nodes that lie in the shared
+// interval but not in its own, and the block of first nodes.
+struct BlockRange { int from, to, first_from, first_to, first; };
+template <int BN>
+__device__ __forceinline__ BlockRange block_range(const KeyBlocks<BN>& all, const TileKeys& own) {
+  BlockRange r = {0, 0, 0, 0, 0};
+  const int shift = all.n_first > 0;
+  if (own.n > own.n_first) {
+    r.from = shift + (own.lo - all.lo) / BN;
+    r.to = shift + (own.lo - all.lo + own.n - own.n_first + BN - 1) / BN;
+  }
+  if (own.n_first > 0) {
+    const int x = max(own.first, all.lo), y = own.first + own.n_first;
+    if (y > x) {
+      r.first_from = shift + (x - all.lo) / BN;
+      r.first_to = shift + (y - all.lo + BN - 1) / BN;
+    }
+    r.first = all.n_first > 0 && own.first == all.first;
+  }
+  return r;
+}
+__device__ __forceinline__ bool in_range(const BlockRange& r, int b) {
+  return (b >= r.from && b < r.to) || (b >= r.first_from && b < r.first_to) || (b == 0 && r.first != 0);
 }
 
 // Two fp32 values as one 16-bit pair: `lo` in the lower half.
@@ -204,6 +300,23 @@ __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&v)[N]
 #pragma unroll
   for (int k = 0; k < N / 16; ++k) tmem_st16(addr + 16 * k, reinterpret_cast<const uint32_t(&)[16]>(v[16 * k]));
 }
+
+// 16 channels of a result row from channel d on, of which those below dim count.
+template <bool HALF>
+__device__ __forceinline__ void store_row(void* row, int d, int dim, bool wide, const float (&x)[16]) {
+  uint4 w[2];
+  uint32_t* u = reinterpret_cast<uint32_t*>(w);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) u[e] = pack16<HALF>(x[2 * e], x[2 * e + 1]);
+  uint8_t* dst = (uint8_t*)row + d * 2;
+  if (wide) {
+    st_global_32B(dst, w[0], w[1]);
+  } else {
+    *reinterpret_cast<uint4*>(dst) = w[0];
+    if (d + 8 < dim) *reinterpret_cast<uint4*>(dst + 16) = w[1];
+  }
+}
+inline bool wide_rows(const void* p, int dim) { return dim % 16 == 0 && reinterpret_cast<uintptr_t>(p) % 32 == 0; }
 
 // An instruction descriptor: fp32 accumulator, 128 rows, n columns; B K-major or MN-major.
 template <bool HALF>

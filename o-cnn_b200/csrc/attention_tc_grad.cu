@@ -20,30 +20,28 @@ constexpr int kBN = 64;                        // columns of a block: keys, or r
 constexpr int kMaxStages = 6;
 
 struct GradArgs {
+  CUtensorMap q, grad, k, v;                   // dq: Q, dO by tile, K, V by block; dkv: Q, dO by block
   AttnArgs a;
   AttnGrad g;
   int* status;
-  int pack_log, stages;
+  int pack_log, stages, wide;
 };
 
 constexpr int tmem_columns(int need) { return need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512; }
 
-template <int DP>
-constexpr int kLoadWarps = DP > 64 ? 2 : 1;      // warps that copy
-
 template <int DP, int W>
 struct DqShape {
-  static constexpr int kThreads = 160 * W + 32 * kLoadWarps<DP>;
+  static constexpr int kThreads = 160 * W + 32;
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTile = 128 * kRowBytes * kPieces;                // Q, then dO
   static constexpr int kBlock = kBN * kRowBytes * kPieces;               // K, then V
   static constexpr int kAcc = 2 * kBN + DP;
   static constexpr int kCols = tmem_columns(W * kAcc);
-  static constexpr size_t smem(int stages) { return (size_t)W * 2 * kTile + (size_t)stages * 2 * kBlock + 1024 + 256; }
+  static constexpr size_t smem(int stages) { return (size_t)W * 2 * kTile + (size_t)stages * 2 * kBlock + 1024 + 320; }
 };
 
 template <int DP, int W, bool HALF, int CTAS>
-__global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_kernel(const GradArgs p) {
+__global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_kernel(const __grid_constant__ GradArgs p) {
   using Shape = DqShape<DP, W>;
   using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
   const AttnArgs& a = p.a;
@@ -53,13 +51,14 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
   uint8_t* skv = stq + W * 2 * Shape::kTile;
   uint64_t* full = reinterpret_cast<uint64_t*>(skv + p.stages * 2 * Shape::kBlock);
   uint64_t* empty = full + kMaxStages;
-  uint64_t* qfull = empty + kMaxStages;
+  uint64_t* clean = empty + kMaxStages;                                    // (the stage's rows are cleared)
+  uint64_t* qfull = clean + kMaxStages;
   uint64_t* sfull = qfull + 1;
   uint64_t* dsfull = sfull + W;
   uint64_t* dqdone = dsfull + W;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dqdone + W);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  int* ranges = reinterpret_cast<int*>(tmem_holder + 2);
+  BlockRange* ranges = reinterpret_cast<BlockRange*>(tmem_holder + 2);
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int nodes = 128 >> p.pack_log, pack = 1 << p.pack_log, r0 = blockIdx.x * (W * nodes);
@@ -67,10 +66,11 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
   const int hk = blockIdx.y / per_kv, h0 = hk * group + (blockIdx.y % per_kv) * pack;
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(smem_u32(&full[s]), 32 * kLoadWarps<DP>);
+      mbar_init(smem_u32(&full[s]), 1);
       mbar_init(smem_u32(&empty[s]), W);
+      mbar_init(smem_u32(&clean[s]), 1);
     }
-    mbar_init(smem_u32(qfull), 128 * W);
+    mbar_init(smem_u32(qfull), 1);
     for (int t = 0; t < W; ++t) {
       mbar_init(smem_u32(&sfull[t]), 1);
       mbar_init(smem_u32(&dsfull[t]), 128);
@@ -80,43 +80,30 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 4 * W) tmem_alloc(tmem_holder, Shape::kCols);
-  const TileKeys keys = attn_tile_keys(a, r0, r0 + W * nodes);
-  const int blocks = (keys.n + kBN - 1) / kBN;
-  if (W > 1 && tid < W) {
-    const TileKeys k = attn_tile_keys(a, r0 + tid * nodes, r0 + (tid + 1) * nodes);
-    const int at = k.lo - keys.lo + keys.n_first, end = at + k.n - k.n_first;
-    ranges[3 * tid] = k.n > 0 ? at / kBN : 0;
-    ranges[3 * tid + 1] = k.n > 0 ? (end + kBN - 1) / kBN : 0;
-    ranges[3 * tid + 2] = k.n > 0 && keys.n_first > 0 && k.first == keys.first;
+  Span f, l;
+  const TileKeys tile_keys = attn_tile_keys(a, r0, r0 + W * nodes, f, l);
+  const KeyBlocks<kBN> keys(tile_keys);
+  const int blocks = keys.count;
+  if (W > 1 && warp < W) {
+    Span x, y;
+    const BlockRange r = block_range<kBN>(keys, attn_tile_keys(a, r0 + warp * nodes, r0 + (warp + 1) * nodes, x, y));
+    if (lane == 0) ranges[warp] = r;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  auto active = [&](int t, int b) {
-    if (W == 1) return true;
-    return (b >= ranges[3 * t] && b < ranges[3 * t + 1]) || (b == 0 && ranges[3 * t + 2] != 0);
-  };
-  const int ksteps = (a.dim + 15) / 16;
+  auto active = [&](int t, int b) { return W == 1 || in_range(ranges[t], b); };
+  const int ksteps = (a.dim + 15) / 16, end = batch_end(a);
+  const bool cleared = a.mask != nullptr || (end < a.n && keys.reaches(end));   // (see clear_rows)
 
   if (warp < 4 * W) {
     // ---------------- rows ----------------
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * Shape::kAcc, acc = lanes + 2 * kBN;
-    if (blocks > 0) {
-      const uint32_t dst = smem_u32(stq + t * 2 * Shape::kTile);
-      const int node = r0 + t * nodes;
-      const PackedRows q = {(const uint8_t*)((const T*)a.q + h0 * a.q_head), (int)(a.q_row * 2), p.pack_log, a.q_head * 2};
-      const PackedRows g = {(const uint8_t*)((const T*)p.g.grad + h0 * p.g.grad_head), (int)(p.g.grad_row * 2), p.pack_log,
-                            p.g.grad_head * 2};
-      auto live = [&](int r) { return node + (r >> p.pack_log) < a.n; };
-      copy_tile<DP, 128, 128>(dst, row, a.dim, a.q, [&](int r) { return q(node, r); }, live);
-      copy_tile<DP, 128, 128>(dst + Shape::kTile, row, a.dim, a.q, [&](int r) { return g(node, r); }, live);
-      cp_async_arrive(smem_u32(qfull));
-    }
     const int i = r0 + t * nodes + (row >> p.pack_log), h = h0 + (row & (pack - 1));
     const bool in = i < a.n;
-    const RowKeys r = in ? attn_row_keys(a, i, attn_span(a, i)) : RowKeys{0, 0, 0, 0};
+    const RowKeys r = in ? attn_row_keys(a, i, attn_span_near(a, i, f, l)) : RowKeys{0, 0, 0, 0};
     const float lse = in ? p.g.lse[(long long)h * a.n + i] : INFINITY;
     float delta = 0.f;
     if (in) {
@@ -139,15 +126,9 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     bool alive = true;
     for (int b = 0; b < blocks && alive; ++b) {
       if (!active(t, b)) continue;
-      uint32_t bits[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        bits[k] = seen_bits(a, keys, r, b * kBN + 32 * k);
-        if (a.mask != nullptr) {
-          const int at = b * kBN + 32 * k + lane;
-          bits[k] &= __ballot_sync(0xffffffffu, at < keys.n && a.mask[keys.key(at)] != 0);
-        }
-      }
+      const int j = keys.key(b);
+      const bool first = keys.is_first(b);
+      const bool all = a.mask == nullptr && !first && __all_sync(0xffffffffu, r.lo <= j && j + kBN <= r.hi);
       alive = mbar_wait(smem_u32(&sfull[t]), done & 1, abort_flag, p.status, kErrGradS);
       alive = __all_sync(0xffffffffu, alive);
       if (!alive) break;
@@ -155,22 +136,25 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       float s[kBN], dp[kBN];
       tmem_load<kBN>(lanes, s);
       tmem_load<kBN>(lanes + kBN, dp);
-      const bool all = __all_sync(0xffffffffu, (bits[0] & bits[1]) == 0xffffffffu);
       tmem_wait_ld();
-      uint32_t w[kBN / 2];
 #pragma unroll
-      for (int e = 0; e < kBN / 2; ++e) {
-        const float2 x = unpair(fma2(pair(s[2 * e], s[2 * e + 1]), c2, lse2));
-        const uint64_t ds = mul2(pair(exp2_approx(x.x), exp2_approx(x.y)), add2(pair(dp[2 * e], dp[2 * e + 1]), delta2));
-        const float2 y = unpair(ds);
-        s[2 * e] = y.x;
-        s[2 * e + 1] = y.y;
+      for (int e = 0; e < kBN; e += 2) {
+        const float2 x = unpair(fma2(pair(s[e], s[e + 1]), c2, lse2));
+        const float2 ds = unpair(mul2(pair(exp2_approx(x.x), exp2_approx(x.y)), add2(pair(dp[e], dp[e + 1]), delta2)));
+        s[e] = ds.x;
+        s[e + 1] = ds.y;
       }
       if (!all) {
 #pragma unroll
-        for (int e = 0; e < kBN; ++e)
-          if (!((bits[e / 32] >> (e & 31)) & 1)) s[e] = 0.f;
+        for (int k = 0; k < 2; ++k) {
+          uint32_t bits = first ? seen_first(keys, r, 32 * k) : seen_bits(a, r, j + 32 * k);
+          if (a.mask != nullptr) bits &= kept_bits(a, j + 32 * k, a.n);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((bits >> e) & 1)) s[32 * k + e] = 0.f;
+        }
       }
+      uint32_t w[kBN / 2];
 #pragma unroll
       for (int e = 0; e < kBN / 2; ++e) w[e] = pack16<HALF>(s[2 * e], s[2 * e + 1]);
       tmem_store<kBN / 2>(lanes, w);
@@ -185,21 +169,27 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       tc_fence_after();
     }
     if (alive) {
+      bool bad = false;
       T* dst = (T*)p.g.dq + ((long long)i * a.heads + h) * a.dim;
-#pragma unroll 1
+#pragma unroll 2
       for (int d = 0; d < a.dim; d += 16) {
-        uint32_t o[16], w[8];
+        float x[16] = {};
         if (done > 0) {
-          tmem_ld16(acc + d, o);
+          tmem_ld16(acc + d, reinterpret_cast<uint32_t(&)[16]>(x));
           tmem_wait_ld();
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          w[e] = done > 0 ? pack16<HALF>(__uint_as_float(o[2 * e]) * a.scale, __uint_as_float(o[2 * e + 1]) * a.scale) : 0u;
-        if (in) {
-          *reinterpret_cast<uint4*>(dst + d) = make_uint4(w[0], w[1], w[2], w[3]);
-          if (d + 8 < a.dim) *reinterpret_cast<uint4*>(dst + d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+        for (int e = 0; e < 16; ++e) {
+          x[e] *= a.scale;
+          bad |= not_finite(x[e]);
         }
+        if (in) store_row<HALF>(dst, d, a.dim, p.wide, x);
+      }
+      unsigned redo = __ballot_sync(0xffffffffu, bad && in);
+      while (redo != 0) {
+        const int at = __ffs(redo) - 1;
+        redo &= redo - 1;
+        attn_dq_row<T>(a, p.g, __shfl_sync(0xffffffffu, i, at), __shfl_sync(0xffffffffu, h, at));
       }
     }
   } else if (warp < 5 * W) {
@@ -212,9 +202,9 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       int n = 0, stage = 0;
       uint32_t phase = 0;
       bool alive = mbar_wait(smem_u32(qfull), 0, abort_flag, p.status, kErrGradTile);
+      uint64_t* ready = cleared ? clean : full;
       auto wait_stage = [&](int s, uint32_t ph) {
-        if (alive) alive = mbar_wait(smem_u32(&full[s]), ph, abort_flag, p.status, kErrGradLoad);
-        proxy_fence();
+        if (alive) alive = mbar_wait(smem_u32(&ready[s]), ph, abort_flag, p.status, kErrGradLoad);
       };
       auto scores = [&](int s) {
         tc_fence_after();
@@ -253,42 +243,53 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       if (!alive)
         for (int it = 0; it < 64; ++it) __nanosleep(1000);       // (products under way end before tensor memory is freed)
     }
-  } else {
-    // ---------------- copies of K and V ----------------
-    const int thread = tid - 160 * W;
-    const uint8_t* const base[2] = {(const uint8_t*)((const T*)a.k + hk * a.k_head),
-                                    (const uint8_t*)((const T*)a.v + hk * a.v_head)};
-    const int stride[2] = {(int)(a.k_row * 2), (int)(a.v_row * 2)};
-    int stage = 0;
-    uint32_t phase = 0;
-    bool alive = true;
-    for (int b = 0; b < blocks && alive; ++b) {
-      uint32_t kept[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int at = b * kBN + 32 * k + lane;
-        kept[k] = __ballot_sync(0xffffffffu, at < keys.n && (a.mask == nullptr || a.mask[keys.key(at)] != 0));
-      }
-      if (b >= p.stages) {
-        alive = mbar_wait(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.status, kErrGradSlot);
-        alive = __all_sync(0xffffffffu, alive);
-        if (!alive) break;
-      }
-      const uint32_t dst = smem_u32(skv + stage * 2 * Shape::kBlock);
-      const int j0 = keys.lo - keys.n_first + b * kBN, nf = keys.n_first - b * kBN, early = keys.first - j0;
-#pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv)
-        copy_tile<DP, kBN, 32 * kLoadWarps<DP>>(
-            dst + kv * Shape::kBlock, thread, a.dim, base[0],
-            [&](int r) { return base[kv] + (long long)(j0 + r + (r < nf ? early : 0)) * stride[kv]; },
-            [&](int r) { return ((r < 32 ? kept[0] : kept[1]) >> (r & 31)) & 1; });
-      cp_async_arrive(smem_u32(&full[stage]));
-      if (++stage == p.stages) {
-        stage = 0;
-        phase ^= 1u;
+  } else if (blocks > 0) {
+    // ---------------- copies ----------------
+    if (lane == 0) {
+      mbar_arrive_expect_tx(smem_u32(qfull), 2 * W * tile_bytes<128>(a.dim));
+      for (int t = 0; t < W; ++t) {
+        const uint32_t dst = smem_u32(stq + t * 2 * Shape::kTile);
+        tma_tile<Shape::kPieces, 128>(dst, &p.q, a.dim, h0, r0 + t * nodes, smem_u32(qfull));
+        tma_tile<Shape::kPieces, 128>(dst + Shape::kTile, &p.grad, a.dim, h0, r0 + t * nodes, smem_u32(qfull));
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    int stage = 0, cstage = 0;
+    uint32_t phase = 1, cphase = 0;
+    bool alive = true;
+    for (int b = 0; b < blocks + (cleared ? 1 : 0) && alive; ++b) {
+      if (b < blocks) {
+        if (b >= p.stages) alive = mbar_wait(smem_u32(&empty[stage]), phase, abort_flag, p.status, kErrGradSlot);
+        if (!alive) break;
+        if (lane == 0) {
+          const uint32_t dst = smem_u32(skv + stage * 2 * Shape::kBlock), bar = smem_u32(&full[stage]);
+          mbar_arrive_expect_tx(bar, 2 * tile_bytes<kBN>(a.dim));
+          tma_tile<Shape::kPieces, kBN>(dst, &p.k, a.dim, hk, keys.key(b), bar);
+          tma_tile<Shape::kPieces, kBN>(dst + Shape::kBlock, &p.v, a.dim, hk, keys.key(b), bar);
+        }
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (cleared && b > 0) {
+        alive = mbar_wait(smem_u32(&full[cstage]), cphase, abort_flag, p.status, kErrGradLoad);
+        alive = __all_sync(0xffffffffu, alive);
+        if (!alive) break;
+        const int j = keys.key(b - 1);
+        for (int kv = 0; kv < 2; ++kv)
+          clear_rows<Shape::kPieces, kBN>(skv + (cstage * 2 + kv) * Shape::kBlock,
+                                          [&](int k) { return kept_bits(a, j + 32 * k, end); });
+        proxy_fence();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&clean[cstage]));
+        if (++cstage == p.stages) {
+          cstage = 0;
+          cphase ^= 1u;
+        }
+      }
+    }
+    if (!alive)
+      for (int it = 0; it < 64; ++it) __nanosleep(1000);         // (copies under way end before the CTA does)
   }
   tc_fence_before();
   __syncthreads();
@@ -296,31 +297,33 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Shape::kCols) : "memory");
 }
 
-// The nodes that see the keys [k0, k1) from within the window, whatever the mask says.
-__device__ __forceinline__ KeyRows attn_tile_rows(AttnArgs a, int k0, int k1) {
-  a.mask = nullptr;
-  const int f = max(k0, attn_offset(a, 0)), l = min(min(k1, a.n), attn_offset(a, a.batch)) - 1;
-  if (f > l) return KeyRows{0, 0};
-  const KeyRows x = attn_key_rows(a, f, attn_span(a, f)), y = attn_key_rows(a, l, attn_span(a, l));
-  return KeyRows{x.lo, y.hi};
+// The nodes that see the keys [k0, k1) from within the window, whatever the mask says, by a whole warp; f and l: the
+// sequences of the first and the last key that is in one.
+__device__ __forceinline__ KeyRows attn_tile_rows(const AttnArgs& a, int k0, int k1, Span& f, Span& l) {
+  const int x = max(k0, attn_offset(a, 0)), y = min(min(k1, a.n), attn_offset(a, a.batch)) - 1;
+  f = l = Span{0, 0, 0};
+  if (x > y) return KeyRows{0, 0};
+  f = attn_span_warp(a, x);
+  l = y < f.end ? f : attn_span_warp(a, y);
+  return KeyRows{attn_rows_of_key(a, x, f).lo, attn_rows_of_key(a, y, l).hi};
 }
 
 template <int DP, int G>
 struct DkvShape {
-  static constexpr int kThreads = 128 * G + 32 + 32 * kLoadWarps<DP>;
+  static constexpr int kThreads = 128 * G + 64;
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTile = 128 * kRowBytes * kPieces;                // K, then V
   static constexpr int kBlock = kBN * kRowBytes * kPieces;               // Q, then dO
   static constexpr int kCols = tmem_columns(G * 2 * kBN + 2 * DP);       // S' and dP' of G blocks, dK, dV
   static constexpr size_t smem(int stages) {
-    return (size_t)2 * kTile + (size_t)stages * 2 * kBlock + G * 4 * kBN * sizeof(float) + 1024 + 256;
+    return (size_t)2 * kTile + (size_t)stages * 2 * kBlock + G * 4 * kBN * sizeof(float) + 1024 + 320;
   }
 };
 
 // One tile of 128 keys.  A block is kBN rows of queries: kBN / pack nodes, pack heads each; G groups of four warps take
 // the blocks in turn, each with S' and dP' of its own.
 template <int DP, int G, bool HALF, int CTAS>
-__global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_kernel(const GradArgs p) {
+__global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_kernel(const __grid_constant__ GradArgs p) {
   using Shape = DkvShape<DP, G>;
   using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
   const AttnArgs& a = p.a;
@@ -331,7 +334,8 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
   float* stats = reinterpret_cast<float*>(sqg + p.stages * 2 * Shape::kBlock);       // [G][2][-lse, -delta][kBN]
   uint64_t* full = reinterpret_cast<uint64_t*>(stats + G * 4 * kBN);
   uint64_t* empty = full + kMaxStages;
-  uint64_t* kvfull = empty + kMaxStages;
+  uint64_t* clean = empty + kMaxStages;                                    // (the stage's rows are cleared)
+  uint64_t* kvfull = clean + kMaxStages;
   uint64_t* sfull = kvfull + 1;
   uint64_t* pfull = sfull + G;
   uint64_t* done = pfull + G;
@@ -342,8 +346,9 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
   const int k0 = blockIdx.x * 128, hk = blockIdx.y, group = a.heads / a.kv_heads;
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(smem_u32(&full[s]), 32 * kLoadWarps<DP>);
+      mbar_init(smem_u32(&full[s]), 1);
       mbar_init(smem_u32(&empty[s]), 1);
+      mbar_init(smem_u32(&clean[s]), 1);
     }
     mbar_init(smem_u32(kvfull), 128 * G);
     for (int t = 0; t < G; ++t) {
@@ -355,7 +360,8 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 4 * G) tmem_alloc(tmem_holder, Shape::kCols);
-  const KeyRows span = attn_tile_rows(a, k0, k0 + 128);
+  Span f, l;
+  const KeyRows span = attn_tile_rows(a, k0, k0 + 128, f, l);
   const int pack = 1 << p.pack_log, nodes = kBN >> p.pack_log;             // nodes of a block
   const int per_head = (max(0, span.hi - span.lo) + nodes - 1) >> (6 - p.pack_log);   // blocks of `pack` heads
   const int blocks = per_head * (group >> p.pack_log);
@@ -364,7 +370,8 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   constexpr int kAcc = G * 2 * kBN;                                        // dK, then dV
-  const int ksteps = (a.dim + 15) / 16;
+  const int ksteps = (a.dim + 15) / 16, end = batch_end(a);
+  const bool cleared = end < a.n && span.hi == end;                        // (its last block holds nobody's nodes)
   // (blocks go head by head: no division where there is only one run of them)
   auto run_of = [&](int b) { return b < per_head ? 0 : b / per_head; };
   auto first_node = [&](int b) { return span.lo + (b - run_of(b) * per_head) * nodes; };
@@ -383,7 +390,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
                                   [&](int r) { return (const uint8_t*)(v + (k0 + r) * a.v_row); }, kept);
       cp_async_arrive(smem_u32(kvfull));
     }
-    const KeyRows kr = j < a.n ? attn_key_rows(a, j, attn_span(a, j)) : KeyRows{0, 0};
+    const KeyRows kr = j < a.n ? attn_key_rows(a, j, attn_span_near(a, j, f, l)) : KeyRows{0, 0};
     const uint64_t c2 = pair(a.scale_log2, a.scale_log2);
     // lse and delta of a block's rows: two threads a row fetch them a block ahead
     auto fetch = [&](int b) {
@@ -459,35 +466,37 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
     tc_fence_after();
     if (alive) {
       const bool in = j < a.n;
-      const FarSums far = in ? far_sums(a, p.g, j, hk) : FarSums{nullptr, 0, 0, 0};
+      const FarSums far = in ? far_sums(a, p.g, j, hk) : FarSums{nullptr, 0, 0};
       // group 0 writes dK, the last one dV (both, where there is one)
 #pragma unroll 1
       for (int which = t == 0 ? 0 : 1; which <= (t == G - 1 ? 1 : 0); ++which) {
         const float f = which == 0 ? a.scale : 1.f;
+        bool bad = false;
         T* dst = (T*)(which == 0 ? p.g.dk : p.g.dv) + ((long long)j * a.kv_heads + hk) * a.dim;
-#pragma unroll 1
+#pragma unroll 2
         for (int d = 0; d < a.dim; d += 16) {
-          uint32_t o[16], w[8];
+          float x[16] = {};
           if (blocks > 0) {
-            tmem_ld16(quarter + kAcc + which * DP + d, o);
+            tmem_ld16(quarter + kAcc + which * DP + d, reinterpret_cast<uint32_t(&)[16]>(x));
             tmem_wait_ld();
           }
-          if (in) {
+          if (far.count > 0) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float x = blocks > 0 ? __uint_as_float(o[e]) : 0.f;
-              if (far.count > 0 && d + e < a.dim) {
-                float y = 0.f;
-                if (which == 0) far.add(d + e, x, y);
-                else far.add(d + e, y, x);
-              }
-              o[e] = __float_as_uint(x * f);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = pack16<HALF>(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
-            *reinterpret_cast<uint4*>(dst + d) = make_uint4(w[0], w[1], w[2], w[3]);
-            if (d + 8 < a.dim) *reinterpret_cast<uint4*>(dst + d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            for (int e = 0; e < 16; ++e)
+              if (d + e < a.dim) x[e] += far.sum(which * a.dim + d + e);
           }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            x[e] *= f;
+            bad |= not_finite(x[e]);
+          }
+          if (in) store_row<HALF>(dst, d, a.dim, p.wide, x);
+        }
+        unsigned redo = __ballot_sync(0xffffffffu, bad && in);
+        while (redo != 0) {
+          const int at = __ffs(redo) - 1;
+          redo &= redo - 1;
+          attn_dkv_row<T>(a, p.g, __shfl_sync(0xffffffffu, j, at), hk, which == 0, which == 1);
         }
       }
     }
@@ -497,16 +506,16 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
       const bool leader = elect_one();
       const uint32_t idesc_s = attn_idesc<HALF>(kBN, false), idesc_o = attn_idesc<HALF>(16 * ksteps, true);
       bool alive = mbar_wait(smem_u32(kvfull), 0, abort_flag, p.status, kErrGradTile);
+      proxy_fence();                                  // (K and V came by cp.async)
       const uint32_t qg = smem_u32(sqg), k = smem_u32(skv);
       int ahead = 0, ahead_stage = 0;
       uint32_t ahead_phase = 0;
       auto scores = [&]() {                            // of the next block that has none yet
         const int t = ahead % G, n = ahead / G;
-        if (alive) alive = mbar_wait(smem_u32(&full[ahead_stage]), ahead_phase, abort_flag, p.status, kErrGradLoad);
+        if (alive) alive = mbar_wait(smem_u32(&(cleared ? clean : full)[ahead_stage]), ahead_phase, abort_flag, p.status, kErrGradLoad);
         // (S' and dP' lie where P' and dS' do: the products that read those have to be through)
         if (alive && n > 0) alive = mbar_wait(smem_u32(&done[t]), (n - 1) & 1, abort_flag, p.status, kErrGradDone);
         if (!alive) return;
-        proxy_fence();
         tc_fence_after();
         if (leader) {
           const uint32_t q = qg + ahead_stage * 2 * Shape::kBlock, d = tmem + t * 2 * kBN;
@@ -542,31 +551,46 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
     }
   } else {
     // ---------------- copies of Q and dO ----------------
-    const int thread = tid - 128 * G - 32;
-    int stage = 0;
-    uint32_t phase = 0;
+    // (rows behind the nodes that see the tile are hidden from all of its keys)
+    int stage = 0, cstage = 0;
+    uint32_t phase = 1, cphase = 0;
     bool alive = true;
-    for (int b = 0; b < blocks && alive; ++b) {
-      if (b >= p.stages) {
-        alive = mbar_wait(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.status, kErrGradSlot);
+    for (int b = 0; b < blocks + (cleared ? 1 : 0); ++b) {
+      if (b < blocks) {
+        if (b >= p.stages) alive = mbar_wait(smem_u32(&empty[stage]), phase, abort_flag, p.status, kErrGradSlot);
+        if (!alive) break;
+        if (lane == 0) {
+          const uint32_t dst = smem_u32(sqg + stage * 2 * Shape::kBlock), bar = smem_u32(&full[stage]);
+          mbar_arrive_expect_tx(bar, 2 * tile_bytes<kBN>(a.dim));
+          tma_tile<Shape::kPieces, kBN>(dst, &p.q, a.dim, first_head(b), first_node(b), bar);
+          tma_tile<Shape::kPieces, kBN>(dst + Shape::kBlock, &p.grad, a.dim, first_head(b), first_node(b), bar);
+        }
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (cleared && b > 0) {
+        alive = mbar_wait(smem_u32(&full[cstage]), cphase, abort_flag, p.status, kErrGradLoad);
         alive = __all_sync(0xffffffffu, alive);
         if (!alive) break;
-      }
-      const uint32_t dst = smem_u32(sqg + stage * 2 * Shape::kBlock);
-      const int i0 = first_node(b), h0 = first_head(b);
-      const PackedRows q = {(const uint8_t*)((const T*)a.q + h0 * a.q_head), (int)(a.q_row * 2), p.pack_log, a.q_head * 2};
-      const PackedRows g = {(const uint8_t*)((const T*)p.g.grad + h0 * p.g.grad_head), (int)(p.g.grad_row * 2), p.pack_log,
-                            p.g.grad_head * 2};
-      auto live = [&](int r) { return i0 + (r >> p.pack_log) < span.hi; };
-      copy_tile<DP, kBN, 32 * kLoadWarps<DP>>(dst, thread, a.dim, a.q, [&](int r) { return q(i0, r); }, live);
-      copy_tile<DP, kBN, 32 * kLoadWarps<DP>>(dst + Shape::kBlock, thread, a.dim, a.q, [&](int r) { return g(i0, r); }, live);
-      cp_async_arrive(smem_u32(&full[stage]));
-      if (++stage == p.stages) {
-        stage = 0;
-        phase ^= 1u;
+        const int live = (end - first_node(b - 1)) << p.pack_log;           // rows before the batch's end
+        if (live < kBN) {
+          for (int qg = 0; qg < 2; ++qg)
+            clear_rows<Shape::kPieces, kBN>(sqg + (cstage * 2 + qg) * Shape::kBlock,
+                                            [&](int k) { return bit_run(0, live - 32 * k); });
+          proxy_fence();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(smem_u32(&clean[cstage]));
+        if (++cstage == p.stages) {
+          cstage = 0;
+          cphase ^= 1u;
+        }
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!alive)
+      for (int it = 0; it < 64; ++it) __nanosleep(1000);         // (copies under way end before the CTA does)
   }
   tc_fence_before();
   __syncthreads();
@@ -577,8 +601,9 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
 template <typename Shape, int CTAS>
 int stages_for() {
   constexpr size_t kMost = (227 * 1024) / CTAS - 1024;
+  static_assert(Shape::smem(3) <= kMost, "with a mask, three stages at least: one is cleared while two are read");
   int stages = kMaxStages;
-  while (stages > 2 && Shape::smem(stages) > kMost) --stages;
+  while (Shape::smem(stages) > kMost) --stages;
   return stages;
 }
 
@@ -590,20 +615,36 @@ int grad_launch(GradArgs& p, cudaStream_t st) {
   auto dkv = attn_tc_dkv_kernel<DP, G, HALF, CTAS_K>;
   const int stages_q = stages_for<Dq, CTAS_Q>(), stages_k = stages_for<Dkv, CTAS_K>();
   static PerDeviceOnce once;
-  const int status = once.run([&]() -> int {
+  int status = once.run([&]() -> int {
     OCNN_CUDA_OK(cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Dq::smem(stages_q)));
     OCNN_CUDA_OK(cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Dkv::smem(stages_k)));
     return OCNN_OK;
   });
   if (status != OCNN_OK) return status;
+  const AttnArgs& a = p.a;
+  constexpr int dtype = HALF ? OCNN_F16 : OCNN_BF16;
+  const int pack = 1 << p.pack_log;
+  auto queries = [&](int rows) -> int {
+    const int s = attn_map(&p.q, a.q, dtype, a.dim, a.heads, a.n, a.q_row, a.q_head, pack, rows >> p.pack_log);
+    return s != OCNN_OK ? s : attn_map(&p.grad, p.g.grad, dtype, a.dim, a.heads, a.n, p.g.grad_row, p.g.grad_head, pack,
+                                       rows >> p.pack_log);
+  };
+  status = queries(128);
+  if (status == OCNN_OK) status = attn_map(&p.k, a.k, dtype, a.dim, a.kv_heads, a.n, a.k_row, a.k_head, 1, kBN);
+  if (status == OCNN_OK) status = attn_map(&p.v, a.v, dtype, a.dim, a.kv_heads, a.n, a.v_row, a.v_head, 1, kBN);
+  if (status != OCNN_OK) return status;
   p.stages = stages_q;
-  dq<<<dim3(ceil_div(p.a.n, W * 128 >> p.pack_log), p.a.heads >> p.pack_log), Dq::kThreads, Dq::smem(stages_q), st>>>(p);
+  p.wide = wide_rows(p.g.dq, a.dim);
+  dq<<<dim3(ceil_div(a.n, W * 128 >> p.pack_log), a.heads >> p.pack_log), Dq::kThreads, Dq::smem(stages_q), st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_dq_kernel");
   if (p.a.sinks > 0) {
     const int far = attn_far_sums(p.a, p.g, HALF ? OCNN_F16 : OCNN_BF16, st);
     if (far != OCNN_OK) return far;
   }
+  status = queries(kBN);
+  if (status != OCNN_OK) return status;
   p.stages = stages_k;
+  p.wide = wide_rows(p.g.dk, a.dim) && wide_rows(p.g.dv, a.dim);
   dkv<<<dim3(ceil_div(p.a.n, 128), p.a.kv_heads), Dkv::kThreads, Dkv::smem(stages_k), st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_dkv_kernel");
   return OCNN_OK;
@@ -619,7 +660,11 @@ int grad_by_width(GradArgs& p, cudaStream_t st) {
 }  // namespace
 
 int attn_tc_backward(const AttnArgs& a, const AttnGrad& g, int dtype, int* status, cudaStream_t st) {
-  GradArgs p = {a, g, status, attn_pack_log(a), 0};
+  GradArgs p;
+  p.a = a;
+  p.g = g;
+  p.status = status;
+  p.pack_log = attn_pack_log(a);
   return dtype == OCNN_F16 ? grad_by_width<true>(p, st) : grad_by_width<false>(p, st);
 }
 

@@ -40,9 +40,13 @@ void need_like(const Tensor& t, const Tensor& like, const char* name, const char
               t.device(), " in ", t.scalar_type(), ", the data on ", like.device(), " in ", like.scalar_type());
 }
 
-// The kernels read whole rows: the last dimension is contiguous, the others may have any stride that a view gives
-// them (an expanded one too).
-Tensor rows_of(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+// The kernels read whole rows: the last dimension is contiguous, the others may have any stride that a view gives them.
+// (An expanded tensor, one row for all, is written out: tiles are not fetched at strides of 0.)
+Tensor rows_of(const Tensor& t) {
+  bool ok = t.size(-1) == 1 || t.stride(-1) == 1;
+  for (int i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.stride(i) != 0 || t.size(i) == 1);
+  return ok ? t : t.contiguous();
+}
 
 // Gradients are formed by kernels: they have no graph of their own.
 void once_only(const char* who) {

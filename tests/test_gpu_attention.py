@@ -101,9 +101,20 @@ def test_lengths_around_a_tile(dtype, n):
 
 @pytest.mark.parametrize('dtype', [F32, BF16])
 @pytest.mark.parametrize('causal', [False, True])
-def test_first_nodes_seen_from_far(dtype, causal):
+@pytest.mark.parametrize('dim', [32, 128])
+def test_first_nodes_seen_from_far(dtype, causal, dim):
   """Sequences over several blocks of the far pass, several sequences in one, first nodes that the mask hides."""
-  compare([1500, 30, 700, 512, 20, 1100], 4, 2, 32, dtype, 16, 4, causal, masked=0.8)
+  compare([1500, 30, 700, 512, 20, 1100], 4, 2, dim, dtype, 16, 4, causal, masked=0.8)
+  compare([40, 300, 5, 1000], 2, 2, dim, dtype, 16, 7, causal)
+
+
+@pytest.mark.parametrize('window,sinks', [(16, 4), (100, 64), (300, 1), (0, 0)])
+@pytest.mark.parametrize('masked', [None, 0.6])
+@pytest.mark.parametrize('heads,kv', [(2, 2), (8, 1)])
+def test_wide_heads(window, sinks, masked, heads, kv):
+  """Two tiles that share their copies of keys and values, of which each needs some."""
+  for causal in (False, True):
+    compare([700, 3, 400, 129], heads, kv, 128, BF16, window, sinks, causal, masked=masked)
 
 
 def test_large_scores():
@@ -146,6 +157,48 @@ def test_hidden_values_have_no_say(dtype):
   rel = (out[far].float() - clean['out'][far].float()).abs().max().item()
   assert rel <= 4 * torch.finfo(dtype).eps * clean['out'].abs().max().item()
   assert not torch.isfinite(out[53:69].float()).all(2).any()
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('dim', [32, 128])
+def test_hidden_values_have_no_say_in_gradients(dtype, dim):
+  """A node whose values are not numbers spoils what it sees and what sees it, no other node and no other sequence."""
+  offsets, n = [0, 150, 400], 400
+  q, k, v, g = inputs(n, 4, 2, dim, dtype, 6)
+  kw = dict(window=9, sinks=2, causal=False)
+  clean = run(q, k, v, offsets, g, **kw)
+  q2, v2 = q.clone(), v.clone()
+  v2[60], q2[300] = math.inf, math.nan                   # 60 is seen by 52 .. 68, whose delta it spoils; 300 sees 292 .. 308
+  got = run(q2, k, v2, offsets, g, **kw)
+  rows = torch.arange(n)
+  near = lambda at, w: (rows - at).abs() < w
+  spoilt = {'out': near(60, 9) | (rows == 300), 'dq': near(60, 9) | (rows == 300),
+            'dk': near(60, 17) | near(300, 9) | (rows < 2) | near(151, 2) & (rows >= 150),
+            'dv': near(60, 17) | near(300, 9) | (rows < 2) | near(151, 2) & (rows >= 150)}
+  for name in got:
+    rest = ~spoilt[name]
+    off = (got[name][rest].double() - clean[name][rest].double()).abs().max().item()
+    assert off <= 16 * torch.finfo(dtype).eps * clean[name].abs().max().item(), name
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('layout', ['heads first', 'expanded keys', 'one head', 'wide rows'])
+def test_layouts(dtype, layout):
+  offsets, n = [0, 90, 201], 201
+  q, k, v, g = inputs(n, 4, 2, 64, dtype, 1)
+  if layout == 'heads first':
+    q, k, v, g = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v, g))
+  elif layout == 'expanded keys':
+    k, g = k[:, :1].expand(n, 2, 64), g[:1].expand(n, 4, 64)
+  elif layout == 'one head':
+    q, k, v, g = q[:, :1], k[:, :1], v[:, 1:], g[:, 3:]
+  else:
+    q, k, v, g = (torch.cat([t, t, t], 2)[..., 64:128] for t in (q, k, v, g))
+  kw = dict(window=40, sinks=1, causal=True)
+  got = run(q, k, v, offsets, g, **kw)
+  want = attention(q, k, v, visible(n, offsets, 40, 1, True, None, 'cuda'), None, g)
+  for name in want:
+    check(got[name], want[name], name)
 
 
 def test_gradient_against_differences():
