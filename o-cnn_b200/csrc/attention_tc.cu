@@ -122,6 +122,14 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
       // does every row of the warp see every key?
       const bool first = keys.is_first(b);
       const bool all = a.mask == nullptr && !first && __all_sync(0xffffffffu, r.lo <= j && j + BN <= r.hi);
+      uint32_t bits[BN / 32];
+      if (!all) {
+#pragma unroll
+        for (int k = 0; k < BN / 32; ++k) {
+          bits[k] = first ? seen_first(keys, r, 32 * k) : seen_bits(a, r, j + 32 * k);
+          if (a.mask != nullptr) bits[k] &= kept_bits(a, j + 32 * k, a.n);
+        }
+      }
       alive = mbar_wait(smem_u32(&sfull[2 * t + place]), (done >> 1) & 1, abort_flag, p.status, kErrAttnS);
       alive = __all_sync(0xffffffffu, alive);
       if (!alive) break;
@@ -132,13 +140,8 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
       if (!all) {
         // (a hidden score is -inf, c > 0: its p is 0)
 #pragma unroll
-        for (int k = 0; k < BN / 32; ++k) {
-          uint32_t bits = first ? seen_first(keys, r, 32 * k) : seen_bits(a, r, j + 32 * k);
-          if (a.mask != nullptr) bits &= kept_bits(a, j + 32 * k, a.n);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((bits >> e) & 1)) s[32 * k + e] = -INFINITY;
-        }
+        for (int e = 0; e < BN; ++e)
+          if (!((bits[e / 32] >> (e & 31)) & 1)) s[e] = -INFINITY;
       }
       float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll

@@ -129,6 +129,14 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       const int j = keys.key(b);
       const bool first = keys.is_first(b);
       const bool all = a.mask == nullptr && !first && __all_sync(0xffffffffu, r.lo <= j && j + kBN <= r.hi);
+      uint32_t bits[2];
+      if (!all) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          bits[k] = first ? seen_first(keys, r, 32 * k) : seen_bits(a, r, j + 32 * k);
+          if (a.mask != nullptr) bits[k] &= kept_bits(a, j + 32 * k, a.n);
+        }
+      }
       alive = mbar_wait(smem_u32(&sfull[t]), done & 1, abort_flag, p.status, kErrGradS);
       alive = __all_sync(0xffffffffu, alive);
       if (!alive) break;
@@ -146,13 +154,8 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       }
       if (!all) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t bits = first ? seen_first(keys, r, 32 * k) : seen_bits(a, r, j + 32 * k);
-          if (a.mask != nullptr) bits &= kept_bits(a, j + 32 * k, a.n);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((bits >> e) & 1)) s[32 * k + e] = 0.f;
-        }
+        for (int e = 0; e < kBN; ++e)
+          if (!((bits[e / 32] >> (e & 31)) & 1)) s[e] = 0.f;
       }
       uint32_t w[kBN / 2];
 #pragma unroll
