@@ -399,73 +399,111 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
     if (redo[r] != 0 && k0 + r < a.n) attn_dkv_row<T>(a, g, k0 + r, hk, true, true);
 }
 
-// The far pass: what the nodes beyond the window add to the gradients of their sequence's first nodes.  A block takes
-// kFarRows nodes of one key head, every warp its share of them; a lane holds four channels of the sums (dim <= 128).
-// Partial sums go to slot block + sequence, which no other pair of block and sequence has: along the packed batch
-// either the block or the sequence moves on.
+// The far pass: what the nodes beyond the window add to the gradients of their sequence's first nodes, kFarSinks of them
+// at a time.  A block takes kFarRows nodes of one key head; a row (a query head of a node) is read once by LPR lanes,
+// 16 bytes of q and dO each, which keep their channels of the sums, so that a warp has 32 / LPR rows under way (65 k nodes,
+// 16 heads of 128, 4 first nodes: 890 us with a row per warp and a channel per lane and load, FIG_FAR now).
+constexpr int kFarSinks = 4;
+
 template <typename T>
-__global__ void __launch_bounds__(256) attn_far_kernel(const AttnArgs a, const AttnGrad g) {
-  const int hk = blockIdx.y, group = a.heads / a.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int r0 = blockIdx.x * kFarRows, r1 = min(a.n, r0 + kFarRows);
-  __shared__ float part[8][2][kMaxHeadDim];
+__device__ __forceinline__ void far_load(const T* p, int left, bool vec, float (&x)[16 / sizeof(T)]) {
+  constexpr int V = 16 / sizeof(T);
+  if (vec) {
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (left > 0) w = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int c = 0; c < V; ++c) x[c] = to_f32(e[c]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < V; ++c) x[c] = c < left ? to_f32(p[c]) : 0.f;
+  }
+}
+
+template <typename T, int LPR>
+__global__ void __launch_bounds__(256) attn_far_kernel(const AttnArgs a, const AttnGrad g, bool vec) {
+  constexpr int V = 16 / sizeof(T), kRows = 256 / LPR;        // rows of a block at a time
+  const int hk = blockIdx.y, group = a.heads / a.kv_heads, tid = threadIdx.x, sub = tid % LPR, row = tid / LPR;
+  const int r0 = blockIdx.x * kFarRows, r1 = min(a.n, r0 + kFarRows), d0 = sub * V, left = a.dim - d0;
+  __shared__ float part[8][2 * kMaxHeadDim];
   for (int i0 = r0; i0 < r1;) {
-    Span s = attn_span(a, i0);
-    if (s.end <= s.start) {                        // outside of every sequence: on to the next one's first node
-      const int next = s.seq < a.batch ? (s.seq == 0 && i0 < attn_offset(a, 0) ? attn_offset(a, 0) : a.n) : a.n;
-      i0 = max(i0 + 1, next);
+    const Span s = attn_span(a, i0);
+    if (s.end <= s.start) {                        // outside of every sequence: on to the first one, or to the end
+      const int begin = attn_offset(a, 0);
+      i0 = i0 < begin ? begin : r1;
       continue;
     }
-    const int end = min(r1, s.end);
-    for (int t = 0; t < a.sinks && s.start + t < s.end; ++t) {
-      const int j = s.start + t;
-      float k[4], v[4], dk[4] = {}, dv[4] = {};
-      const bool kept = a.mask == nullptr || a.mask[j] != 0;
-      const bool any = kept && end > j + (long long)a.window;
+    const int end = min(r1, s.end), sinks = min(a.sinks, s.end - s.start);
+    for (int t0 = 0; t0 < sinks; t0 += kFarSinks) {
+      float k[kFarSinks][V], v[kFarSinks][V], dk[kFarSinks][V] = {}, dv[kFarSinks][V] = {};
+      bool kept[kFarSinks];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int d = lane + 32 * c;
-        k[c] = any && d < a.dim ? to_f32(((const T*)a.k)[j * a.k_row + hk * a.k_head + d]) : 0.f;
-        v[c] = any && d < a.dim ? to_f32(((const T*)a.v)[j * a.v_row + hk * a.v_head + d]) : 0.f;
+      for (int t = 0; t < kFarSinks; ++t) {
+        const int j = s.start + t0 + t;
+        kept[t] = t0 + t < sinks && (a.mask == nullptr || a.mask[j] != 0);
+        far_load<T>((const T*)a.k + j * a.k_row + hk * a.k_head + d0, kept[t] ? left : 0, vec, k[t]);
+        far_load<T>((const T*)a.v + j * a.v_row + hk * a.v_head + d0, kept[t] ? left : 0, vec, v[t]);
       }
-      if (any) {
-        for (int i = max(i0, j + a.window) + warp; i < end; i += 8) {
-          for (int hg = 0; hg < group; ++hg) {
-            const int h = hk * group + hg;
-            float q[4], o[4], x = 0.f, y = 0.f;
+      // the rows that see the first of them from far; the others' turn comes a node later each
+      const int from = s.end - s.start - t0 > a.window ? max(i0, s.start + t0 + a.window) : end;
+      const int count = (end - from) * group;
+      for (int e = row; e - row < count; e += kRows) {         // (all lanes of a warp go round together)
+        const bool in = e < count;
+        const int i = from + (in ? e / group : 0), h = hk * group + (in ? e % group : 0);
+        float q[V], o[V];
+        far_load<T>((const T*)a.q + i * a.q_row + h * a.q_head + d0, in ? left : 0, vec, q);
+        far_load<T>((const T*)g.grad + i * g.grad_row + h * g.grad_head + d0, in ? left : 0, vec, o);
+        const float lse = in ? g.lse[(long long)h * a.n + i] : 0.f, delta = in ? g.delta[(long long)h * a.n + i] : 0.f;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int d = lane + 32 * c;
-              q[c] = d < a.dim ? to_f32(((const T*)a.q)[i * a.q_row + h * a.q_head + d]) : 0.f;
-              o[c] = d < a.dim ? to_f32(((const T*)g.grad)[i * g.grad_row + h * g.grad_head + d]) : 0.f;
-              x = fmaf(q[c], k[c], x);
-              y = fmaf(o[c], v[c], y);
-            }
-            x = warp_sum(x);
-            y = warp_sum(y);
-            const float p = exp2f(x * a.scale_log2 - g.lse[(long long)h * a.n + i]);
-            const float ds = p * (y - g.delta[(long long)h * a.n + i]);
+        for (int t = 0; t < kFarSinks; ++t) {
+          if (t0 + t >= sinks) break;
+          float x = 0.f, y = 0.f;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              dk[c] = fmaf(ds, q[c], dk[c]);
-              dv[c] = fmaf(p, o[c], dv[c]);
-            }
+          for (int c = 0; c < V; ++c) {
+            x = fmaf(q[c], k[t][c], x);
+            y = fmaf(o[c], v[t][c], y);
+          }
+#pragma unroll
+          for (int m = LPR / 2; m > 0; m >>= 1) {
+            x += __shfl_xor_sync(0xffffffffu, x, m);
+            y += __shfl_xor_sync(0xffffffffu, y, m);
+          }
+          const bool seen = in && kept[t] && i - (s.start + t0 + t) >= a.window;
+          const float p = seen ? exp2f(x * a.scale_log2 - lse) : 0.f, ds = seen ? p * (y - delta) : 0.f;
+#pragma unroll
+          for (int c = 0; c < V; ++c) {
+            dk[t][c] += seen ? ds * q[c] : 0.f;
+            dv[t][c] += seen ? p * o[c] : 0.f;
           }
         }
       }
-      __syncthreads();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        part[warp][0][lane + 32 * c] = dk[c];
-        part[warp][1][lane + 32 * c] = dv[c];
-      }
-      __syncthreads();
-      float* dst = far_slot(a, g, blockIdx.x + s.seq, hk, t);
-      for (int e = threadIdx.x; e < 2 * kMaxHeadDim; e += 256) {
-        const int which = e / kMaxHeadDim, d = e % kMaxHeadDim;
-        if (d >= a.dim) continue;
-        float x = 0.f;
-        for (int w = 0; w < 8; ++w) x += part[w][which][d];
-        dst[which * a.dim + d] = x;
+      for (int t = 0; t < kFarSinks; ++t) {
+        if (t0 + t >= sinks) break;
+#pragma unroll
+        for (int c = 0; c < V; ++c)
+#pragma unroll
+          for (int m = LPR; m < 32; m <<= 1) {
+            dk[t][c] += __shfl_xor_sync(0xffffffffu, dk[t][c], m);
+            dv[t][c] += __shfl_xor_sync(0xffffffffu, dv[t][c], m);
+          }
+        __syncthreads();
+        if ((tid & 31) < LPR) {
+#pragma unroll
+          for (int c = 0; c < V; ++c) {
+            if (c >= left) break;
+            part[tid >> 5][d0 + c] = dk[t][c];
+            part[tid >> 5][a.dim + d0 + c] = dv[t][c];
+          }
+        }
+        __syncthreads();
+        float* dst = far_slot(a, g, blockIdx.x + s.seq, hk, t0 + t);
+        for (int e = tid; e < 2 * a.dim; e += 256) {
+          float x = 0.f;
+#pragma unroll
+          for (int w = 0; w < 8; ++w) x += part[w][e];
+          dst[e] = x;
+        }
       }
     }
     i0 = s.end;
@@ -474,7 +512,17 @@ __global__ void __launch_bounds__(256) attn_far_kernel(const AttnArgs a, const A
 
 template <typename T>
 int far_launch(const AttnArgs& a, const AttnGrad& g, cudaStream_t st) {
-  attn_far_kernel<T><<<dim3(ceil_div(a.n, kFarRows), a.kv_heads), 256, 0, st>>>(a, g);
+  constexpr int V = 16 / sizeof(T);
+  auto on = [&](const void* p, long long row, long long head) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % V == 0 && head % V == 0;
+  };
+  const bool vec = a.dim % V == 0 && on(a.q, a.q_row, a.q_head) && on(a.k, a.k_row, a.k_head) &&
+                   on(a.v, a.v_row, a.v_head) && on(g.grad, g.grad_row, g.grad_head);
+  const dim3 grid(ceil_div(a.n, kFarRows), a.kv_heads);
+  if (a.dim <= 4 * V) attn_far_kernel<T, 4><<<grid, 256, 0, st>>>(a, g, vec);
+  else if (a.dim <= 8 * V) attn_far_kernel<T, 8><<<grid, 256, 0, st>>>(a, g, vec);
+  else if (a.dim <= 16 * V) attn_far_kernel<T, 16><<<grid, 256, 0, st>>>(a, g, vec);
+  else attn_far_kernel<T, 32><<<grid, 256, 0, st>>>(a, g, vec);
   OCNN_LAUNCH_OK("attn_far_kernel");
   return OCNN_OK;
 }

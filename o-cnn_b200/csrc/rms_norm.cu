@@ -258,32 +258,28 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_backward_kernel(const N
   }
 }
 
-// gw[c] = the blocks' sums, in order: 32 channels per block, 8 runs of slots side by side.
+// gw[c] = the blocks' sums, in order: 32 channels per block, 32 runs of slots side by side.
 template <typename T>
-__global__ void __launch_bounds__(256) rms_norm_weight_kernel(const float* partial, int slots, int channels, void* gw,
-                                                              int w_f32) {
+__global__ void __launch_bounds__(1024) rms_norm_weight_kernel(const float* partial, int slots, int channels, void* gw,
+                                                               int w_f32) {
   grid_dependency_trigger();
   grid_dependency_wait();
-  __shared__ float part[8][32];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), run = threadIdx.x >> 5;
-  const int per = (slots + 7) / 8;
-  float x[4] = {};
+  __shared__ float part[32][33];
+  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float x = 0.f;
   if (c < channels) {
-    const int end = min(slots, (run + 1) * per);
-    int s = run * per;
-    for (; s + 4 <= end; s += 4)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] += partial[(long long)(s + u) * channels + c];
-    for (; s < end; ++s) x[0] += partial[(long long)s * channels + c];
+#pragma unroll 8
+    for (int s = run; s < slots; s += 32) x += partial[(long long)s * channels + c];
   }
-  part[run][threadIdx.x & 31] = (x[0] + x[1]) + (x[2] + x[3]);
+  part[run][lane] = x;
   __syncthreads();
-  if (run == 0 && c < channels) {
-    float y = 0.f;
+  float y = part[lane][run];                     // (warp `run` adds channel `run`)
 #pragma unroll
-    for (int r = 0; r < 8; ++r) y += part[r][threadIdx.x];
-    if (w_f32) ((float*)gw)[c] = y;
-    else norm_set(((T*)gw)[c], y);
+  for (int m = 16; m > 0; m >>= 1) y += __shfl_xor_sync(0xffffffffu, y, m);
+  const int out = blockIdx.x * 32 + run;
+  if (lane == 0 && out < channels) {
+    if (w_f32) ((float*)gw)[out] = y;
+    else norm_set(((T*)gw)[out], y);
   }
 }
 
@@ -400,7 +396,7 @@ int ocnn_add_rms_norm_backward(const void* x_dev, int64_t x_row, const void* res
   if (status != OCNN_OK || grad_weight_dev == nullptr) return status;
   auto sum = dtype == OCNN_F32 ? rms_norm_weight_kernel<float>
              : dtype == OCNN_BF16 ? rms_norm_weight_kernel<__nv_bfloat16> : rms_norm_weight_kernel<__half>;
-  OCNN_CUDA_OK(launch_chained(sum, dim3(ceil_div(channels, 32)), dim3(256), 0, st, (const float*)a.partial, blocks,
+  OCNN_CUDA_OK(launch_chained(sum, dim3(ceil_div(channels, 32)), dim3(1024), 0, st, (const float*)a.partial, blocks,
                               channels, grad_weight_dev, weight_dtype == OCNN_F32 ? 1 : 0));
   OCNN_LAUNCH_OK("rms_norm_weight_kernel");
   return OCNN_OK;

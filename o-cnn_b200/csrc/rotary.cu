@@ -19,7 +19,7 @@ struct RotaryArgs {
   void* y;
   const double* freqs;
   long long rows, row, head;
-  int heads, dim, axes, pairs, rows_per_block, float_positions, inverse, head_items;
+  int heads, dim, axes, pairs, rows_per_block, float_positions, inverse;
   int begin[kMaxAxes + 1];                  // axis a turns the pairs [begin[a], begin[a + 1])
 };
 
@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
   extern __shared__ float2 turn[];          // [rows_per_block][pairs]
   const long long r0 = (long long)blockIdx.x * a.rows_per_block;
   const int rows = (int)min((long long)a.rows_per_block, a.rows - r0);
-  for (int e = threadIdx.x; e < rows * a.pairs; e += kRotThreads) {
+  for (int e = threadIdx.x; e < rows * a.pairs; e += blockDim.x) {
     const int r = e / a.pairs, t = e - r * a.pairs;
     int axis = 0;
     while (t >= a.begin[axis + 1]) ++axis;
@@ -57,50 +57,55 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
     turn[e] = make_float2(c, a.inverse ? -s : s);
   }
   __syncthreads();
-  const int half = a.dim >> 1, runs = half / V, row_items = a.heads * runs, items = rows * row_items;
-  for (int e0 = threadIdx.x; e0 < items; e0 += 2 * kRotThreads) {
-    Pack<T, V> lo[2], hi[2];
-    const T* src[2];
-    T* dst[2];
-    int at[2], first[2];
+  // A thread has one item of a row, in every rows_at_a_time-th row (or, of rows with more items than threads, several).
+  const int half = a.dim >> 1, runs = half / V, row_items = a.heads * runs;
+  const int across = min(row_items, (int)blockDim.x), step = blockDim.x / across;
+  for (int item = threadIdx.x % across; item < row_items; item += across) {
+    const int h = item / runs, t = (item - h * runs) * V, c = INTERLEAVED ? 2 * t : t, live = min(V, a.pairs - t);
+    const int mine = threadIdx.x / across;
+    const T* src = (const T*)a.x + (r0 + mine) * a.row + h * a.head + c;
+    T* dst = (T*)a.y + ((r0 + mine) * a.heads + h) * a.dim + c;
+    const long long src_step = step * a.row, dst_step = (long long)step * a.heads * a.dim;
+    constexpr int U = 4;
+    for (int r = mine; r < rows; r += U * step) {
+      Pack<T, V> lo[U], hi[U];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int e = e0 + u * kRotThreads;
-      if (e >= items) break;
-      const int r = e / row_items, rest = e - r * row_items, h = rest / runs, t = (rest - h * runs) * V;
-      first[u] = t;
-      at[u] = r * a.pairs + t;
-      const int c = INTERLEAVED ? 2 * t : t;
-      src[u] = (const T*)a.x + (r0 + r) * a.row + h * a.head + c;
-      dst[u] = (T*)a.y + ((r0 + r) * a.heads + h) * a.dim + c;
-      lo[u] = *reinterpret_cast<const Pack<T, V>*>(src[u]);
-      hi[u] = *reinterpret_cast<const Pack<T, V>*>(src[u] + (INTERLEAVED ? V : half));
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (e0 + u * kRotThreads >= items) break;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (first[u] + i >= a.pairs) break;   // (behind the last axis' pairs: as they are, whatever they are)
-        const float2 w = turn[at[u] + i];
-        // interleaved: pair i is elements 2i, 2i + 1 of the run of 2V
-        T& x1 = INTERLEAVED ? (2 * i < V ? lo[u].x[(2 * i) % V] : hi[u].x[(2 * i) % V]) : lo[u].x[i];
-        T& x2 = INTERLEAVED ? (2 * i + 1 < V ? lo[u].x[(2 * i + 1) % V] : hi[u].x[(2 * i + 1) % V]) : hi[u].x[i];
-        const float f1 = rot_f32(x1), f2 = rot_f32(x2);
-        rot_set(x1, f1 * w.x - f2 * w.y);
-        rot_set(x2, f2 * w.x + f1 * w.y);
+      for (int u = 0; u < U; ++u) {
+        if (r + u * step >= rows) break;
+        lo[u] = *reinterpret_cast<const Pack<T, V>*>(src + u * src_step);
+        hi[u] = *reinterpret_cast<const Pack<T, V>*>(src + u * src_step + (INTERLEAVED ? V : half));
       }
-      *reinterpret_cast<Pack<T, V>*>(dst[u]) = lo[u];
-      *reinterpret_cast<Pack<T, V>*>(dst[u] + (INTERLEAVED ? V : half)) = hi[u];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (r + u * step >= rows) break;
+        const float2* w = turn + (r + u * step) * a.pairs + t;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (i >= live) break;                 // (behind the last axis' pairs: as they are, whatever they are)
+          // interleaved: pair i is elements 2i, 2i + 1 of the run of 2V
+          T& x1 = INTERLEAVED ? (2 * i < V ? lo[u].x[(2 * i) % V] : hi[u].x[(2 * i) % V]) : lo[u].x[i];
+          T& x2 = INTERLEAVED ? (2 * i + 1 < V ? lo[u].x[(2 * i + 1) % V] : hi[u].x[(2 * i + 1) % V]) : hi[u].x[i];
+          const float f1 = rot_f32(x1), f2 = rot_f32(x2);
+          rot_set(x1, f1 * w[i].x - f2 * w[i].y);
+          rot_set(x2, f2 * w[i].x + f1 * w[i].y);
+        }
+        *reinterpret_cast<Pack<T, V>*>(dst + u * dst_step) = lo[u];
+        *reinterpret_cast<Pack<T, V>*>(dst + u * dst_step + (INTERLEAVED ? V : half)) = hi[u];
+      }
+      src += U * src_step;
+      dst += U * dst_step;
     }
   }
 }
 
 template <typename T, int V>
 int rotary_launch(RotaryArgs& a, bool interleaved, cudaStream_t st) {
-  // nodes per block: four items a thread, but no more than 16 KB of cosines and sines, and enough blocks for the SMs
+  // As many threads as make whole rows (256 at most), and nodes per block: eight a thread, but no more than 16 KB of
+  // cosines and sines, and enough blocks for the SMs.
   const int row_items = a.heads * (a.dim / 2 / V);
-  long long r = (4 * kRotThreads + row_items - 1) / row_items;
+  const int threads = row_items >= kRotThreads ? kRotThreads : kRotThreads / row_items * row_items;
+  const int step = row_items >= kRotThreads ? 1 : kRotThreads / row_items;
+  long long r = 8LL * step;
   if (a.pairs > 0 && r * a.pairs > 2048) r = 2048 / a.pairs;
   const long long spread = (a.rows + 4LL * sm_count() - 1) / (4LL * sm_count());
   if (r > spread) r = spread;
@@ -109,8 +114,8 @@ int rotary_launch(RotaryArgs& a, bool interleaved, cudaStream_t st) {
   const long long blocks = (a.rows + r - 1) / r;
   OCNN_REQUIRE(blocks < (1LL << 31), "ocnn_octree_rotary: too many rows");
   const size_t smem = (size_t)r * a.pairs * sizeof(float2);
-  if (interleaved) rotary_kernel<T, V, true><<<(unsigned)blocks, kRotThreads, smem, st>>>(a);
-  else rotary_kernel<T, V, false><<<(unsigned)blocks, kRotThreads, smem, st>>>(a);
+  if (interleaved) rotary_kernel<T, V, true><<<(unsigned)blocks, threads, smem, st>>>(a);
+  else rotary_kernel<T, V, false><<<(unsigned)blocks, threads, smem, st>>>(a);
   OCNN_LAUNCH_OK("rotary_kernel");
   return OCNN_OK;
 }

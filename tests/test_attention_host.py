@@ -66,7 +66,7 @@ def test_step(kw, heads, window, status):
     setattr(c, name, value)
   s = (I64 * 2)(128, 32)
   assert L.ocnn_octree_attention_step(ctypes.byref(c), P(64), s, P(64), s, P(64), s, P(64), heads, window, 0,
-                                      ctypes.c_float(1.0), None) == status
+                                      ctypes.c_float(1.0), P(64), None) == status
 
 
 def test_rotary_and_norm():
