@@ -717,7 +717,7 @@ typedef struct ocnn_attention_cache {
 int ocnn_octree_attention_step(const ocnn_attention_cache* cache, const void* q_dev, const int64_t q_stride[2],
                                const void* k_dev, const int64_t k_stride[2], const void* v_dev,
                                const int64_t v_stride[2], void* out_dev, int heads, int window, int sinks,
-                               float scale, int32_t* status_dev, void* stream);
+                               float scale, void* stream);
 
 #ifdef __cplusplus
 }

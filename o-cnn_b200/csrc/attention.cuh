@@ -49,7 +49,7 @@ inline int attn_pack_log(const AttnArgs& a) {
 
 int attn_tc_forward(const AttnArgs& a, int dtype, void* out, float* lse, int* status, cudaStream_t st);
 int attn_tc_backward(const AttnArgs& a, const AttnGrad& g, int dtype, int* status, cudaStream_t st);
-int attn_far_sums(const AttnArgs& a, const AttnGrad& g, int dtype, cudaStream_t st);
+int attn_far_mma(const AttnArgs& a, const AttnGrad& g, int dtype, cudaStream_t st);   // 16-bit rows on 16-byte boundaries
 int attn_simt_forward(const AttnArgs& a, int dtype, void* out, float* lse, bool vec, cudaStream_t st);
 int attn_simt_backward(const AttnArgs& a, const AttnGrad& g, int dtype, bool vec, cudaStream_t st);
 
@@ -278,7 +278,7 @@ __device__ void attn_dkv_row(const AttnArgs& a, const AttnGrad& g, int j, int hk
 // sequence.  It is summed in blocks of kFarRows nodes, each block's share of a sequence in a slot of its own, and the
 // kernel that writes the keys' gradients adds the slots in order: no atomics, the same bits every time.  Slot = block +
 // sequence: along the packed batch either the block or the sequence moves on, so no two pairs share one.
-constexpr int kFarRows = 512;
+constexpr int kFarRows = 256;
 inline int far_slots(int n, int batch) { return ceil_div(n, kFarRows) + batch; }
 __device__ __forceinline__ float* far_slot(const AttnArgs& a, const AttnGrad& g, int slot, int hk, int sink) {
   return g.far + (((long long)slot * a.kv_heads + hk) * a.sinks + sink) * (2 * a.dim);

@@ -401,8 +401,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
 
 // The far pass: what the nodes beyond the window add to the gradients of their sequence's first nodes, kFarSinks of them
 // at a time.  A block takes kFarRows nodes of one key head; a row (a query head of a node) is read once by LPR lanes,
-// 16 bytes of q and dO each, which keep their channels of the sums, so that a warp has 32 / LPR rows under way (65 k nodes,
-// 16 heads of 128, 4 first nodes: 890 us with a row per warp and a channel per lane and load, FIG_FAR now).
+// 16 bytes of q and dO each, which keep their channels of the sums, so that a warp has 32 / LPR rows under way.
 constexpr int kFarSinks = 4;
 
 template <typename T>
@@ -421,7 +420,7 @@ __device__ __forceinline__ void far_load(const T* p, int left, bool vec, float (
 }
 
 template <typename T, int LPR>
-__global__ void __launch_bounds__(256) attn_far_kernel(const AttnArgs a, const AttnGrad g, bool vec) {
+__global__ void __launch_bounds__(256, 2) attn_far_kernel(const AttnArgs a, const AttnGrad g, bool vec) {
   constexpr int V = 16 / sizeof(T), kRows = 256 / LPR;        // rows of a block at a time
   const int hk = blockIdx.y, group = a.heads / a.kv_heads, tid = threadIdx.x, sub = tid % LPR, row = tid / LPR;
   const int r0 = blockIdx.x * kFarRows, r1 = min(a.n, r0 + kFarRows), d0 = sub * V, left = a.dim - d0;
@@ -577,10 +576,6 @@ int by_type(int dtype, int dim, F f) {
 
 }  // namespace
 
-int attn_far_sums(const AttnArgs& a, const AttnGrad& g, int dtype, cudaStream_t st) {
-  return dtype == OCNN_F32 ? far_launch<float>(a, g, st)
-         : dtype == OCNN_BF16 ? far_launch<__nv_bfloat16>(a, g, st) : far_launch<__half>(a, g, st);
-}
 int attn_simt_forward(const AttnArgs& a, int dtype, void* out, float* lse, bool vec, cudaStream_t st) {
   return by_type(dtype, a.dim, [&](auto t, auto dp) -> int {
     return forward_launch<decltype(t), decltype(dp)::value>(a, out, lse, vec, st);

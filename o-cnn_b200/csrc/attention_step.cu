@@ -9,14 +9,15 @@
 // sequence's key head, each CTA a stretch of the visible positions, each warp its rows with a running maximum and sum;
 // the parts are joined in shared memory, first the warps', then the CTAs' through the cluster's: one launch, no
 // workspace, the same bits every time.
-//   16-bit caches: a warp copies rows into a ring of stages (one bulk copy per row: rolled caches and the new row need no
-//   case of their own) and four warps multiply them with mma.sync, 16 query heads at a time.  On the CUDA cores, a product
-//   and a shuffle per value for each query head, 64 sequences of 4100 rows, 16 heads over 4 of 128, took 510 us.
+//   16-bit caches: every warp copies its rows, 16 at a time, into a ring of its own (cp.async, one row after the other:
+//   rolled caches and the new row need no case of their own) and multiplies them with mma.sync, 16 query heads at a time.
+//   On the CUDA cores, a product and a shuffle per value for each query head, 64 sequences of 4100 rows, 16 heads over 4
+//   of 128, took 510 us, with a bulk copy per row (about 65 cycles each, one after the other) 302 us, now FIG_STEP.
 //   fp32 caches: a warp reads whole rows, 16 bytes a lane, on the CUDA cores.
 #include <cooperative_groups.h>
 
 #include "attention.cuh"
-#include "tc.cuh"
+#include "mma.cuh"
 
 namespace ocnn {
 namespace {
@@ -30,7 +31,6 @@ struct StepArgs {
   long long kc_seq, kc_pos, kc_head, vc_seq, vc_pos, vc_head;
   void* out;
   const int* lengths;
-  int* status;
   int batch, heads, kv_heads, dim, capacity, window, sinks, rolls;
   float scale_log2;
 };
@@ -225,207 +225,154 @@ __global__ void __launch_bounds__(kStepThreads) attn_step_kernel(const StepArgs 
 }
 
 // ---- 16-bit caches ------------------------------------------------------------------------------------------------
-constexpr int kMmaKeys = 64, kMmaWarps = 4, kMmaHeads = 16;    // rows of a stage, warps that multiply, query heads of a CTA
-
-enum : int { kErrStepFull = 31, kErrStepEmpty = 32 };
-
-__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ void ldmatrix4t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-template <bool HALF>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (HALF)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
+constexpr int kMmaWarps = 4, kMmaHeads = 16, kMmaRows = 16;    // warps, query heads of a CTA, rows of a tile
 
 template <int DP>
 struct StepShape {
   static constexpr int kPitch = DP * 2 + 16;                   // (an odd number of 16-byte pieces: ldmatrix meets no bank twice)
-  static constexpr int kStage = 2 * kMmaKeys * kPitch;         // K, then V
-  static constexpr int kStages = DP > 64 ? 3 : 4;
-  static constexpr int kJoin = kMmaWarps * kMmaHeads * (DP + 2) * 4;
-  static constexpr size_t smem() { return kStages * kStage > kJoin ? kStages * kStage : kJoin; }
+  static constexpr int kTile = 2 * kMmaRows * kPitch;          // K, then V
+  static constexpr int kTiles = DP > 64 ? 2 : 3;               // of a warp's ring
+  static constexpr int kRing = kMmaWarps * kTiles * kTile, kJoin = kMmaWarps * kMmaHeads * (DP + 2) * 4;
+  static constexpr int kBytes = kRing > kJoin ? kRing : kJoin;
 };
 
 template <bool HALF, int DP>
-__global__ void __launch_bounds__(32 * (kMmaWarps + 1)) attn_step_mma_kernel(const StepArgs a) {
+__global__ void __launch_bounds__(32 * kMmaWarps) attn_step_mma_kernel(const StepArgs a) {
   using Shape = StepShape<DP>;
   using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
-  constexpr int KS = DP / 16, kThreads = 32 * (kMmaWarps + 1);
+  constexpr int KS = DP / 16, kThreads = 32 * kMmaWarps, kChunks = DP / 8, kStep = 32 / kChunks;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int group = a.heads / a.kv_heads, chunks = (group + kMmaHeads - 1) / kMmaHeads;
   const int hk = blockIdx.y / chunks, g0 = (blockIdx.y % chunks) * kMmaHeads, b = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[Shape::kStages], empty[Shape::kStages];
-  __shared__ volatile int abort_flag;
   const StepKeys keys(a, b);
-  // this CTA's stretch, in whole stages
-  const int stages = (keys.n + kMmaKeys - 1) / kMmaKeys, per = (stages + parts - 1) / parts;
-  const int t_begin = min(part * per * kMmaKeys, keys.n), t_end = min((part + 1) * per * kMmaKeys, keys.n);
-  const int count = (t_end - t_begin + kMmaKeys - 1) / kMmaKeys;
-  if (tid == 0) {
-    for (int s = 0; s < Shape::kStages; ++s) {
-      mbar_init(smem_u32(&full[s]), 1);
-      mbar_init(smem_u32(&empty[s]), kMmaWarps);
-    }
-    abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  // What the copies leave out and the products read: rows behind the last one, channels up to the next multiple of 16.
-  if (a.dim % 16 != 0 || (t_end - t_begin) % kMmaKeys != 0) {
-    const int slot = (count - 1) % Shape::kStages, from = (t_end - t_begin) - (count - 1) * kMmaKeys;
-    for (int e = tid; e < Shape::kStages * 2 * kMmaKeys; e += kThreads) {
-      const int r = e % kMmaKeys, s = e / (2 * kMmaKeys);
-      if (count == 0 || !((s == slot && r >= from) || a.dim % 16 != 0)) continue;
-      uint8_t* row = smem + e * Shape::kPitch;
-      for (int c = (s == slot && r >= from) ? 0 : a.dim * 2; c < (a.dim + 15) / 16 * 32; c += 16)
-        *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  }
-  __syncthreads();
-  const int ksteps = (a.dim + 15) / 16;
-  float o[2 * KS][4] = {}, top[2] = {-INFINITY, -INFINITY}, total[2] = {};
+  // this CTA's stretch of the list, in whole rounds of its warps
+  constexpr int kRound = kMmaWarps * kMmaRows;
+  const int rounds = (keys.n + kRound - 1) / kRound, per = (rounds + parts - 1) / parts * kRound;
+  const int t_begin = min(part * per, keys.n), t_end = min(t_begin + per, keys.n);
+  const int ksteps = (a.dim + 15) / 16, full = a.dim / 8;
 
-  if (warp == kMmaWarps) {
-    // ---------------- copies: a lane per row ----------------
-    const T* kc = (const T*)a.kc + b * a.kc_seq + hk * a.kc_head;
-    const T* vc = (const T*)a.vc + b * a.vc_seq + hk * a.vc_head;
-    const T* kn = (const T*)a.k + b * a.k_row + hk * a.k_head;
-    const T* vn = (const T*)a.v + b * a.v_row + hk * a.v_head;
-    const uint32_t bytes = a.dim * 2;
-    bool alive = true;
-    for (int i = 0; i < count; ++i) {
-      const int s = i % Shape::kStages;
-      if (i >= Shape::kStages)
-        alive = mbar_wait(smem_u32(&empty[s]), (i / Shape::kStages - 1) & 1, &abort_flag, a.status, kErrStepEmpty);
-      alive = __all_sync(0xffffffffu, alive);
-      if (!alive) break;
-      const int t0 = t_begin + i * kMmaKeys, rows = min(kMmaKeys, t_end - t0);
-      const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem + s * Shape::kStage);
-      if (lane == 0) mbar_arrive_expect_tx(bar, 2 * rows * bytes);
-      __syncwarp();
-      for (int r = lane; r < rows; r += 32) {
-        const int x = keys.position(t0 + r), place = step_place(a, x);
-        const bool newest = x == keys.p;                        // (its place in the cache is being written)
-        bulk_copy(dst + r * Shape::kPitch, newest ? kn : kc + place * a.kc_pos, bytes, bar);
-        bulk_copy(dst + (kMmaKeys + r) * Shape::kPitch, newest ? vn : vc + place * a.vc_pos, bytes, bar);
+  uint8_t* ring = smem + warp * Shape::kTiles * Shape::kTile;
+  const uint8_t* kc = (const uint8_t*)((const T*)a.kc + b * a.kc_seq + hk * a.kc_head);
+  const uint8_t* vc = (const uint8_t*)((const T*)a.vc + b * a.vc_seq + hk * a.vc_head);
+  const uint8_t* kn = (const uint8_t*)((const T*)a.k + b * a.k_row + hk * a.k_head);
+  const uint8_t* vn = (const uint8_t*)((const T*)a.v + b * a.v_row + hk * a.v_head);
+  auto fetch = [&](int i) {                                     // tile i of this warp, if there is one
+    const int t0 = t_begin + i * kRound + warp * kMmaRows;
+    if (t0 < t_end) {
+      const int x = keys.position(min(t0 + (lane & 15), t_end - 1));
+      const int where = t0 + (lane & 15) < t_end ? (x == keys.p ? -1 : step_place(a, x)) : -2;   // -1: the new row, -2: none
+      const uint32_t dst = smem_u32(ring + i % Shape::kTiles * Shape::kTile);
+      const int c = lane % kChunks;
+#pragma unroll
+      for (int it = 0; it < kMmaRows / kStep; ++it) {
+        const int r = it * kStep + lane / kChunks, place = __shfl_sync(0xffffffffu, where, r);
+        if (c >= 2 * ksteps) continue;                          // (zeros up to a multiple of 16 channels, and in rows there are none of)
+        const uint32_t bytes = place >= -1 && c < full ? 16u : 0u;
+        const uint8_t* k = place < 0 ? kn : kc + place * (a.kc_pos * 2);
+        const uint8_t* v = place < 0 ? vn : vc + place * (a.vc_pos * 2);
+        cp_async16(dst + r * Shape::kPitch + c * 16, bytes != 0 ? k + c * 16 : kn, bytes);
+        cp_async16(dst + (kMmaRows + r) * Shape::kPitch + c * 16, bytes != 0 ? v + c * 16 : vn, bytes);
       }
     }
-    if (!alive)
-      for (int it = 0; it < 64; ++it) __nanosleep(1000);        // (copies under way end before the CTA does)
-  } else {
-    // ---------------- products: 16 rows of every stage a warp ----------------
-    uint32_t q[KS][4];
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
 #pragma unroll
-    for (int k = 0; k < KS; ++k)
+  for (int i = 0; i < Shape::kTiles - 1; ++i) fetch(i);
+
+  uint32_t q[KS][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int g = g0 + (lane >> 2) + 8 * (e & 1), d = 16 * k + 2 * (lane & 3) + 8 * (e >> 1);
-        q[k][e] = g < group && d < a.dim
-                      ? *reinterpret_cast<const uint32_t*>((const T*)a.q + b * a.q_row + (hk * group + g) * a.q_head + d)
-                      : 0u;
-      }
-    bool alive = true;
-    for (int i = 0; i < count; ++i) {
-      const int s = i % Shape::kStages;
-      alive = mbar_wait(smem_u32(&full[s]), (i / Shape::kStages) & 1, &abort_flag, a.status, kErrStepFull);
-      alive = __all_sync(0xffffffffu, alive);
-      if (!alive) break;
-      const int t0 = t_begin + i * kMmaKeys + 16 * warp;
-      if (t0 < t_end) {
-        const uint32_t kb = smem_u32(smem + s * Shape::kStage) + 16 * warp * Shape::kPitch;
-        // K: tiles (8 rows, 8 channels): rows 0-7 and 8-15, channels 0-7 and 8-15 of each step
-        const uint32_t ka = kb + ((lane & 7) + ((lane >> 4) & 1) * 8) * Shape::kPitch + ((lane >> 3) & 1) * 16;
-        float sc[2][4] = {};
+  for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          if (k >= ksteps) break;
-          uint32_t f[4];
-          ldmatrix4(ka + 32 * k, f);
-          mma16816<HALF>(sc[0], q[k], f[0], f[1]);
-          mma16816<HALF>(sc[1], q[k], f[2], f[3]);
-        }
-        uint32_t w[4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {                            // query heads lane / 4 and lane / 4 + 8
-          float x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int t = t0 + 8 * (e >> 1) + 2 * (lane & 3) + (e & 1);
-            x[e] = t < t_end ? sc[e >> 1][2 * h + (e & 1)] * a.scale_log2 : -INFINITY;
-          }
-          float m = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          m = fmaxf(top[h], fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2)));
-          const float base = m == -INFINITY ? 0.f : m;
-          if (__any_sync(0xffffffffu, m != top[h])) {
-            const float keep = exp2_approx(top[h] - base);
-            top[h] = m;
-            total[h] *= keep;
-#pragma unroll
-            for (int n = 0; n < 2 * KS; ++n) {
-              o[n][2 * h] *= keep;
-              o[n][2 * h + 1] *= keep;
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = exp2_approx(x[e] - base);
-            total[h] += x[e];
-          }
-          // (rounded to the data's type for the product; the sum is of the unrounded values)
-          w[h] = pack2(x[0], x[1], HALF);
-          w[2 + h] = pack2(x[2], x[3], HALF);
-        }
-        // V: the same tiles read the other way
-        const uint32_t va = kb + kMmaKeys * Shape::kPitch + ((lane & 7) + ((lane >> 3) & 1) * 8) * Shape::kPitch +
-                            ((lane >> 4) & 1) * 16;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          if (k >= ksteps) break;
-          uint32_t f[4];
-          ldmatrix4t(va + 32 * k, f);
-          mma16816<HALF>(o[2 * k], w, f[0], f[1]);
-          mma16816<HALF>(o[2 * k + 1], w, f[2], f[3]);
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
+    for (int e = 0; e < 4; ++e) {
+      const int g = g0 + (lane >> 2) + 8 * (e & 1), d = 16 * k + 2 * (lane & 3) + 8 * (e >> 1);
+      q[k][e] = g < group && d < a.dim
+                    ? *reinterpret_cast<const uint32_t*>((const T*)a.q + b * a.q_row + (hk * group + g) * a.q_head + d)
+                    : 0u;
     }
+  float o[2 * KS][4] = {}, top[2] = {-INFINITY, -INFINITY}, total[2] = {};
+  for (int i = 0; t_begin + i * kRound < t_end; ++i) {
+    fetch(i + Shape::kTiles - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(Shape::kTiles - 1) : "memory");
+    __syncwarp();
+    const int t0 = t_begin + i * kRound + warp * kMmaRows;
+    if (t0 < t_end) {
+      const uint32_t kb = smem_u32(ring + i % Shape::kTiles * Shape::kTile);
+      float sc[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        if (k >= ksteps) break;
+        uint32_t f[4];
+        ldmatrix4(rows_frag(kb, Shape::kPitch) + 32 * k, f);
+        mma16816<HALF>(sc[0], q[k], f[0], f[1]);
+        mma16816<HALF>(sc[1], q[k], f[2], f[3]);
+      }
+      uint32_t w[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {                              // query heads lane / 4 and lane / 4 + 8
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = t0 + 8 * (e >> 1) + 2 * (lane & 3) + (e & 1);
+          x[e] = t < t_end ? sc[e >> 1][2 * h + (e & 1)] * a.scale_log2 : -INFINITY;
+        }
+        float m = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(top[h], fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2)));
+        const float base = m == -INFINITY ? 0.f : m;
+        if (__any_sync(0xffffffffu, m != top[h])) {
+          const float keep = exp2_approx(top[h] - base);
+          top[h] = m;
+          total[h] *= keep;
+#pragma unroll
+          for (int n = 0; n < 2 * KS; ++n) {
+            o[n][2 * h] *= keep;
+            o[n][2 * h + 1] *= keep;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = exp2_approx(x[e] - base);
+          total[h] += x[e];
+        }
+        // (rounded to the data's type for the product; the sum is of the unrounded values)
+        w[h] = pack2(x[0], x[1], HALF);
+        w[2 + h] = pack2(x[2], x[3], HALF);
+      }
+      const uint32_t vb = columns_frag(kb + kMmaRows * Shape::kPitch, Shape::kPitch);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        if (k >= ksteps) break;
+        uint32_t f[4];
+        ldmatrix4t(vb + 32 * k, f);
+        mma16816<HALF>(o[2 * k], w, f[0], f[1]);
+        mma16816<HALF>(o[2 * k + 1], w, f[2], f[3]);
+      }
+    }
+    __syncwarp();                                               // (the tile is read: the next copies may go there)
   }
-  // ---------------- the warps' parts, in the stages' place ----------------
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  // ---------------- the warps' parts, in the rings' place ----------------
   __syncthreads();
   float* so = reinterpret_cast<float*>(smem);                   // [warp][head][DP], then maxima and sums
   float* sm = so + kMmaWarps * kMmaHeads * DP;
   float* sl = sm + kMmaWarps * kMmaHeads;
-  if (warp < kMmaWarps) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int head = (lane >> 2) + 8 * h;
-      float l = total[h];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      if ((lane & 3) == 0) {
-        sm[warp * kMmaHeads + head] = top[h];
-        sl[warp * kMmaHeads + head] = l;
-      }
-#pragma unroll
-      for (int n = 0; n < 2 * KS; ++n)
-        *reinterpret_cast<float2*>(so + (warp * kMmaHeads + head) * DP + 8 * n + 2 * (lane & 3)) =
-            make_float2(o[n][2 * h], o[n][2 * h + 1]);
+  for (int h = 0; h < 2; ++h) {
+    const int head = (lane >> 2) + 8 * h;
+    float l = total[h];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if ((lane & 3) == 0) {
+      sm[warp * kMmaHeads + head] = top[h];
+      sl[warp * kMmaHeads + head] = l;
     }
+#pragma unroll
+    for (int n = 0; n < 2 * KS; ++n)
+      *reinterpret_cast<float2*>(so + (warp * kMmaHeads + head) * DP + 8 * n + 2 * (lane & 3)) =
+          make_float2(o[n][2 * h], o[n][2 * h + 1]);
   }
   __syncthreads();
   const int heads = min(kMmaHeads, group - g0);
@@ -467,12 +414,11 @@ __global__ void __launch_bounds__(32 * (kMmaWarps + 1)) attn_step_mma_kernel(con
     ((T*)a.out)[((long long)b * a.heads + hk * group + g0 + head) * a.dim + d] = from_f32<T>(y);
   }
   if (part == 0 && g0 == 0 && keys.live && tid < a.dim / 4) {   // the new row: dim / 8 pieces of K, then of V
-    const int piece = tid % (a.dim / 8) * 8, place = step_place(a, keys.p);
-    const bool v = tid >= a.dim / 8;
-    T* dst = (v ? (T*)a.vc + b * a.vc_seq + place * a.vc_pos + hk * a.vc_head
-                : (T*)a.kc + b * a.kc_seq + place * a.kc_pos + hk * a.kc_head) + piece;
-    const T* src = (v ? (const T*)a.v + b * a.v_row + hk * a.v_head : (const T*)a.k + b * a.k_row + hk * a.k_head) + piece;
-    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+    const int piece = tid % full * 16, place = step_place(a, keys.p);
+    const bool v = tid >= full;
+    uint8_t* dst = (v ? (uint8_t*)((T*)a.vc + b * a.vc_seq + place * a.vc_pos + hk * a.vc_head)
+                      : (uint8_t*)((T*)a.kc + b * a.kc_seq + place * a.kc_pos + hk * a.kc_head)) + piece;
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>((v ? vn : kn) + piece);
   }
   if (parts > 1) cluster.sync();                                // (no CTA leaves while its shared memory is read)
 }
@@ -483,22 +429,22 @@ int step_mma_launch(const StepArgs& a, int parts, cudaStream_t st) {
   static PerDeviceOnce once;
   const int status = once.run([&]() -> int {
     OCNN_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    OCNN_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)StepShape<DP>::smem()));
+    OCNN_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, StepShape<DP>::kBytes));
     return OCNN_OK;
   });
   if (status != OCNN_OK) return status;
   const int chunks = ceil_div(a.heads / a.kv_heads, kMmaHeads);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(parts, a.kv_heads * chunks, a.batch);
-  cfg.blockDim = dim3(32 * (kMmaWarps + 1));
-  cfg.dynamicSmemBytes = StepShape<DP>::smem();
+  cfg.blockDim = dim3(32 * kMmaWarps);
+  cfg.dynamicSmemBytes = StepShape<DP>::kBytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = parts;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
   OCNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, a));
   OCNN_LAUNCH_OK("attn_step_mma_kernel");
   return OCNN_OK;
@@ -565,7 +511,7 @@ using namespace ocnn;
 extern "C" int ocnn_octree_attention_step(const ocnn_attention_cache* c, const void* q_dev, const int64_t q_stride[2],
                                           const void* k_dev, const int64_t k_stride[2], const void* v_dev,
                                           const int64_t v_stride[2], void* out_dev, int heads, int window, int sinks,
-                                          float scale, int32_t* status_dev, void* stream) {
+                                          float scale, void* stream) {
   OCNN_REQUIRE(c != nullptr && c->batch >= 0 && c->capacity >= 1 && c->kv_heads >= 1 && c->dim >= 1,
                "ocnn_octree_attention_step: bad cache");
   OCNN_REQUIRE(c->dtype >= OCNN_F32 && c->dtype <= OCNN_F16, "ocnn_octree_attention_step: bad dtype %d", c->dtype);
@@ -577,7 +523,7 @@ extern "C" int ocnn_octree_attention_step(const ocnn_attention_cache* c, const v
     return fail(OCNN_ERR_UNSUPPORTED, "ocnn_octree_attention_step: heads of %d channels (multiples of 16 bytes up to %d)",
                 c->dim, kMaxHeadDim);
   if (c->batch == 0) return OCNN_OK;
-  OCNN_REQUIRE(q_dev && k_dev && v_dev && out_dev && c->k_dev && c->v_dev && c->lengths_dev && status_dev,
+  OCNN_REQUIRE(q_dev && k_dev && v_dev && out_dev && c->k_dev && c->v_dev && c->lengths_dev,
                "ocnn_octree_attention_step: null pointer");
   OCNN_REQUIRE(on16(q_dev, {q_stride[0], q_stride[1]}, size) && on16(k_dev, {k_stride[0], k_stride[1]}, size) &&
                    on16(v_dev, {v_stride[0], v_stride[1]}, size) &&
@@ -597,14 +543,12 @@ extern "C" int ocnn_octree_attention_step(const ocnn_attention_cache* c, const v
   a.sinks = window == 0 ? 0 : sinks;
   a.rolls = window > 0 && (long long)window + sinks <= c->capacity;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.status = status_dev;
-  // CTAs per sequence and key head: until the GPU has two per SM (each keeps a ring of stages full; fp32: four, with eight
-  // warps of loads), as long as each still has 64 rows to read.
+  // CTAs per sequence and key head: until the GPU has four per SM, as long as each still has 64 rows to read.
   const bool f32 = c->dtype == OCNN_F32;
   const long long pairs = (long long)a.batch * a.kv_heads;
   const long long most = a.rolls ? (long long)window + sinks : c->capacity;
   int parts = 1;
-  while (parts < 16 && pairs * parts < (f32 ? 4LL : 2LL) * sm_count() && most >= 2LL * parts * 64) parts *= 2;
+  while (parts < 16 && pairs * parts < 4LL * sm_count() && most >= 2LL * parts * 64) parts *= 2;
   cudaStream_t st = (cudaStream_t)stream;
   if (f32) return step_by_width<float>(a, parts, st);
   return c->dtype == OCNN_F16 ? step_mma_by_width<true>(a, parts, st) : step_mma_by_width<false>(a, parts, st);

@@ -641,7 +641,7 @@ int grad_launch(GradArgs& p, cudaStream_t st) {
   dq<<<dim3(ceil_div(a.n, W * 128 >> p.pack_log), a.heads >> p.pack_log), Dq::kThreads, Dq::smem(stages_q), st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_dq_kernel");
   if (p.a.sinks > 0) {
-    const int far = attn_far_sums(p.a, p.g, HALF ? OCNN_F16 : OCNN_BF16, st);
+    const int far = attn_far_mma(p.a, p.g, HALF ? OCNN_F16 : OCNN_BF16, st);
     if (far != OCNN_OK) return far;
   }
   status = queries(kBN);

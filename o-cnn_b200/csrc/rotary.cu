@@ -41,7 +41,7 @@ __device__ __forceinline__ void rot_set(__half& y, float x) { y = __float2half(x
 // An item is V pairs of one head of one node.  Pairs side by side: two runs of V channels, half a head apart;
 // interleaved: one run of 2V channels (as two packs).
 template <typename T, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kRotThreads, 4) rotary_kernel(const RotaryArgs a) {
   extern __shared__ float2 turn[];          // [rows_per_block][pairs]
   const long long r0 = (long long)blockIdx.x * a.rows_per_block;
   const int rows = (int)min((long long)a.rows_per_block, a.rows - r0);
@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a)
     const T* src = (const T*)a.x + (r0 + mine) * a.row + h * a.head + c;
     T* dst = (T*)a.y + ((r0 + mine) * a.heads + h) * a.dim + c;
     const long long src_step = step * a.row, dst_step = (long long)step * a.heads * a.dim;
-    constexpr int U = 4;
+    constexpr int U = 2;
     for (int r = mine; r < rows; r += U * step) {
       Pack<T, V> lo[U], hi[U];
 #pragma unroll

@@ -380,7 +380,7 @@ Tensor octree_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, 
   OCNN_CALL(ocnn_octree_attention_step(&c, qr.data_ptr(), qs, kr.data_ptr(), ks, vr.data_ptr(), vs, out.data_ptr(),
                                        (int)q.size(1), (int)window, (int)sinks,
                                        (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)dim)),
-                                       ocnn_tc_status(q.device()).data_ptr<int32_t>(), current_stream()));
+                                       current_stream()));
   for (const Tensor* t : {&k_cache, &v_cache})
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return out;
