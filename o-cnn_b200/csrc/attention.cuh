@@ -73,27 +73,38 @@ __device__ __forceinline__ Span attn_span(const AttnArgs& a, int i) {
   return s;
 }
 
-// The same by a whole warp, which looks at 32 offsets at a time (a search node by node is a chain of loads).
-__device__ __forceinline__ Span attn_span_warp(const AttnArgs& a, int i) {
-  const int lane = threadIdx.x & 31;
-  int first = 0, step = 1, left = a.batch + 1;            // candidates first, first + step, ...
-  while (step * 32 < left) step *= 32;
-  int last = 0;
-  for (;; step /= 32) {
-    const int b = first + lane * step;
-    const unsigned under = __ballot_sync(0xffffffffu, b <= a.batch && attn_offset(a, min(b, a.batch)) <= i);
-    last = under == 0 ? first : first + (31 - __clz(under)) * step;
-    if (step == 1) break;
-    first = last;
+// The same by whole warps, for several nodes: a warp reads the offsets once, a lane each (a search node by node is a chain of
+// loads); of more than 32 it keeps every step-th and looks at 32 at a time from there.
+struct WarpOffsets {
+  int mine, step;                                        // offset of sequence lane * step, clamped
+  __device__ __forceinline__ explicit WarpOffsets(const AttnArgs& a) {
+    step = 1;
+    while (step * 32 < a.batch + 1) step *= 32;
+    const int b = (threadIdx.x & 31) * step;
+    mine = b <= a.batch ? attn_offset(a, b) : INT_MAX;
   }
-  Span s = {0, 0, last};
-  if (i >= a.n || last >= a.batch) return s;
-  const int start = attn_offset(a, last), end = attn_offset(a, last + 1);
-  if (i < start || i >= end) return s;
-  s.start = start;
-  s.end = end;
-  return s;
-}
+  __device__ __forceinline__ int begin() const { return __shfl_sync(0xffffffffu, mine, 0); }
+  __device__ __forceinline__ int end(const AttnArgs& a) const {
+    return step == 1 ? __shfl_sync(0xffffffffu, mine, a.batch) : attn_offset(a, a.batch);
+  }
+  __device__ __forceinline__ Span span(const AttnArgs& a, int i) const {
+    unsigned under = __ballot_sync(0xffffffffu, mine <= i);
+    int last = under == 0 ? 0 : (31 - __clz(under)) * step;
+    for (int s = step / 32; s >= 1; s /= 32) {
+      const int b = last + (threadIdx.x & 31) * s;
+      under = __ballot_sync(0xffffffffu, b <= a.batch && attn_offset(a, min(b, a.batch)) <= i);
+      last = under == 0 ? last : last + (31 - __clz(under)) * s;
+    }
+    Span s = {0, 0, last};
+    if (i >= a.n || last >= a.batch) return s;
+    const int start = step == 1 ? __shfl_sync(0xffffffffu, mine, last) : attn_offset(a, last);
+    const int end = step == 1 ? __shfl_sync(0xffffffffu, mine, last + 1) : attn_offset(a, last + 1);
+    if (i < start || i >= end) return s;
+    s.start = start;
+    s.end = end;
+    return s;
+  }
+};
 // Node i's, where the nodes of a tile are known to lie between those of spans f and l.
 __device__ __forceinline__ Span attn_span_near(const AttnArgs& a, int i, const Span& f, const Span& l) {
   if (i >= f.start && i < f.end) return f;
@@ -276,35 +287,28 @@ __device__ void attn_dkv_row(const AttnArgs& a, const AttnGrad& g, int j, int hk
 // ---- first nodes seen from far behind -----------------------------------------------------------------------
 // What the nodes behind the window add to the gradients of their sequence's first nodes comes from all over the
 // sequence.  It is summed in blocks of kFarRows nodes, each block's share of a sequence in a slot of its own, and the
-// kernel that writes the keys' gradients adds the slots in order: no atomics, the same bits every time.  Slot = block +
+// slots are added up in order: no atomics, the same bits every time.  Slot = block +
 // sequence: along the packed batch either the block or the sequence moves on, so no two pairs share one.
 constexpr int kFarRows = 256;
 inline int far_slots(int n, int batch) { return ceil_div(n, kFarRows) + batch; }
 __device__ __forceinline__ float* far_slot(const AttnArgs& a, const AttnGrad& g, int slot, int hk, int sink) {
   return g.far + (((long long)slot * a.kv_heads + hk) * a.sinks + sink) * (2 * a.dim);
 }
-// The slots of key j: first, step between slots and their number (0 for a key that nobody sees from far).
-struct FarSums {
-  const float* at;
-  long long step;
-  int count;
-  // of dK's channel d, and of dV's at dim + d
-  __device__ __forceinline__ float sum(int d) const {
-    float x = 0.f;
-    for (int s = 0; s < count; ++s) x += at[s * step + d];
-    return x;
-  }
-};
-__device__ __forceinline__ FarSums far_sums(const AttnArgs& a, const AttnGrad& g, int j, int hk) {
-  FarSums f = {nullptr, 0, 0};
-  if (a.sinks == 0) return f;
-  const Span s = attn_span(a, j);
-  if (j - s.start >= a.sinks || s.end - j <= a.window || (a.mask != nullptr && a.mask[j] == 0)) return f;
+// Key j's slots: the first one's number, and how many there are (0: nobody sees it from far).  A kernel of their own adds
+// them up into the first, which the gradients' kernel reads.
+struct FarSlots { int first, count; };
+__device__ __forceinline__ FarSlots far_slots_of(const AttnArgs& a, int j, const Span& s) {
+  if (j - s.start >= a.sinks || s.end - j <= a.window || (a.mask != nullptr && a.mask[j] == 0)) return {0, 0};
   const int first = (j + a.window) / kFarRows;
-  f.at = far_slot(a, g, first + s.seq, hk, j - s.start);
-  f.step = (long long)a.kv_heads * a.sinks * 2 * a.dim;
-  f.count = (s.end - 1) / kFarRows - first + 1;
-  return f;
+  return {first + s.seq, (s.end - 1) / kFarRows - first + 1};
 }
+// The sums of dK's channels for key j, then of dV's; NULL where nobody sees it from far.
+__device__ __forceinline__ const float* far_sums(const AttnArgs& a, const AttnGrad& g, int j, int hk) {
+  if (a.sinks == 0) return nullptr;
+  const Span s = attn_span(a, j);
+  const FarSlots f = far_slots_of(a, j, s);
+  return f.count > 0 ? far_slot(a, g, f.first, hk, j - s.start) : nullptr;
+}
+int attn_far_join(const AttnArgs& a, const AttnGrad& g, cudaStream_t st);
 
 }  // namespace ocnn

@@ -201,7 +201,39 @@ int far_mma_by_width(const AttnArgs& a, const AttnGrad& g, cudaStream_t st) {
   return far_mma_launch<HALF, 128>(a, g, st);
 }
 
+// Adds a first node's slots up into the first of them: a block per sequence, key head and first node; its threads are runs
+// of slots x channels.
+constexpr int kJoinThreads = 512;
+__global__ void __launch_bounds__(kJoinThreads) attn_far_join_kernel(const AttnArgs a, const AttnGrad g) {
+  __shared__ float part[kJoinThreads];
+  const int b = blockIdx.x, hk = blockIdx.y, t = blockIdx.z, width = 2 * a.dim, runs = kJoinThreads / width;
+  const Span s = {attn_offset(a, b), attn_offset(a, b + 1), b};
+  const int j = s.start + t;
+  if (j >= s.end) return;
+  const FarSlots f = far_slots_of(a, j, s);
+  if (f.count < 2) return;
+  const int run = threadIdx.x / width, e = threadIdx.x - run * width;
+  float x = 0.f;
+  if (run < runs) {
+#pragma unroll 8
+    for (int k = run; k < f.count; k += runs) x += far_slot(a, g, f.first + k, hk, t)[e];
+  }
+  part[threadIdx.x] = x;
+  __syncthreads();
+  if (run == 0) {
+    for (int k = 1; k < runs; ++k) x += part[k * width + e];
+    far_slot(a, g, f.first, hk, t)[e] = x;
+  }
+}
+
 }  // namespace
+
+int attn_far_join(const AttnArgs& a, const AttnGrad& g, cudaStream_t st) {
+  if (a.batch == 0) return OCNN_OK;
+  attn_far_join_kernel<<<dim3(a.batch, a.kv_heads, a.sinks), kJoinThreads, 0, st>>>(a, g);
+  OCNN_LAUNCH_OK("attn_far_join_kernel");
+  return OCNN_OK;
+}
 
 int attn_far_mma(const AttnArgs& a, const AttnGrad& g, int dtype, cudaStream_t st) {
   return dtype == OCNN_F16 ? far_mma_by_width<true>(a, g, st) : far_mma_by_width<false>(a, g, st);

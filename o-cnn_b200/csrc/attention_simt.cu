@@ -380,14 +380,14 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int j = k0 + 4 * ty + r;
-    const FarSums far = j < a.n ? far_sums(a, g, j, hk) : FarSums{nullptr, 0, 0};
+    const float* far = j < a.n ? far_sums(a, g, j, hk) : nullptr;
     bool bad = false;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const int d = out_col<DP>(c);
       bad |= not_finite(dk[r][c]) | not_finite(dv[r][c]);
       if (j >= a.n || d >= a.dim) continue;
-      const float x = dk[r][c] + far.sum(d), y = dv[r][c] + far.sum(a.dim + d);
+      const float x = dk[r][c] + (far != nullptr ? far[d] : 0.f), y = dv[r][c] + (far != nullptr ? far[a.dim + d] : 0.f);
       ((T*)g.dk)[((long long)j * a.kv_heads + hk) * a.dim + d] = from_f32<T>(x * a.scale);
       ((T*)g.dv)[((long long)j * a.kv_heads + hk) * a.dim + d] = from_f32<T>(y);
     }
@@ -553,7 +553,8 @@ int backward_launch(const AttnArgs& a, const AttnGrad& g, bool vec, cudaStream_t
   attn_simt_dq_kernel<T, DP><<<dim3(ceil_div(a.n, kB), a.heads), kThreads, dq_bytes, st>>>(a, g, vec);
   OCNN_LAUNCH_OK("attn_simt_dq_kernel");
   if (a.sinks > 0) {
-    const int far = far_launch<T>(a, g, st);
+    int far = far_launch<T>(a, g, st);
+    if (far == OCNN_OK) far = attn_far_join(a, g, st);
     if (far != OCNN_OK) return far;
   }
   attn_simt_dkv_kernel<T, DP><<<dim3(ceil_div(a.n, kB), a.kv_heads), kThreads, dkv_bytes, st>>>(a, g, vec);

@@ -87,13 +87,14 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 4 * W) tmem_alloc(tmem_holder, Shape::kCols);
+  const WarpOffsets offsets(a);
   Span f, l;
-  const TileKeys tile_keys = attn_tile_keys(a, r0, r0 + W * nodes, f, l);
+  const TileKeys tile_keys = attn_tile_keys(a, offsets, r0, r0 + W * nodes, f, l);
   const KeyBlocks<BN> keys(tile_keys);
   const int blocks = keys.count;
   if (W > 1 && warp < W) {
     Span x, y;
-    const BlockRange r = block_range<BN>(keys, attn_tile_keys(a, r0 + warp * nodes, r0 + (warp + 1) * nodes, x, y));
+    const BlockRange r = block_range<BN>(keys, attn_tile_keys(a, offsets, r0 + warp * nodes, r0 + (warp + 1) * nodes, x, y));
     if (lane == 0) ranges[warp] = r;
   }
   tc_fence_before();
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   auto active = [&](int t, int b) { return W == 1 || in_range(ranges[t], b); };
-  const int ksteps = (a.dim + 15) / 16, end = batch_end(a);
+  const int ksteps = (a.dim + 15) / 16, end = min(a.n, offsets.end(a));
   const bool cleared = a.mask != nullptr || (end < a.n && keys.reaches(end));   // (see clear_rows)
 
   if (warp < 4 * W) {
@@ -110,6 +111,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
     const uint32_t quarter = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * Shape::kAcc, acc = quarter + 2 * BN;
     const int i = r0 + t * nodes + (row >> p.pack_log), h = h0 + (row & (pack - 1));
     const RowKeys r = i < a.n ? attn_row_keys(a, i, attn_span_near(a, i, f, l)) : RowKeys{0, 0, 0, 0};
+    const FullBlocks whole(keys, r, a.mask != nullptr, std::integral_constant<int, BN>());
     const float c = a.scale_log2;
     const uint64_t c2 = pair(c, c);
     float ref = -INFINITY, total = 0.f;                                    // the reference, in powers of two
@@ -119,9 +121,8 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
       if (!active(t, b)) continue;
       const int place = done & 1, j = keys.key(b);
       const uint32_t lanes = quarter + place * BN;
-      // does every row of the warp see every key?
       const bool first = keys.is_first(b);
-      const bool all = a.mask == nullptr && !first && __all_sync(0xffffffffu, r.lo <= j && j + BN <= r.hi);
+      const bool all = whole.has(b);
       uint32_t bits[BN / 32];
       if (!all) {
 #pragma unroll

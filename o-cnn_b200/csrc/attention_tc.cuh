@@ -135,13 +135,13 @@ inline int attn_map(CUtensorMap* map, const void* base, int dtype, int dim, int 
 // ---- the keys of a tile of queries ------------------------------------------------------------------------------
 // The keys that the nodes [r0, r1) see between them (TileKeys), by a whole warp.  Windows move on with the nodes, so the
 // first and the last node that are in a sequence say it all; their sequences go to f and l.
-__device__ __forceinline__ TileKeys attn_tile_keys(const AttnArgs& a, int r0, int r1, Span& f, Span& l) {
+__device__ __forceinline__ TileKeys attn_tile_keys(const AttnArgs& a, const WarpOffsets& offsets, int r0, int r1, Span& f, Span& l) {
   TileKeys t = {0, 0, 0, 0};
-  const int x = max(r0, attn_offset(a, 0)), y = min(min(r1, a.n), attn_offset(a, a.batch)) - 1;
+  const int x = max(r0, offsets.begin()), y = min(min(r1, a.n), offsets.end(a)) - 1;
   f = l = Span{0, 0, 0};
   if (x > y) return t;
-  f = attn_span_warp(a, x);
-  l = y < f.end ? f : attn_span_warp(a, y);
+  f = offsets.span(a, x);
+  l = y < f.end ? f : offsets.span(a, y);
   const RowKeys rx = attn_row_keys(a, x, f), ry = attn_row_keys(a, y, l);
   t.lo = rx.lo;
   if (a.sinks > 0) {
@@ -201,8 +201,18 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, Kept kept) {
     }
   }
 }
-// Where the last sequence ends; what lies behind is nobody's.
-__device__ __forceinline__ int batch_end(const AttnArgs& a) { return min(a.n, attn_offset(a, a.batch)); }
+// Blocks [from, to) of the windows' interval of which every row of the warp sees every key.
+struct FullBlocks {
+  int from, to;
+  template <int BN>
+  __device__ __forceinline__ FullBlocks(const KeyBlocks<BN>& k, const RowKeys& r, bool masked, std::integral_constant<int, BN>) {
+    const int lo = __reduce_max_sync(0xffffffffu, r.lo), hi = __reduce_min_sync(0xffffffffu, r.hi);
+    const int shift = k.n_first > 0;
+    from = shift + (max(lo - k.lo, 0) + BN - 1) / BN;
+    to = masked || hi <= k.lo ? 0 : shift + (hi - k.lo) / BN;
+  }
+  __device__ __forceinline__ bool has(int b) const { return b >= from && b < to; }
+};
 
 // Which blocks a tile of several that share their copies needs: an interval, those of first nodes that lie in the shared
 // interval but not in its own, and the block of first nodes.

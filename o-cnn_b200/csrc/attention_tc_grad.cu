@@ -80,13 +80,14 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 4 * W) tmem_alloc(tmem_holder, Shape::kCols);
+  const WarpOffsets offsets(a);
   Span f, l;
-  const TileKeys tile_keys = attn_tile_keys(a, r0, r0 + W * nodes, f, l);
+  const TileKeys tile_keys = attn_tile_keys(a, offsets, r0, r0 + W * nodes, f, l);
   const KeyBlocks<kBN> keys(tile_keys);
   const int blocks = keys.count;
   if (W > 1 && warp < W) {
     Span x, y;
-    const BlockRange r = block_range<kBN>(keys, attn_tile_keys(a, r0 + warp * nodes, r0 + (warp + 1) * nodes, x, y));
+    const BlockRange r = block_range<kBN>(keys, attn_tile_keys(a, offsets, r0 + warp * nodes, r0 + (warp + 1) * nodes, x, y));
     if (lane == 0) ranges[warp] = r;
   }
   tc_fence_before();
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   auto active = [&](int t, int b) { return W == 1 || in_range(ranges[t], b); };
-  const int ksteps = (a.dim + 15) / 16, end = batch_end(a);
+  const int ksteps = (a.dim + 15) / 16, end = min(a.n, offsets.end(a));
   const bool cleared = a.mask != nullptr || (end < a.n && keys.reaches(end));   // (see clear_rows)
 
   if (warp < 4 * W) {
@@ -121,6 +122,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       }
       p.g.delta[(long long)h * a.n + i] = delta;
     }
+    const FullBlocks whole(keys, r, a.mask != nullptr, std::integral_constant<int, kBN>());
     const uint64_t c2 = pair(a.scale_log2, a.scale_log2), lse2 = pair(-lse, -lse), delta2 = pair(-delta, -delta);
     int done = 0;
     bool alive = true;
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       if (!active(t, b)) continue;
       const int j = keys.key(b);
       const bool first = keys.is_first(b);
-      const bool all = a.mask == nullptr && !first && __all_sync(0xffffffffu, r.lo <= j && j + kBN <= r.hi);
+      const bool all = whole.has(b);
       uint32_t bits[2];
       if (!all) {
 #pragma unroll
@@ -302,12 +304,12 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
 
 // The nodes that see the keys [k0, k1) from within the window, whatever the mask says, by a whole warp; f and l: the
 // sequences of the first and the last key that is in one.
-__device__ __forceinline__ KeyRows attn_tile_rows(const AttnArgs& a, int k0, int k1, Span& f, Span& l) {
-  const int x = max(k0, attn_offset(a, 0)), y = min(min(k1, a.n), attn_offset(a, a.batch)) - 1;
+__device__ __forceinline__ KeyRows attn_tile_rows(const AttnArgs& a, const WarpOffsets& offsets, int k0, int k1, Span& f, Span& l) {
+  const int x = max(k0, offsets.begin()), y = min(min(k1, a.n), offsets.end(a)) - 1;
   f = l = Span{0, 0, 0};
   if (x > y) return KeyRows{0, 0};
-  f = attn_span_warp(a, x);
-  l = y < f.end ? f : attn_span_warp(a, y);
+  f = offsets.span(a, x);
+  l = y < f.end ? f : offsets.span(a, y);
   return KeyRows{attn_rows_of_key(a, x, f).lo, attn_rows_of_key(a, y, l).hi};
 }
 
@@ -363,8 +365,9 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 4 * G) tmem_alloc(tmem_holder, Shape::kCols);
+  const WarpOffsets offsets(a);
   Span f, l;
-  const KeyRows span = attn_tile_rows(a, k0, k0 + 128, f, l);
+  const KeyRows span = attn_tile_rows(a, offsets, k0, k0 + 128, f, l);
   const int pack = 1 << p.pack_log, nodes = kBN >> p.pack_log;             // nodes of a block
   const int per_head = (max(0, span.hi - span.lo) + nodes - 1) >> (6 - p.pack_log);   // blocks of `pack` heads
   const int blocks = per_head * (group >> p.pack_log);
@@ -373,7 +376,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
   constexpr int kAcc = G * 2 * kBN;                                        // dK, then dV
-  const int ksteps = (a.dim + 15) / 16, end = batch_end(a);
+  const int ksteps = (a.dim + 15) / 16, end = min(a.n, offsets.end(a));
   const bool cleared = end < a.n && span.hi == end;                        // (its last block holds nobody's nodes)
   // (blocks go head by head: no division where there is only one run of them)
   auto run_of = [&](int b) { return b < per_head ? 0 : b / per_head; };
@@ -469,7 +472,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
     tc_fence_after();
     if (alive) {
       const bool in = j < a.n;
-      const FarSums far = in ? far_sums(a, p.g, j, hk) : FarSums{nullptr, 0, 0};
+      const float* far = in ? far_sums(a, p.g, j, hk) : nullptr;
       // group 0 writes dK, the last one dV (both, where there is one)
 #pragma unroll 1
       for (int which = t == 0 ? 0 : 1; which <= (t == G - 1 ? 1 : 0); ++which) {
@@ -483,10 +486,10 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
             tmem_ld16(quarter + kAcc + which * DP + d, reinterpret_cast<uint32_t(&)[16]>(x));
             tmem_wait_ld();
           }
-          if (far.count > 0) {
+          if (far != nullptr) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              if (d + e < a.dim) x[e] += far.sum(which * a.dim + d + e);
+              if (d + e < a.dim) x[e] += far[which * a.dim + d + e];
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -643,6 +646,8 @@ int grad_launch(GradArgs& p, cudaStream_t st) {
   if (p.a.sinks > 0) {
     const int far = attn_far_mma(p.a, p.g, HALF ? OCNN_F16 : OCNN_BF16, st);
     if (far != OCNN_OK) return far;
+    const int joined = attn_far_join(p.a, p.g, st);
+    if (joined != OCNN_OK) return joined;
   }
   status = queries(kBN);
   if (status != OCNN_OK) return status;
