@@ -22,41 +22,42 @@ struct AttnFwdArgs {
   void* out;
   float* lse;
   int* status;
-  int pack_log, slots, wide;
+  int pack_log, stages, wide;
 };
 
 enum : int { kErrAttnQ = 11, kErrAttnLoad = 12, kErrAttnSlot = 13, kErrAttnP = 14, kErrAttnS = 15, kErrAttnO = 16 };
 
-constexpr int kMaxSlots = 8;
+constexpr int kMaxStages = 6;
 
-template <int DP, int W, int BN>
+// NB: places for a tile's scores (1: none ahead of its rows; more CTAs per SM cover the wait).
+template <int DP, int W, int BN, int NB>
 struct FwdShape {
   static constexpr int kThreads = 160 * W + 32;                          // rows, products, copies
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTileQ = 128 * kRowBytes * kPieces;
-  static constexpr int kSlot = BN * kRowBytes * kPieces;
-  static constexpr int kAcc = 2 * BN + DP;                               // two places for S, and O
+  static constexpr int kBlock = BN * kRowBytes * kPieces;                // K, then V
+  static constexpr int kAcc = NB * BN + DP;                              // places for S, and O
   static constexpr int kCols = W * kAcc <= 128 ? 128 : W * kAcc <= 256 ? 256 : 512;
-  static constexpr size_t smem(int slots) { return (size_t)W * kTileQ + (size_t)slots * kSlot + 1024 + 512; }
+  static constexpr size_t smem(int stages) { return (size_t)W * kTileQ + (size_t)stages * 2 * kBlock + 1024 + 512; }
 };
 
-template <int DP, int W, int BN, bool HALF, int CTAS>
-__global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
+template <int DP, int W, int BN, int NB, bool HALF, int CTAS>
+__global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
     attn_tc_kernel(const __grid_constant__ AttnFwdArgs p) {
-  using Shape = FwdShape<DP, W, BN>;
+  using Shape = FwdShape<DP, W, BN, NB>;
   using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
   const AttnArgs& a = p.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sq = smem;
   uint8_t* skv = sq + W * Shape::kTileQ;
-  uint64_t* full = reinterpret_cast<uint64_t*>(skv + p.slots * Shape::kSlot);
-  uint64_t* empty = full + kMaxSlots;
-  uint64_t* clean = empty + kMaxSlots;                                     // (the slot's rows are cleared)
-  uint64_t* qfull = clean + kMaxSlots;
+  uint64_t* full = reinterpret_cast<uint64_t*>(skv + p.stages * 2 * Shape::kBlock);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* clean = empty + kMaxStages;                                     // (the slot's rows are cleared)
+  uint64_t* qfull = clean + kMaxStages;
   uint64_t* sfull = qfull + 1;                                             // [tile][place]
-  uint64_t* pfull = sfull + 2 * W;
-  uint64_t* pvdone = pfull + 2 * W;
+  uint64_t* pfull = sfull + NB * W;
+  uint64_t* pvdone = pfull + NB * W;
   uint64_t* ofull = pvdone + W;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(ofull + W);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
@@ -69,16 +70,16 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
   const int hk = blockIdx.y / per_kv, h0 = hk * group + (blockIdx.y % per_kv) * pack;
 
   if (tid == 0) {
-    for (int s = 0; s < p.slots; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
       mbar_init(smem_u32(&empty[s]), W);
       mbar_init(smem_u32(&clean[s]), 1);
     }
     mbar_init(smem_u32(qfull), 1);
     for (int t = 0; t < W; ++t) {
-      for (int k = 0; k < 2; ++k) {
-        mbar_init(smem_u32(&sfull[2 * t + k]), 1);
-        mbar_init(smem_u32(&pfull[2 * t + k]), 128);
+      for (int k = 0; k < NB; ++k) {
+        mbar_init(smem_u32(&sfull[NB * t + k]), 1);
+        mbar_init(smem_u32(&pfull[NB * t + k]), 128);
       }
       mbar_init(smem_u32(&pvdone[t]), 1);
       mbar_init(smem_u32(&ofull[t]), 1);
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
   if (warp < 4 * W) {
     // ---------------- rows ----------------
     const int t = warp >> 2, row = tid & 127;
-    const uint32_t quarter = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * Shape::kAcc, acc = quarter + 2 * BN;
+    const uint32_t quarter = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * Shape::kAcc, acc = quarter + NB * BN;
     const int i = r0 + t * nodes + (row >> p.pack_log), h = h0 + (row & (pack - 1));
     const RowKeys r = i < a.n ? attn_row_keys(a, i, attn_span_near(a, i, f, l)) : RowKeys{0, 0, 0, 0};
     const FullBlocks whole(keys, r, a.mask != nullptr, std::integral_constant<int, BN>());
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
     bool alive = true;
     for (int b = 0; b < blocks && alive; ++b) {
       if (!active(t, b)) continue;
-      const int place = done & 1, j = keys.key(b);
+      const int place = done % NB, j = keys.key(b);
       const uint32_t lanes = quarter + place * BN;
       const bool first = keys.is_first(b);
       const bool all = whole.has(b);
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
           if (a.mask != nullptr) bits[k] &= kept_bits(a, j + 32 * k, a.n);
         }
       }
-      alive = mbar_wait(smem_u32(&sfull[2 * t + place]), (done >> 1) & 1, abort_flag, p.status, kErrAttnS);
+      alive = mbar_wait(smem_u32(&sfull[NB * t + place]), (done / NB) & 1, abort_flag, p.status, kErrAttnS);
       alive = __all_sync(0xffffffffu, alive);
       if (!alive) break;
       tc_fence_after();
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
       total = sum.x + sum.y;
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(smem_u32(&pfull[2 * t + place]));
+      mbar_arrive(smem_u32(&pfull[NB * t + place]));
       ++done;
     }
     // ---------------- O / sum ----------------
@@ -234,50 +235,45 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
       const uint32_t idesc_s = attn_idesc<HALF>(BN, false), idesc_o = attn_idesc<HALF>(16 * ksteps, true);
       const uint32_t q = smem_u32(sq + t * Shape::kTileQ), kv = smem_u32(skv), d = tmem + t * Shape::kAcc;
       uint64_t* ready = cleared ? clean : full;
-      // K of block b lies in slot 2 b, V in slot 2 b + 1, modulo the ring
-      int ks = 0, vs = 1, scored = 0, n = 0;
-      uint32_t kp = 0, vp = 0;
-      auto on = [&](int& slot, uint32_t& phase) {
-        slot += 2;
-        if (slot >= p.slots) {
-          slot -= p.slots;
-          phase ^= 1u;
-        }
-      };
+      BlockRange range;
+      if (W > 1) range = ranges[t];
+      auto needs = [&](int b) { return W == 1 || in_range(range, b); };
+      int scored = 0, n = 0, stage = 0;
+      uint32_t phase = 0;
       bool alive = mbar_wait(smem_u32(qfull), 0, abort_flag, p.status, kErrAttnQ);
-      auto scores = [&](int b) {
-        if (alive) alive = mbar_wait(smem_u32(&ready[ks]), kp, abort_flag, p.status, kErrAttnLoad);
-        if (alive && active(t, b)) {
-          // (the place's last P has to be through)
-          if (scored > 1) alive = mbar_wait(smem_u32(&pvdone[t]), (scored - 2) & 1, abort_flag, p.status, kErrAttnO);
-          if (alive) {
-            tc_fence_after();
-            if (leader) {
-              product_channels<DP / 16, 128, BN>(d + (scored & 1) * BN, q, kv + ks * Shape::kSlot, ksteps, idesc_s);
-              umma_commit(smem_u32(&sfull[2 * t + (scored & 1)]));
-            }
-            ++scored;
-          }
+      auto scores = [&](int s) {
+        // (the place's last P has to be through)
+        if (scored >= NB) alive = mbar_wait(smem_u32(&pvdone[t]), (scored - NB) & 1, abort_flag, p.status, kErrAttnO);
+        if (!alive) return;
+        tc_fence_after();
+        if (leader) {
+          product_channels<DP / 16, 128, BN>(d + scored % NB * BN, q, kv + s * 2 * Shape::kBlock, ksteps, idesc_s);
+          umma_commit(smem_u32(&sfull[NB * t + scored % NB]));
         }
-        if (alive && leader && 2 * b + p.slots < 2 * blocks) umma_commit(smem_u32(&empty[ks]));
-        on(ks, kp);
+        ++scored;
       };
-      scores(0);
+      if (alive) alive = mbar_wait(smem_u32(&ready[0]), 0, abort_flag, p.status, kErrAttnLoad);
+      if (alive && needs(0)) scores(0);
       for (int b = 0; b < blocks && alive; ++b) {
-        if (b + 1 < blocks) scores(b + 1);
-        if (alive) alive = mbar_wait(smem_u32(&ready[vs]), vp, abort_flag, p.status, kErrAttnLoad);
-        if (alive && active(t, b)) {
-          alive = mbar_wait(smem_u32(&pfull[2 * t + (n & 1)]), (n >> 1) & 1, abort_flag, p.status, kErrAttnP);
+        const int next = stage + 1 == p.stages ? 0 : stage + 1;
+        const uint32_t next_phase = next == 0 ? phase ^ 1u : phase;
+        const bool more = b + 1 < blocks;
+        if (more) alive = mbar_wait(smem_u32(&ready[next]), next_phase, abort_flag, p.status, kErrAttnLoad);
+        if (NB > 1 && alive && more && needs(b + 1)) scores(next);
+        if (alive && needs(b)) {
+          alive = mbar_wait(smem_u32(&pfull[NB * t + n % NB]), (n / NB) & 1, abort_flag, p.status, kErrAttnP);
           if (!alive) break;
           tc_fence_after();
           if (leader) {
-            product_rows<BN>(d + 2 * BN, d + (n & 1) * BN, kv + vs * Shape::kSlot, idesc_o, n == 0);
+            product_rows<BN>(d + NB * BN, d + n % NB * BN, kv + stage * 2 * Shape::kBlock + Shape::kBlock, idesc_o, n == 0);
             umma_commit(smem_u32(&pvdone[t]));
           }
           ++n;
         }
-        if (alive && leader && 2 * b + 1 + p.slots < 2 * blocks) umma_commit(smem_u32(&empty[vs]));
-        on(vs, vp);
+        if (alive && leader && b + p.stages < blocks) umma_commit(smem_u32(&empty[stage]));
+        if (NB == 1 && alive && more && needs(b + 1)) scores(next);
+        stage = next;
+        phase = next_phase;
       }
       if (leader) umma_commit(smem_u32(&ofull[t]));              // (a barrier of its own: rows cannot tell pvdone's phases apart)
       if (!alive)
@@ -290,35 +286,38 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
       for (int t = 0; t < W; ++t)
         tma_tile<Shape::kPieces, 128>(smem_u32(sq + t * Shape::kTileQ), &p.q, a.dim, h0, r0 + t * nodes, smem_u32(qfull));
     }
-    int slot = 0, cslot = 0;
+    int stage = 0, cstage = 0;
     uint32_t phase = 1, cphase = 0;
     bool alive = true;
-    for (int c = 0; c < 2 * blocks + (cleared ? 1 : 0) && alive; ++c) {
-      if (c < 2 * blocks) {
-        if (c >= p.slots) alive = mbar_wait(smem_u32(&empty[slot]), phase, abort_flag, p.status, kErrAttnSlot);
+    for (int b = 0; b < blocks + (cleared ? 1 : 0) && alive; ++b) {
+      if (b < blocks) {
+        if (b >= p.stages) alive = mbar_wait(smem_u32(&empty[stage]), phase, abort_flag, p.status, kErrAttnSlot);
         if (!alive) break;
         if (lane == 0) {
-          mbar_arrive_expect_tx(smem_u32(&full[slot]), tile_bytes<BN>(a.dim));
-          tma_tile<Shape::kPieces, BN>(smem_u32(skv + slot * Shape::kSlot), (c & 1) == 0 ? &p.k : &p.v, a.dim, hk,
-                                       keys.key(c >> 1), smem_u32(&full[slot]));
+          const uint32_t dst = smem_u32(skv + stage * 2 * Shape::kBlock), bar = smem_u32(&full[stage]);
+          mbar_arrive_expect_tx(bar, 2 * tile_bytes<BN>(a.dim));
+          tma_tile<Shape::kPieces, BN>(dst, &p.k, a.dim, hk, keys.key(b), bar);
+          tma_tile<Shape::kPieces, BN>(dst + Shape::kBlock, &p.v, a.dim, hk, keys.key(b), bar);
         }
-        if (++slot == p.slots) {
-          slot = 0;
+        if (++stage == p.stages) {
+          stage = 0;
           phase ^= 1u;
         }
       }
-      // the slot before has landed or is about to
-      if (cleared && c > 0) {
-        alive = mbar_wait(smem_u32(&full[cslot]), cphase, abort_flag, p.status, kErrAttnLoad);
+      // the stage before has landed or is about to
+      if (cleared && b > 0) {
+        alive = mbar_wait(smem_u32(&full[cstage]), cphase, abort_flag, p.status, kErrAttnLoad);
         alive = __all_sync(0xffffffffu, alive);
         if (!alive) break;
-        const int j = keys.key((c - 1) >> 1);
-        clear_rows<Shape::kPieces, BN>(skv + cslot * Shape::kSlot, [&](int k) { return kept_bits(a, j + 32 * k, end); });
+        const int j = keys.key(b - 1);
+        for (int kv = 0; kv < 2; ++kv)
+          clear_rows<Shape::kPieces, BN>(skv + (cstage * 2 + kv) * Shape::kBlock,
+                                         [&](int k) { return kept_bits(a, j + 32 * k, end); });
         proxy_fence();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&clean[cslot]));
-        if (++cslot == p.slots) {
-          cslot = 0;
+        if (lane == 0) mbar_arrive(smem_u32(&clean[cstage]));
+        if (++cstage == p.stages) {
+          cstage = 0;
           cphase ^= 1u;
         }
       }
@@ -332,16 +331,16 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN>::kThreads, CTAS)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Shape::kCols) : "memory");
 }
 
-template <int DP, int W, int BN, bool HALF, int CTAS>
+template <int DP, int W, int BN, int NB, bool HALF, int CTAS>
 int fwd_launch(AttnFwdArgs& p, cudaStream_t st) {
-  using Shape = FwdShape<DP, W, BN>;
+  using Shape = FwdShape<DP, W, BN, NB>;
   constexpr size_t kMost = (227 * 1024) / CTAS - 1024;
   constexpr int dtype = HALF ? OCNN_F16 : OCNN_BF16;
-  int slots = kMaxSlots;
-  static_assert(Shape::smem(3) <= kMost, "with a mask, three slots at least: one is cleared while two are read");
-  while (Shape::smem(slots) > kMost) --slots;
-  p.slots = slots;
-  const size_t bytes = Shape::smem(slots);
+  int stages = kMaxStages;
+  static_assert(Shape::smem(3) <= kMost, "with a mask, three stages at least: one is cleared while two are read");
+  while (Shape::smem(stages) > kMost) --stages;
+  p.stages = stages;
+  const size_t bytes = Shape::smem(stages);
   const AttnArgs& a = p.a;
   int status = attn_map(&p.q, a.q, dtype, a.dim, a.heads, a.n, a.q_row, a.q_head, 1 << p.pack_log, 128 >> p.pack_log);
   if (status == OCNN_OK) status = attn_map(&p.k, a.k, dtype, a.dim, a.kv_heads, a.n, a.k_row, a.k_head, 1, BN);
@@ -349,22 +348,25 @@ int fwd_launch(AttnFwdArgs& p, cudaStream_t st) {
   if (status != OCNN_OK) return status;
   static PerDeviceOnce once;
   status = once.run([&]() -> int {
-    OCNN_CUDA_OK(cudaFuncSetAttribute(attn_tc_kernel<DP, W, BN, HALF, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    OCNN_CUDA_OK(cudaFuncSetAttribute(attn_tc_kernel<DP, W, BN, NB, HALF, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)bytes));
     return OCNN_OK;
   });
   if (status != OCNN_OK) return status;
   const int nodes = W * 128 >> p.pack_log;
-  attn_tc_kernel<DP, W, BN, HALF, CTAS><<<dim3(ceil_div(a.n, nodes), a.heads >> p.pack_log), Shape::kThreads, bytes, st>>>(p);
+  attn_tc_kernel<DP, W, BN, NB, HALF, CTAS><<<dim3(ceil_div(a.n, nodes), a.heads >> p.pack_log), Shape::kThreads, bytes, st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_kernel");
   return OCNN_OK;
 }
 
 template <bool HALF>
 int fwd_by_width(AttnFwdArgs& p, cudaStream_t st) {
-  if (p.a.dim <= 32) return fwd_launch<32, 1, 64, HALF, 2>(p, st);
-  if (p.a.dim <= 64) return fwd_launch<64, 1, 64, HALF, 2>(p, st);
-  return fwd_launch<128, 2, 64, HALF, 1>(p, st);
+  // Up to 64 channels a tile's tensor memory is a quarter of the SM's with one place for scores, and three CTAs share an SM:
+  // 60 k nodes, 8 heads of 32, window 256: 159 us; with two places and two CTAs 178.  At 128 channels there is room for two
+  // tiles, which share their copies of K and V and have two places each.
+  if (p.a.dim <= 32) return fwd_launch<32, 1, 64, 1, HALF, 3>(p, st);
+  if (p.a.dim <= 64) return fwd_launch<64, 1, 64, 1, HALF, 3>(p, st);
+  return fwd_launch<128, 2, 64, 2, HALF, 1>(p, st);
 }
 
 }  // namespace

@@ -252,11 +252,17 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 template <int KS, int ROWS_A, int ROWS_B>
 __device__ __forceinline__ void product_channels(uint32_t d, uint32_t a, uint32_t b, int ksteps, uint32_t idesc) {
   const uint64_t da = smem_desc_sw128(a), db = smem_desc_sw128(b);
-#pragma unroll
-  for (int k = 0; k < KS; ++k) {
-    if (k >= ksteps) break;
+  auto step = [&](int k) {
     umma_bf16(d, da + (k >> 2) * (ROWS_A * kRowBytes >> 4) + (k & 3) * 2, db + (k >> 2) * (ROWS_B * kRowBytes >> 4) + (k & 3) * 2,
               idesc, k > 0 ? 1u : 0u);
+  };
+  if (ksteps == KS) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) step(k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+      if (k < ksteps) step(k);
   }
 }
 // Products over a block's rows: D[128 x channels] (+)= P[128 x ROWS] B, P in tensor memory.

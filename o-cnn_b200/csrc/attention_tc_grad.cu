@@ -204,6 +204,9 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       const bool leader = elect_one();
       const uint32_t idesc_s = attn_idesc<HALF>(kBN, false), idesc_o = attn_idesc<HALF>(16 * ksteps, true);
       const uint32_t q = smem_u32(stq + t * 2 * Shape::kTile), kv = smem_u32(skv), d = tmem + t * Shape::kAcc;
+      BlockRange range;
+      if (W > 1) range = ranges[t];
+      auto needs = [&](int b) { return W == 1 || in_range(range, b); };
       int n = 0, stage = 0;
       uint32_t phase = 0;
       bool alive = mbar_wait(smem_u32(qfull), 0, abort_flag, p.status, kErrGradTile);
@@ -221,12 +224,12 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
         }
       };
       wait_stage(0, 0);
-      if (alive && active(t, 0)) scores(0);
+      if (alive && needs(0)) scores(0);
       for (int b = 0; b < blocks && alive; ++b) {
         const int next = stage + 1 == p.stages ? 0 : stage + 1;
         const uint32_t next_phase = next == 0 ? phase ^ 1u : phase;
         if (b + 1 < blocks) wait_stage(next, next_phase);
-        if (alive && active(t, b)) {
+        if (alive && needs(b)) {
           alive = mbar_wait(smem_u32(&dsfull[t]), n & 1, abort_flag, p.status, kErrGradP);
           if (!alive) break;
           tc_fence_after();
@@ -237,7 +240,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
           ++n;
         }
         if (alive && leader && b + p.stages < blocks) umma_commit(smem_u32(&empty[stage]));
-        if (alive && b + 1 < blocks && active(t, b + 1)) {
+        if (alive && b + 1 < blocks && needs(b + 1)) {
           // (S lies where dS does: the product that reads dS has to be through)
           if (n > 0) alive = mbar_wait(smem_u32(&dqdone[t]), (n - 1) & 1, abort_flag, p.status, kErrGradDone);
           if (alive) scores(next);
