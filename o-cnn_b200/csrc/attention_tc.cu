@@ -3,11 +3,11 @@
 // A CTA takes W tiles of 128 rows against the keys that they see, in blocks of BN keys.  A row is a query head of a node:
 // P heads that share a key head stand side by side (P the largest power of two in the group), so that 128 / P nodes share
 // each copy of keys and values and the tile's windows overlap more.  Per block and tile
-//     S = Q K^T (tensor memory) -> p = exp2(S scale - m) -> P (tensor memory) -> O += P V
+//     S = Q K^T (tensor memory) -> p = exp2(S scale - m) -> P (tensor memory, in S's place) -> O += P V
 // with 128 threads per tile, one row each, between the two products.  m is the row's reference: its running maximum, but
 // moved only when a block exceeds it by more than 8 (any reference gives the same quotient as long as nothing overflows,
 // and 2^8 is far from that), so O is hardly ever scaled.  P is rounded to the data's type, which is what the product takes;
-// its sum is of the unrounded values.
+// its sum is of the unrounded values.  Scores have two places, so that a block's are ready when its rows come to it.
 //
 // Roles: 4 W warps of rows, W warps that issue products (one thread of each), one warp that brings Q and the blocks of K
 // and V by TMA into a ring of slots (and clears the rows that the mask hides: see clear_rows).
@@ -36,10 +36,7 @@ struct FwdShape {
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTileQ = 128 * kRowBytes * kPieces;
   static constexpr int kBlock = BN * kRowBytes * kPieces;                // K, then V
-  // P has columns of its own where they are to be had: the next scores may then be formed as soon as its rows have read
-  // the last ones, while they are still at work on them.
-  static constexpr bool kApart = NB == 1 && W == 1 && BN + DP + BN / 2 <= 128;
-  static constexpr int kAcc = NB * BN + DP + (kApart ? BN / 2 : 0);      // places for S, O, P
+  static constexpr int kAcc = NB * BN + DP;                              // places for S, and O
   static constexpr int kCols = W * kAcc <= 128 ? 128 : W * kAcc <= 256 ? 256 : 512;
   static constexpr size_t smem(int stages) { return (size_t)W * kTileQ + (size_t)stages * 2 * kBlock + 1024 + 512; }
 };
@@ -62,8 +59,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
   uint64_t* pfull = sfull + NB * W;
   uint64_t* pvdone = pfull + NB * W;
   uint64_t* ofull = pvdone + W;
-  uint64_t* sread = ofull + W;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sread + W);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(ofull + W);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   BlockRange* ranges = reinterpret_cast<BlockRange*>(tmem_holder + 2);
 
@@ -87,7 +83,6 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
       }
       mbar_init(smem_u32(&pvdone[t]), 1);
       mbar_init(smem_u32(&ofull[t]), 1);
-      mbar_init(smem_u32(&sread[t]), 128);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -122,22 +117,13 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
     const uint64_t c2 = pair(c, c);
     float ref = -INFINITY, total = 0.f;                                    // the reference, in powers of two
     int done = 0;
-    uint32_t formed = 0;                                                   // the scores' barrier's answer, asked ahead
     bool alive = true;
     for (int b = 0; b < blocks && alive; ++b) {
       if (!active(t, b)) continue;
-      const int place = done % NB;
+      const int place = done % NB, j = keys.key(b);
       const uint32_t lanes = quarter + place * BN;
-      if (!__all_sync(0xffffffffu, formed != 0))
-        alive = mbar_wait(smem_u32(&sfull[NB * t + place]), (done / NB) & 1, abort_flag, p.status, kErrAttnS);
-      alive = __all_sync(0xffffffffu, alive);
-      if (!alive) break;
-      tc_fence_after();
-      float s[BN];
-      tmem_load<BN>(lanes, s);
-      const uint32_t added = done > 0 ? mbar_ask(smem_u32(&pvdone[t]), (done - 1) & 1) : 1u;
-      const int j = keys.key(b);
-      const bool first = keys.is_first(b), all = whole.has(b);
+      const bool first = keys.is_first(b);
+      const bool all = whole.has(b);
       uint32_t bits[BN / 32];
       if (!all) {
 #pragma unroll
@@ -146,11 +132,13 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
           if (a.mask != nullptr) bits[k] &= kept_bits(a, j + 32 * k, a.n);
         }
       }
+      alive = mbar_wait(smem_u32(&sfull[NB * t + place]), (done / NB) & 1, abort_flag, p.status, kErrAttnS);
+      alive = __all_sync(0xffffffffu, alive);
+      if (!alive) break;
+      tc_fence_after();
+      float s[BN];
+      tmem_load<BN>(lanes, s);
       tmem_wait_ld();
-      if (Shape::kApart) {
-        tc_fence_before();
-        mbar_arrive(smem_u32(&sread[t]));
-      }
       if (!all) {
         // (a hidden score is -inf, c > 0: its p is 0)
 #pragma unroll
@@ -162,22 +150,18 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
       for (int e = 4; e < BN; e += 2) tops[(e / 2) & 3] = max3(tops[(e / 2) & 3], s[e], s[e + 1]);
       const float top = max3(fmaxf(tops[0], tops[1]), tops[2], tops[3]) * c;
       const bool move = top > ref + 8.f;                                   // (from -inf too)
-      const bool moves = __any_sync(0xffffffffu, move);
-      if (done > 0 && (Shape::kApart || moves)) {
-        // (the last block's product may still be reading P and adding to O)
-        if (!__all_sync(0xffffffffu, added != 0))
-          alive = mbar_wait(smem_u32(&pvdone[t]), (done - 1) & 1, abort_flag, p.status, kErrAttnO);
-        alive = __all_sync(0xffffffffu, alive);
-        if (!alive) break;
-        tc_fence_after();
-      }
-      if (moves) {
+      if (__any_sync(0xffffffffu, move)) {
         const float keep = move ? exp2_approx(ref - top) : 1.f;
         if (move) {
           ref = top;
           total *= keep;
         }
         if (done > 0) {
+          // (the last block's product may still be adding to O)
+          alive = mbar_wait(smem_u32(&pvdone[t]), (done - 1) & 1, abort_flag, p.status, kErrAttnO);
+          alive = __all_sync(0xffffffffu, alive);
+          if (!alive) break;
+          tc_fence_after();
 #pragma unroll 1
           for (int d = 0; d < a.dim; d += 16) {
             uint32_t o[16];
@@ -202,9 +186,8 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
           sums[e & 1] = add2(sums[e & 1], pair(px, py));
           w[e] = pack16<HALF>(px, py);
         }
-        tmem_st16((Shape::kApart ? acc + DP : lanes) + 16 * k, w);         // (else where the scores lay: all read)
+        tmem_st16(lanes + 16 * k, w);                                      // (where the scores lay: all read)
       }
-      formed = NB > 1 || Shape::kApart ? mbar_ask(smem_u32(&sfull[NB * t + (done + 1) % NB]), ((done + 1) / NB) & 1) : 0u;
       const float2 sum = unpair(add2(sums[0], sums[1]));
       total = sum.x + sum.y;
       tmem_wait_st();
@@ -258,13 +241,9 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
       int scored = 0, n = 0, stage = 0;
       uint32_t phase = 0;
       bool alive = mbar_wait(smem_u32(qfull), 0, abort_flag, p.status, kErrAttnQ);
-      // Scores ahead of their rows need their place: its last P through, or (apart) its last scores read.
-      constexpr bool kAhead = NB > 1 || Shape::kApart;
-      constexpr int kBehind = Shape::kApart ? 1 : NB;
-      const uint32_t place_bar = smem_u32(Shape::kApart ? &sread[t] : &pvdone[t]);
-      auto scores = [&](int s, uint32_t free) {
-        if (scored >= kBehind && !free)
-          alive = mbar_wait(place_bar, (scored - kBehind) & 1, abort_flag, p.status, kErrAttnO);
+      auto scores = [&](int s) {
+        // (the place's last P has to be through)
+        if (scored >= NB) alive = mbar_wait(smem_u32(&pvdone[t]), (scored - NB) & 1, abort_flag, p.status, kErrAttnO);
         if (!alive) return;
         tc_fence_after();
         if (leader) {
@@ -274,30 +253,25 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
         ++scored;
       };
       if (alive) alive = mbar_wait(smem_u32(&ready[0]), 0, abort_flag, p.status, kErrAttnLoad);
-      if (alive && needs(0)) scores(0, 0u);
+      if (alive && needs(0)) scores(0);
       for (int b = 0; b < blocks && alive; ++b) {
         const int next = stage + 1 == p.stages ? 0 : stage + 1;
         const uint32_t next_phase = next == 0 ? phase ^ 1u : phase;
         const bool more = b + 1 < blocks;
-        // (all asked before the first is waited for)
-        const uint32_t loaded = mbar_ask(smem_u32(&ready[next]), next_phase);
-        const uint32_t free = kAhead && scored >= kBehind ? mbar_ask(place_bar, (scored - kBehind) & 1) : 0u;
-        const uint32_t formed = mbar_ask(smem_u32(&pfull[NB * t + n % NB]), (n / NB) & 1);
-        if (more && !loaded) alive = mbar_wait(smem_u32(&ready[next]), next_phase, abort_flag, p.status, kErrAttnLoad);
-        if (kAhead && alive && more && needs(b + 1)) scores(next, free);
+        if (more) alive = mbar_wait(smem_u32(&ready[next]), next_phase, abort_flag, p.status, kErrAttnLoad);
+        if (NB > 1 && alive && more && needs(b + 1)) scores(next);
         if (alive && needs(b)) {
-          if (!formed) alive = mbar_wait(smem_u32(&pfull[NB * t + n % NB]), (n / NB) & 1, abort_flag, p.status, kErrAttnP);
+          alive = mbar_wait(smem_u32(&pfull[NB * t + n % NB]), (n / NB) & 1, abort_flag, p.status, kErrAttnP);
           if (!alive) break;
           tc_fence_after();
           if (leader) {
-            product_rows<BN>(d + NB * BN, Shape::kApart ? d + NB * BN + DP : d + n % NB * BN,
-                             kv + stage * 2 * Shape::kBlock + Shape::kBlock, idesc_o, n == 0);
+            product_rows<BN>(d + NB * BN, d + n % NB * BN, kv + stage * 2 * Shape::kBlock + Shape::kBlock, idesc_o, n == 0);
             umma_commit(smem_u32(&pvdone[t]));
           }
           ++n;
         }
         if (alive && leader && b + p.stages < blocks) umma_commit(smem_u32(&empty[stage]));
-        if (!kAhead && alive && more && needs(b + 1)) scores(next, 0u);
+        if (NB == 1 && alive && more && needs(b + 1)) scores(next);
         stage = next;
         phase = next_phase;
       }

@@ -6,8 +6,8 @@
 // Two kernels, one over tiles of queries and one over tiles of keys, each forming s, dO . v and p for itself: seven
 // products instead of five, but every sum stays in tensor memory, in one order, and is written once; one kernel would
 // have to add dq into fp32 in global memory, with atomics whose order changes the result.
-//   queries: S = Q K^T, dP = dO V^T -> dS (tensor memory) -> dQ += dS K
-//   keys:    S' = K Q^T, dP' = V dO^T -> P', dS' (tensor memory) -> dV += P' dO, dK += dS' Q
+//   queries: S = Q K^T, dP = dO V^T -> dS (tensor memory, in S's place) -> dQ += dS K
+//   keys:    S' = K Q^T, dP' = V dO^T -> P', dS' (in place) -> dV += P' dO, dK += dS' Q
 // P and dS are rounded to the data's type, which is what the products take.  Roles and tiles as in attention_tc.cu.
 #include "attention_tc.cuh"
 
@@ -35,10 +35,7 @@ struct DqShape {
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTile = 128 * kRowBytes * kPieces;                // Q, then dO
   static constexpr int kBlock = kBN * kRowBytes * kPieces;               // K, then V
-  // dS has columns of its own where they are to be had: the next S and dP may then be formed as soon as its rows have read
-  // the last ones.
-  static constexpr bool kApart = W == 1 && 2 * kBN + DP + kBN / 2 <= 256;
-  static constexpr int kAcc = 2 * kBN + DP + (kApart ? kBN / 2 : 0);
+  static constexpr int kAcc = 2 * kBN + DP;                              // S, dP, dQ
   static constexpr int kCols = tmem_columns(W * kAcc);
   static constexpr size_t smem(int stages) { return (size_t)W * 2 * kTile + (size_t)stages * 2 * kBlock + 1024 + 384; }
 };
@@ -59,8 +56,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
   uint64_t* sfull = qfull + 1;
   uint64_t* dsfull = sfull + W;
   uint64_t* dqdone = dsfull + W;
-  uint64_t* sread = dqdone + W;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sread + W);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(dqdone + W);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   BlockRange* ranges = reinterpret_cast<BlockRange*>(tmem_holder + 2);
 
@@ -79,7 +75,6 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       mbar_init(smem_u32(&sfull[t]), 1);
       mbar_init(smem_u32(&dsfull[t]), 128);
       mbar_init(smem_u32(&dqdone[t]), 1);
-      mbar_init(smem_u32(&sread[t]), 128);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -130,19 +125,16 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     const FullBlocks whole(keys, r, a.mask != nullptr, std::integral_constant<int, kBN>());
     const uint64_t c2 = pair(a.scale_log2, a.scale_log2), lse2 = pair(-lse, -lse), delta2 = pair(-delta, -delta);
     int done = 0;
-    uint32_t formed = 0;                                                   // the scores' barrier's answer, asked ahead
     bool alive = true;
     for (int b = 0; b < blocks && alive; ++b) {
       if (!active(t, b)) continue;
-      if (!__all_sync(0xffffffffu, formed != 0))
-        alive = mbar_wait(smem_u32(&sfull[t]), done & 1, abort_flag, p.status, kErrGradS);
+      alive = mbar_wait(smem_u32(&sfull[t]), done & 1, abort_flag, p.status, kErrGradS);
       alive = __all_sync(0xffffffffu, alive);
       if (!alive) break;
       tc_fence_after();
       float s[kBN], dp[kBN];
       tmem_load<kBN>(lanes, s);
       tmem_load<kBN>(lanes + kBN, dp);
-      const uint32_t added = Shape::kApart && done > 0 ? mbar_ask(smem_u32(&dqdone[t]), (done - 1) & 1) : 1u;
       const int j = keys.key(b);
       const bool first = keys.is_first(b), all = whole.has(b);
       uint32_t bits[2];
@@ -154,10 +146,6 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
         }
       }
       tmem_wait_ld();
-      if (Shape::kApart) {
-        tc_fence_before();
-        mbar_arrive(smem_u32(&sread[t]));
-      }
 #pragma unroll
       for (int e = 0; e < kBN; e += 2) {
         const float2 x = unpair(fma2(pair(s[e], s[e + 1]), c2, lse2));
@@ -173,16 +161,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       uint32_t w[kBN / 2];
 #pragma unroll
       for (int e = 0; e < kBN / 2; ++e) w[e] = pack16<HALF>(s[2 * e], s[2 * e + 1]);
-      if (Shape::kApart && done > 0) {
-        // (the last block's product may still be reading dS)
-        if (!__all_sync(0xffffffffu, added != 0))
-          alive = mbar_wait(smem_u32(&dqdone[t]), (done - 1) & 1, abort_flag, p.status, kErrGradDone);
-        alive = __all_sync(0xffffffffu, alive);
-        if (!alive) break;
-        tc_fence_after();
-      }
-      formed = Shape::kApart ? mbar_ask(smem_u32(&sfull[t]), (done + 1) & 1) : 0u;
-      tmem_store<kBN / 2>(Shape::kApart ? acc + DP : lanes, w);
+      tmem_store<kBN / 2>(lanes, w);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(smem_u32(&dsfull[t]));
@@ -240,10 +219,9 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
           umma_commit(smem_u32(&sfull[t]));
         }
       };
-      // S and dP need their place: (apart) read by the rows, else the product that reads dS through.
-      auto next_scores = [&](int s, uint32_t free) {
-        if (Shape::kApart && !free) alive = mbar_wait(smem_u32(&sread[t]), n & 1, abort_flag, p.status, kErrGradP);
-        if (!Shape::kApart && n > 0) alive = mbar_wait(smem_u32(&dqdone[t]), (n - 1) & 1, abort_flag, p.status, kErrGradDone);
+      // S and dP need their place: the product that reads dS through.
+      auto next_scores = [&](int s) {
+        if (n > 0) alive = mbar_wait(smem_u32(&dqdone[t]), (n - 1) & 1, abort_flag, p.status, kErrGradDone);
         if (alive) scores(s);
       };
       if (alive) alive = mbar_wait(smem_u32(&ready[0]), 0, abort_flag, p.status, kErrGradLoad);
@@ -254,22 +232,20 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
         const bool more = b + 1 < blocks;
         // (all asked before the first is waited for)
         const uint32_t loaded = mbar_ask(smem_u32(&ready[next]), next_phase);
-        const uint32_t free = Shape::kApart ? mbar_ask(smem_u32(&sread[t]), n & 1) : 0u;
         const uint32_t formed = mbar_ask(smem_u32(&dsfull[t]), n & 1);
         if (more && !loaded) alive = mbar_wait(smem_u32(&ready[next]), next_phase, abort_flag, p.status, kErrGradLoad);
-        if (Shape::kApart && alive && more) next_scores(next, free);           // (W = 1: every block is needed)
         if (alive && needs(b)) {
           if (!formed) alive = mbar_wait(smem_u32(&dsfull[t]), n & 1, abort_flag, p.status, kErrGradP);
           if (!alive) break;
           tc_fence_after();
           if (leader) {
-            product_rows<kBN>(d + 2 * kBN, Shape::kApart ? d + 2 * kBN + DP : d, kv + stage * 2 * Shape::kBlock, idesc_o, n == 0);
+            product_rows<kBN>(d + 2 * kBN, d, kv + stage * 2 * Shape::kBlock, idesc_o, n == 0);
             umma_commit(smem_u32(&dqdone[t]));
           }
           ++n;
         }
         if (alive && leader && b + p.stages < blocks) umma_commit(smem_u32(&empty[stage]));
-        if (!Shape::kApart && alive && more && needs(b + 1)) next_scores(next, 0u);
+        if (alive && more && needs(b + 1)) next_scores(next);
         stage = next;
         phase = next_phase;
       }
@@ -347,8 +323,7 @@ struct DkvShape {
   static constexpr int kPieces = DP / 64 > 0 ? DP / 64 : 1;
   static constexpr int kTile = 128 * kRowBytes * kPieces;                // K, then V
   static constexpr int kBlock = kBN * kRowBytes * kPieces;               // Q, then dO
-  static constexpr bool kApart = G == 1 && 2 * kBN + 2 * DP + kBN <= 256;  // (as in DqShape: P' and dS')
-  static constexpr int kCols = tmem_columns(G * 2 * kBN + 2 * DP + (kApart ? kBN : 0));   // S' and dP' of G blocks, dK, dV
+  static constexpr int kCols = tmem_columns(G * 2 * kBN + 2 * DP);         // S' and dP' of G blocks, dK, dV
   static constexpr size_t smem(int stages) {
     return (size_t)2 * kTile + (size_t)stages * 2 * kBlock + G * 4 * kBN * sizeof(float) + 1024 + 384;
   }
@@ -373,8 +348,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
   uint64_t* sfull = kvfull + 1;
   uint64_t* pfull = sfull + G;
   uint64_t* done = pfull + G;
-  uint64_t* sread = done + G;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sread + G);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + G);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -390,7 +364,6 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
       mbar_init(smem_u32(&sfull[t]), 1);
       mbar_init(smem_u32(&pfull[t]), 128);
       mbar_init(smem_u32(&done[t]), 1);
-      mbar_init(smem_u32(&sread[t]), 128);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -406,8 +379,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  constexpr int kAcc = G * 2 * kBN;                                        // dK, then dV (then P' and dS')
-  constexpr int kProb = Shape::kApart ? kAcc + 2 * DP : 0, kScore = Shape::kApart ? kProb + kBN / 2 : kBN;   // P', dS'
+  constexpr int kAcc = G * 2 * kBN;                                        // dK, then dV
   const int ksteps = (a.dim + 15) / 16, end = min(a.n, offsets.end(a));
   const bool cleared = end < a.n && span.hi == end;                        // (its last block holds nobody's nodes)
   // (blocks go head by head: no division where there is only one run of them)
@@ -448,11 +420,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
       ahead = fetch(b + G);
       const int i0 = first_node(b);
       const int lo = (max(kr.lo, i0) - i0) << p.pack_log, hi = (max(min(kr.hi, i0 + nodes), i0) - i0) << p.pack_log;
-      // (apart: the last block's products may still be reading P' and dS')
-      const uint32_t formed = mbar_ask(smem_u32(&sfull[t]), n & 1);
-      const uint32_t added = Shape::kApart && n > 0 ? mbar_ask(smem_u32(&done[t]), (n - 1) & 1) : 1u;
-      if (alive && !formed) alive = mbar_wait(smem_u32(&sfull[t]), n & 1, abort_flag, p.status, kErrGradS);
-      if (alive && !added) alive = mbar_wait(smem_u32(&done[t]), (n - 1) & 1, abort_flag, p.status, kErrGradDone);
+      if (alive) alive = mbar_wait(smem_u32(&sfull[t]), n & 1, abort_flag, p.status, kErrGradS);
       alive = __all_sync(0xffffffffu, alive);
       if (alive) {
         tc_fence_after();
@@ -466,10 +434,6 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
             tmem_load<32>(lanes + 32 * k, s);
             tmem_load<32>(lanes + kBN + 32 * k, dp);
             tmem_wait_ld();
-            if (Shape::kApart && k == 1) {
-              tc_fence_before();
-              mbar_arrive(smem_u32(&sread[t]));
-            }
             uint32_t w[16], v[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 4) {
@@ -493,9 +457,9 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
                 v[(e + u) / 2] = pack16<HALF>(ds.x, ds.y);
               }
             }
-            // (not apart: P' lies where the scores of the first 32 columns lay, dS' likewise: all read by now)
-            tmem_st16((Shape::kApart ? quarter : lanes) + kProb + 16 * k, w);
-            tmem_st16((Shape::kApart ? quarter : lanes) + kScore + 16 * k, v);
+            // P' lies where the scores of the first 32 columns lay, dS' likewise: all read by now
+            tmem_st16(lanes + 16 * k, w);
+            tmem_st16(lanes + kBN + 16 * k, v);
           }
         };
         if (all) form(std::true_type());
@@ -561,10 +525,10 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
       uint32_t ahead_phase = 0;
       auto scores = [&]() {                            // of the next block that has none yet
         const int t = ahead % G, n = ahead / G;
-        const uint32_t bar = smem_u32(&(cleared ? clean : full)[ahead_stage]), held = smem_u32(&(Shape::kApart ? sread : done)[t]);
+        const uint32_t bar = smem_u32(&(cleared ? clean : full)[ahead_stage]), held = smem_u32(&done[t]);
         const uint32_t loaded = mbar_ask(bar, ahead_phase), free = n > 0 ? mbar_ask(held, (n - 1) & 1) : 1u;
         if (alive && !loaded) alive = mbar_wait(bar, ahead_phase, abort_flag, p.status, kErrGradLoad);
-        // (S' and dP' lie where P' and dS' do: the products that read those have to be through; apart: they have to be read)
+        // (S' and dP' lie where P' and dS' do: the products that read those have to be through)
         if (alive && !free) alive = mbar_wait(held, (n - 1) & 1, abort_flag, p.status, kErrGradDone);
         if (!alive) return;
         tc_fence_after();
@@ -584,19 +548,18 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
       int stage = 0;
       for (int b = 0; b < blocks && alive; ++b) {
         const int t = b % G;
-        if (Shape::kApart && ahead < blocks) scores();
-        if (alive) alive = mbar_wait(smem_u32(&pfull[t]), (b / G) & 1, abort_flag, p.status, kErrGradP);
+        alive = mbar_wait(smem_u32(&pfull[t]), (b / G) & 1, abort_flag, p.status, kErrGradP);
         if (!alive) break;
         tc_fence_after();
         if (leader) {
           const uint32_t q = qg + stage * 2 * Shape::kBlock, d = tmem + t * 2 * kBN;
-          product_rows<kBN>(tmem + kAcc + DP, (Shape::kApart ? tmem : d) + kProb, q + Shape::kBlock, idesc_o, b == 0);   // dV += P' dO
-          product_rows<kBN>(tmem + kAcc, (Shape::kApart ? tmem : d) + kScore, q, idesc_o, b == 0);                       // dK += dS' Q
+          product_rows<kBN>(tmem + kAcc + DP, d, q + Shape::kBlock, idesc_o, b == 0);    // dV += P' dO
+          product_rows<kBN>(tmem + kAcc, d + kBN, q, idesc_o, b == 0);                   // dK += dS' Q
           umma_commit(smem_u32(&done[t]));
           if (b + p.stages < blocks) umma_commit(smem_u32(&empty[stage]));
         }
         if (++stage == p.stages) stage = 0;
-        if (!Shape::kApart && ahead < blocks) scores();
+        if (ahead < blocks) scores();
       }
       if (!alive)
         for (int it = 0; it < 64; ++it) __nanosleep(1000);       // (products under way end before tensor memory is freed)
