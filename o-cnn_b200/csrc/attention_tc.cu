@@ -41,7 +41,7 @@ struct FwdShape {
   static constexpr size_t smem(int stages) { return (size_t)W * kTileQ + (size_t)stages * 2 * kBlock + 1024 + 512; }
 };
 
-template <int DP, int W, int BN, int NB, bool HALF, int CTAS>
+template <int DP, int W, int BN, int NB, bool HALF, bool MASKED, int CTAS>
 __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
     attn_tc_kernel(const __grid_constant__ AttnFwdArgs p) {
   using Shape = FwdShape<DP, W, BN, NB>;
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
   const uint32_t tmem = *tmem_holder;
   auto active = [&](int t, int b) { return W == 1 || in_range(ranges[t], b); };
   const int ksteps = (a.dim + 15) / 16, end = min(a.n, offsets.end(a));
-  const bool cleared = a.mask != nullptr || (end < a.n && keys.reaches(end));   // (see clear_rows)
+  const bool cleared = MASKED || (end < a.n && keys.reaches(end));   // (see clear_rows)
 
   if (warp < 4 * W) {
     // ---------------- rows ----------------
@@ -112,13 +112,19 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
     const uint32_t quarter = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * Shape::kAcc, acc = quarter + NB * BN;
     const int i = r0 + t * nodes + (row >> p.pack_log), h = h0 + (row & (pack - 1));
     const RowKeys r = i < a.n ? attn_row_keys(a, i, attn_span_near(a, i, f, l)) : RowKeys{0, 0, 0, 0};
-    const FullBlocks whole(keys, r, a.mask != nullptr, std::integral_constant<int, BN>());
+    const FullBlocks whole(keys, r, MASKED, std::integral_constant<int, BN>());
     const float c = a.scale_log2;
     const uint64_t c2 = pair(c, c);
     float ref = -INFINITY, total = 0.f;                                    // the reference, in powers of two
     int done = 0;
     bool alive = true;
+    KeptKeys<BN> kept, ahead;
+    if (MASKED && blocks > 0) ahead.ask(a, keys.key(0), a.n);
     for (int b = 0; b < blocks && alive; ++b) {
+      if (MASKED) {
+        kept = ahead;
+        if (b + 1 < blocks) ahead.ask(a, keys.key(b + 1), a.n);
+      }
       if (!active(t, b)) continue;
       const int place = done % NB, j = keys.key(b);
       const uint32_t lanes = quarter + place * BN;
@@ -129,7 +135,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
 #pragma unroll
         for (int k = 0; k < BN / 32; ++k) {
           bits[k] = first ? seen_first(keys, r, 32 * k) : seen_bits(a, r, j + 32 * k);
-          if (a.mask != nullptr) bits[k] &= kept_bits(a, j + 32 * k, a.n);
+          if (MASKED) bits[k] &= kept.bits(k);
         }
       }
       alive = mbar_wait(smem_u32(&sfull[NB * t + place]), (done / NB) & 1, abort_flag, p.status, kErrAttnS);
@@ -287,7 +293,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
         tma_tile<Shape::kPieces, 128>(smem_u32(sq + t * Shape::kTileQ), &p.q, a.dim, h0, r0 + t * nodes, smem_u32(qfull));
     }
     int stage = 0, cstage = 0;
-    uint32_t phase = 1, cphase = 0;
+    uint32_t phase = 1, cphase = 0, words[BN / 32];
     bool alive = true;
     for (int b = 0; b < blocks + (cleared ? 1 : 0) && alive; ++b) {
       if (b < blocks) {
@@ -304,15 +310,14 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
           phase ^= 1u;
         }
       }
-      // the stage before has landed or is about to
+      KeptKeys<BN> kept;
+      if (cleared && b < blocks) kept.ask(a, keys.key(b), end);
+      // the stage before has landed or is about to: its V (a hidden key's score is not read)
       if (cleared && b > 0) {
         alive = mbar_wait(smem_u32(&full[cstage]), cphase, abort_flag, p.status, kErrAttnLoad);
         alive = __all_sync(0xffffffffu, alive);
         if (!alive) break;
-        const int j = keys.key(b - 1);
-        for (int kv = 0; kv < 2; ++kv)
-          clear_rows<Shape::kPieces, BN>(skv + (cstage * 2 + kv) * Shape::kBlock,
-                                         [&](int k) { return kept_bits(a, j + 32 * k, end); });
+        clear_rows<Shape::kPieces, BN>(skv + (cstage * 2 + 1) * Shape::kBlock, [&](int k) { return words[k]; });
         proxy_fence();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&clean[cstage]));
@@ -320,6 +325,10 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
           cstage = 0;
           cphase ^= 1u;
         }
+      }
+      if (cleared) {
+#pragma unroll
+        for (int k = 0; k < BN / 32; ++k) words[k] = kept.bits(k);
       }
     }
     if (!alive)
@@ -331,8 +340,8 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Shape::kCols) : "memory");
 }
 
-template <int DP, int W, int BN, int NB, bool HALF, int CTAS>
-int fwd_launch(AttnFwdArgs& p, cudaStream_t st) {
+template <int DP, int W, int BN, int NB, bool HALF, bool MASKED, int CTAS>
+int fwd_launch_kernel(AttnFwdArgs& p, cudaStream_t st) {
   using Shape = FwdShape<DP, W, BN, NB>;
   constexpr size_t kMost = (227 * 1024) / CTAS - 1024;
   constexpr int dtype = HALF ? OCNN_F16 : OCNN_BF16;
@@ -348,15 +357,21 @@ int fwd_launch(AttnFwdArgs& p, cudaStream_t st) {
   if (status != OCNN_OK) return status;
   static PerDeviceOnce once;
   status = once.run([&]() -> int {
-    OCNN_CUDA_OK(cudaFuncSetAttribute(attn_tc_kernel<DP, W, BN, NB, HALF, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    OCNN_CUDA_OK(cudaFuncSetAttribute(attn_tc_kernel<DP, W, BN, NB, HALF, MASKED, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)bytes));
     return OCNN_OK;
   });
   if (status != OCNN_OK) return status;
   const int nodes = W * 128 >> p.pack_log;
-  attn_tc_kernel<DP, W, BN, NB, HALF, CTAS><<<dim3(ceil_div(a.n, nodes), a.heads >> p.pack_log), Shape::kThreads, bytes, st>>>(p);
+  attn_tc_kernel<DP, W, BN, NB, HALF, MASKED, CTAS><<<dim3(ceil_div(a.n, nodes), a.heads >> p.pack_log), Shape::kThreads, bytes, st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_kernel");
   return OCNN_OK;
+}
+
+template <int DP, int W, int BN, int NB, bool HALF, int CTAS>
+int fwd_launch(AttnFwdArgs& p, cudaStream_t st) {
+  return p.a.mask != nullptr ? fwd_launch_kernel<DP, W, BN, NB, HALF, true, CTAS>(p, st)
+                             : fwd_launch_kernel<DP, W, BN, NB, HALF, false, CTAS>(p, st);
 }
 
 template <bool HALF>

@@ -192,11 +192,20 @@ template <int BN>
 __device__ __forceinline__ uint32_t seen_first(const KeyBlocks<BN>& k, const RowKeys& r, int c) {
   return r.first > r.start && r.start == k.first ? bit_run(-c, min(k.n_first, r.first - r.start) - c) : 0u;
 }
-// Which of the 32 keys from j on the mask keeps, if they lie before node `end`.
-__device__ __forceinline__ uint32_t kept_bits(const AttnArgs& a, int j, int end) {
-  const int at = j + (threadIdx.x & 31);
-  return __ballot_sync(0xffffffffu, at < end && (a.mask == nullptr || a.mask[at] != 0));
-}
+// Which keys of a block the mask keeps, of those before node `end`: read for a block ahead (`ask`), and then formed into a bit
+// per key by the whole warp (`bits`, for 32 keys each).
+template <int BN>
+struct KeptKeys {
+  unsigned char mine[BN / 32];
+  __device__ __forceinline__ void ask(const AttnArgs& a, int j, int end) {
+#pragma unroll
+    for (int k = 0; k < BN / 32; ++k) {
+      const int at = j + 32 * k + (threadIdx.x & 31);
+      mine[k] = at >= end ? 0 : a.mask == nullptr ? 1 : a.mask[at];
+    }
+  }
+  __device__ __forceinline__ uint32_t bits(int k) const { return __ballot_sync(0xffffffffu, mine[k] != 0); }
+};
 
 // Zeros in the rows of a tile that `kept` (32 rows from 32 k on) leaves out, by a whole warp: what lies there, behind the
 // mask or behind the last sequence, may not be a number, and a product with a probability of 0 would be none.

@@ -40,7 +40,7 @@ struct DqShape {
   static constexpr size_t smem(int stages) { return (size_t)W * 2 * kTile + (size_t)stages * 2 * kBlock + 1024 + 384; }
 };
 
-template <int DP, int W, bool HALF, int CTAS>
+template <int DP, int W, bool HALF, bool MASKED, int CTAS>
 __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_kernel(const __grid_constant__ GradArgs p) {
   using Shape = DqShape<DP, W>;
   using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
   const uint32_t tmem = *tmem_holder;
   auto active = [&](int t, int b) { return W == 1 || in_range(ranges[t], b); };
   const int ksteps = (a.dim + 15) / 16, end = min(a.n, offsets.end(a));
-  const bool cleared = a.mask != nullptr || (end < a.n && keys.reaches(end));   // (see clear_rows)
+  const bool cleared = MASKED || (end < a.n && keys.reaches(end));   // (see clear_rows)
 
   if (warp < 4 * W) {
     // ---------------- rows ----------------
@@ -122,11 +122,17 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       }
       p.g.delta[(long long)h * a.n + i] = delta;
     }
-    const FullBlocks whole(keys, r, a.mask != nullptr, std::integral_constant<int, kBN>());
+    const FullBlocks whole(keys, r, MASKED, std::integral_constant<int, kBN>());
     const uint64_t c2 = pair(a.scale_log2, a.scale_log2), lse2 = pair(-lse, -lse), delta2 = pair(-delta, -delta);
     int done = 0;
     bool alive = true;
+    KeptKeys<kBN> kept, ahead;
+    if (MASKED && blocks > 0) ahead.ask(a, keys.key(0), a.n);
     for (int b = 0; b < blocks && alive; ++b) {
+      if (MASKED) {
+        kept = ahead;
+        if (b + 1 < blocks) ahead.ask(a, keys.key(b + 1), a.n);
+      }
       if (!active(t, b)) continue;
       alive = mbar_wait(smem_u32(&sfull[t]), done & 1, abort_flag, p.status, kErrGradS);
       alive = __all_sync(0xffffffffu, alive);
@@ -142,7 +148,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           bits[k] = first ? seen_first(keys, r, 32 * k) : seen_bits(a, r, j + 32 * k);
-          if (a.mask != nullptr) bits[k] &= kept_bits(a, j + 32 * k, a.n);
+          if (MASKED) bits[k] &= kept.bits(k);
         }
       }
       tmem_wait_ld();
@@ -263,7 +269,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
       }
     }
     int stage = 0, cstage = 0;
-    uint32_t phase = 1, cphase = 0;
+    uint32_t phase = 1, cphase = 0, words[2];
     bool alive = true;
     for (int b = 0; b < blocks + (cleared ? 1 : 0) && alive; ++b) {
       if (b < blocks) {
@@ -280,14 +286,14 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
           phase ^= 1u;
         }
       }
+      KeptKeys<kBN> kept;
+      if (cleared && b < blocks) kept.ask(a, keys.key(b), end);
+      // the stage before has landed or is about to: its K (V is read for dP only, and a hidden key's dP is not)
       if (cleared && b > 0) {
         alive = mbar_wait(smem_u32(&full[cstage]), cphase, abort_flag, p.status, kErrGradLoad);
         alive = __all_sync(0xffffffffu, alive);
         if (!alive) break;
-        const int j = keys.key(b - 1);
-        for (int kv = 0; kv < 2; ++kv)
-          clear_rows<Shape::kPieces, kBN>(skv + (cstage * 2 + kv) * Shape::kBlock,
-                                          [&](int k) { return kept_bits(a, j + 32 * k, end); });
+        clear_rows<Shape::kPieces, kBN>(skv + cstage * 2 * Shape::kBlock, [&](int k) { return words[k]; });
         proxy_fence();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&clean[cstage]));
@@ -295,6 +301,10 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
           cstage = 0;
           cphase ^= 1u;
         }
+      }
+      if (cleared) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) words[k] = kept.bits(k);
       }
     }
     if (!alive)
@@ -626,12 +636,13 @@ template <int DP, int W, int G, bool HALF, int CTAS_Q, int CTAS_K>
 int grad_launch(GradArgs& p, cudaStream_t st) {
   using Dq = DqShape<DP, W>;
   using Dkv = DkvShape<DP, G>;
-  auto dq = attn_tc_dq_kernel<DP, W, HALF, CTAS_Q>;
+  auto dq = attn_tc_dq_kernel<DP, W, HALF, false, CTAS_Q>, dq_masked = attn_tc_dq_kernel<DP, W, HALF, true, CTAS_Q>;
   auto dkv = attn_tc_dkv_kernel<DP, G, HALF, CTAS_K>;
   const int stages_q = stages_for<Dq, CTAS_Q>(), stages_k = stages_for<Dkv, CTAS_K>();
   static PerDeviceOnce once;
   int status = once.run([&]() -> int {
     OCNN_CUDA_OK(cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Dq::smem(stages_q)));
+    OCNN_CUDA_OK(cudaFuncSetAttribute(dq_masked, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Dq::smem(stages_q)));
     OCNN_CUDA_OK(cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Dkv::smem(stages_k)));
     return OCNN_OK;
   });
@@ -650,6 +661,7 @@ int grad_launch(GradArgs& p, cudaStream_t st) {
   if (status != OCNN_OK) return status;
   p.stages = stages_q;
   p.wide = wide_rows(p.g.dq, a.dim);
+  if (a.mask != nullptr) dq = dq_masked;
   dq<<<dim3(ceil_div(a.n, W * 128 >> p.pack_log), a.heads >> p.pack_log), Dq::kThreads, Dq::smem(stages_q), st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_dq_kernel");
   if (p.a.sinks > 0) {
