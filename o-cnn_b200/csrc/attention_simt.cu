@@ -39,31 +39,30 @@ __device__ __forceinline__ void load_rows(float* dst, const void* base, long lon
   }
 }
 
-// acc[r][c] = A row (4 ty + r) . B row (tx + 16 c)
+// acc[r][c] = A row (4 ty + r) . B row (tx + 16 c), even and odd channels side by side in one instruction
 template <int DP>
 __device__ __forceinline__ void tile_dot(const float* A, const float* B, float (&acc)[4][4]) {
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) acc[r][c] = 0.f;
+  uint64_t sum[4][4] = {};
 #pragma unroll 4
   for (int d = 0; d < DP; d += 4) {
-    float4 x[4], y[4];
+    ulonglong2 x[4], y[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const float4*>(A + (4 * ty + r) * (DP + kPad) + d);
+    for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const ulonglong2*>(A + (4 * ty + r) * (DP + kPad) + d);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) y[c] = *reinterpret_cast<const float4*>(B + (tx + 16 * c) * (DP + kPad) + d);
+    for (int c = 0; c < 4; ++c) y[c] = *reinterpret_cast<const ulonglong2*>(B + (tx + 16 * c) * (DP + kPad) + d);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        acc[r][c] = fmaf(x[r].x, y[c].x, acc[r][c]);
-        acc[r][c] = fmaf(x[r].y, y[c].y, acc[r][c]);
-        acc[r][c] = fmaf(x[r].z, y[c].z, acc[r][c]);
-        acc[r][c] = fmaf(x[r].w, y[c].w, acc[r][c]);
-      }
+      for (int c = 0; c < 4; ++c) sum[r][c] = fma2(x[r].y, y[c].y, fma2(x[r].x, y[c].x, sum[r][c]));
   }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float2 f = unpair(sum[r][c]);
+      acc[r][c] = f.x + f.y;
+    }
 }
 
 constexpr int kPRow = kB + 4;
@@ -71,9 +70,9 @@ constexpr int kPRow = kB + 4;
 template <int DP>
 __device__ __forceinline__ int out_col(int c) { return 2 * (threadIdx.x & 15) + 32 * (c >> 1) + (c & 1); }
 
-// acc[r][c] += sum over the kB columns of P row (4 ty + r) * B row: out = P B
+// acc[r] += sum over the kB columns of P row (4 ty + r) * B row: out = P B, a thread's channels in pairs
 template <int DP>
-__device__ __forceinline__ void tile_mul(const float* P, const float* B, float (&acc)[4][DP / 16]) {
+__device__ __forceinline__ void tile_mul(const float* P, const float* B, uint64_t (&acc)[4][DP / 32]) {
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
 #pragma unroll 2
   for (int j = 0; j < kB; j += 4) {
@@ -82,18 +81,24 @@ __device__ __forceinline__ void tile_mul(const float* P, const float* B, float (
     for (int r = 0; r < 4; ++r) p[r] = *reinterpret_cast<const float4*>(P + (4 * ty + r) * kPRow + j);
 #pragma unroll
     for (int jj = 0; jj < 4; ++jj) {
+      uint64_t v[DP / 32];
 #pragma unroll
-      for (int c = 0; c < DP / 16; c += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(B + (j + jj) * (DP + kPad) + 2 * tx + 16 * c);
+      for (int c = 0; c < DP / 32; ++c)
+        v[c] = *reinterpret_cast<const uint64_t*>(B + (j + jj) * (DP + kPad) + 2 * tx + 32 * c);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float x = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
-          acc[r][c] = fmaf(x, v.x, acc[r][c]);
-          acc[r][c + 1] = fmaf(x, v.y, acc[r][c + 1]);
-        }
+      for (int r = 0; r < 4; ++r) {
+        const float x = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
+        const uint64_t xx = pair(x, x);
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) acc[r][c] = fma2(xx, v[c], acc[r][c]);
       }
     }
   }
+}
+template <int N>
+__device__ __forceinline__ float channel(const uint64_t (&acc)[N], int c) {
+  const float2 f = unpair(acc[c / 2]);
+  return (c & 1) ? f.y : f.x;
 }
 
 __device__ __forceinline__ float row_max(float x) {
@@ -162,7 +167,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const AttnArgs a, T
   const TileKeys keys = query_tile(a, r0, rows, ext);
   load_rows<T, DP>(sq, a.q, a.q_row, h * a.q_head, a.dim, vec, [&](int r) { return r0 + r < a.n ? r0 + r : -1; });
 
-  float acc[4][DP / 16] = {}, top[4], total[4] = {};
+  uint64_t acc[4][DP / 32] = {};
+  float top[4], total[4] = {};
 #pragma unroll
   for (int r = 0; r < 4; ++r) top[r] = -INFINITY;
   for (int t0 = 0; t0 < keys.n; t0 += kB) {
@@ -192,18 +198,18 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const AttnArgs a, T
       }
       m = fmaxf(top[r], row_max(m));
       const float base = m == -INFINITY ? 0.f : m;          // a row that has seen nothing yet
-      const float keep = exp2f(top[r] - base);
+      const float keep = exp2_approx(top[r] - base);
       top[r] = m;
       float sum = 0.f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float p = exp2f(s[r][c] - base);
+        const float p = exp2_approx(s[r][c] - base);
         sp[(4 * ty + r) * kPRow + tx + 16 * c] = p;
         sum += p;
       }
       total[r] = total[r] * keep + sum;
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) acc[r][c] *= keep;
+      for (int c = 0; c < DP / 32; ++c) acc[r][c] = fma2(acc[r][c], pair(keep, keep), 0);
     }
     __syncwarp();                                            // (a row of P is written and read by one half warp)
     tile_mul<DP>(sp, sv, acc);
@@ -216,9 +222,10 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const AttnArgs a, T
     if (i < a.n) {
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
-        bad |= not_finite(acc[r][c]);
+        const float x = channel(acc[r], c);
+        bad |= not_finite(x);
         const int d = out_col<DP>(c);
-        if (d < a.dim) out[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(sum == 0.f ? 0.f : acc[r][c] * inv);
+        if (d < a.dim) out[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(sum == 0.f ? 0.f : x * inv);
       }
       if (tx == 0 && lse != nullptr) lse[(long long)h * a.n + i] = sum == 0.f ? INFINITY : top[r] + log2f(sum);
     }
@@ -260,7 +267,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const AttnArgs a
     delta[r] = row_sum(x);
     if (tx == 0 && i < a.n) g.delta[(long long)h * a.n + i] = delta[r];
   }
-  float acc[4][DP / 16] = {};
+  uint64_t acc[4][DP / 32] = {};
   for (int t0 = 0; t0 < keys.n; t0 += kB) {
     auto row_of = [&](int t) {
       if (t0 + t >= keys.n) return -1;
@@ -284,7 +291,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const AttnArgs a
       for (int c = 0; c < 4; ++c) {
         const bool seen = j[c] >= 0 && attn_sees(rk, j[c]);
         sp[(4 * ty + r) * kPRow + tx + 16 * c] =
-            seen ? exp2f(s[r][c] * a.scale_log2 - lse[r]) * (dp[r][c] - delta[r]) : 0.f;
+            seen ? exp2_approx(s[r][c] * a.scale_log2 - lse[r]) * (dp[r][c] - delta[r]) : 0.f;
       }
     }
     __syncwarp();
@@ -297,8 +304,9 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const AttnArgs a
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const int d = out_col<DP>(c);
-      bad |= not_finite(acc[r][c]);
-      if (i < a.n && d < a.dim) ((T*)g.dq)[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(acc[r][c] * a.scale);
+      const float x = channel(acc[r], c);
+      bad |= not_finite(x);
+      if (i < a.n && d < a.dim) ((T*)g.dq)[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(x * a.scale);
     }
     const unsigned any = __ballot_sync(0xffffffffu, bad);
     if (tx == 0) redo[4 * ty + r] = (any >> (tid & 16)) & 0xffffu;
@@ -342,7 +350,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
   auto key = [&](int t) { return rows[t].hi > rows[t].lo ? k0 + t : -1; };
   load_rows<T, DP>(sk, a.k, a.k_row, hk * a.k_head, a.dim, vec, key);
   load_rows<T, DP>(sv, a.v, a.v_row, hk * a.v_head, a.dim, vec, key);
-  float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
+  uint64_t dk[4][DP / 32] = {}, dv[4][DP / 32] = {};
   for (int hg = 0; hg < group; ++hg) {
     const int h = hk * group + hg;
     for (int i0 = ext[0]; i0 < ext[1]; i0 += kB) {
@@ -367,7 +375,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
         const KeyRows kr = rows[4 * ty + r];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const float p = i[c] >= kr.lo && i[c] < kr.hi ? exp2f(s[r][c] * a.scale_log2 - lse[c]) : 0.f;
+          const float p = i[c] >= kr.lo && i[c] < kr.hi ? exp2_approx(s[r][c] * a.scale_log2 - lse[c]) : 0.f;
           sp[(4 * ty + r) * kPRow + tx + 16 * c] = p;
           sd[(4 * ty + r) * kPRow + tx + 16 * c] = p == 0.f ? 0.f : p * (dp[r][c] - delta[c]);
         }
@@ -385,9 +393,11 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const int d = out_col<DP>(c);
-      bad |= not_finite(dk[r][c]) | not_finite(dv[r][c]);
+      float x = channel(dk[r], c), y = channel(dv[r], c);
+      bad |= not_finite(x) | not_finite(y);
       if (j >= a.n || d >= a.dim) continue;
-      const float x = dk[r][c] + (far != nullptr ? far[d] : 0.f), y = dv[r][c] + (far != nullptr ? far[a.dim + d] : 0.f);
+      x += far != nullptr ? far[d] : 0.f;
+      y += far != nullptr ? far[a.dim + d] : 0.f;
       ((T*)g.dk)[((long long)j * a.kv_heads + hk) * a.dim + d] = from_f32<T>(x * a.scale);
       ((T*)g.dv)[((long long)j * a.kv_heads + hk) * a.dim + d] = from_f32<T>(y);
     }

@@ -296,22 +296,7 @@ __device__ __forceinline__ void product_rows(uint32_t d, uint32_t p, uint32_t b,
   for (int k = 0; k < ROWS / 16; ++k) umma_ts(d, p + 8 * k, db + k * (16 * kRowBytes >> 4), idesc, !first || k > 0 ? 1u : 0u);
 }
 
-// ---- two fp32 values per instruction (sm_100) -------------------------------------------------------------------
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-  uint64_t p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
-  return p;
-}
-__device__ __forceinline__ float2 unpair(uint64_t p) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
-  return f;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
+// ---- values by twos and threes (sm_100) -----------------------------------------------------------------------
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
