@@ -79,7 +79,7 @@ int ocnn_octree_attention(const ocnn_attention* p, void* out_dev, float* lse_dev
 size_t ocnn_octree_attention_backward_workspace_bytes(const ocnn_attention* p) {
   if (check(p, "ocnn_octree_attention_backward_workspace_bytes") != OCNN_OK || p->n == 0) return 0;
   const AttnArgs a = args_of(p);
-  return (delta_floats(p) + (size_t)far_slots(a.n, a.batch) * a.kv_heads * a.sinks * 2 * a.dim) * sizeof(float);
+  return (32 + delta_floats(p) + (size_t)far_slots(a.n, a.batch) * a.kv_heads * a.sinks * 2 * a.dim) * sizeof(float);
 }
 
 int ocnn_octree_attention_backward(const ocnn_attention* p, const void* out_dev, const float* lse_dev,
@@ -97,7 +97,8 @@ int ocnn_octree_attention_backward(const ocnn_attention* p, const void* out_dev,
   AttnGrad g = {};
   g.out = out_dev, g.grad = grad_dev, g.grad_row = grad_stride[0], g.grad_head = grad_stride[1];
   g.lse = lse_dev;
-  g.delta = (float*)workspace_dev;
+  g.largest = (unsigned*)workspace_dev;
+  g.delta = (float*)workspace_dev + 32;
   g.far = g.delta + delta_floats(p);
   g.dq = dq_dev, g.dk = dk_dev, g.dv = dv_dev;
   if (on_tensor_cores(p) && near_rows(grad_stride) && on_boundary(grad_dev, grad_stride, p->dim, 8, 2) &&

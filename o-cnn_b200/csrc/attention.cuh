@@ -36,8 +36,19 @@ struct AttnGrad {
   long long grad_row, grad_head;
   const float* lse;
   float *delta, *far;
+  unsigned* largest;                          // float16: the largest |dO| (its bits), written by the queries' kernel
   void *dq, *dk, *dv;
 };
+
+// float16 holds nothing below 2^-24, and p of a long sequence and dO of a mean loss are small: a product's operands are kept
+// at powers of two that bring dO to 1 and p to 2^10 at most, which the results are divided by.  (Nothing is lost or rounded by
+// that; with dO near 1 and 60 k keys dV was off by 1e-3, now as bfloat16's exponent would have it.)
+constexpr float kProbUp = 1024.f;
+__device__ __forceinline__ float down_to_one(float largest) {       // 2^-e for 2^e <= largest < 2^(e + 1)
+  if (!(largest > 0.f)) return 1.f;
+  const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -100), 100);
+  return __uint_as_float((unsigned)(127 - e) << 23);
+}
 
 // Heads of a node that stand side by side in a tensor-core tile: the largest power of two in the group.
 inline int attn_pack_log(const AttnArgs& a) {

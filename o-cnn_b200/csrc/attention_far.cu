@@ -31,6 +31,9 @@ __global__ void __launch_bounds__(32 * kFarWarps) attn_far_mma_kernel(const Attn
   const int hk = blockIdx.y, group = a.heads / a.kv_heads;
   const int r0 = blockIdx.x * kFarRows, r1 = min(a.n, r0 + kFarRows);
   const int ksteps = (a.dim + 15) / 16, full = a.dim / 8;
+  // p is kept at p * prob_up, ds at ds * down, as in the other kernels
+  constexpr float prob_up = HALF ? kProbUp : 1.f, prob_log = HALF ? 10.f : 0.f;
+  const float down = HALF ? down_to_one(__uint_as_float(*g.largest)) : 1.f, after = down / prob_up;
   uint8_t* ring = smem + warp * 2 * Shape::kTile;
   const uint8_t* qb = (const uint8_t*)((const T*)a.q + (long long)hk * group * a.q_head);
   const uint8_t* gb = (const uint8_t*)((const T*)g.grad + (long long)hk * group * g.grad_head);
@@ -130,9 +133,9 @@ __global__ void __launch_bounds__(32 * kFarWarps) attn_far_mma_kernel(const Attn
 #pragma unroll
             for (int h = 0; h < 2; ++h) {                        // first nodes lane / 4, lane / 4 + 8
               const bool seen = kept[h] && i >= 0 && i - (first + (lane >> 2) + 8 * h) >= a.window;
-              const float x = seen ? exp2_approx(sc[half][2 * h + e] * a.scale_log2 - lse) : 0.f;
+              const float x = seen ? exp2_approx(sc[half][2 * h + e] * a.scale_log2 + (prob_log - lse)) : 0.f;
               p[h][e] = x;
-              ds[h][e] = seen ? x * (dp[half][2 * h + e] - delta) : 0.f;
+              ds[h][e] = seen ? x * ((dp[half][2 * h + e] - delta) * after) : 0.f;
             }
           }
 #pragma unroll
@@ -172,7 +175,7 @@ __global__ void __launch_bounds__(32 * kFarWarps) attn_far_mma_kernel(const Attn
           float x = 0.f;
 #pragma unroll
           for (int w = 0; w < kFarWarps; ++w) x += part[(w * 16 + t) * DP + d];
-          far_slot(a, g, blockIdx.x + s.seq, hk, t0 + t)[which * a.dim + d] = x;
+          far_slot(a, g, blockIdx.x + s.seq, hk, t0 + t)[which * a.dim + d] = x * (which == 0 ? 1.f / down : 1.f / prob_up);
         }
       }
       __syncthreads();

@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     const bool in = i < a.n;
     const RowKeys r = in ? attn_row_keys(a, i, attn_span_near(a, i, f, l)) : RowKeys{0, 0, 0, 0};
     const float lse = in ? p.g.lse[(long long)h * a.n + i] : INFINITY;
-    float delta = 0.f;
+    float delta = 0.f, largest = 0.f;
     if (in) {
       const T* go = (const T*)p.g.grad + i * p.g.grad_row + h * p.g.grad_head;
       const T* o = (const T*)p.g.out + ((long long)i * a.heads + h) * a.dim;
@@ -118,12 +118,22 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
           const float2 u = unpack2(xs[e], HALF), v = unpack2(ys[e], HALF);
           delta = fmaf(u.x, v.x, delta);
           delta = fmaf(u.y, v.y, delta);
+          if (HALF) {
+            if (!not_finite(u.x)) largest = fmaxf(largest, fabsf(u.x));
+            if (!not_finite(u.y)) largest = fmaxf(largest, fabsf(u.y));
+          }
         }
       }
       p.g.delta[(long long)h * a.n + i] = delta;
     }
+    if (HALF) {
+      const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
+      if (lane == 0 && most != 0) atomicMax(p.g.largest, most);             // (a maximum: whatever the order)
+    }
+    const float down = HALF ? down_to_one(largest) : 1.f;                   // dS of this row is kept at dS * down
     const FullBlocks whole(keys, r, MASKED, std::integral_constant<int, kBN>());
-    const uint64_t c2 = pair(a.scale_log2, a.scale_log2), lse2 = pair(-lse, -lse), delta2 = pair(-delta, -delta);
+    const uint64_t c2 = pair(a.scale_log2, a.scale_log2), lse2 = pair(-lse, -lse), delta2 = pair(-delta * down, -delta * down),
+                   down2 = pair(down, down);
     int done = 0;
     bool alive = true;
     KeptKeys<kBN> kept, ahead;
@@ -155,7 +165,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
 #pragma unroll
       for (int e = 0; e < kBN; e += 2) {
         const float2 x = unpair(fma2(pair(s[e], s[e + 1]), c2, lse2));
-        const float2 ds = unpair(mul2(pair(exp2_approx(x.x), exp2_approx(x.y)), add2(pair(dp[e], dp[e + 1]), delta2)));
+        const float2 ds = unpair(mul2(pair(exp2_approx(x.x), exp2_approx(x.y)), fma2(pair(dp[e], dp[e + 1]), down2, delta2)));
         s[e] = ds.x;
         s[e + 1] = ds.y;
       }
@@ -180,6 +190,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     }
     if (alive) {
       bool bad = false;
+      const float up = a.scale / down;
       T* dst = (T*)p.g.dq + ((long long)i * a.heads + h) * a.dim;
 #pragma unroll 2
       for (int d = 0; d < a.dim; d += 16) {
@@ -190,7 +201,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          x[e] *= a.scale;
+          x[e] *= up;
           bad |= not_finite(x[e]);
         }
         if (in) store_row<HALF>(dst, d, a.dim, p.wide, x);
@@ -412,12 +423,16 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
     }
     const KeyRows kr = j < a.n ? attn_key_rows(a, j, attn_span_near(a, j, f, l)) : KeyRows{0, 0};
     const uint64_t c2 = pair(a.scale_log2, a.scale_log2);
+    // P' is kept at P' * prob_up, dS' at dS' * down
+    constexpr float prob_up = HALF ? kProbUp : 1.f, prob_log = HALF ? 10.f : 0.f;
+    const float down = HALF ? down_to_one(__uint_as_float(*p.g.largest)) : 1.f, after = down / prob_up;
+    const uint64_t after2 = pair(after, after);
     // lse and delta of a block's rows: two threads a row fetch them a block ahead
     auto fetch = [&](int b) {
       const int r = row & (kBN - 1), i = first_node(b) + (r >> p.pack_log);
       if (b >= blocks || i >= span.hi) return row < kBN ? -INFINITY : 0.f;
       const long long at = (long long)(first_head(b) + (r & (pack - 1))) * a.n + i;
-      return row < kBN ? -p.g.lse[at] : -p.g.delta[at];
+      return row < kBN ? prob_log - p.g.lse[at] : -p.g.delta[at] * after;
     };
     float ahead = t < blocks ? fetch(t) : 0.f;
     int n = 0;
@@ -457,7 +472,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
                   if (!((bits[k] >> (e + u)) & 1)) px = 0.f;
                   if (!((bits[k] >> (e + u + 1)) & 1)) py = 0.f;
                 }
-                float2 ds = unpair(mul2(pair(px, py), add2(pair(dp[e + u], dp[e + u + 1]), u == 0 ? delta.x : delta.y)));
+                float2 ds = unpair(mul2(pair(px, py), fma2(pair(dp[e + u], dp[e + u + 1]), after2, u == 0 ? delta.x : delta.y)));
                 if (!ALL) {
                   // (a hidden row's dP may be anything)
                   if (px == 0.f) ds.x = 0.f;
@@ -493,7 +508,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
       // group 0 writes dK, the last one dV (both, where there is one)
 #pragma unroll 1
       for (int which = t == 0 ? 0 : 1; which <= (t == G - 1 ? 1 : 0); ++which) {
-        const float f = which == 0 ? a.scale : 1.f;
+        const float f = which == 0 ? a.scale : 1.f, kept = which == 0 ? 1.f / down : 1.f / prob_up;
         bool bad = false;
         T* dst = (T*)(which == 0 ? p.g.dk : p.g.dv) + ((long long)j * a.kv_heads + hk) * a.dim;
 #pragma unroll 2
@@ -503,6 +518,8 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
             tmem_ld16(quarter + kAcc + which * DP + d, reinterpret_cast<uint32_t(&)[16]>(x));
             tmem_wait_ld();
           }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] *= kept;
           if (far != nullptr) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -662,6 +679,7 @@ int grad_launch(GradArgs& p, cudaStream_t st) {
   p.stages = stages_q;
   p.wide = wide_rows(p.g.dq, a.dim);
   if (a.mask != nullptr) dq = dq_masked;
+  if (HALF) OCNN_CUDA_OK(cudaMemsetAsync(p.g.largest, 0, sizeof(unsigned), st));
   dq<<<dim3(ceil_div(a.n, W * 128 >> p.pack_log), a.heads >> p.pack_log), Dq::kThreads, Dq::smem(stages_q), st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_dq_kernel");
   if (p.a.sinks > 0) {

@@ -117,6 +117,26 @@ def test_wide_heads(window, sinks, masked, heads, kv):
     compare([700, 3, 400, 129], heads, kv, 128, BF16, window, sinks, causal, masked=masked)
 
 
+def test_small_gradients_in_half():
+  """float16 with gradients far below 1, over many keys: probabilities and their gradients are smaller than its smallest
+  numbers, the results are not.  Where p and ds are rounded, the bounds count half a step of their own, not of float16's
+  smallest number: they are kept at powers of two that bring them into its range (dq, dk: relative to the largest dO)."""
+  n = 6000
+  q, k, v, g = inputs(n, 1, 1, 64, F16, 11)
+  q, v = 0.2 * q, 16 * v
+  g = (g.float() * 2.0 ** -6).to(F16)
+  got = run(q, k, v, [0, n], g)
+  see = torch.ones(n, n, dtype=torch.bool, device='cuda')
+  wide = {name: (value, bound) for name, (value, bound) in
+          attention(q.float(), k.float(), v.float(), see, None, g.float()).items()}
+  u = 2.0 ** -11
+  for name, heavy in (('dv', 1.0), ('dq', 1.0), ('dk', 1.0)):
+    value = wide[name][0]
+    off = (got[name].double() - value).norm() / value.norm()
+    step = 2.0 ** -25 * math.sqrt(value.numel()) / value.norm()           # (the result's own smallest numbers)
+    assert off <= 3 * u + step, (name, off.item(), step.item())
+
+
 def test_large_scores():
   """Scores far apart and far from zero: the running maximum, not the scores, decides what is kept."""
   q, k, v, g = inputs(300, 2, 2, 64, F32, 3)
