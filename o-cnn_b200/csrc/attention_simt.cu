@@ -41,11 +41,11 @@ __device__ __forceinline__ void load_rows(float* dst, const void* base, long lon
 
 // acc[r][c] = A row (4 ty + r) . B row (tx + 16 c), even and odd channels side by side in one instruction
 template <int DP>
-__device__ __forceinline__ void tile_dot(const float* A, const float* B, float (&acc)[4][4]) {
+__device__ __forceinline__ void tile_dot(const float* A, const float* B, int dim, float (&acc)[4][4]) {
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   uint64_t sum[4][4] = {};
-#pragma unroll 4
-  for (int d = 0; d < DP; d += 4) {
+#pragma unroll 2
+  for (int d = 0; d < dim; d += 4) {                   // (rows hold zeros behind dim)
     ulonglong2 x[4], y[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const ulonglong2*>(A + (4 * ty + r) * (DP + kPad) + d);
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const AttnArgs a, T
     for (int c = 0; c < 4; ++c) j[c] = row_of(tx + 16 * c);
     __syncthreads();
     float s[4][4];
-    tile_dot<DP>(sq, sk, s);
+    tile_dot<DP>(sq, sk, a.dim, s);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const RowKeys rk = rows[4 * ty + r];
@@ -282,8 +282,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const AttnArgs a
     for (int c = 0; c < 4; ++c) j[c] = row_of(tx + 16 * c);
     __syncthreads();
     float s[4][4], dp[4][4];
-    tile_dot<DP>(sq, sk, s);
-    tile_dot<DP>(sg, sv, dp);
+    tile_dot<DP>(sq, sk, a.dim, s);
+    tile_dot<DP>(sg, sv, a.dim, dp);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const RowKeys rk = rows[4 * ty + r];
@@ -368,8 +368,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
       }
       __syncthreads();
       float s[4][4], dp[4][4];
-      tile_dot<DP>(sk, sq, s);
-      tile_dot<DP>(sv, sg, dp);
+      tile_dot<DP>(sk, sq, a.dim, s);
+      tile_dot<DP>(sv, sg, a.dim, dp);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const KeyRows kr = rows[4 * ty + r];
