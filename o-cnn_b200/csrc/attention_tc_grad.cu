@@ -128,12 +128,14 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     }
     if (HALF) {
       const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
-      if (lane == 0 && most != 0) atomicMax(p.g.largest, most);             // (a maximum: whatever the order)
+      // (a warp's nodes are in one chunk; a maximum is the same in any order)
+      const int chunk = (r0 + t * nodes + (((warp & 3) * 32) >> p.pack_log)) >> kChunkLog;
+      if (lane == 0 && most != 0) atomicMax(p.g.largest + chunk, most);
     }
-    const float down = HALF ? down_to_one(largest) : 1.f;                   // dS of this row is kept at dS * down
+    const float kept_at = HALF ? grad_scale(largest) : 1.f;                 // dS of this row is kept at dS * kept_at
     const FullBlocks whole(keys, r, MASKED, std::integral_constant<int, kBN>());
-    const uint64_t c2 = pair(a.scale_log2, a.scale_log2), lse2 = pair(-lse, -lse), delta2 = pair(-delta * down, -delta * down),
-                   down2 = pair(down, down);
+    const uint64_t c2 = pair(a.scale_log2, a.scale_log2), lse2 = pair(-lse, -lse), delta2 = pair(-delta * kept_at, -delta * kept_at),
+                   kept2 = pair(kept_at, kept_at);
     int done = 0;
     bool alive = true;
     KeptKeys<kBN> kept, ahead;
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
 #pragma unroll
       for (int e = 0; e < kBN; e += 2) {
         const float2 x = unpair(fma2(pair(s[e], s[e + 1]), c2, lse2));
-        const float2 ds = unpair(mul2(pair(exp2_approx(x.x), exp2_approx(x.y)), fma2(pair(dp[e], dp[e + 1]), down2, delta2)));
+        const float2 ds = unpair(mul2(pair(exp2_approx(x.x), exp2_approx(x.y)), fma2(pair(dp[e], dp[e + 1]), kept2, delta2)));
         s[e] = ds.x;
         s[e + 1] = ds.y;
       }
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     }
     if (alive) {
       bool bad = false;
-      const float up = a.scale / down;
+      const float up = a.scale / kept_at;
       T* dst = (T*)p.g.dq + ((long long)i * a.heads + h) * a.dim;
 #pragma unroll 2
       for (int d = 0; d < a.dim; d += 16) {
@@ -423,9 +425,9 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
     }
     const KeyRows kr = j < a.n ? attn_key_rows(a, j, attn_span_near(a, j, f, l)) : KeyRows{0, 0};
     const uint64_t c2 = pair(a.scale_log2, a.scale_log2);
-    // P' is kept at P' * prob_up, dS' at dS' * down
-    constexpr float prob_up = HALF ? kProbUp : 1.f, prob_log = HALF ? 10.f : 0.f;
-    const float down = HALF ? down_to_one(__uint_as_float(*p.g.largest)) : 1.f, after = down / prob_up;
+    // P' is kept at P' * prob_up, dS' at dS' * kept_at
+    constexpr float prob_up = HALF ? kProbUp : 1.f, prob_log = HALF ? kProbUpLog : 0.f;
+    const float kept_at = HALF && blocks > 0 ? grad_scale_of(p.g.largest, span.lo, span.hi) : 1.f, after = kept_at / prob_up;
     const uint64_t after2 = pair(after, after);
     // lse and delta of a block's rows: two threads a row fetch them a block ahead
     auto fetch = [&](int b) {
@@ -508,7 +510,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
       // group 0 writes dK, the last one dV (both, where there is one)
 #pragma unroll 1
       for (int which = t == 0 ? 0 : 1; which <= (t == G - 1 ? 1 : 0); ++which) {
-        const float f = which == 0 ? a.scale : 1.f, kept = which == 0 ? 1.f / down : 1.f / prob_up;
+        const float f = which == 0 ? a.scale : 1.f, back = which == 0 ? 1.f / kept_at : 1.f / prob_up;
         bool bad = false;
         T* dst = (T*)(which == 0 ? p.g.dk : p.g.dv) + ((long long)j * a.kv_heads + hk) * a.dim;
 #pragma unroll 2
@@ -519,7 +521,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
             tmem_wait_ld();
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] *= kept;
+          for (int e = 0; e < 16; ++e) x[e] *= back;
           if (far != nullptr) {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -679,7 +681,7 @@ int grad_launch(GradArgs& p, cudaStream_t st) {
   p.stages = stages_q;
   p.wide = wide_rows(p.g.dq, a.dim);
   if (a.mask != nullptr) dq = dq_masked;
-  if (HALF) OCNN_CUDA_OK(cudaMemsetAsync(p.g.largest, 0, sizeof(unsigned), st));
+  if (HALF) OCNN_CUDA_OK(cudaMemsetAsync(p.g.largest, 0, grad_chunks(a.n) * sizeof(unsigned), st));
   dq<<<dim3(ceil_div(a.n, W * 128 >> p.pack_log), a.heads >> p.pack_log), Dq::kThreads, Dq::smem(stages_q), st>>>(p);
   OCNN_LAUNCH_OK("attn_tc_dq_kernel");
   if (p.a.sinks > 0) {

@@ -357,6 +357,7 @@ Tensor octree_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, 
     TORCH_CHECK(aligned(*t), who, ": the caches' rows must be contiguous and start on 16-byte boundaries");
     TORCH_CHECK(at::has_internal_overlap(*t) != at::MemOverlap::Yes, who, ": the caches' places must not overlap");
   }
+  TORCH_CHECK(k_cache.numel() == 0 || k_cache.data_ptr() != v_cache.data_ptr(), who, ": the caches are the same memory");
   c10::cuda::CUDAGuard guard(q.device());
   auto row = [&](const Tensor& t) { return aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous); };
   const Tensor qr = row(q), kr = row(k), vr = row(v), len = lengths.contiguous();

@@ -137,6 +137,32 @@ def test_small_gradients_in_half():
     assert off <= 3 * u + step, (name, off.item(), step.item())
 
 
+def test_a_large_gradient_among_small_ones_in_half():
+  """One node's gradient 2^16 times the others': what does not see it keeps its precision (as above)."""
+  n = 3000
+  q, k, v, g = inputs(n, 2, 1, 32, F16, 12)
+  g = (g.float() * 2.0 ** -7).to(F16)
+  g[1500] = 2.0 ** 9
+  kw = dict(window=40, sinks=1, causal=False)
+  got = run(q, k, v, [0, n], g, **kw)
+  see = visible(n, [0, n], 40, 1, False, None, 'cuda')
+  far = (torch.arange(n, device='cuda') - 1500).abs() > 600         # (its chunk of 256 nodes, and windows around it)
+  far[0] = False                                                    # (the first node is seen by all)
+  u = 2.0 ** -11
+  for name, (value, _) in attention(q.float(), k.float(), v.float(), see, None, g.float()).items():
+    rows = far if name in ('dk', 'dv') else torch.arange(n, device='cuda') != 1500
+    off = (got[name].double() - value)[rows].norm() / value[rows].norm()
+    step = 2.0 ** -25 * math.sqrt(value[rows].numel()) / value[rows].norm()
+    assert off <= 3 * u + step, (name, off.item(), step.item())
+
+
+def test_many_short_sequences():
+  lengths = np.random.default_rng(3).integers(0, 4, 2500)
+  for dtype in (F32, BF16):
+    compare(list(lengths[:900]), 2, 1, 32, dtype, 2, 1, False)
+    compare(list(lengths), 1, 1, 16, dtype, 0, 0, True)
+
+
 def test_large_scores():
   """Scores far apart and far from zero: the running maximum, not the scores, decides what is kept."""
   q, k, v, g = inputs(300, 2, 2, 64, F32, 3)
@@ -378,7 +404,7 @@ def test_step_full_cache_and_refusals():
   bad = [(q, k, v, caches[0], caches[1], lengths.long()), (q, k, v, caches[0][:1], caches[1][:1], lengths),
          (q, k, v, caches[0].float(), caches[1].float(), lengths), (q[:, :3], k, v, caches[0], caches[1], lengths),
          (q, k, v, caches[0][:, :1].expand(2, 8, 2, 32), caches[1], lengths), (q, k, v, caches[0], caches[1], lengths.cpu()),
-         (q.cpu(), k, v, caches[0], caches[1], lengths)]
+         (q.cpu(), k, v, caches[0], caches[1], lengths), (q, k, v, caches[0], caches[0], lengths)]
   for args in bad:
     with pytest.raises(RuntimeError):
       ocnn.octree_attention_step(*args)
