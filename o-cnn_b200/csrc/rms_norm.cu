@@ -8,10 +8,12 @@
 // kept between the two.
 //
 // Bound: HBM.  Forward 2 rows read and 2 written, backward 4 read and 1 written.  A row is taken by as few lanes as hold
-// it in two to four vectors each (8 channels of 16 bits or 4 of 32), so that a warp has several rows in flight and the
-// statistics are a few shuffles; a row of more than 4 vectors x 32 lanes takes a block, and one that even a block cannot
-// keep in registers is read twice (the second time from L2).  gw: every thread keeps the sums of its own channels over
+// it in one vector each (8 channels of 16 bits or 4 of 32), so that a warp has several rows in flight and the statistics are
+// a few shuffles; wider ones by a warp with two or four vectors a lane, one of more than 4 vectors x 32 lanes by a block,
+// and one that even a block cannot keep in registers is read twice (the second time from L2).  gw: every thread keeps the sums of its own channels over
 // the rows of its block, a block's sums go to a slot of the workspace, and a second launch adds the slots in order.
+#include <atomic>
+
 #include "common.cuh"
 
 namespace ocnn {
@@ -283,12 +285,10 @@ __global__ void __launch_bounds__(1024) rms_norm_weight_kernel(const float* part
   }
 }
 
-// Blocks of a backward pass: its rows, at most four per SM (each leaves a slot of sums).  `blocks` below: a forward pass
-// where it is NULL, else where a backward pass says how many it took.
-int norm_blocks(long long rows, int rows_per_block) {
-  const long long need = (rows + rows_per_block - 1) / rows_per_block, cap = 4LL * sm_count();
-  return (int)(need < cap ? need : cap);
-}
+// Blocks of a backward pass, each of which leaves a slot of sums: its rows, at most as many as run at once (592 blocks where
+// 444 run leave a half-empty second wave: 68 us against 56 for 250 k rows of 96 channels of 16 bits) and kNormBlocks per SM.
+// `blocks` below: a forward pass where it is NULL, else where a backward pass says how many it took.
+constexpr int kNormBlocks = 6;
 
 template <typename T, int V, int LANES, int K>
 int norm_launch(const NormArgs& a, int* blocks_out, cudaStream_t st) {
@@ -300,20 +300,31 @@ int norm_launch(const NormArgs& a, int* blocks_out, cudaStream_t st) {
     OCNN_LAUNCH_OK("rms_norm_kernel");
     return OCNN_OK;
   }
-  const int blocks = *blocks_out = norm_blocks(a.rows, kRows);
   const size_t smem = K > 0 && a.partial != nullptr ? (size_t)kRows * LANES * K * V * 4 : 0;
+  static std::atomic<int> at_once{0};
+  int per_sm = at_once.load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    OCNN_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, rms_norm_backward_kernel<T, V, LANES, K>, kNormThreads,
+                                                               (size_t)kRows * LANES * K * V * 4));
+    per_sm = per_sm < 1 ? 1 : per_sm < kNormBlocks ? per_sm : kNormBlocks;
+    at_once.store(per_sm, std::memory_order_relaxed);
+  }
+  const long long need = (a.rows + kRows - 1) / kRows, cap = (long long)per_sm * sm_count();
+  const int blocks = *blocks_out = (int)(need < cap ? need : cap);
   OCNN_CUDA_OK(launch_chained(rms_norm_backward_kernel<T, V, LANES, K>, dim3(blocks), dim3(kNormThreads), smem, st, a));
   OCNN_LAUNCH_OK("rms_norm_backward_kernel");
   return OCNN_OK;
 }
 
-// Lanes per row: the fewest whose two vectors hold it; a whole warp, then a block, with up to four.
+// Lanes per row: the fewest of which each has one vector (with two, twice the registers hold half the rows: the gradient of
+// 61 k rows of 96 fp32 channels 30 us against 20); a whole warp, then a block, with up to four.
 template <typename T, int V>
 int norm_by_width(const NormArgs& a, int* blocks, cudaStream_t st) {
   const int vectors = (a.channels + V - 1) / V;
-  if (vectors <= 8) return norm_launch<T, V, 4, 2>(a, blocks, st);
-  if (vectors <= 16) return norm_launch<T, V, 8, 2>(a, blocks, st);
-  if (vectors <= 32) return norm_launch<T, V, 16, 2>(a, blocks, st);
+  if (vectors <= 4) return norm_launch<T, V, 4, 1>(a, blocks, st);
+  if (vectors <= 8) return norm_launch<T, V, 8, 1>(a, blocks, st);
+  if (vectors <= 16) return norm_launch<T, V, 16, 1>(a, blocks, st);
+  if (vectors <= 32) return norm_launch<T, V, 32, 1>(a, blocks, st);
   if (vectors <= 64) return norm_launch<T, V, 32, 2>(a, blocks, st);
   if (vectors <= 128) return norm_launch<T, V, 32, 4>(a, blocks, st);
   if (vectors <= 4 * kNormThreads) return norm_launch<T, V, kNormThreads, 4>(a, blocks, st);
@@ -361,7 +372,7 @@ int ocnn_add_rms_norm(const void* x_dev, int64_t x_row, const void* residual_dev
 }
 
 size_t ocnn_add_rms_norm_backward_workspace_bytes(int channels) {
-  return channels > 0 ? (size_t)4 * sm_count() * channels * sizeof(float) : 0;
+  return channels > 0 ? (size_t)kNormBlocks * sm_count() * channels * sizeof(float) : 0;
 }
 
 int ocnn_add_rms_norm_backward(const void* x_dev, int64_t x_row, const void* residual_dev, int64_t residual_row,
