@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 4 * W) tmem_alloc(tmem_holder, Shape::kCols);
+  grid_dependency_wait();
   const WarpOffsets offsets(a);
   Span f, l;
   const TileKeys tile_keys = attn_tile_keys(a, offsets, r0, r0 + W * nodes, f, l);
@@ -363,7 +364,8 @@ int fwd_launch_kernel(AttnFwdArgs& p, cudaStream_t st) {
   });
   if (status != OCNN_OK) return status;
   const int nodes = W * 128 >> p.pack_log;
-  attn_tc_kernel<DP, W, BN, NB, HALF, MASKED, CTAS><<<dim3(ceil_div(a.n, nodes), a.heads >> p.pack_log), Shape::kThreads, bytes, st>>>(p);
+  OCNN_CUDA_OK(launch_chained(attn_tc_kernel<DP, W, BN, NB, HALF, MASKED, CTAS>,
+                              dim3(ceil_div(a.n, nodes), a.heads >> p.pack_log), dim3(Shape::kThreads), bytes, st, p));
   OCNN_LAUNCH_OK("attn_tc_kernel");
   return OCNN_OK;
 }

@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 4 * W) tmem_alloc(tmem_holder, Shape::kCols);
+  grid_dependency_wait();
   const WarpOffsets offsets(a);
   Span f, l;
   const TileKeys tile_keys = attn_tile_keys(a, offsets, r0, r0 + W * nodes, f, l);
@@ -392,6 +393,7 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 4 * G) tmem_alloc(tmem_holder, Shape::kCols);
+  grid_dependency_wait();
   const WarpOffsets offsets(a);
   Span f, l;
   const KeyRows span = attn_tile_rows(a, offsets, k0, k0 + 128, f, l);
@@ -682,7 +684,8 @@ int grad_launch(GradArgs& p, cudaStream_t st) {
   p.wide = wide_rows(p.g.dq, a.dim);
   if (a.mask != nullptr) dq = dq_masked;
   if (HALF) OCNN_CUDA_OK(cudaMemsetAsync(p.g.largest, 0, grad_chunks(a.n) * sizeof(unsigned), st));
-  dq<<<dim3(ceil_div(a.n, W * 128 >> p.pack_log), a.heads >> p.pack_log), Dq::kThreads, Dq::smem(stages_q), st>>>(p);
+  OCNN_CUDA_OK(launch_chained(dq, dim3(ceil_div(a.n, W * 128 >> p.pack_log), a.heads >> p.pack_log), dim3(Dq::kThreads),
+                              Dq::smem(stages_q), st, p));
   OCNN_LAUNCH_OK("attn_tc_dq_kernel");
   if (p.a.sinks > 0) {
     const int far = attn_far_mma(p.a, p.g, HALF ? OCNN_F16 : OCNN_BF16, st);
@@ -694,7 +697,7 @@ int grad_launch(GradArgs& p, cudaStream_t st) {
   if (status != OCNN_OK) return status;
   p.stages = stages_k;
   p.wide = wide_rows(p.g.dk, a.dim) && wide_rows(p.g.dv, a.dim);
-  dkv<<<dim3(ceil_div(p.a.n, 128), p.a.kv_heads), Dkv::kThreads, Dkv::smem(stages_k), st>>>(p);
+  OCNN_CUDA_OK(launch_chained(dkv, dim3(ceil_div(p.a.n, 128), p.a.kv_heads), dim3(Dkv::kThreads), Dkv::smem(stages_k), st, p));
   OCNN_LAUNCH_OK("attn_tc_dkv_kernel");
   return OCNN_OK;
 }
