@@ -9,6 +9,12 @@ constexpr int kB = 64;                        // queries and keys per tile
 constexpr int kThreads = 256;                 // 16 x 16: thread (ty, tx) has rows 4 ty .. 4 ty + 3, columns tx + 16 c
 constexpr int kPad = 4;                       // a row of DP + 4 floats: 16 rows 16 bytes each hit distinct banks
 
+// Bound: instruction issue (fp32 products have no tensor pipe of their accuracy here) and, between a tile's barriers, the
+// latency of its loads, which other thread blocks cover: of up to 32 channels three per SM (80 registers), of 64 two.
+// Blocks of 16 columns that none of a warp's eight rows sees are left out.  Forward and gradients of 20 k nodes, 4 heads of
+// 24, window 64: 325 us (88 + 108 + 132 in the kernels); two blocks per SM and every column of a tile computed: 380.
+template <int DP> constexpr int kPerSm = DP == 32 ? 3 : DP == 64 ? 2 : 1;
+
 // Rows of a [n, heads, dim] tensor as floats, zeros for row < 0 and behind dim.  `index` gives the row for 0 .. kB - 1.
 template <typename T, int DP, typename Index>
 __device__ __forceinline__ void load_rows(float* dst, const void* base, long long row, long long head_offset, int dim,
@@ -39,66 +45,108 @@ __device__ __forceinline__ void load_rows(float* dst, const void* base, long lon
   }
 }
 
-// acc[r][c] = A row (4 ty + r) . B row (tx + 16 c), even and odd channels side by side in one instruction
+// Which blocks of 16 columns hold anything that one of the warp's eight rows sees: bit c for columns 16 c .. 16 c + 15.
+// `seen`: bit 4 r + c where the thread's row r sees its column tx + 16 c.
+__device__ __forceinline__ unsigned live_columns(unsigned seen) {
+  unsigned live = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) live |= __any_sync(0xffffffffu, (seen & (0x1111u << c)) != 0) ? 1u << c : 0u;
+  return live;
+}
+
+// acc[r][c] = A row (4 ty + r) . B row (tx + 16 (c0 + c)), even and odd channels side by side in one instruction, for
+// kDotCols blocks of columns: of 32 channels two at a time, since the sums of four do not fit the registers of three
+// thread blocks per SM.
+template <int DP> constexpr int kDotCols = DP == 32 ? 2 : 4;
 template <int DP>
-__device__ __forceinline__ void tile_dot(const float* A, const float* B, int dim, float (&acc)[4][4]) {
+__device__ __forceinline__ void tile_dot(const float* A, const float* B, int dim, int c0, float (&acc)[4][kDotCols<DP>]) {
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  uint64_t sum[4][4] = {};
-#pragma unroll 2
-  for (int d = 0; d < dim; d += 4) {                   // (rows hold zeros behind dim)
-    ulonglong2 x[4], y[4];
+  uint64_t sum[4][kDotCols<DP>] = {};
+#pragma unroll 1
+  for (int d = 0; d < dim; d += 4) {                     // (rows hold zeros behind dim)
+    ulonglong2 x[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const ulonglong2*>(A + (4 * ty + r) * (DP + kPad) + d);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) y[c] = *reinterpret_cast<const ulonglong2*>(B + (tx + 16 * c) * (DP + kPad) + d);
+    for (int c = 0; c < kDotCols<DP>; ++c) {
+      const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(B + (tx + 16 * (c0 + c)) * (DP + kPad) + d);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) sum[r][c] = fma2(x[r].y, y[c].y, fma2(x[r].x, y[c].x, sum[r][c]));
+      for (int r = 0; r < 4; ++r) sum[r][c] = fma2(x[r].y, y.y, fma2(x[r].x, y.x, sum[r][c]));
+    }
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < kDotCols<DP>; ++c) {
       const float2 f = unpair(sum[r][c]);
       acc[r][c] = f.x + f.y;
     }
 }
+template <int DP>
+__device__ __forceinline__ bool any_live(unsigned live, int c0) { return (live >> c0 & ((1u << kDotCols<DP>) - 1)) != 0; }
 
 constexpr int kPRow = kB + 4;
-// A thread's columns of a [kB][DP] tile: pairs 2 tx + 32 c (two adjacent floats a lane).
+// out = P B, where P has a row of kB columns per row of the tile and B a row of DP channels per column.  A thread sums
+// channels in fours, 4 l + 64 q with l = tx, so that a value of P is used for four at a time.  Of 32 channels there are
+// only eight fours: lanes tx and tx + 8 take the same one and every second four columns each, and exchange halves at the end.
+template <int DP> constexpr int kOutPairs = DP == 32 ? 2 : DP / 32;
 template <int DP>
-__device__ __forceinline__ int out_col(int c) { return 2 * (threadIdx.x & 15) + 32 * (c >> 1) + (c & 1); }
-
-// acc[r] += sum over the kB columns of P row (4 ty + r) * B row: out = P B, a thread's channels in pairs
+struct OutTile { uint64_t sum[4][kOutPairs<DP>]; };
 template <int DP>
-__device__ __forceinline__ void tile_mul(const float* P, const float* B, uint64_t (&acc)[4][DP / 32]) {
+__device__ __forceinline__ void tile_mul(const float* P, const float* B, unsigned live, OutTile<DP>& out) {
+  constexpr int kSplit = DP == 32 ? 2 : 1;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-#pragma unroll 2
-  for (int j = 0; j < kB; j += 4) {
-    float4 p[4];
+  const int l = DP == 32 ? tx & 7 : tx, shift = DP == 32 ? 4 * (tx >> 3) : 0;
+#pragma unroll 1
+  for (int j0 = 0; j0 < kB; j0 += 16) {
+    if (!(live >> (j0 / 16) & 1)) continue;
+#pragma unroll 1
+    for (int jj = 0; jj < 16; jj += 4 * kSplit) {
+      const int j = j0 + jj + shift;
+      float4 p[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) p[r] = *reinterpret_cast<const float4*>(P + (4 * ty + r) * kPRow + j);
+      for (int r = 0; r < 4; ++r) p[r] = *reinterpret_cast<const float4*>(P + (4 * ty + r) * kPRow + j);
 #pragma unroll
-    for (int jj = 0; jj < 4; ++jj) {
-      uint64_t v[DP / 32];
+      for (int k = 0; k < 4; ++k) {
+        ulonglong2 v[kOutPairs<DP> / 2];
 #pragma unroll
-      for (int c = 0; c < DP / 32; ++c)
-        v[c] = *reinterpret_cast<const uint64_t*>(B + (j + jj) * (DP + kPad) + 2 * tx + 32 * c);
+        for (int q = 0; q < kOutPairs<DP> / 2; ++q)
+          v[q] = *reinterpret_cast<const ulonglong2*>(B + (j + k) * (DP + kPad) + 4 * l + 64 * q);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float x = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
-        const uint64_t xx = pair(x, x);
+        for (int r = 0; r < 4; ++r) {
+          const float x = k == 0 ? p[r].x : k == 1 ? p[r].y : k == 2 ? p[r].z : p[r].w;
+          const uint64_t xx = pair(x, x);
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) acc[r][c] = fma2(xx, v[c], acc[r][c]);
+          for (int q = 0; q < kOutPairs<DP> / 2; ++q) {
+            out.sum[r][2 * q] = fma2(xx, v[q].x, out.sum[r][2 * q]);
+            out.sum[r][2 * q + 1] = fma2(xx, v[q].y, out.sum[r][2 * q + 1]);
+          }
+        }
       }
     }
   }
 }
-template <int N>
-__device__ __forceinline__ float channel(const uint64_t (&acc)[N], int c) {
-  const float2 f = unpair(acc[c / 2]);
-  return (c & 1) ? f.y : f.x;
+// A thread's share of row r, DP / 16 channels: the c-th is channel out_col(c).
+template <int DP>
+__device__ __forceinline__ int out_col(int c) {
+  const int tx = threadIdx.x & 15;
+  return DP == 32 ? 4 * (tx & 7) + 2 * (tx >> 3) + c : 4 * tx + 64 * (c >> 2) + (c & 3);
+}
+template <int DP>
+__device__ __forceinline__ void out_row(const OutTile<DP>& out, int r, float (&x)[DP / 16]) {
+  if (DP == 32) {
+    const bool upper = (threadIdx.x & 8) != 0;
+    const float2 low = unpair(out.sum[r][0]), high = unpair(out.sum[r][1]);
+    x[0] = (upper ? high.x : low.x) + __shfl_xor_sync(0xffffffffu, upper ? low.x : high.x, 8);
+    x[1] = (upper ? high.y : low.y) + __shfl_xor_sync(0xffffffffu, upper ? low.y : high.y, 8);
+  } else {
+#pragma unroll
+    for (int q = 0; q < DP / 32; ++q) {
+      const float2 f = unpair(out.sum[r][q]);
+      x[2 * q] = f.x;
+      x[2 * q + 1] = f.y;
+    }
+  }
 }
 
 __device__ __forceinline__ float row_max(float x) {
@@ -154,7 +202,7 @@ __device__ __forceinline__ TileKeys query_tile(const AttnArgs& a, int r0, RowKey
 
 // One tile of 64 queries of one head: a pass over the keys that they see, with a running maximum and sum per row.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_simt_kernel(const AttnArgs a, T* out, float* lse, bool vec) {
+__global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_kernel(const AttnArgs a, T* out, float* lse, bool vec) {
   extern __shared__ float smem[];
   float* sq = smem;
   float* sk = sq + kB * (DP + kPad);
@@ -167,7 +215,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const AttnArgs a, T
   const TileKeys keys = query_tile(a, r0, rows, ext);
   load_rows<T, DP>(sq, a.q, a.q_row, h * a.q_head, a.dim, vec, [&](int r) { return r0 + r < a.n ? r0 + r : -1; });
 
-  uint64_t acc[4][DP / 32] = {};
+  OutTile<DP> acc = {};
   float top[4], total[4] = {};
 #pragma unroll
   for (int r = 0; r < 4; ++r) top[r] = -INFINITY;
@@ -185,17 +233,31 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const AttnArgs a, T
 #pragma unroll
     for (int c = 0; c < 4; ++c) j[c] = row_of(tx + 16 * c);
     __syncthreads();
-    float s[4][4];
-    tile_dot<DP>(sq, sk, a.dim, s);
+    unsigned seen = 0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const RowKeys rk = rows[4 * ty + r];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) seen |= j[c] >= 0 && attn_sees(rk, j[c]) ? 1u << (4 * r + c) : 0u;
+    }
+    const unsigned live = live_columns(seen);
+    if (live == 0) continue;
+    float s[4][4];
+#pragma unroll
+    for (int c0 = 0; c0 < 4; c0 += kDotCols<DP>) {
+      float x[4][kDotCols<DP>] = {};
+      if (any_live<DP>(live, c0)) tile_dot<DP>(sq, sk, a.dim, c0, x);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < kDotCols<DP>; ++c)
+          s[r][c0 + c] = seen >> (4 * r + c0 + c) & 1 ? x[r][c] * a.scale_log2 : -INFINITY;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
       float m = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        s[r][c] = j[c] >= 0 && attn_sees(rk, j[c]) ? s[r][c] * a.scale_log2 : -INFINITY;
-        m = fmaxf(m, s[r][c]);
-      }
+      for (int c = 0; c < 4; ++c) m = fmaxf(m, s[r][c]);
       m = fmaxf(top[r], row_max(m));
       const float base = m == -INFINITY ? 0.f : m;          // a row that has seen nothing yet
       const float keep = exp2_approx(top[r] - base);
@@ -209,23 +271,24 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const AttnArgs a, T
       }
       total[r] = total[r] * keep + sum;
 #pragma unroll
-      for (int c = 0; c < DP / 32; ++c) acc[r][c] = fma2(acc[r][c], pair(keep, keep), 0);
+      for (int q = 0; q < kOutPairs<DP>; ++q) acc.sum[r][q] = fma2(acc.sum[r][q], pair(keep, keep), 0);
     }
     __syncwarp();                                            // (a row of P is written and read by one half warp)
-    tile_mul<DP>(sp, sv, acc);
+    tile_mul<DP>(sp, sv, live, acc);
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int i = r0 + 4 * ty + r;
     const float sum = row_sum(total[r]), inv = sum == 0.f ? 0.f : 1.f / sum;
     bool bad = not_finite(sum);
+    float x[DP / 16];
+    out_row<DP>(acc, r, x);
     if (i < a.n) {
 #pragma unroll
       for (int c = 0; c < DP / 16; ++c) {
-        const float x = channel(acc[r], c);
-        bad |= not_finite(x);
+        bad |= not_finite(x[c]);
         const int d = out_col<DP>(c);
-        if (d < a.dim) out[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(sum == 0.f ? 0.f : x * inv);
+        if (d < a.dim) out[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(sum == 0.f ? 0.f : x[c] * inv);
       }
       if (tx == 0 && lse != nullptr) lse[(long long)h * a.n + i] = sum == 0.f ? INFINITY : top[r] + log2f(sum);
     }
@@ -240,7 +303,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(const AttnArgs a, T
 // Gradient of the queries of one tile, and delta_i = dO_i . o_i for the keys' gradients.
 //     p = exp2(s - lse), ds = p (dO . v - delta), dq = scale sum_j ds k_j
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const AttnArgs a, const AttnGrad g, bool vec) {
+__global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_dq_kernel(const AttnArgs a, const AttnGrad g, bool vec) {
   extern __shared__ float smem[];
   float* sq = smem;
   float* sg = sq + kB * (DP + kPad);
@@ -267,7 +330,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const AttnArgs a
     delta[r] = row_sum(x);
     if (tx == 0 && i < a.n) g.delta[(long long)h * a.n + i] = delta[r];
   }
-  uint64_t acc[4][DP / 32] = {};
+  OutTile<DP> acc = {};
   for (int t0 = 0; t0 < keys.n; t0 += kB) {
     auto row_of = [&](int t) {
       if (t0 + t >= keys.n) return -1;
@@ -281,32 +344,42 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const AttnArgs a
 #pragma unroll
     for (int c = 0; c < 4; ++c) j[c] = row_of(tx + 16 * c);
     __syncthreads();
-    float s[4][4], dp[4][4];
-    tile_dot<DP>(sq, sk, a.dim, s);
-    tile_dot<DP>(sg, sv, a.dim, dp);
+    unsigned seen = 0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const RowKeys rk = rows[4 * ty + r];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const bool seen = j[c] >= 0 && attn_sees(rk, j[c]);
-        sp[(4 * ty + r) * kPRow + tx + 16 * c] =
-            seen ? exp2_approx(s[r][c] * a.scale_log2 - lse[r]) * (dp[r][c] - delta[r]) : 0.f;
-      }
+      for (int c = 0; c < 4; ++c) seen |= j[c] >= 0 && attn_sees(rk, j[c]) ? 1u << (4 * r + c) : 0u;
+    }
+    const unsigned live = live_columns(seen);
+    if (live == 0) continue;
+#pragma unroll
+    for (int c0 = 0; c0 < 4; c0 += kDotCols<DP>) {
+      if (!any_live<DP>(live, c0)) continue;
+      float s[4][kDotCols<DP>], dp[4][kDotCols<DP>];
+      tile_dot<DP>(sq, sk, a.dim, c0, s);
+      tile_dot<DP>(sg, sv, a.dim, c0, dp);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < kDotCols<DP>; ++c)
+          sp[(4 * ty + r) * kPRow + tx + 16 * (c0 + c)] =
+              seen >> (4 * r + c0 + c) & 1 ? exp2_approx(s[r][c] * a.scale_log2 - lse[r]) * (dp[r][c] - delta[r]) : 0.f;
     }
     __syncwarp();
-    tile_mul<DP>(sp, sk, acc);
+    tile_mul<DP>(sp, sk, live, acc);
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int i = r0 + 4 * ty + r;
     bool bad = false;
+    float x[DP / 16];
+    out_row<DP>(acc, r, x);
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const int d = out_col<DP>(c);
-      const float x = channel(acc[r], c);
-      bad |= not_finite(x);
-      if (i < a.n && d < a.dim) ((T*)g.dq)[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(x * a.scale);
+      bad |= not_finite(x[c]);
+      if (i < a.n && d < a.dim) ((T*)g.dq)[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(x[c] * a.scale);
     }
     const unsigned any = __ballot_sync(0xffffffffu, bad);
     if (tx == 0) redo[4 * ty + r] = (any >> (tid & 16)) & 0xffffu;
@@ -320,7 +393,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dq_kernel(const AttnArgs a
 // by head of the group; what the far pass has summed for first nodes is added at the end.
 //     dv_j = sum_i p_ij dO_i, dk_j = scale sum_i ds_ij q_i
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs a, const AttnGrad g, bool vec) {
+__global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_dkv_kernel(const AttnArgs a, const AttnGrad g, bool vec) {
   extern __shared__ float smem[];
   float* sk = smem;
   float* sv = sk + kB * (DP + kPad);
@@ -350,7 +423,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
   auto key = [&](int t) { return rows[t].hi > rows[t].lo ? k0 + t : -1; };
   load_rows<T, DP>(sk, a.k, a.k_row, hk * a.k_head, a.dim, vec, key);
   load_rows<T, DP>(sv, a.v, a.v_row, hk * a.v_head, a.dim, vec, key);
-  uint64_t dk[4][DP / 32] = {}, dv[4][DP / 32] = {};
+  OutTile<DP> dk = {}, dv = {};
   for (int hg = 0; hg < group; ++hg) {
     const int h = hk * group + hg;
     for (int i0 = ext[0]; i0 < ext[1]; i0 += kB) {
@@ -367,22 +440,34 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
         delta[c] = i[c] >= 0 ? g.delta[(long long)h * a.n + i[c]] : 0.f;
       }
       __syncthreads();
-      float s[4][4], dp[4][4];
-      tile_dot<DP>(sk, sq, a.dim, s);
-      tile_dot<DP>(sv, sg, a.dim, dp);
+      unsigned seen = 0;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const KeyRows kr = rows[4 * ty + r];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float p = i[c] >= kr.lo && i[c] < kr.hi ? exp2_approx(s[r][c] * a.scale_log2 - lse[c]) : 0.f;
-          sp[(4 * ty + r) * kPRow + tx + 16 * c] = p;
-          sd[(4 * ty + r) * kPRow + tx + 16 * c] = p == 0.f ? 0.f : p * (dp[r][c] - delta[c]);
-        }
+        for (int c = 0; c < 4; ++c) seen |= i[c] >= kr.lo && i[c] < kr.hi ? 1u << (4 * r + c) : 0u;
+      }
+      const unsigned live = live_columns(seen);
+      if (live == 0) continue;
+#pragma unroll
+      for (int c0 = 0; c0 < 4; c0 += kDotCols<DP>) {
+        if (!any_live<DP>(live, c0)) continue;
+        float s[4][kDotCols<DP>], dp[4][kDotCols<DP>];
+        tile_dot<DP>(sk, sq, a.dim, c0, s);
+        tile_dot<DP>(sv, sg, a.dim, c0, dp);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < kDotCols<DP>; ++c) {
+            const int at = (4 * ty + r) * kPRow + tx + 16 * (c0 + c);
+            const float p = seen >> (4 * r + c0 + c) & 1 ? exp2_approx(s[r][c] * a.scale_log2 - lse[c0 + c]) : 0.f;
+            sp[at] = p;
+            sd[at] = p == 0.f ? 0.f : p * (dp[r][c] - delta[c0 + c]);
+          }
       }
       __syncwarp();
-      tile_mul<DP>(sp, sg, dv);
-      tile_mul<DP>(sd, sq, dk);
+      tile_mul<DP>(sp, sg, live, dv);
+      tile_mul<DP>(sd, sq, live, dk);
     }
   }
 #pragma unroll
@@ -390,10 +475,13 @@ __global__ void __launch_bounds__(kThreads) attn_simt_dkv_kernel(const AttnArgs 
     const int j = k0 + 4 * ty + r;
     const float* far = j < a.n ? far_sums(a, g, j, hk) : nullptr;
     bool bad = false;
+    float dk_row[DP / 16], dv_row[DP / 16];
+    out_row<DP>(dk, r, dk_row);
+    out_row<DP>(dv, r, dv_row);
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const int d = out_col<DP>(c);
-      float x = channel(dk[r], c), y = channel(dv[r], c);
+      float x = dk_row[c], y = dv_row[c];
       bad |= not_finite(x) | not_finite(y);
       if (j >= a.n || d >= a.dim) continue;
       x += far != nullptr ? far[d] : 0.f;

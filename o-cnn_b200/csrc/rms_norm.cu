@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(1024) rms_norm_weight_kernel(const float* part
 }
 
 // Blocks of a backward pass, each of which leaves a slot of sums: its rows, at most as many as run at once (592 blocks where
-// 444 run leave a half-empty second wave: 68 us against 56 for 250 k rows of 96 channels of 16 bits) and kNormBlocks per SM.
+// 444 run leave a half-empty second wave: 68 us against 56 for 250 k rows of 128 channels of 16 bits) and kNormBlocks per SM.
 // `blocks` below: a forward pass where it is NULL, else where a backward pass says how many it took.
 constexpr int kNormBlocks = 6;
 
