@@ -690,7 +690,7 @@ int ocnn_add_rms_norm_backward(const void* x_dev, int64_t x_row, const void* res
 typedef struct ocnn_attention {
   const void *q_dev, *k_dev, *v_dev;
   int64_t q_stride[2], k_stride[2], v_stride[2];    /* node, head */
-  const int32_t* offsets_dev;                       /* batch + 1, ascending */
+  const int32_t* offsets_dev;                       /* batch + 1 (up to 2^24), ascending */
   const uint8_t* mask_dev;                          /* n, or NULL */
   int32_t batch, n, heads, kv_heads, dim, window, sinks, causal, dtype;
   float scale;

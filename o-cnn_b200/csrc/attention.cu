@@ -17,6 +17,8 @@ int check(const ocnn_attention* a, const char* who) {
   if (a->dim > kMaxHeadDim || a->sinks > kMaxSinks || a->heads > 65535)
     return fail(OCNN_ERR_UNSUPPORTED, "%s: heads of %d channels with %d first nodes (up to %d and %d)", who, a->dim,
                 a->sinks, kMaxHeadDim, kMaxSinks);
+  if (a->batch > kMaxSequences)
+    return fail(OCNN_ERR_UNSUPPORTED, "%s: %d sequences (up to %d)", who, a->batch, kMaxSequences);
   OCNN_REQUIRE(a->n == 0 || (a->q_dev && a->k_dev && a->v_dev && a->offsets_dev), "%s: null pointer", who);
   return OCNN_OK;
 }

@@ -15,6 +15,7 @@
 
 namespace ocnn {
 
+constexpr int kMaxSequences = 1 << 24;         // (the search in steps of 32 stays below 2^31)
 constexpr int kMaxSinks = 64;                 // first nodes that stay visible: "a few" (the far pass keeps their sums)
 constexpr int kMaxHeadDim = 128;
 

@@ -53,6 +53,12 @@ void once_only(const char* who) {
   TORCH_CHECK(!at::GradMode::is_enabled(), who, ": its gradient cannot be differentiated again (create_graph)");
 }
 
+// Nor do forward-mode derivatives pass through them.
+void no_tangent(std::initializer_list<Tensor> tensors, const char* who) {
+  for (const Tensor& t : tensors)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), who, ": it has no forward-mode derivative");
+}
+
 Tensor empty_rows(const Tensor& like) { return torch::empty(like.sizes(), like.options()); }
 
 // ---- rotary positions -----------------------------------------------------------------------------------------
@@ -109,6 +115,7 @@ struct Rotary : public torch::autograd::Function<Rotary> {
 
 Tensor octree_rotary(const Tensor& data, const Tensor& positions, const Tensor& freqs, const vector<int64_t>& sections,
                      bool interleaved) {
+  no_tangent({data}, "octree_rotary");
   if (at::GradMode::is_enabled() && data.requires_grad())
     return Rotary::apply(data, positions, freqs, sections, interleaved);
   return rotary_call(data, positions, freqs, sections, interleaved, false);
@@ -194,6 +201,7 @@ struct AddRmsNorm : public torch::autograd::Function<AddRmsNorm> {
 // (norm, sum): sum is data + residual, data itself without a residual.
 vector<Tensor> add_rms_norm(const Tensor& data, const c10::optional<Tensor>& residual, const Tensor& weight, double eps) {
   const bool has = residual.has_value() && residual->defined();
+  no_tangent({data, weight, has ? *residual : Tensor()}, "add_rms_norm");
   vector<Tensor> out;
   if (at::GradMode::is_enabled() && (data.requires_grad() || weight.requires_grad() || (has && residual->requires_grad())))
     out = AddRmsNorm::apply(data, residual, weight, eps);
@@ -224,7 +232,7 @@ Operands operands(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   TORCH_CHECK(window >= 0 && window < (1LL << 31) && sinks >= 0 && sinks <= 64, who, ": window ", window, " with ", sinks,
               " first nodes (0 or more; 0 to 64)");
   TORCH_CHECK(offsets.device() == q.device() && offsets.scalar_type() == torch::kInt32 && offsets.dim() == 1 &&
-                  offsets.size(0) >= 1,
+                  offsets.size(0) >= 1 && offsets.size(0) < (1LL << 31),
               who, ": offsets must hold batch + 1 int32 values, on the data's device");
   Operands o;
   o.q = rows_of(q);
@@ -312,6 +320,7 @@ struct Attention : public torch::autograd::Function<Attention> {
 
 Tensor octree_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, int64_t window,
                         int64_t sinks, bool causal, const c10::optional<Tensor>& mask, c10::optional<double> scale) {
+  no_tangent({q, k, v}, "octree_attention");
   const double s = scale.has_value() ? *scale : q.dim() == 3 && q.size(2) > 0 ? 1.0 / std::sqrt((double)q.size(2)) : 1.0;
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return Attention::apply(q, k, v, offsets, mask, window, sinks, causal, s);
@@ -327,6 +336,7 @@ Tensor octree_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, 
   TORCH_CHECK(!(at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                k_cache.requires_grad() || v_cache.requires_grad())),
               who, ": it has no gradient (call it under torch.no_grad())");
+  no_tangent({q, k, v, k_cache, v_cache}, who);
   need_like(k, q, "k", who);
   need_like(v, q, "v", who);
   need_like(k_cache, q, "k_cache", who);

@@ -97,3 +97,9 @@ def test_no_cpu_path():
                lambda: ocnn.add_rms_norm(x, None, torch.ones(16))):
     with pytest.raises(RuntimeError, match='CUDA'):
       call()
+
+
+def test_attention_of_too_many_sequences():
+  a = attention(batch=(1 << 24) + 1)
+  assert L.ocnn_octree_attention(ctypes.byref(a), P(64), None, P(64), None) == UNSUPPORTED
+  assert L.ocnn_octree_attention_backward_workspace_bytes(ctypes.byref(a)) == 0
