@@ -82,7 +82,8 @@ def octree_attention_step(q, k, v, k_cache, v_cache, lengths, window=0, sinks=0,
 
 
 class AddRMSNorm(_nn.Module):
-  """`add_rms_norm` on node data [1, C, H, 1]: forward(data, residual=None) -> (norm, sum), channels_last."""
+  """`add_rms_norm` on node data [1, C, H, 1]: forward(data, residual=None) -> (norm, sum), channels_last, in the wider of
+  the two's types."""
 
   def __init__(self, channels, eps=1e-6):
     super().__init__()
@@ -90,6 +91,9 @@ class AddRMSNorm(_nn.Module):
     self.weight = _nn.Parameter(torch.ones(channels))
 
   def forward(self, data, residual=None):
+    if residual is not None and residual.dtype != data.dtype:    # (autocast: a 16-bit branch joins float32 data)
+      dtype = torch.promote_types(data.dtype, residual.dtype)
+      data, residual = data.to(dtype), residual.to(dtype)
     norm, total = add_rms_norm(_rows(data), None if residual is None else _rows(residual), self.weight, self.eps)
     return _nodes(norm), _nodes(total)
 

@@ -313,3 +313,34 @@ def test_modules_keep_their_frequencies():
   for bad in ((30, 4, None), (32, 4, 3), (12, 4, 4)):
     with pytest.raises(ValueError):
       ocnn.OctreeAttention(*bad)
+
+
+def test_no_forward_mode_derivatives():
+  from torch.autograd import forward_ad
+  q, w = randn(6, 2, 16), randn(16)
+  cache = torch.zeros(6, 4, 2, 16, device='cuda')
+  off, lengths = (torch.tensor(x, dtype=torch.int32, device='cuda') for x in ([0, 6], [0] * 6))
+  with forward_ad.dual_level():
+    dual = forward_ad.make_dual(q, torch.ones_like(q))
+    for call in (lambda: ocnn.octree_attention(q, dual, q, off), lambda: ocnn.add_rms_norm(q, dual, w),
+                 lambda: ocnn.octree_attention_step(dual, q, q, cache, cache.clone(), lengths),
+                 lambda: ocnn.octree_rotary(dual, q[:, 0, :3], ocnn.rotary_freqs([4, 2, 2]), [4, 2, 2])):
+      with pytest.raises(RuntimeError, match='forward-mode'):
+        call()
+
+
+def test_block_under_autocast():
+  """Products and attention in bfloat16, norms and the residual in float32: no more roundings than bfloat16 data has
+  (test_block), so its bound holds."""
+  torch.manual_seed(0)
+  _, seq = a_level(4)
+  block = ocnn.OctreeAttentionBlock(64, 4, kv_heads=2, window=40, sinks=1).cuda()
+  data = randn(1, 64, seq.positions.shape[0], 1).contiguous(memory_format=torch.channels_last)
+  want = block_reference(block, data, seq, None)
+  leaf = data.clone().requires_grad_()
+  with torch.autocast('cuda', dtype=BF16):
+    out = block(leaf, seq)
+  assert out.dtype == F32
+  assert (out[0, :, :, 0].t().double() - want).abs().max().item() <= 32 * 2.0 ** -8 * want.abs().max().item()
+  out.sum().backward()
+  assert leaf.grad.dtype == F32 and all(p.grad is not None and torch.isfinite(p.grad).all() for p in block.parameters())
