@@ -7,6 +7,8 @@
 // Bound: HBM, every channel read and written once.  The angles of a node are the same for all its heads: a block forms
 // the cosines and sines of its nodes once, in shared memory.  An angle is formed and brought into one turn in 64 bits
 // (a position of 2^16 times a frequency of 1 has lost 2^-8 of a turn in 32), sine and cosine of the rest in 32.
+#include <cstring>
+
 #include "common.cuh"
 
 namespace ocnn {
@@ -38,10 +40,35 @@ __device__ __forceinline__ void rot_set(float& y, float x) { y = x; }
 __device__ __forceinline__ void rot_set(__nv_bfloat16& y, float x) { y = __float2bfloat16(x); }
 __device__ __forceinline__ void rot_set(__half& y, float x) { y = __float2half(x); }
 
+// 16 bytes at a time, the first to leave the caches when something else needs the room.
+template <typename P>
+__device__ __forceinline__ P read_once(const void* p) {
+  P x;
+  if constexpr (sizeof(P) == 16) {
+    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p));
+    memcpy(&x, &w, 16);
+  } else {
+    x = *reinterpret_cast<const P*>(p);
+  }
+  return x;
+}
+template <typename P>
+__device__ __forceinline__ void write_once(void* p, const P& x) {
+  if constexpr (sizeof(P) == 16) {
+    uint4 w;
+    memcpy(&w, &x, 16);
+    __stcs(reinterpret_cast<uint4*>(p), w);
+  } else {
+    *reinterpret_cast<P*>(p) = x;
+  }
+}
+
+// One item at a time on six blocks per SM: 250 k nodes of 16 heads of 32 in bf16 104 us, 61 k of 8 heads of 24 in fp32 22
+// (two items, which leave four blocks: 106 and 26; without that hint to the caches 110 and 23).
 // An item is V pairs of one head of one node.  Pairs side by side: two runs of V channels, half a head apart;
 // interleaved: one run of 2V channels (as two packs).
 template <typename T, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRotThreads, 4) rotary_kernel(const RotaryArgs a) {
+__global__ void __launch_bounds__(kRotThreads, 6) rotary_kernel(const RotaryArgs a) {
   extern __shared__ float2 turn[];          // [rows_per_block][pairs]
   const long long r0 = (long long)blockIdx.x * a.rows_per_block;
   const int rows = (int)min((long long)a.rows_per_block, a.rows - r0);
@@ -66,34 +93,21 @@ __global__ void __launch_bounds__(kRotThreads, 4) rotary_kernel(const RotaryArgs
     const T* src = (const T*)a.x + (r0 + mine) * a.row + h * a.head + c;
     T* dst = (T*)a.y + ((r0 + mine) * a.heads + h) * a.dim + c;
     const long long src_step = step * a.row, dst_step = (long long)step * a.heads * a.dim;
-    constexpr int U = 2;
-    for (int r = mine; r < rows; r += U * step) {
-      Pack<T, V> lo[U], hi[U];
+    for (int r = mine; r < rows; r += step, src += src_step, dst += dst_step) {
+      Pack<T, V> lo = read_once<Pack<T, V>>(src), hi = read_once<Pack<T, V>>(src + (INTERLEAVED ? V : half));
+      const float2* w = turn + r * a.pairs + t;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (r + u * step >= rows) break;
-        lo[u] = *reinterpret_cast<const Pack<T, V>*>(src + u * src_step);
-        hi[u] = *reinterpret_cast<const Pack<T, V>*>(src + u * src_step + (INTERLEAVED ? V : half));
+      for (int i = 0; i < V; ++i) {
+        if (i >= live) break;                   // (behind the last axis' pairs: as they are, whatever they are)
+        // interleaved: pair i is elements 2i, 2i + 1 of the run of 2V
+        T& x1 = INTERLEAVED ? (2 * i < V ? lo.x[(2 * i) % V] : hi.x[(2 * i) % V]) : lo.x[i];
+        T& x2 = INTERLEAVED ? (2 * i + 1 < V ? lo.x[(2 * i + 1) % V] : hi.x[(2 * i + 1) % V]) : hi.x[i];
+        const float f1 = rot_f32(x1), f2 = rot_f32(x2);
+        rot_set(x1, f1 * w[i].x - f2 * w[i].y);
+        rot_set(x2, f2 * w[i].x + f1 * w[i].y);
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (r + u * step >= rows) break;
-        const float2* w = turn + (r + u * step) * a.pairs + t;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (i >= live) break;                 // (behind the last axis' pairs: as they are, whatever they are)
-          // interleaved: pair i is elements 2i, 2i + 1 of the run of 2V
-          T& x1 = INTERLEAVED ? (2 * i < V ? lo[u].x[(2 * i) % V] : hi[u].x[(2 * i) % V]) : lo[u].x[i];
-          T& x2 = INTERLEAVED ? (2 * i + 1 < V ? lo[u].x[(2 * i + 1) % V] : hi[u].x[(2 * i + 1) % V]) : hi[u].x[i];
-          const float f1 = rot_f32(x1), f2 = rot_f32(x2);
-          rot_set(x1, f1 * w[i].x - f2 * w[i].y);
-          rot_set(x2, f2 * w[i].x + f1 * w[i].y);
-        }
-        *reinterpret_cast<Pack<T, V>*>(dst + u * dst_step) = lo[u];
-        *reinterpret_cast<Pack<T, V>*>(dst + u * dst_step + (INTERLEAVED ? V : half)) = hi[u];
-      }
-      src += U * src_step;
-      dst += U * dst_step;
+      write_once(dst, lo);
+      write_once(dst + (INTERLEAVED ? V : half), hi);
     }
   }
 }
