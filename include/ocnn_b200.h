@@ -684,7 +684,8 @@ int ocnn_add_rms_norm_backward(const void* x_dev, int64_t x_row, const void* res
  *   causal:  j <= i and (i - j < window or j - start < sinks);   else:  |i - j| < window or j - start < sinks
  * (window 0: every key) and mask[j] != 0 (mask NULL: all).  out_i = sum_j softmax_j(scale * q_i . k_j) v_j, zeros for a
  * node that sees nothing and for nodes outside of every sequence.  q: heads, k and v: kv_heads (a divisor of heads),
- * dim up to 128, sinks up to 64.  out: contiguous; lse: [heads][n] fp32 for the backward pass, or NULL.
+ * dim up to 128, sinks up to 64.  out: contiguous; lse: what the backward pass needs of
+ * this one, or NULL: ocnn_octree_attention_saved_bytes for [heads][n] fp32 and, of 16-bit data, what rounding took from out.
  * The backward pass takes the same structure, out and lse of the forward pass and the gradient of out; dq, dk, dv:
  * contiguous.  status_dev: as in ocnn_octree_conv_tc. */
 typedef struct ocnn_attention {
@@ -695,6 +696,7 @@ typedef struct ocnn_attention {
   int32_t batch, n, heads, kv_heads, dim, window, sinks, causal, dtype;
   float scale;
 } ocnn_attention;
+size_t ocnn_octree_attention_saved_bytes(const ocnn_attention* attention);
 int ocnn_octree_attention(const ocnn_attention* attention, void* out_dev, float* lse_dev, int32_t* status_dev,
                           void* stream);
 size_t ocnn_octree_attention_backward_workspace_bytes(const ocnn_attention* attention);

@@ -77,9 +77,15 @@ int ocnn_octree_attention(const ocnn_attention* p, void* out_dev, float* lse_dev
   if (status != OCNN_OK || p->n == 0) return status;
   OCNN_REQUIRE(out_dev && status_dev, "ocnn_octree_attention: null pointer");
   const AttnArgs a = args_of(p);
-  if (on_tensor_cores(p) && reinterpret_cast<uintptr_t>(out_dev) % 16 == 0)
+  if (on_tensor_cores(p) && (reinterpret_cast<uintptr_t>(out_dev) | reinterpret_cast<uintptr_t>(lse_dev)) % 16 == 0)
     return attn_tc_forward(a, p->dtype, out_dev, lse_dev, status_dev, (cudaStream_t)stream);
   return attn_simt_forward(a, p->dtype, out_dev, lse_dev, all_on_boundary(p, 4), (cudaStream_t)stream);
+}
+
+size_t ocnn_octree_attention_saved_bytes(const ocnn_attention* p) {
+  if (check(p, "ocnn_octree_attention_saved_bytes") != OCNN_OK || p->n == 0) return 0;
+  const AttnArgs a = args_of(p);
+  return attn_lse_floats(a) * sizeof(float) + (p->dtype == OCNN_F32 ? 0 : (size_t)a.n * a.heads * a.dim * 2);
 }
 
 size_t ocnn_octree_attention_backward_workspace_bytes(const ocnn_attention* p) {
@@ -108,8 +114,8 @@ int ocnn_octree_attention_backward(const ocnn_attention* p, const void* out_dev,
   g.far = g.delta + delta_floats(p);
   g.dq = dq_dev, g.dk = dk_dev, g.dv = dv_dev;
   if (on_tensor_cores(p) && map_strides(grad_stride, a.n, a.heads) && on_boundary(grad_dev, grad_stride, p->dim, 8, 2) &&
-      (reinterpret_cast<uintptr_t>(out_dev) | reinterpret_cast<uintptr_t>(dq_dev) | reinterpret_cast<uintptr_t>(dk_dev) |
-       reinterpret_cast<uintptr_t>(dv_dev)) % 16 == 0)
+      (reinterpret_cast<uintptr_t>(out_dev) | reinterpret_cast<uintptr_t>(lse_dev) | reinterpret_cast<uintptr_t>(dq_dev) |
+       reinterpret_cast<uintptr_t>(dk_dev) | reinterpret_cast<uintptr_t>(dv_dev)) % 16 == 0)
     return attn_tc_backward(a, g, p->dtype, status_dev, (cudaStream_t)stream);
   const bool vec = all_on_boundary(p, 4) && on_boundary(grad_dev, grad_stride, p->dim, 4, size_of(p->dtype)) &&
                    reinterpret_cast<uintptr_t>(out_dev) % (4 * size_of(p->dtype)) == 0;

@@ -276,6 +276,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_kernel(const A
     __syncwarp();                                            // (a row of P is written and read by one half warp)
     tile_mul<DP>(sp, sv, live, acc);
   }
+  T* rest = attn_rest<T>(a, lse);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int i = r0 + 4 * ty + r;
@@ -288,7 +289,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_kernel(const A
       for (int c = 0; c < DP / 16; ++c) {
         bad |= not_finite(x[c]);
         const int d = out_col<DP>(c);
-        if (d < a.dim) out[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(sum == 0.f ? 0.f : x[c] * inv);
+        if (d >= a.dim) continue;
+        const long long at = ((long long)i * a.heads + h) * a.dim + d;
+        const float y = sum == 0.f ? 0.f : x[c] * inv;
+        out[at] = from_f32<T>(y);
+        if (sizeof(T) == 2 && rest != nullptr) rest[at] = from_f32<T>(rounded_off<T>(y));
       }
       if (tx == 0 && lse != nullptr) lse[(long long)h * a.n + i] = sum == 0.f ? INFINITY : top[r] + log2f(sum);
     }
@@ -326,7 +331,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_dq_kernel(cons
     const int i = r0 + 4 * ty + r;
     lse[r] = i < a.n ? g.lse[(long long)h * a.n + i] : INFINITY;
     float x = 0.f;
-    for (int d = tx; d < DP; d += 16) x = fmaf(sg[(4 * ty + r) * (DP + kPad) + d], sk[(4 * ty + r) * (DP + kPad) + d], x);
+    for (int d = tx; d < DP; d += 16) {
+      float o = sk[(4 * ty + r) * (DP + kPad) + d];
+      if (sizeof(T) == 2 && i < a.n && d < a.dim) o += to_f32(attn_rest<T>(a, g.lse)[((long long)i * a.heads + h) * a.dim + d]);
+      x = fmaf(sg[(4 * ty + r) * (DP + kPad) + d], o, x);
+    }
     delta[r] = row_sum(x);
     if (tx == 0 && i < a.n) g.delta[(long long)h * a.n + i] = delta[r];
   }

@@ -111,14 +111,16 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
     if (in) {
       const T* go = (const T*)p.g.grad + i * p.g.grad_row + h * p.g.grad_head;
       const T* o = (const T*)p.g.out + ((long long)i * a.heads + h) * a.dim;
+      const T* rest = attn_rest<T>(a, p.g.lse) + ((long long)i * a.heads + h) * a.dim;
       for (int d = 0; d < a.dim; d += 8) {
         const uint4 x = *reinterpret_cast<const uint4*>(go + d), y = *reinterpret_cast<const uint4*>(o + d);
-        const uint32_t *xs = &x.x, *ys = &y.x;
+        const uint4 z = *reinterpret_cast<const uint4*>(rest + d);
+        const uint32_t *xs = &x.x, *ys = &y.x, *zs = &z.x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 u = unpack2(xs[e], HALF), v = unpack2(ys[e], HALF);
-          delta = fmaf(u.x, v.x, delta);
-          delta = fmaf(u.y, v.y, delta);
+          const float2 u = unpack2(xs[e], HALF), v = unpack2(ys[e], HALF), w = unpack2(zs[e], HALF);
+          delta = fmaf(u.x, v.x + w.x, delta);
+          delta = fmaf(u.y, v.y + w.y, delta);
           if (HALF) {
             if (!not_finite(u.x)) largest = fmaxf(largest, fabsf(u.x));
             if (!not_finite(u.y)) largest = fmaxf(largest, fabsf(u.y));

@@ -274,7 +274,8 @@ Tensor attention_call(const Operands& o, Tensor* lse) {
   c10::cuda::CUDAGuard guard(o.q.device());
   const Tensor status = ocnn_tc_status(o.q.device());
   Tensor out = torch::empty({o.q.size(0), o.q.size(1), o.q.size(2)}, o.q.options());
-  if (lse != nullptr) *lse = torch::empty({o.q.size(1), o.q.size(0)}, o.q.options().dtype(torch::kFloat32));
+  if (lse != nullptr)
+    *lse = torch::empty({(int64_t)ocnn_octree_attention_saved_bytes(&o.a) / 4 + 1}, o.q.options().dtype(torch::kFloat32));
   OCNN_CALL(ocnn_octree_attention(&o.a, out.data_ptr(), lse != nullptr ? lse->data_ptr<float>() : nullptr,
                                   status.data_ptr<int32_t>(), current_stream()));
   return out;

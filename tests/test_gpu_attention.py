@@ -431,3 +431,19 @@ def test_step_in_a_graph():
     graph.replay()
     want = ocnn.octree_attention_step(q, k, v, *twins, torch.full_like(lengths, t), 16)
     assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(caches, twins))
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16])
+@pytest.mark.parametrize('dim,causal', [(32, True), (128, False), (20, True)])
+def test_gradients_are_rounded_twice_at_most(dtype, dim, causal):
+  """A gradient's terms are rounded once (p, ds), and so is their sum: two independent errors of one size, 1.42 times that of
+  a result that is only rounded; no third of that size (out's own rounding, through delta) joins them: 1.74 with it."""
+  lengths = [700, 300]
+  offsets, n = offsets_of(lengths), 1000
+  q, k, v, g = inputs(n, 4, 4, dim, dtype, 5)
+  got = run(q, k, v, offsets, g, window=16, causal=causal)
+  want = attention(q, k, v, visible(n, offsets, 16, 0, causal, None, 'cuda'), None, g)
+  for name in ('out', 'dq', 'dk', 'dv'):
+    value = want[name][0]
+    once = (value.to(dtype).double() - value).norm()
+    assert (got[name].detach().double() - value).norm() <= 1.5 * once, name
