@@ -232,7 +232,8 @@ __device__ __forceinline__ float warp_sum(float x) {
 // ---- rows key by key ----------------------------------------------------------------------------------------
 // A tile multiplies a hidden pair's probability, 0, by whatever the hidden value is: 0 x inf is not 0.  A row whose
 // result is not finite is therefore formed once more by its warp, from the keys that it sees only (where one of those
-// is not finite the result stays what it is).
+// is not finite the result is none either, however small its probability).  A row without a visible key is zeros; one whose
+// visible scores are all -inf has no softmax: NaN.
 template <typename T>
 __device__ void attn_forward_row(const AttnArgs& a, int i, int h, T* out, float* lse) {
   const int lane = threadIdx.x & 31;
@@ -243,10 +244,12 @@ __device__ void attn_forward_row(const AttnArgs& a, int i, int h, T* out, float*
 #pragma unroll
   for (int c = 0; c < 4; ++c) qv[c] = lane + 32 * c < a.dim ? to_f32(q[lane + 32 * c]) : 0.f;
   float top = -INFINITY, total = 0.f;
+  bool sees = false;
   const int n_first = max(0, min(r.first, r.lo) - r.start), behind = max(r.hi, r.first);
   for (int t = 0; t < n_first + behind - r.lo; ++t) {
     const int j = t < n_first ? r.start + t : r.lo + t - n_first;
     if (!attn_sees(r, j) || (a.mask != nullptr && a.mask[j] == 0)) continue;
+    sees = true;
     const T* k = (const T*)a.k + j * a.k_row + hk * a.k_head;
     const T* v = (const T*)a.v + j * a.v_row + hk * a.v_head;
     float s = 0.f;
@@ -254,25 +257,27 @@ __device__ void attn_forward_row(const AttnArgs& a, int i, int h, T* out, float*
     for (int c = 0; c < 4; ++c)
       if (lane + 32 * c < a.dim) s += qv[c] * to_f32(k[lane + 32 * c]);
     s = warp_sum(s) * a.scale_log2;
-    const float m = fmaxf(top, s), keep = m == -INFINITY ? 1.f : exp2f(top - m);
-    const float p = m == -INFINITY ? 0.f : exp2f(s - m);
+    const float last = top;
+    // (fmaxf passes a NaN score by, the exponential does not: it stays in the sum whatever the maximum is)
+    top = fmaxf(top, s);
+    const float base = top == -INFINITY ? 0.f : top, keep = exp2f(last - base), p = exp2f(s - base);
     total = total * keep + p;
-    top = m;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (lane + 32 * c < a.dim) acc[c] = acc[c] * keep + (p == 0.f ? 0.f : p * to_f32(v[lane + 32 * c]));
+      if (lane + 32 * c < a.dim) acc[c] = acc[c] * keep + p * to_f32(v[lane + 32 * c]);
   }
+  if (sees && total == 0.f) total = NAN;
   T* rest = attn_rest<T>(a, lse);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     if (lane + 32 * c < a.dim) {
       const long long at = ((long long)i * a.heads + h) * a.dim + lane + 32 * c;
-      const float x = total == 0.f ? 0.f : acc[c] / total;
+      const float x = sees ? acc[c] / total : 0.f;
       out[at] = from_f32<T>(x);
       if (rest != nullptr) rest[at] = from_f32<T>(rounded_off<T>(x));
     }
   if (lse != nullptr && lane == 0)
-    lse[(long long)h * a.n + i] = total == 0.f ? INFINITY : top + log2f(total);
+    lse[(long long)h * a.n + i] = sees ? top + log2f(total) : INFINITY;
 }
 
 // Gradient of query i of head h from the keys that it sees, and of key j from the queries that see it: as
@@ -301,9 +306,9 @@ __device__ void attn_dq_row(const AttnArgs& a, const AttnGrad& g, int i, int h) 
     float k[4], v[4];
     attn_row<T>(a.k, j * a.k_row + hk * a.k_head, a.dim, k);
     attn_row<T>(a.v, j * a.v_row + hk * a.v_head, a.dim, v);
-    const float p = exp2f(attn_dot(q, k) * a.scale_log2 - lse), ds = p == 0.f ? 0.f : p * (attn_dot(go, v) - delta);
+    const float p = exp2f(attn_dot(q, k) * a.scale_log2 - lse), ds = p * (attn_dot(go, v) - delta);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc[c] += ds == 0.f ? 0.f : ds * k[c];
+    for (int c = 0; c < 4; ++c) acc[c] += ds * k[c];
   }
 #pragma unroll
   for (int c = 0; c < 4; ++c)
@@ -325,11 +330,11 @@ __device__ void attn_dkv_row(const AttnArgs& a, const AttnGrad& g, int j, int hk
       attn_row<T>(a.q, i * a.q_row + h * a.q_head, a.dim, q);
       attn_row<T>(g.grad, i * g.grad_row + h * g.grad_head, a.dim, go);
       const float p = exp2f(attn_dot(q, k) * a.scale_log2 - g.lse[(long long)h * a.n + i]);
-      const float ds = p == 0.f ? 0.f : p * (attn_dot(go, v) - g.delta[(long long)h * a.n + i]);
+      const float ds = p * (attn_dot(go, v) - g.delta[(long long)h * a.n + i]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        dk[c] += ds == 0.f ? 0.f : ds * q[c];
-        dv[c] += p == 0.f ? 0.f : p * go[c];
+        dk[c] += ds * q[c];
+        dv[c] += p * go[c];
       }
     }
   }

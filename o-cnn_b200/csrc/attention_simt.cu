@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_kernel(const A
 
   OutTile<DP> acc = {};
   float top[4], total[4] = {};
+  unsigned ever = 0;                                         // as `seen`, of all tiles so far
 #pragma unroll
   for (int r = 0; r < 4; ++r) top[r] = -INFINITY;
   for (int t0 = 0; t0 < keys.n; t0 += kB) {
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_kernel(const A
 #pragma unroll
       for (int c = 0; c < 4; ++c) seen |= j[c] >= 0 && attn_sees(rk, j[c]) ? 1u << (4 * r + c) : 0u;
     }
+    ever |= seen;
     const unsigned live = live_columns(seen);
     if (live == 0) continue;
     float s[4][4];
@@ -280,7 +282,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_kernel(const A
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int i = r0 + 4 * ty + r;
-    const float sum = row_sum(total[r]), inv = sum == 0.f ? 0.f : 1.f / sum;
+    const bool sees = (__ballot_sync(0xffffffffu, (ever >> (4 * r) & 15u) != 0) >> (tid & 16) & 0xffffu) != 0;
+    float sum = row_sum(total[r]);
+    if (sees && sum == 0.f) sum = NAN;                       // scores of -inf alone have no softmax
+    const float inv = sees ? 1.f / sum : 0.f;
     bool bad = not_finite(sum);
     float x[DP / 16];
     out_row<DP>(acc, r, x);
@@ -291,11 +296,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_kernel(const A
         const int d = out_col<DP>(c);
         if (d >= a.dim) continue;
         const long long at = ((long long)i * a.heads + h) * a.dim + d;
-        const float y = sum == 0.f ? 0.f : x[c] * inv;
+        const float y = sees ? x[c] * inv : 0.f;
         out[at] = from_f32<T>(y);
         if (sizeof(T) == 2 && rest != nullptr) rest[at] = from_f32<T>(rounded_off<T>(y));
       }
-      if (tx == 0 && lse != nullptr) lse[(long long)h * a.n + i] = sum == 0.f ? INFINITY : top[r] + log2f(sum);
+      if (tx == 0 && lse != nullptr) lse[(long long)h * a.n + i] = sees ? top[r] + log2f(sum) : INFINITY;
     }
     const unsigned any = __ballot_sync(0xffffffffu, bad);
     if (tx == 0) redo[4 * ty + r] = (any >> (tid & 16)) & 0xffffu;
@@ -469,9 +474,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_dkv_kernel(con
 #pragma unroll
           for (int c = 0; c < kDotCols<DP>; ++c) {
             const int at = (4 * ty + r) * kPRow + tx + 16 * (c0 + c);
-            const float p = seen >> (4 * r + c0 + c) & 1 ? exp2_approx(s[r][c] * a.scale_log2 - lse[c0 + c]) : 0.f;
+            const bool see = seen >> (4 * r + c0 + c) & 1;
+            const float p = see ? exp2_approx(s[r][c] * a.scale_log2 - lse[c0 + c]) : 0.f;
             sp[at] = p;
-            sd[at] = p == 0.f ? 0.f : p * (dp[r][c] - delta[c0 + c]);
+            sd[at] = see ? p * (dp[r][c] - delta[c0 + c]) : 0.f;
           }
       }
       __syncwarp();

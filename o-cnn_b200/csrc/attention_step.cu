@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kStepThreads) attn_step_kernel(const StepArgs 
       l += f * *cluster.map_shared_rank(&sl[0][g], c);
       x += f * *cluster.map_shared_rank(&so[0][g][d], c);
     }
-    const float y = keys.full ? __int_as_float(0x7fc00000) : l == 0.f ? 0.f : x / l;
+    const float y = keys.full ? __int_as_float(0x7fc00000) : keys.n == 0 ? 0.f : x / l;
     ((T*)a.out)[((long long)b * a.heads + hk * group + g0 + g) * a.dim + d] = from_f32<T>(y);
   }
   if (part == 0 && g0 == 0 && keys.live && tid < 2 * LPK && in) {    // (lanes 0 .. 2 LPK - 1 hold every d0 twice)
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(32 * kMmaWarps) attn_step_mma_kernel(const Ste
       l += f * *cluster.map_shared_rank(sl + head, c);
       x += f * *cluster.map_shared_rank(so + head * DP + d, c);
     }
-    const float y = keys.full ? __int_as_float(0x7fc00000) : l == 0.f ? 0.f : x / l;
+    const float y = keys.full ? __int_as_float(0x7fc00000) : keys.n == 0 ? 0.f : x / l;
     ((T*)a.out)[((long long)b * a.heads + hk * group + g0 + head) * a.dim + d] = from_f32<T>(y);
   }
   if (part == 0 && g0 == 0 && keys.live && tid < a.dim / 4) {   // the new row: dim / 8 pieces of K, then of V

@@ -117,6 +117,8 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
     const float c = a.scale_log2;
     const uint64_t c2 = pair(c, c);
     float ref = -INFINITY, total = 0.f;                                    // the reference, in powers of two
+    uint32_t seen = r.hi > r.lo;                                           // (a node in a sequence sees itself, unless hidden)
+    if (MASKED) seen = 0;
     int done = 0;
     bool alive = true;
     KeptKeys<BN> kept, ahead;
@@ -137,6 +139,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
         for (int k = 0; k < BN / 32; ++k) {
           bits[k] = first ? seen_first(keys, r, 32 * k) : seen_bits(a, r, j + 32 * k);
           if (MASKED) bits[k] &= kept.bits(k);
+          if (MASKED) seen |= bits[k];
         }
       }
       alive = mbar_wait(smem_u32(&sfull[NB * t + place]), (done / NB) & 1, abort_flag, p.status, kErrAttnS);
@@ -207,7 +210,8 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
     alive = __all_sync(0xffffffffu, alive);
     tc_fence_after();
     if (alive) {
-      const bool none = total == 0.f;
+      const bool none = seen == 0;
+      if (!none && total == 0.f) total = NAN;                              // scores of -inf alone have no softmax
       const float inv = none ? 0.f : 1.f / total;
       bool bad = not_finite(total);
       T* dst = (T*)p.out + ((long long)i * a.heads + h) * a.dim;

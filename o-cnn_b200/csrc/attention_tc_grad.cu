@@ -481,8 +481,8 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
                 float2 ds = unpair(mul2(pair(px, py), fma2(pair(dp[e + u], dp[e + u + 1]), after2, u == 0 ? delta.x : delta.y)));
                 if (!ALL) {
                   // (a hidden row's dP may be anything)
-                  if (px == 0.f) ds.x = 0.f;
-                  if (py == 0.f) ds.y = 0.f;
+                  if (!((bits[k] >> (e + u)) & 1)) ds.x = 0.f;
+                  if (!((bits[k] >> (e + u + 1)) & 1)) ds.y = 0.f;
                 }
                 w[(e + u) / 2] = pack16<HALF>(px, py);
                 v[(e + u) / 2] = pack16<HALF>(ds.x, ds.y);

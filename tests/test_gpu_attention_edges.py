@@ -1,0 +1,93 @@
+"""Attention where its results are easily lost."""
+import math
+
+import pytest
+import torch
+
+import ocnn
+from attention_reference import visible
+from test_gpu_attention import inputs, run
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+# ---- values that are no numbers -------------------------------------------------------------------------------------
+def row_by_row(q, k, v, see, grad):
+  """The definition in 64 bits, every row from the keys that it sees alone: a row that sees nothing is zeros, and a visible
+  value that is no number goes where its product goes (0 x inf is none either)."""
+  scale = q.shape[2] ** -0.5
+  q, k, v, grad, see = (t.detach().cpu() for t in (q, k, v, grad, see))
+  q, k, v, grad = (t.double() for t in (q, k, v, grad))
+  group = q.shape[1] // k.shape[1]
+  res = {'out': torch.zeros_like(q), 'dq': torch.zeros_like(q), 'dk': torch.zeros_like(k), 'dv': torch.zeros_like(v)}
+  for i in range(q.shape[0]):
+    keys = see[i].nonzero()[:, 0]
+    for h in range(q.shape[1] if keys.numel() else 0):
+      kh, vh, go = k[keys, h // group], v[keys, h // group], grad[i, h]
+      p = torch.softmax((kh * q[i, h]).sum(1) * scale, 0)
+      out = (p[:, None] * vh).sum(0)
+      ds = p * ((vh * go).sum(1) - (out * go).sum()) * scale
+      res['out'][i, h] = out
+      res['dq'][i, h] = (ds[:, None] * kh).sum(0)
+      res['dk'][keys, h // group] += ds[:, None] * q[i, h]
+      res['dv'][keys, h // group] += p[:, None] * go
+  return res
+
+
+def spoil(what, q, k, v, g):
+  if what == 'query':
+    q[40], q[90, 1] = math.nan, math.nan
+  elif what == 'key':                         # (seen by 32 .. 48 both ways: by 48 as the first of its window)
+    k[40] = math.nan
+    k[100, :, 3] = math.inf
+  elif what == 'all keys minus infinity':     # (30 .. 42 see nothing else)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    k[22:51, :, 0] = -math.inf
+  elif what == 'value of a weak key':         # (its probability is 0 in 32 bits)
+    q[:, :, 0], k[:, :, 0] = 30.0, 0.0
+    k[60, :, 0], v[60, :, 5] = -60.0, math.inf
+  elif what == 'gradient':
+    g[70, 0], g[75, :, 2] = math.inf, math.nan
+  else:
+    g[:] = math.inf
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('dim', [32, 128])
+@pytest.mark.parametrize('masked,causal', [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize('what', ['query', 'key', 'all keys minus infinity', 'value of a weak key', 'gradient', 'every gradient'])
+def test_what_is_no_number_is_seen(dtype, dim, masked, causal, what):
+  """Without first nodes, so that a row's first key may be the one that is no number.  What is finite in the definition is
+  finite here, and what is not is not.  Off by a few roundings to the data's type, and by those of a score's terms in 32
+  bits, which add up to less than 16 in size."""
+  n, offsets = 130, [0, 70, 130]
+  q, k, v, g = inputs(n, 2, 1, dim, dtype, 21)
+  spoil(what, q, k, v, g)
+  mask = None
+  if masked:
+    mask = torch.rand(n, generator=torch.Generator(device='cuda').manual_seed(3), device='cuda') < 0.6
+    mask[:12], mask[40], mask[22] = False, True, True                       # (rows 0 .. 3 see nothing)
+  got = run(q, k, v, offsets, g, window=9, causal=causal, mask=mask)
+  quiet = run(q, k, v, offsets, window=9, causal=causal, mask=mask)['out']
+  want = row_by_row(q, k, v, visible(n, offsets, 9, 0, causal, mask, 'cuda'), g)
+  assert masked or not all(want[name].isfinite().all() for name in want)
+  assert torch.equal(quiet.nan_to_num(), got['out'].nan_to_num())
+  for name in want:
+    value, fine = got[name].detach().double().cpu(), want[name].isfinite()
+    assert torch.equal(value.isfinite(), fine), name
+    if fine.any():
+      off = (value - want[name])[fine].abs().max().item()
+      assert off <= (16 * torch.finfo(dtype).eps + (dim + 4) * 2.0 ** -20) * want[name][fine].abs().max().item(), name
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+def test_a_step_that_sees_minus_infinity_alone(dtype):
+  """Scores of minus infinity and nothing else: softmax has no value there; a sequence that is passed over has zeros."""
+  q, k, v, _ = inputs(3, 4, 2, 32, dtype)
+  caches = [torch.randn(3, 40, 2, 32, device='cuda').to(dtype) for _ in range(2)]
+  q[0, :, 0], k[0, :, 0], caches[0][0, :, :, 0] = 1.0, -math.inf, -math.inf
+  lengths = torch.tensor([30, 30, -1], dtype=torch.int32, device='cuda')
+  out = ocnn.octree_attention_step(q, k, v, *caches, lengths, 0)
+  assert out[0].isnan().all() and out[1].isfinite().all() and not out[2].any()
