@@ -9,6 +9,7 @@
 // sequence's key head, each CTA a stretch of the visible positions, each warp its rows with a running maximum and sum;
 // the parts are joined in shared memory, first the warps', then the CTAs' through the cluster's: one launch, no
 // workspace, the same bits every time.
+// float16 holds nothing below 2^-24: the rounded p, at most 1, is kept at 2^15 p there.
 //   16-bit caches: every warp copies its rows, 16 at a time, into a ring of its own (cp.async, one row after the other:
 //   rolled caches and the new row need no case of their own) and multiplies them with mma.sync, 16 query heads at a time.
 //   On the CUDA cores, a product and a shuffle per value for each query head, 64 sequences of 4100 rows, 16 heads over 4
@@ -241,6 +242,7 @@ __global__ void __launch_bounds__(32 * kMmaWarps) attn_step_mma_kernel(const Ste
   using Shape = StepShape<DP>;
   using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
   constexpr int KS = DP / 16, kThreads = 32 * kMmaWarps, kChunks = DP / 8, kStep = 32 / kChunks;
+  constexpr float up = HALF ? 15.f : 0.f;                        // (p is kept at 2^up p, and so is its sum)
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int group = a.heads / a.kv_heads, chunks = (group + kMmaHeads - 1) / kMmaHeads;
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(32 * kMmaWarps) attn_step_mma_kernel(const Ste
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] = exp2_approx(x[e] - base);
+          x[e] = exp2_approx(x[e] + (up - base));
           total[h] += x[e];
         }
         // (rounded to the data's type for the product; the sum is of the unrounded values)

@@ -7,7 +7,8 @@
 // with 128 threads per tile, one row each, between the two products.  m is the row's reference: its running maximum, but
 // moved only when a block exceeds it by more than 8 (any reference gives the same quotient as long as nothing overflows,
 // and 2^8 is far from that), so O is hardly ever scaled.  P is rounded to the data's type, which is what the product takes;
-// its sum is of the unrounded values.  Scores have two places, so that a block's are ready when its rows come to it.
+// its sum is of the unrounded values.  float16 holds nothing below 2^-24: there p is kept at 2^7 p, 2^15 at most (of 10^5 keys at
+// 2^-25 of the strongest, 0.3 % of their values would be lost otherwise).  Scores have two places, so that a block's are ready when its rows come to it.
 //
 // Roles: 4 W warps of rows, W warps that issue products (one thread of each), one warp that brings Q and the blocks of K
 // and V by TMA into a ring of slots (and clears the rows that the mask hides: see clear_rows).
@@ -116,6 +117,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
     const FullBlocks whole(keys, r, MASKED, std::integral_constant<int, BN>());
     const float c = a.scale_log2;
     const uint64_t c2 = pair(c, c);
+    constexpr float up = HALF ? 7.f : 0.f;                                 // (p is kept at 2^up p, and so is its sum)
     float ref = -INFINITY, total = 0.f;                                    // the reference, in powers of two
     uint32_t seen = r.hi > r.lo;                                           // (a node in a sequence sees itself, unless hidden)
     if (MASKED) seen = 0;
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
         }
       }
       const float base = ref == -INFINITY ? 0.f : ref;
-      const uint64_t base2 = pair(-base, -base);
+      const uint64_t base2 = pair(up - base, up - base);
       uint64_t sums[2] = {pair(total, 0.f), 0};
 #pragma unroll
       for (int k = 0; k < BN / 32; ++k) {
@@ -243,7 +245,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
           if (i < a.n) store_row<HALF>(rest, d, a.dim, p.wide, x);
         }
       }
-      if (i < a.n && p.lse != nullptr) p.lse[(long long)h * a.n + i] = none ? INFINITY : ref + log2f(total);
+      if (i < a.n && p.lse != nullptr) p.lse[(long long)h * a.n + i] = none ? INFINITY : ref + (log2f(total) - up);
       unsigned redo = __ballot_sync(0xffffffffu, bad && i < a.n);
       while (redo != 0) {
         const int at = __ffs(redo) - 1;

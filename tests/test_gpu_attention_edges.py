@@ -91,3 +91,51 @@ def test_a_step_that_sees_minus_infinity_alone(dtype):
   lengths = torch.tensor([30, 30, -1], dtype=torch.int32, device='cuda')
   out = ocnn.octree_attention_step(q, k, v, *caches, lengths, 0)
   assert out[0].isnan().all() and out[1].isfinite().all() and not out[2].any()
+
+
+# ---- weak keys in float16 ---------------------------------------------------------------------------------------------
+def weak_keys(n, dim, least):
+  """One strong key of value 1 and n - 1 about 2^-25 as strong of value 16: keys, values, the output, and how far it may be off
+  when probabilities are kept in float16 at a power of two where its smallest step is `least` of the strongest: half of that
+  step each, u = 2^-11 of the larger ones and of the result, 2^-20 for the sums in 32 bits and (dim + 4) 2^-24 of a score."""
+  gen = torch.Generator(device='cuda').manual_seed(1)
+  k = torch.zeros(n, 1, dim, device='cuda', dtype=F16)
+  k[1:, 0, 0] = -(16.5 + 2 * torch.rand(n - 1, generator=gen, device='cuda')).to(F16)
+  v = torch.full_like(k, 16.0)
+  v[0] = 1.0
+  return (k, v) + weak_output(k, v, least)
+
+
+def weak_output(k, v, least):
+  """(output, bound) of weak_keys, for those keys and values."""
+  p = torch.softmax(k[:, 0, 0].double(), 0)
+  out = (p * v[:, 0, 0].double()).sum()
+  heavy = out * (2.0 ** -11 + 2.0 ** -20 + (k.shape[2] + 4) * 2.0 ** -24 * 18.5)
+  return out.item(), (2.0 ** -11 * out + heavy + 0.5 * least * v.double()[:, 0, 0].sum()).item()
+
+
+@pytest.mark.parametrize('dim', [16, 64, 128])
+def test_many_weak_keys_in_half(dim):
+  """The reference may lie 2^8 below the maximum, never above it; p is kept at 2^7 p at least."""
+  n = 100000
+  k, v, value, bound = weak_keys(n, dim, 2.0 ** -24 / 2.0 ** 7)
+  q = torch.zeros(n, 1, dim, device='cuda', dtype=F16)
+  q[:, 0, 0] = 1.0
+  out = ocnn.octree_attention(q, k, v, torch.tensor([0, n], dtype=torch.int32, device='cuda'), scale=1.0)
+  assert value > 1.01 and (out.double() - value).abs().max().item() <= bound
+
+
+@pytest.mark.parametrize('dim,n', [(8, 100000), (40, 40000), (72, 40000)])
+def test_many_weak_keys_in_a_step_in_half(dim, n):
+  """More sequences than there is room for clusters of several CTAs, so that four warps share a sequence: a strong key for
+  each (rows come to them in sixteens), p at 2^15 p."""
+  k, v, _, _ = weak_keys(n, dim, 0.0)
+  k[0:64:16, 0, 0], v[0:64:16] = 0.0, 1.0
+  value, bound = weak_output(k, v, 2.0 ** -24 / 2.0 ** 15)
+  q = torch.zeros(600, 1, dim, device='cuda', dtype=F16)
+  q[..., 0] = 1.0
+  caches = [t[None].repeat(600, 1, 1, 1) for t in (k, v)]
+  lengths = torch.full((600,), n - 1, dtype=torch.int32, device='cuda')
+  new = [t[-1:].expand(600, 1, dim) for t in (k, v)]
+  out = ocnn.octree_attention_step(q, *new, *caches, lengths, scale=1.0)
+  assert (out.double() - value).abs().max().item() <= bound
