@@ -147,6 +147,7 @@ class AttentionCache:
     at, left = node - ends[b], ends[b + 1] - node
     keep = inside & ((at < sinks) | (left <= capacity - sinks))
     place = torch.where(at < capacity, at, sinks + (at - sinks) % max(capacity - sinks, 1))
+    keep &= place < capacity                 # (more first nodes than places: what does not fit has none)
     b, place = b[keep], place[keep]
     self.k[b, place] = k[keep].detach()
     self.v[b, place] = v[keep].detach()

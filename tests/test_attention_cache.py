@@ -1,0 +1,34 @@
+"""The attention layer's cache and its refusals, on the CPU."""
+import pytest
+import torch
+
+import ocnn
+
+
+def filled(lengths, capacity, sinks, first=0, tail=0):
+  """(cache, packed keys): key of node t of sequence b is 1000 b + t + 1."""
+  cache = ocnn.AttentionCache(len(lengths), capacity, 1, 8, torch.float32, 'cpu')
+  keys = torch.cat([torch.zeros(first)] + [1000.0 * b + 1 + torch.arange(float(n)) for b, n in enumerate(lengths)] +
+                   [torch.zeros(tail)])
+  rows = keys[:, None, None].expand(-1, 1, 8)
+  offsets = torch.tensor([first + sum(lengths[:b]) for b in range(len(lengths) + 1)], dtype=torch.int32)
+  cache.fill(rows, -rows, offsets, sinks)
+  return cache
+
+
+@pytest.mark.parametrize('capacity,sinks', [(1, 0), (2, 4), (4, 4), (3, 5), (8, 3), (8, 0), (16, 64)])
+def test_fill(capacity, sinks):
+  """Every position that a place is for lies there, the last that came to it; more first nodes than the cache has room for are
+  a cache that does not roll: as many positions as it holds."""
+  lengths = [0, 1, capacity, capacity + 1, 3 * capacity + 2]
+  cache = filled(lengths, capacity, sinks, first=2, tail=3)
+  assert cache.lengths.tolist() == lengths
+  for b, n in enumerate(lengths):
+    places = {}
+    for x in range(n):
+      place = x if x < capacity else sinks + (x - sinks) % (capacity - sinks) if sinks < capacity else None
+      if place is not None:
+        places[place] = 1000 * b + x + 1
+    got = cache.k[b, :, 0, 0]
+    assert got.tolist() == [float(places.get(place, 0)) for place in range(capacity)], (b, n)
+    assert torch.equal(cache.v[b], -cache.k[b])
