@@ -139,6 +139,8 @@ class AttentionCache:
     """The nodes of a packed batch (as in `octree_attention`), as many of each sequence as `step` will look at: all, or
     the first `sinks` and the last capacity - sinks."""
     capacity = self.k.shape[1]
+    if offsets.shape[0] != self.lengths.shape[0] + 1:
+      raise RuntimeError('AttentionCache.fill: {} sequences for a cache of {}'.format(offsets.shape[0] - 1, self.lengths.shape[0]))
     node = torch.arange(k.shape[0], device=k.device)
     ends = offsets.long()
     b = torch.searchsorted(ends, node, right=True) - 1

@@ -32,3 +32,18 @@ def test_fill(capacity, sinks):
     got = cache.k[b, :, 0, 0]
     assert got.tolist() == [float(places.get(place, 0)) for place in range(capacity)], (b, n)
     assert torch.equal(cache.v[b], -cache.k[b])
+
+
+def test_fill_of_another_batch():
+  for sequences in (1, 2, 4):
+    cache = ocnn.AttentionCache(3, 8, 1, 8, torch.float32, 'cpu')
+    offsets = torch.arange(sequences + 1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match='sequences'):
+      cache.fill(torch.zeros(sequences, 1, 8), torch.zeros(sequences, 1, 8), offsets)
+    assert not cache.lengths.any()
+
+
+def test_fill_of_no_sequences():
+  cache = ocnn.AttentionCache(0, 8, 1, 8, torch.float32, 'cpu')
+  cache.fill(torch.zeros(2, 1, 8), torch.zeros(2, 1, 8), torch.zeros(1, dtype=torch.int32))
+  assert cache.lengths.shape == (0,)
