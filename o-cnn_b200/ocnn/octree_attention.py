@@ -190,7 +190,10 @@ class OctreeAttention(_nn.Module):
     return qk[:, :self.heads], qk[:, self.heads:], rows[:, turned:]
 
   def forward(self, data, sequence, mask=None, residual=None, cache=None):
-    """data [1, C, H, 1]; sequence: `octree_sequence` of its level.  cache: an AttentionCache to fill for `step`."""
+    """data [1, C, H, 1]; sequence: `octree_sequence` of its level.  cache: an AttentionCache to fill for `step`, which sees
+    every node of it: not beside a mask."""
+    if mask is not None and cache is not None:
+      raise RuntimeError('OctreeAttention: a step would see the nodes that the mask hides (a cache beside a mask)')
     q, k, v = self._heads(data.contiguous(memory_format=torch.channels_last), sequence.positions)
     out = octree_attention(q, k, v, sequence.offsets, self.window, self.sinks, self.causal, mask)
     if cache is not None:

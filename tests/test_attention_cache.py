@@ -47,3 +47,12 @@ def test_fill_of_no_sequences():
   cache = ocnn.AttentionCache(0, 8, 1, 8, torch.float32, 'cpu')
   cache.fill(torch.zeros(2, 1, 8), torch.zeros(2, 1, 8), torch.zeros(1, dtype=torch.int32))
   assert cache.lengths.shape == (0,)
+
+
+def test_no_mask_beside_a_cache():
+  """A step cannot know which of the cache's nodes were hidden."""
+  cache = ocnn.AttentionCache(1, 8, 4, 8, torch.float32, 'cpu')
+  data, mask = torch.zeros(1, 32, 5, 1), torch.ones(5, dtype=torch.bool)
+  seq = ocnn.OctreeSequence(torch.tensor([0, 5], dtype=torch.int32), torch.zeros(5, 3))
+  with pytest.raises(RuntimeError, match='mask'):
+    ocnn.OctreeAttention(32, 4, causal=True)(data, seq, mask, cache=cache)
