@@ -4,6 +4,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -53,10 +54,15 @@ void once_only(const char* who) {
   TORCH_CHECK(!at::GradMode::is_enabled(), who, ": its gradient cannot be differentiated again (create_graph)");
 }
 
-// Nor do forward-mode derivatives pass through them.
-void no_tangent(std::initializer_list<Tensor> tensors, const char* who) {
-  for (const Tensor& t : tensors)
-    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), who, ": it has no forward-mode derivative");
+// Nor do forward-mode derivatives pass through them, and neither a tracer nor a torch.func transform would see what they do.
+void plain_call(std::initializer_list<Tensor> tensors, const char* who) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), who, ": it cannot be traced (torch.jit.trace)");
+  for (const Tensor& t : tensors) {
+    if (!t.defined()) continue;
+    TORCH_CHECK(!t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper})),
+                who, ": it cannot be transformed (torch.func)");
+    TORCH_CHECK(!t._fw_grad(0).defined(), who, ": it has no forward-mode derivative");
+  }
 }
 
 Tensor empty_rows(const Tensor& like) { return torch::empty(like.sizes(), like.options()); }
@@ -115,7 +121,7 @@ struct Rotary : public torch::autograd::Function<Rotary> {
 
 Tensor octree_rotary(const Tensor& data, const Tensor& positions, const Tensor& freqs, const vector<int64_t>& sections,
                      bool interleaved) {
-  no_tangent({data}, "octree_rotary");
+  plain_call({data}, "octree_rotary");
   if (at::GradMode::is_enabled() && data.requires_grad())
     return Rotary::apply(data, positions, freqs, sections, interleaved);
   return rotary_call(data, positions, freqs, sections, interleaved, false);
@@ -201,7 +207,7 @@ struct AddRmsNorm : public torch::autograd::Function<AddRmsNorm> {
 // (norm, sum): sum is data + residual, data itself without a residual.
 vector<Tensor> add_rms_norm(const Tensor& data, const c10::optional<Tensor>& residual, const Tensor& weight, double eps) {
   const bool has = residual.has_value() && residual->defined();
-  no_tangent({data, weight, has ? *residual : Tensor()}, "add_rms_norm");
+  plain_call({data, weight, has ? *residual : Tensor()}, "add_rms_norm");
   vector<Tensor> out;
   if (at::GradMode::is_enabled() && (data.requires_grad() || weight.requires_grad() || (has && residual->requires_grad())))
     out = AddRmsNorm::apply(data, residual, weight, eps);
@@ -321,7 +327,7 @@ struct Attention : public torch::autograd::Function<Attention> {
 
 Tensor octree_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets, int64_t window,
                         int64_t sinks, bool causal, const c10::optional<Tensor>& mask, c10::optional<double> scale) {
-  no_tangent({q, k, v}, "octree_attention");
+  plain_call({q, k, v}, "octree_attention");
   const double s = scale.has_value() ? *scale : q.dim() == 3 && q.size(2) > 0 ? 1.0 / std::sqrt((double)q.size(2)) : 1.0;
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
     return Attention::apply(q, k, v, offsets, mask, window, sinks, causal, s);
@@ -332,12 +338,12 @@ Tensor octree_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, 
                              const Tensor& v_cache, const Tensor& lengths, int64_t window, int64_t sinks,
                              c10::optional<double> scale) {
   const char* who = "octree_attention_step";
+  plain_call({q, k, v, k_cache, v_cache}, who);
   TORCH_CHECK(q.is_cuda(), who, ": the data tensor must be a CUDA tensor (there is no CPU path)");
   TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, who, ": q, k and v must have shape [batch, heads, dim]");
   TORCH_CHECK(!(at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
                                                k_cache.requires_grad() || v_cache.requires_grad())),
               who, ": it has no gradient (call it under torch.no_grad())");
-  no_tangent({q, k, v, k_cache, v_cache}, who);
   need_like(k, q, "k", who);
   need_like(v, q, "v", who);
   need_like(k_cache, q, "k_cache", who);

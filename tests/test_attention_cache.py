@@ -56,3 +56,26 @@ def test_no_mask_beside_a_cache():
   seq = ocnn.OctreeSequence(torch.tensor([0, 5], dtype=torch.int32), torch.zeros(5, 3))
   with pytest.raises(RuntimeError, match='mask'):
     ocnn.OctreeAttention(32, 4, causal=True)(data, seq, mask, cache=cache)
+
+
+def test_tracing_is_refused():
+  """A recording would hold none of the kernels' work."""
+  x, off = torch.zeros(4, 2, 16), torch.tensor([0, 4], dtype=torch.int32)
+  pos, freqs = torch.zeros(4, 1, dtype=torch.int32), ocnn.rotary_freqs([2], device='cpu')
+  for call in (lambda x: ocnn.octree_attention(x, x, x, off), lambda x: ocnn.octree_rotary(x, pos, freqs, [2]),
+               lambda x: ocnn.add_rms_norm(x, None, torch.ones(16)),
+               lambda x: ocnn.octree_attention_step(x, x, x, x[:, None], x[:, None], torch.zeros(4, dtype=torch.int32))):
+    with pytest.raises(RuntimeError, match='traced'):
+      torch.jit.trace(call, (x,), check_trace=False)
+
+
+def test_transforms_are_refused():
+  x, off = torch.zeros(4, 2, 16), torch.tensor([0, 4], dtype=torch.int32)
+  pos, freqs = torch.zeros(4, 1, dtype=torch.int32), ocnn.rotary_freqs([2], device='cpu')
+  calls = (lambda x: ocnn.octree_attention(x, x, x, off), lambda x: ocnn.octree_rotary(x, pos, freqs, [2]),
+           lambda x: ocnn.add_rms_norm(x, None, torch.ones(16))[0])
+  for call in calls:
+    with pytest.raises(RuntimeError, match='torch.func'):
+      torch.func.grad(lambda x: call(x).sum())(x)
+    with pytest.raises(RuntimeError, match='torch.func'):
+      torch.vmap(call)(x[None])
