@@ -17,7 +17,7 @@ import torch
 from torch import nn as _nn
 
 from . import nn
-from .modules import OctreeConv1x1
+from .modules import OctreeConv1x1, _stock_conv1x1, hooked
 
 OctreeSequence = collections.namedtuple('OctreeSequence', ['offsets', 'positions'])
 OctreeSequence.__doc__ = """The nodes of a level as sequences, one per shape: `offsets` int32 [batch + 1], and the cell
@@ -112,8 +112,24 @@ def _nodes(rows):
   return rows.view(1, rows.shape[0], 1, rows.shape[1]).permute(0, 3, 1, 2)
 
 
+def _called(layer, data):
+  """A layer whose product someone asked to see (hooks; a weight that a hook forms) or replaced: its own call."""
+  autocast = torch.is_autocast_enabled('cuda')
+  x = data
+  if not autocast:                                       # (a Conv1d takes data of its parameters' type alone)
+    x = data.to(next((p.dtype for p in layer.parameters()), data.dtype))
+  out = layer(x) if type(layer) is not OctreeConv1x1 or hooked(layer) else layer.conv1x1(x.squeeze(-1)).unsqueeze(-1)
+  return out if autocast else out.to(data.dtype)
+
+
 def _linear(layer, data, residual=None, relu=False):
   """An OctreeConv1x1 on channels_last data, whose output is channels_last too, in the data's type."""
+  if type(layer) is not OctreeConv1x1 or not _stock_conv1x1(layer.conv1x1) or hooked(layer, layer.conv1x1):
+    out = _called(layer, data)
+    if residual is not None:
+      out = out + residual
+    out = torch.relu(out) if relu else out
+    return out.contiguous(memory_format=torch.channels_last)
   conv = layer.conv1x1
   if torch.is_grad_enabled() and (data.requires_grad or conv.weight.requires_grad or
                                   (residual is not None and residual.requires_grad)):
