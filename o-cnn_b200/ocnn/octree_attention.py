@@ -131,8 +131,7 @@ def _linear(layer, data, residual=None, relu=False):
     out = torch.relu(out) if relu else out
     return out.contiguous(memory_format=torch.channels_last)
   conv = layer.conv1x1
-  if torch.is_grad_enabled() and (data.requires_grad or conv.weight.requires_grad or
-                                  (residual is not None and residual.requires_grad)):
+  if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (data, conv.weight, conv.bias, residual)):
     rows = _rows(data)
     bias = None if conv.bias is None else conv.bias.to(rows.dtype)
     out = _nodes(torch.nn.functional.linear(rows, conv.weight[:, :, 0].to(rows.dtype), bias))

@@ -95,3 +95,12 @@ def test_a_replaced_product(autocast):
   assert (got - want).abs().max() <= tol * want.abs().max() and (quiet - want).abs().max() <= tol * want.abs().max()
   got.sum().backward()
   assert adapter.up.weight.grad is not None and adapter.base.weight.grad is not None
+
+
+def test_biases_alone_are_trained():
+  net, x, seq = block(), nodes(50, 32), sequence([30, 20])
+  for name, p in net.named_parameters():
+    p.requires_grad_(name.endswith('bias'))
+  out = net(x, seq)
+  out.sum().backward()
+  assert net.fc1.conv1x1.bias.grad.any() and torch.equal(net.fc2.conv1x1.bias.grad, torch.full((32,), 50.0, device='cuda'))
