@@ -123,7 +123,8 @@ def _called(layer, data):
 
 
 def _linear(layer, data, residual=None, relu=False):
-  """An OctreeConv1x1 on channels_last data, whose output is channels_last too, in the data's type."""
+  """An OctreeConv1x1 on channels_last data, whose output is channels_last too, in the data's type (under autocast: in that
+  one's, or the residual's)."""
   if type(layer) is not OctreeConv1x1 or not _stock_conv1x1(layer.conv1x1) or hooked(layer, layer.conv1x1):
     out = _called(layer, data)
     if residual is not None:
@@ -138,7 +139,12 @@ def _linear(layer, data, residual=None, relu=False):
     if residual is not None:
       out = out + residual
     return torch.relu(out) if relu else out
-  return layer.run(data, residual=residual, relu=relu)
+  if torch.is_autocast_enabled('cuda'):                  # (as torch's linear does above)
+    data = data.to(torch.get_autocast_dtype('cuda'))
+  if residual is None or residual.dtype == data.dtype:
+    return layer.run(data, residual=residual, relu=relu)
+  out = layer.run(data) + residual
+  return torch.relu(out) if relu else out
 
 
 class AttentionCache:
@@ -166,9 +172,12 @@ class AttentionCache:
     place = torch.where(at < capacity, at, sinks + (at - sinks) % max(capacity - sinks, 1))
     keep &= place < capacity                 # (more first nodes than places: what does not fit has none)
     b, place = b[keep], place[keep]
-    self.k[b, place] = k[keep].detach()
-    self.v[b, place] = v[keep].detach()
+    self.k[b, place], self.v[b, place] = self.typed(k[keep].detach(), v[keep].detach())
     self.lengths.copy_(ends[1:] - ends[:-1])
+
+  def typed(self, *rows):
+    """Rows as autocast's products give them, in the cache's type."""
+    return [x.to(self.k.dtype) for x in rows] if torch.is_autocast_enabled('cuda') else rows
 
 
 class OctreeAttention(_nn.Module):
@@ -221,6 +230,7 @@ class OctreeAttention(_nn.Module):
       raise RuntimeError('OctreeAttention.step: only a causal layer can be run node by node')
     with torch.no_grad():
       q, k, v = self._heads(data.contiguous(memory_format=torch.channels_last), positions)
+      q, k, v = cache.typed(q, k, v)
       out = octree_attention_step(q, k, v, cache.k, cache.v, cache.lengths, self.window, self.sinks)
       cache.lengths += (cache.lengths >= 0).to(torch.int32)
       return _linear(self.proj, _nodes(out.reshape(out.shape[0], -1)), residual)

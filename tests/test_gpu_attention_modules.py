@@ -1,4 +1,6 @@
 """The attention layer's modules as a network uses them: hooks and replaced layers, autocast, empty levels, caches."""
+import sys
+
 import pytest
 import torch
 
@@ -80,7 +82,7 @@ class Adapter(torch.nn.Module):
     return self.base(x) + self.up(self.down(x))
 
 
-@pytest.mark.parametrize('autocast', [False])
+@pytest.mark.parametrize('autocast', [False, True])
 def test_a_replaced_product(autocast):
   net, x, seq = block(), nodes(50, 32), sequence([30, 20])
   plain = block()
@@ -104,3 +106,22 @@ def test_biases_alone_are_trained():
   out = net(x, seq)
   out.sum().backward()
   assert net.fc1.conv1x1.bias.grad.any() and torch.equal(net.fc2.conv1x1.bias.grad, torch.full((32,), 50.0, device='cuda'))
+
+
+# ---- autocast -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', [BF16, F16])
+def test_autocast_without_gradients(dtype, monkeypatch):
+  """As in training: products and attention in the 16-bit type, norms and the residual in the data's."""
+  module = sys.modules['ocnn.octree_attention']
+  net, x, seq = block(causal=True), nodes(50, 32), sequence([30, 20])
+  types, plain = [], module.octree_attention
+  monkeypatch.setattr(module, 'octree_attention', lambda q, *a, **kw: types.append(q.dtype) or plain(q, *a, **kw))
+  with torch.autocast('cuda', dtype=dtype):
+    want = net(x, seq)
+    with torch.no_grad():
+      for cache in [ocnn.AttentionCache(2, 40, 2, 8, t) for t in (dtype, F32)]:
+        got = net(x, seq, cache=cache)
+        assert net.step(nodes(2, 32), torch.zeros(2, 3, device='cuda'), cache).dtype == F32
+  assert types == [dtype] * 3 and got.dtype == want.dtype == F32
+  # (both are within 32 half steps of the definition: six roundings on the way)
+  assert (got - want).abs().max().item() <= 64 * torch.finfo(dtype).eps / 2 * want.abs().max().item()
