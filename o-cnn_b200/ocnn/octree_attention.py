@@ -132,7 +132,8 @@ def _linear(layer, data, residual=None, relu=False):
     out = torch.relu(out) if relu else out
     return out.contiguous(memory_format=torch.channels_last)
   conv = layer.conv1x1
-  if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (data, conv.weight, conv.bias, residual)):
+  if data.shape[2] == 0 or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in
+                                                           (data, conv.weight, conv.bias, residual)):
     rows = _rows(data)
     bias = None if conv.bias is None else conv.bias.to(rows.dtype)
     out = _nodes(torch.nn.functional.linear(rows, conv.weight[:, :, 0].to(rows.dtype), bias))
@@ -222,7 +223,7 @@ class OctreeAttention(_nn.Module):
     out = octree_attention(q, k, v, sequence.offsets, self.window, self.sinks, self.causal, mask)
     if cache is not None:
       cache.fill(k, v, sequence.offsets, self.sinks)
-    return _linear(self.proj, _nodes(out.reshape(out.shape[0], -1)), residual)
+    return _linear(self.proj, _nodes(out.flatten(1)), residual)
 
   def step(self, data, positions, cache, residual=None):
     """One new node per sequence: data [1, C, batch, 1], their cells [batch, 3].  The cache takes them in."""
@@ -233,7 +234,7 @@ class OctreeAttention(_nn.Module):
       q, k, v = cache.typed(q, k, v)
       out = octree_attention_step(q, k, v, cache.k, cache.v, cache.lengths, self.window, self.sinks)
       cache.lengths += (cache.lengths >= 0).to(torch.int32)
-      return _linear(self.proj, _nodes(out.reshape(out.shape[0], -1)), residual)
+      return _linear(self.proj, _nodes(out.flatten(1)), residual)
 
   def extra_repr(self):
     return 'channels={}, heads={}, kv_heads={}, window={}, sinks={}, causal={}'.format(

@@ -125,3 +125,22 @@ def test_autocast_without_gradients(dtype, monkeypatch):
   assert types == [dtype] * 3 and got.dtype == want.dtype == F32
   # (both are within 32 half steps of the definition: six roundings on the way)
   assert (got - want).abs().max().item() <= 64 * torch.finfo(dtype).eps / 2 * want.abs().max().item()
+
+
+# ---- levels and batches of no or one node ---------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('n', [0])
+def test_hardly_any_nodes(n, dtype):
+  net, seq = block(causal=True), sequence([0, n])
+  leaf = nodes(n, 32, dtype).requires_grad_()
+  out = net(leaf, seq)
+  assert out.shape == (1, 32, n, 1) and out.dtype == dtype
+  out.sum().backward()
+  assert leaf.grad.shape == leaf.shape and all(bool(p.grad.any()) == bool(n) for p in net.parameters() if p.dim() < 3)
+  with torch.no_grad():
+    quiet = net(leaf, seq)
+    assert quiet.shape == (1, 32, n, 1)
+    # (both within 32 half steps of the definition)
+    assert n == 0 or (quiet - out).abs().max() <= 64 * max(torch.finfo(dtype).eps / 2, 2.0 ** -20) * out.abs().max()
+    cache = ocnn.AttentionCache(n, 16, 2, 8, dtype)
+    assert net.step(leaf, torch.zeros(n, 3, device='cuda'), cache).shape == (1, 32, n, 1)
