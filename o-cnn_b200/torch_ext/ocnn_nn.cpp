@@ -544,6 +544,14 @@ ConvShape conv_shape(const OctreeRef& o, const DataRef& x, int depth, const vect
   return s;
 }
 
+// Whether a's elements lie as b's do.  (A dimension of one may have any stride: the data of a single node.)
+bool same_layout(const Tensor& a, const Tensor& b) {
+  if (a.sizes() != b.sizes()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+
 ocnn_conv_epilogue make_epilogue(const c10::optional<Tensor>& scale, const c10::optional<Tensor>& bias,
                                  const c10::optional<Tensor>& residual, bool relu, int cout,
                                  const Tensor& y) {
@@ -561,8 +569,7 @@ ocnn_conv_epilogue make_epilogue(const c10::optional<Tensor>& scale, const c10::
     ep.bias_dev = bias->data_ptr<float>();
   }
   if (residual.has_value() && residual->defined()) {
-    TORCH_CHECK(residual->is_cuda() && residual->sizes() == y.sizes() &&
-                    residual->strides() == y.strides() && residual->scalar_type() == y.scalar_type(),
+    TORCH_CHECK(residual->is_cuda() && same_layout(*residual, y) && residual->scalar_type() == y.scalar_type(),
                 "residual must match the output's shape, dtype and memory layout");
     ep.residual_dev = residual->data_ptr();
   }

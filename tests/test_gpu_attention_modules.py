@@ -129,7 +129,7 @@ def test_autocast_without_gradients(dtype, monkeypatch):
 
 # ---- levels and batches of no or one node ---------------------------------------------------------------------------------
 @pytest.mark.parametrize('dtype', [F32, BF16])
-@pytest.mark.parametrize('n', [0])
+@pytest.mark.parametrize('n', [0, 1])
 def test_hardly_any_nodes(n, dtype):
   net, seq = block(causal=True), sequence([0, n])
   leaf = nodes(n, 32, dtype).requires_grad_()
