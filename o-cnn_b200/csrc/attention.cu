@@ -91,7 +91,7 @@ size_t ocnn_octree_attention_saved_bytes(const ocnn_attention* p) {
 size_t ocnn_octree_attention_backward_workspace_bytes(const ocnn_attention* p) {
   if (check(p, "ocnn_octree_attention_backward_workspace_bytes") != OCNN_OK || p->n == 0) return 0;
   const AttnArgs a = args_of(p);
-  return (chunk_words(p) + delta_floats(p) + (size_t)far_slots(a.n, a.batch) * a.kv_heads * a.sinks * 2 * a.dim) * sizeof(float);
+  return (chunk_words(p) + delta_floats(p) + (size_t)far_slots(a) * a.kv_heads * a.sinks * 2 * a.dim) * sizeof(float);
 }
 
 int ocnn_octree_attention_backward(const ocnn_attention* p, const void* out_dev, const float* lse_dev,

@@ -350,10 +350,18 @@ __device__ void attn_dkv_row(const AttnArgs& a, const AttnGrad& g, int j, int hk
 // ---- first nodes seen from far behind -----------------------------------------------------------------------
 // What the nodes behind the window add to the gradients of their sequence's first nodes comes from all over the
 // sequence.  It is summed in blocks of kFarRows nodes, each block's share of a sequence in a slot of its own, and the
-// slots are added up in order: no atomics, the same bits every time.  Slot = block +
-// sequence: along the packed batch either the block or the sequence moves on, so no two pairs share one.
+// slots are added up in order: no atomics, the same bits every time.  Slot = block + the sequence's number: along the packed
+// batch either the block or the sequence moves on, so no two pairs share one.  Only sequences longer than the window have
+// anything from far: where there cannot be as many as the batch holds, start / (window + 1) numbers them instead, which is another
+// one for each (10^5 short sequences of 10 nodes under a window of 1000: 4905 slots, not 103907).
 constexpr int kFarRows = 256;
-inline int far_slots(int n, int batch) { return ceil_div(n, kFarRows) + batch; }
+__host__ __device__ inline bool far_by_start(const AttnArgs& a) { return a.batch > a.n / (a.window + 1) + 1; }
+inline int far_slots(const AttnArgs& a) {
+  return ceil_div(a.n, kFarRows) + (far_by_start(a) ? a.n / (a.window + 1) + 1 : a.batch);
+}
+__device__ __forceinline__ int far_number(const AttnArgs& a, const Span& s) {
+  return far_by_start(a) ? s.start / (a.window + 1) : s.seq;
+}
 __device__ __forceinline__ float* far_slot(const AttnArgs& a, const AttnGrad& g, int slot, int hk, int sink) {
   return g.far + (((long long)slot * a.kv_heads + hk) * a.sinks + sink) * (2 * a.dim);
 }
@@ -363,7 +371,7 @@ struct FarSlots { int first, count; };
 __device__ __forceinline__ FarSlots far_slots_of(const AttnArgs& a, int j, const Span& s) {
   if (j - s.start >= a.sinks || s.end - j <= a.window || (a.mask != nullptr && a.mask[j] == 0)) return {0, 0};
   const int first = (j + a.window) / kFarRows;
-  return {first + s.seq, (s.end - 1) / kFarRows - first + 1};
+  return {first + far_number(a, s), (s.end - 1) / kFarRows - first + 1};
 }
 // The sums of dK's channels for key j, then of dV's; NULL where nobody sees it from far.
 __device__ __forceinline__ const float* far_sums(const AttnArgs& a, const AttnGrad& g, int j, int hk) {

@@ -44,6 +44,10 @@ __global__ void __launch_bounds__(32 * kFarWarps) attn_far_mma_kernel(const Attn
       i0 = i0 < begin ? begin : r1;
       continue;
     }
+    if (s.end - s.start <= a.window) {             // nobody here sees a first node from far
+      i0 = s.end;
+      continue;
+    }
     const int end = min(r1, s.end), sinks = min(a.sinks, s.end - s.start);
     for (int t0 = 0; t0 < sinks; t0 += 16) {
       const int first = s.start + t0, many = min(16, sinks - t0);
@@ -175,7 +179,7 @@ __global__ void __launch_bounds__(32 * kFarWarps) attn_far_mma_kernel(const Attn
           float x = 0.f;
 #pragma unroll
           for (int w = 0; w < kFarWarps; ++w) x += part[(w * 16 + t) * DP + d];
-          far_slot(a, g, blockIdx.x + s.seq, hk, t0 + t)[which * a.dim + d] = x * (which == 0 ? 1.f / kept_at : 1.f / prob_up);
+          far_slot(a, g, blockIdx.x + far_number(a, s), hk, t0 + t)[which * a.dim + d] = x * (which == 0 ? 1.f / kept_at : 1.f / prob_up);
         }
       }
       __syncthreads();

@@ -79,3 +79,17 @@ def test_transforms_are_refused():
       torch.func.grad(lambda x: call(x).sum())(x)
     with pytest.raises(RuntimeError, match='torch.func'):
       torch.vmap(call)(x[None])
+
+
+def test_workspace_of_many_short_sequences():
+  """Slots for sums from far are made for sequences that can have them: those longer than the window."""
+  import ctypes
+  import test_attention_host as host
+  need = host.L.ocnn_octree_attention_backward_workspace_bytes
+  slot = 4 * 16 * 2 * 64 * 4                                              # key heads, first nodes, dK and dV, fp32
+  rest = (1000000 // 256 + 64 + 8 * 1000000) * 4
+  a = dict(n=1000000, heads=8, kv_heads=4, dim=64, sinks=16)
+  many = need(ctypes.byref(host.attention(batch=100000, window=1000, **a)))
+  assert many <= rest + (1000000 // 256 + 1000000 // 1001 + 2) * slot
+  few = need(ctypes.byref(host.attention(batch=10, window=1000, **a)))
+  assert (1000000 // 256) * slot <= few <= rest + (1000000 // 256 + 1 + 10) * slot

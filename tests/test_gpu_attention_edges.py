@@ -1,12 +1,13 @@
 """Attention where its results are easily lost."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
 import ocnn
 from attention_reference import visible
-from test_gpu_attention import inputs, run
+from test_gpu_attention import compare, inputs, run
 
 pytestmark = pytest.mark.gpu
 
@@ -139,3 +140,14 @@ def test_many_weak_keys_in_a_step_in_half(dim, n):
   new = [t[-1:].expand(600, 1, dim) for t in (k, v)]
   out = ocnn.octree_attention_step(q, *new, *caches, lengths, scale=1.0)
   assert (out.double() - value).abs().max().item() <= bound
+
+
+# ---- many sequences, first nodes seen from far ------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('longest,count', [(40, 150), (24, 700), (17, 900)])
+def test_first_nodes_of_many_short_sequences(dtype, longest, count):
+  """Sequences shorter and longer than the window side by side, more of them than could be longer than it, and fewer."""
+  lengths = np.random.default_rng(longest).integers(0, longest + 1, count)
+  compare(list(lengths), 2, 1, 32, dtype, 16, 3, False)
+  compare(list(lengths), 2, 1, 32, dtype, 1, 2, True, masked=0.8)
+
