@@ -14,11 +14,11 @@ int check(const ocnn_attention* a, const char* who) {
   OCNN_REQUIRE(a->dtype >= OCNN_F32 && a->dtype <= OCNN_F16, "%s: bad dtype %d", who, a->dtype);
   OCNN_REQUIRE(a->heads % a->kv_heads == 0, "%s: %d heads over %d key heads", who, a->heads, a->kv_heads);
   OCNN_REQUIRE(a->window >= 0 && a->sinks >= 0, "%s: window and sinks must not be negative", who);
-  if (a->dim > kMaxHeadDim || a->sinks > kMaxSinks || a->heads > 65535)
+  if (a->dim > kMaxHeadDim || a->sinks > kMaxSinks)
     return fail(OCNN_ERR_UNSUPPORTED, "%s: heads of %d channels with %d first nodes (up to %d and %d)", who, a->dim,
                 a->sinks, kMaxHeadDim, kMaxSinks);
-  if (a->batch > kMaxSequences)
-    return fail(OCNN_ERR_UNSUPPORTED, "%s: %d sequences (up to %d)", who, a->batch, kMaxSequences);
+  if (a->batch > kMaxSequences || a->heads > 65535)                   // (heads: the grid's y)
+    return fail(OCNN_ERR_UNSUPPORTED, "%s: %d sequences, %d heads (up to %d and 65535)", who, a->batch, a->heads, kMaxSequences);
   OCNN_REQUIRE(a->n == 0 || (a->q_dev && a->k_dev && a->v_dev && a->offsets_dev), "%s: null pointer", who);
   return OCNN_OK;
 }

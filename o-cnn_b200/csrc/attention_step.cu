@@ -521,7 +521,9 @@ extern "C" int ocnn_octree_attention_step(const ocnn_attention_cache* c, const v
                c->kv_heads);
   OCNN_REQUIRE(window >= 0 && sinks >= 0, "ocnn_octree_attention_step: window and sinks must not be negative");
   const int size = c->dtype == OCNN_F32 ? 4 : 2;
-  if (c->dim > kMaxHeadDim || c->dim * size % 16 != 0 || c->batch > 65535 || heads > 65535)
+  if (c->batch > 65535 || heads > 65535)                       // (the grid's y and z)
+    return fail(OCNN_ERR_UNSUPPORTED, "ocnn_octree_attention_step: %d sequences, %d heads (up to 65535 each)", c->batch, heads);
+  if (c->dim > kMaxHeadDim || c->dim * size % 16 != 0)
     return fail(OCNN_ERR_UNSUPPORTED, "ocnn_octree_attention_step: heads of %d channels (multiples of 16 bytes up to %d)",
                 c->dim, kMaxHeadDim);
   if (c->batch == 0) return OCNN_OK;

@@ -93,3 +93,20 @@ def test_workspace_of_many_short_sequences():
   assert many <= rest + (1000000 // 256 + 1000000 // 1001 + 2) * slot
   few = need(ctypes.byref(host.attention(batch=10, window=1000, **a)))
   assert (1000000 // 256) * slot <= few <= rest + (1000000 // 256 + 1 + 10) * slot
+
+
+def test_too_many_sequences_or_heads():
+  """The message says what is too many."""
+  import ctypes
+  import test_attention_host as host
+  cache = host.Cache(k=64, v=64, ks=(host.I64 * 3)(2048, 64, 32), vs=(host.I64 * 3)(2048, 64, 32), lengths=64, batch=65536,
+                     capacity=32, kv_heads=2, dim=32, dtype=1)
+  s, p = (host.I64 * 2)(128, 32), host.P(64)
+  step = lambda heads: host.L.ocnn_octree_attention_step(ctypes.byref(cache), p, s, p, s, p, s, p, heads, 0, 0,
+                                                         ctypes.c_float(1.0), None)
+  assert step(4) == host.UNSUPPORTED and b'65536 sequences, 4 heads' in host.L.ocnn_last_error()
+  cache.batch = 2
+  assert step(65536) == host.UNSUPPORTED and b'2 sequences, 65536 heads' in host.L.ocnn_last_error()
+  a = host.attention(heads=65536, kv_heads=1)
+  assert host.L.ocnn_octree_attention(ctypes.byref(a), p, None, p, None) == host.UNSUPPORTED
+  assert b'65536 heads' in host.L.ocnn_last_error()
