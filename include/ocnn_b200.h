@@ -687,7 +687,7 @@ int ocnn_add_rms_norm_backward(const void* x_dev, int64_t x_row, const void* res
  * dim up to 128, sinks up to 64.  out: contiguous; lse: what the backward pass needs of
  * this one, or NULL: ocnn_octree_attention_saved_bytes for [heads][n] fp32 and, of 16-bit data, what rounding took from out.
  * The backward pass takes the same structure, out and lse of the forward pass and the gradient of out; dq, dk, dv:
- * contiguous.  status_dev: as in ocnn_octree_conv_tc. */
+ * contiguous; dk and dv both NULL: of the queries alone.  status_dev: as in ocnn_octree_conv_tc. */
 typedef struct ocnn_attention {
   const void *q_dev, *k_dev, *v_dev;
   int64_t q_stride[2], k_stride[2], v_stride[2];    /* node, head */

@@ -100,7 +100,7 @@ int ocnn_octree_attention_backward(const ocnn_attention* p, const void* out_dev,
                                    void* stream) {
   const int status = check(p, "ocnn_octree_attention_backward");
   if (status != OCNN_OK || p->n == 0) return status;
-  OCNN_REQUIRE(out_dev && lse_dev && grad_dev && grad_stride && dq_dev && dk_dev && dv_dev && status_dev,
+  OCNN_REQUIRE(out_dev && lse_dev && grad_dev && grad_stride && dq_dev && (dk_dev == nullptr) == (dv_dev == nullptr) && status_dev,
                "ocnn_octree_attention_backward: null pointer");
   const size_t need = ocnn_octree_attention_backward_workspace_bytes(p);
   if (workspace_dev == nullptr || workspace_bytes < need)

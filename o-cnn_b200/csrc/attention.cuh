@@ -47,7 +47,7 @@ struct AttnGrad {
   const float* lse;
   float *delta, *far;
   unsigned* largest;                          // float16: per 256 nodes the largest |dO| (its bits), by the queries' kernel
-  void *dq, *dk, *dv;
+  void *dq, *dk, *dv;                         // dk and dv NULL: not asked for
 };
 
 // float16 holds nothing below 2^-24, and p of a long sequence and dO of a mean loss are small: the operands of the gradients'

@@ -669,6 +669,7 @@ int backward_launch(const AttnArgs& a, const AttnGrad& g, bool vec, cudaStream_t
   if (status != OCNN_OK) return status;
   attn_simt_dq_kernel<T, DP><<<dim3(ceil_div(a.n, kB), a.heads), kThreads, dq_bytes, st>>>(a, g, vec);
   OCNN_LAUNCH_OK("attn_simt_dq_kernel");
+  if (g.dk == nullptr) return OCNN_OK;
   if (a.sinks > 0) {
     int far = far_launch<T>(a, g, st);
     if (far == OCNN_OK) far = attn_far_join(a, g, st);

@@ -689,6 +689,7 @@ int grad_launch(GradArgs& p, cudaStream_t st) {
   OCNN_CUDA_OK(launch_chained(dq, dim3(ceil_div(a.n, W * 128 >> p.pack_log), a.heads >> p.pack_log), dim3(Dq::kThreads),
                               Dq::smem(stages_q), st, p));
   OCNN_LAUNCH_OK("attn_tc_dq_kernel");
+  if (p.g.dk == nullptr) return OCNN_OK;
   if (p.a.sinks > 0) {
     const int far = attn_far_mma(p.a, p.g, HALF ? OCNN_F16 : OCNN_BF16, st);
     if (far != OCNN_OK) return far;

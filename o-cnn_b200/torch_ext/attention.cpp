@@ -310,12 +310,15 @@ struct Attention : public torch::autograd::Function<Attention> {
                                 ctx->saved_data["scale"].toDouble());
     c10::cuda::CUDAGuard guard(o.q.device());
     const Tensor g = rows_of(grads[0]), status = ocnn_tc_status(o.q.device());
-    Tensor dq = empty_rows(saved[0]), dk = empty_rows(saved[1]), dv = empty_rows(saved[2]);
+    // (the queries' kernel forms what the keys' needs; keys and values are one kernel)
+    const bool keys = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
+    Tensor dq = empty_rows(saved[0]), dk = keys ? empty_rows(saved[1]) : Tensor(), dv = keys ? empty_rows(saved[2]) : Tensor();
     const size_t bytes = ocnn_octree_attention_backward_workspace_bytes(&o.a);
     const Tensor ws = torch::empty({(int64_t)bytes}, o.q.options().dtype(torch::kUInt8));
     const int64_t stride[2] = {g.stride(0), g.stride(1)};
     OCNN_CALL(ocnn_octree_attention_backward(&o.a, saved[5].data_ptr(), saved[6].data_ptr<float>(), g.data_ptr(), stride,
-                                             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), bytes,
+                                             dq.data_ptr(), keys ? dk.data_ptr() : nullptr, keys ? dv.data_ptr() : nullptr,
+                                             ws.data_ptr(), bytes,
                                              status.data_ptr<int32_t>(), current_stream()));
     variable_list res(9);
     res[0] = dq;

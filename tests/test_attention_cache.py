@@ -110,3 +110,13 @@ def test_too_many_sequences_or_heads():
   a = host.attention(heads=65536, kv_heads=1)
   assert host.L.ocnn_octree_attention(ctypes.byref(a), p, None, p, None) == host.UNSUPPORTED
   assert b'65536 heads' in host.L.ocnn_last_error()
+
+
+def test_gradients_of_keys_without_those_of_values():
+  import ctypes
+  import test_attention_host as host
+  a, p, s = host.attention(), host.P(64), (host.I64 * 2)(128, 32)
+  call = lambda dq, dk, dv: host.L.ocnn_octree_attention_backward(ctypes.byref(a), p, p, p, s, dq, dk, dv, p, ctypes.c_size_t(0), p,
+                                                                  None)
+  assert [call(p, None, p), call(p, p, None), call(None, p, p)] == [host.INVALID] * 3
+  assert call(p, None, None) == host.CAPACITY

@@ -151,3 +151,26 @@ def test_first_nodes_of_many_short_sequences(dtype, longest, count):
   compare(list(lengths), 2, 1, 32, dtype, 16, 3, False)
   compare(list(lengths), 2, 1, 32, dtype, 1, 2, True, masked=0.8)
 
+
+# ---- gradients that are not asked for ---------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+def test_gradients_of_queries_alone(dtype):
+  """Frozen keys and values: the same bits for the queries, and the keys' kernels do not run."""
+  q, k, v, g = inputs(900, 4, 2, 32, dtype, 4)
+  off = torch.tensor([0, 500, 900], dtype=torch.int32, device='cuda')
+  kw = dict(window=40, sinks=2)
+  want = run(q, k, v, [0, 500, 900], g, **kw)
+  leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+
+  def launches(asked):
+    given = [leaf if at in asked else leaf.detach() for at, leaf in enumerate(leaves)]
+    out = ocnn.octree_attention(*given, off, **kw)
+    before = ocnn.nn.launch_count()
+    got = torch.autograd.grad(out, [given[at] for at in asked], g)
+    for at, x in zip(asked, got):
+      assert torch.equal(x, want[('dq', 'dk', 'dv')[at]])
+    return ocnn.nn.launch_count() - before
+  every = launches((0, 1, 2))
+  assert launches((0,)) < every
+  assert launches((1,)) == launches((2,)) == launches((1, 2)) == every
+
