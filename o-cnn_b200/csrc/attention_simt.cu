@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_kernel(const A
     float sum = row_sum(total[r]);
     if (sees && sum == 0.f) sum = NAN;                       // scores of -inf alone have no softmax
     const float inv = sees ? 1.f / sum : 0.f;
-    bool bad = not_finite(sum);
+    bool bad = false;
     float x[DP / 16];
     out_row<DP>(acc, r, x);
     if (i < a.n) {
@@ -302,12 +302,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_kernel(const A
       }
       if (tx == 0 && lse != nullptr) lse[(long long)h * a.n + i] = sees ? top[r] + log2f(sum) : INFINITY;
     }
-    const unsigned any = __ballot_sync(0xffffffffu, bad);
+    // (a sum that is no number is the row's own doing: a hidden key is not in it)
+    const unsigned any = __ballot_sync(0xffffffffu, bad && !not_finite(sum));
     if (tx == 0) redo[4 * ty + r] = (any >> (tid & 16)) & 0xffffu;
   }
   __syncthreads();
   for (int r = tid >> 5; r < kB; r += kThreads / 32)
-    if (redo[r] != 0 && r0 + r < a.n) attn_forward_row<T>(a, r0 + r, h, out, lse);
+    if (redo[r] != 0 && r0 + r < a.n && !attn_row_is_spoilt<T>(a, r0 + r, h, out)) attn_forward_row<T>(a, r0 + r, h, out, lse);
 }
 
 // Gradient of the queries of one tile, and delta_i = dO_i . o_i for the keys' gradients.
@@ -395,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_dq_kernel(cons
       bad |= not_finite(x[c]);
       if (i < a.n && d < a.dim) ((T*)g.dq)[((long long)i * a.heads + h) * a.dim + d] = from_f32<T>(x[c] * a.scale);
     }
-    const unsigned any = __ballot_sync(0xffffffffu, bad);
+    const unsigned any = __ballot_sync(0xffffffffu, bad && !attn_query_is_spoilt(lse[r], delta[r]));
     if (tx == 0) redo[4 * ty + r] = (any >> (tid & 16)) & 0xffffu;
   }
   __syncthreads();
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_dkv_kernel(con
   for (int r = 0; r < 4; ++r) {
     const int j = k0 + 4 * ty + r;
     const float* far = j < a.n ? far_sums(a, g, j, hk) : nullptr;
-    bool bad = false;
+    bool bad_dk = false, bad_dv = false;
     float dk_row[DP / 16], dv_row[DP / 16];
     out_row<DP>(dk, r, dk_row);
     out_row<DP>(dv, r, dv_row);
@@ -497,19 +498,24 @@ __global__ void __launch_bounds__(kThreads, kPerSm<DP>) attn_simt_dkv_kernel(con
     for (int c = 0; c < DP / 16; ++c) {
       const int d = out_col<DP>(c);
       float x = dk_row[c], y = dv_row[c];
-      bad |= not_finite(x) | not_finite(y);
+      bad_dk |= not_finite(x);
+      bad_dv |= not_finite(y);
       if (j >= a.n || d >= a.dim) continue;
       x += far != nullptr ? far[d] : 0.f;
       y += far != nullptr ? far[a.dim + d] : 0.f;
       ((T*)g.dk)[((long long)j * a.kv_heads + hk) * a.dim + d] = from_f32<T>(x * a.scale);
       ((T*)g.dv)[((long long)j * a.kv_heads + hk) * a.dim + d] = from_f32<T>(y);
     }
-    const unsigned any = __ballot_sync(0xffffffffu, bad);
-    if (tx == 0) redo[4 * ty + r] = (any >> (tid & 16)) & 0xffffu;
+    const unsigned any_dk = __ballot_sync(0xffffffffu, bad_dk), any_dv = __ballot_sync(0xffffffffu, bad_dv);
+    if (tx == 0) redo[4 * ty + r] = ((any_dk >> (tid & 16)) & 0xffffu ? 1 : 0) + ((any_dv >> (tid & 16)) & 0xffffu ? 2 : 0);
   }
   __syncthreads();
-  for (int r = tid >> 5; r < kB; r += kThreads / 32)
-    if (redo[r] != 0 && k0 + r < a.n) attn_dkv_row<T>(a, g, k0 + r, hk, true, true);
+  for (int r = tid >> 5; r < kB; r += kThreads / 32) {
+    if (k0 + r >= a.n) continue;
+    const bool dk_too = (redo[r] & 1) && !attn_key_is_spoilt<T>(a, g, k0 + r, hk, false);
+    const bool dv_too = (redo[r] & 2) && !attn_key_is_spoilt<T>(a, g, k0 + r, hk, true);
+    if (dk_too || dv_too) attn_dkv_row<T>(a, g, k0 + r, hk, dk_too, dv_too);
+  }
 }
 
 // The far pass: what the nodes beyond the window add to the gradients of their sequence's first nodes, kFarSinks of them

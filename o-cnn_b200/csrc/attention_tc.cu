@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
       const bool none = seen == 0;
       if (!none && total == 0.f) total = NAN;                              // scores of -inf alone have no softmax
       const float inv = none ? 0.f : 1.f / total;
-      bool bad = not_finite(total);
+      bool bad = false;
       T* dst = (T*)p.out + ((long long)i * a.heads + h) * a.dim;
 #pragma unroll 2
       for (int d = 0; d < a.dim; d += 16) {
@@ -246,11 +246,13 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
         }
       }
       if (i < a.n && p.lse != nullptr) p.lse[(long long)h * a.n + i] = none ? INFINITY : ref + (log2f(total) - up);
-      unsigned redo = __ballot_sync(0xffffffffu, bad && i < a.n);
+      // (a total that is no number is the row's own doing: a hidden key is not in it)
+      unsigned redo = __ballot_sync(0xffffffffu, bad && i < a.n && !not_finite(total));
+      __syncwarp();
       while (redo != 0) {
-        const int at = __ffs(redo) - 1;
+        const int at = __ffs(redo) - 1, ri = __shfl_sync(0xffffffffu, i, at), rh = __shfl_sync(0xffffffffu, h, at);
         redo &= redo - 1;
-        attn_forward_row<T>(a, __shfl_sync(0xffffffffu, i, at), __shfl_sync(0xffffffffu, h, at), (T*)p.out, p.lse);
+        if (!attn_row_is_spoilt<T>(a, ri, rh, (const T*)p.out)) attn_forward_row<T>(a, ri, rh, (T*)p.out, p.lse);
       }
     }
   } else if (warp < 5 * W) {

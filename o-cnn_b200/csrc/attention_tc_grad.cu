@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(DqShape<DP, W>::kThreads, CTAS) attn_tc_dq_ker
         }
         if (in) store_row<HALF>(dst, d, a.dim, p.wide, x);
       }
-      unsigned redo = __ballot_sync(0xffffffffu, bad && in);
+      unsigned redo = __ballot_sync(0xffffffffu, bad && in && !attn_query_is_spoilt(lse, delta));
       while (redo != 0) {
         const int at = __ffs(redo) - 1;
         redo &= redo - 1;
@@ -539,10 +539,11 @@ __global__ void __launch_bounds__(DkvShape<DP, G>::kThreads, CTAS) attn_tc_dkv_k
           if (in) store_row<HALF>(dst, d, a.dim, p.wide, x);
         }
         unsigned redo = __ballot_sync(0xffffffffu, bad && in);
+        __syncwarp();
         while (redo != 0) {
-          const int at = __ffs(redo) - 1;
+          const int rj = __shfl_sync(0xffffffffu, j, __ffs(redo) - 1);
           redo &= redo - 1;
-          attn_dkv_row<T>(a, p.g, __shfl_sync(0xffffffffu, j, at), hk, which == 0, which == 1);
+          if (!attn_key_is_spoilt<T>(a, p.g, rj, hk, which == 1)) attn_dkv_row<T>(a, p.g, rj, hk, which == 0, which == 1);
         }
       }
     }

@@ -94,6 +94,28 @@ def test_a_step_that_sees_minus_infinity_alone(dtype):
   assert out[0].isnan().all() and out[1].isfinite().all() and not out[2].any()
 
 
+@pytest.mark.parametrize('what', ['dO', 'k', 'v'])
+def test_a_step_that_overflows_is_not_slow(what):
+  """Values that are no numbers everywhere, as loss scaling brings them about, are no reason to form rows key by key (which took
+  a hundred times as long): a pass takes no more than ten times one of numbers."""
+  n = 20000
+  q, k, v, g = inputs(n, 8, 2, 64, F16, 1)
+  kw = dict(window=500, sinks=2)
+  bad = {'dO': g, 'k': k, 'v': v}[what].clone()
+  spoilt = [bad.fill_(math.inf) if name == what else x for name, x in (('q', q), ('k', k), ('v', v), ('dO', g))]
+  times = []
+  for t in ([q, k, v, g], spoilt):
+    run(*t[:3], [0, n], t[3], **kw)
+    ends = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    ends[0].record()
+    for _ in range(3):
+      run(*t[:3], [0, n], t[3], **kw)
+    ends[1].record()
+    torch.cuda.synchronize()
+    times.append(ends[0].elapsed_time(ends[1]))
+  assert times[1] <= 10 * times[0], times
+
+
 # ---- weak keys in float16 ---------------------------------------------------------------------------------------------
 def weak_keys(n, dim, least):
   """One strong key of value 1 and n - 1 about 2^-25 as strong of value 16: keys, values, the output, and how far it may be off
