@@ -196,3 +196,59 @@ def test_gradients_of_queries_alone(dtype):
   assert launches((0,)) < every
   assert launches((1,)) == launches((2,)) == launches((1, 2)) == every
 
+
+# ---- two streams at once ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+def test_two_streams_at_once(dtype):
+  """Forward passes and gradients of different inputs on two streams that do not wait for each other: the bits of the same
+  passes one after the other."""
+  kw = dict(window=300, sinks=4, causal=True)
+  off = [0, 2500, 4100]
+  sets = [inputs(4100, 4, 2, 64, dtype, seed) for seed in range(6)]
+  want = [run(*s[:3], off, s[3], **kw) for s in sets]
+  torch.cuda.synchronize()
+  streams = [torch.cuda.Stream() for _ in range(2)]
+  got = []
+  for at, s in enumerate(sets):
+    with torch.cuda.stream(streams[at % 2]):
+      got.append(run(*s[:3], off, s[3], **kw))
+  torch.cuda.synchronize()
+  for a, b in zip(got, want):
+    for name in b:
+      assert torch.equal(a[name], b[name]), name
+
+
+# ---- the norm's gradients, as near as the kernel forms them -------------------------------------------------------------
+def norm_gradients(x, r, w, eps, gy, gs):
+  """{name: (value, bound)} in 64 bits.  The sum x + r enters as 32 bits hold it, so that a result is off by its own rounding
+  and by those in 32 bits: up to 37 additions for a mean (32 in a thread, five between lanes; the root halves them) and a
+  dozen products and sums, 2^-24 each: 2^-19 of every term; gw adds its rows besides."""
+  u = torch.finfo(x.dtype).eps / 2
+  x, r, gy, gs = (t.detach().double() for t in (x, r, gy, gs))
+  wide = w.detach().double()
+  x = x + r
+  inv = (x.pow(2).mean(1, keepdim=True) + eps).rsqrt()
+  unit, wg = x * inv, gy * wide
+  g = gs + inv * (wg - unit * (wg * unit).mean(1, keepdim=True))
+  heavy = gs.abs() + inv * (wg.abs() + unit.abs() * (wg * unit).abs().mean(1, keepdim=True))
+  gw, terms = (gy * unit).sum(0), (gy * unit).abs().sum(0)
+  return {'g': (g, u * g.abs() + 2.0 ** -19 * heavy),
+          'gw': (gw, torch.finfo(w.dtype).eps / 2 * gw.abs() + (2.0 ** -19 + x.shape[0] * 2.0 ** -24) * terms)}
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16])
+@pytest.mark.parametrize('rows,channels', [(40, 8), (61, 96), (64, 128), (33, 1000)])
+def test_norm_gradients_from_the_unrounded_sum(dtype, rows, channels):
+  """A gradient formed from the stored sum, which is rounded to 16 bits, is outside of these bounds: shown beside."""
+  make = lambda seed: torch.randn(rows, channels, generator=torch.Generator(device='cuda').manual_seed(seed), device='cuda')
+  x, r, gy, gs = make(0).to(dtype), (3 * make(1)).to(dtype), make(2).to(dtype), make(3).to(dtype)
+  w = (1 + 0.2 * make(4)[0]).contiguous()
+  leaves = [t.detach().requires_grad_() for t in (x, r, w)]
+  gx, gr, gw = torch.autograd.grad(ocnn.add_rms_norm(*leaves, 1e-5), leaves, (gy, gs))
+  want = norm_gradients(x, r, w, 1e-5, gy, gs)
+  least = torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+  for got, name in ((gx, 'g'), (gr, 'g'), (gw, 'gw')):
+    off = (got.double() - want[name][0]).abs()
+    assert bool((off <= want[name][1] + least).all()), (name, (off / want[name][1]).max().item())
+  stored = norm_gradients((x + r), torch.zeros_like(r), w, 1e-5, gy, gs)['gw'][0]
+  assert bool(((stored - want['gw'][0]).abs() > want['gw'][1]).any())
