@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(32 * kFarWarps) attn_far_mma_kernel(const Attn
       i0 = s.end;
       continue;
     }
-    const int end = min(r1, s.end), sinks = min(a.sinks, s.end - s.start);
+    const int end = min(r1, s.end), sinks = min(a.sinks, s.end - s.start), slot = blockIdx.x + far_number(a, s);
     for (int t0 = 0; t0 < sinks; t0 += 16) {
       const int first = s.start + t0, many = min(16, sinks - t0);
       // rows that see the first of these nodes from far (the others' begin a node later each), heads side by side
@@ -85,8 +85,8 @@ __global__ void __launch_bounds__(32 * kFarWarps) attn_far_mma_kernel(const Attn
         }
         return r;
       };
-      auto fetch = [&](const Row& row, int slot) {
-        const uint32_t dst = smem_u32(ring + slot * Shape::kTile);
+      auto fetch = [&](const Row& row, int place) {
+        const uint32_t dst = smem_u32(ring + place * Shape::kTile);
         const int c = lane % kChunks;
 #pragma unroll
         for (int it = 0; it < kFarTile / kStep; ++it) {
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(32 * kFarWarps) attn_far_mma_kernel(const Attn
           float x = 0.f;
 #pragma unroll
           for (int w = 0; w < kFarWarps; ++w) x += part[(w * 16 + t) * DP + d];
-          far_slot(a, g, blockIdx.x + far_number(a, s), hk, t0 + t)[which * a.dim + d] = x * (which == 0 ? 1.f / kept_at : 1.f / prob_up);
+          far_slot(a, g, slot, hk, t0 + t)[which * a.dim + d] = x * (which == 0 ? 1.f / kept_at : 1.f / prob_up);
         }
       }
       __syncthreads();

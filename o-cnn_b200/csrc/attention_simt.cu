@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(256, 2) attn_far_kernel(const AttnArgs a, cons
       i0 = s.end;
       continue;
     }
-    const int end = min(r1, s.end), sinks = min(a.sinks, s.end - s.start);
+    const int end = min(r1, s.end), sinks = min(a.sinks, s.end - s.start), slot = blockIdx.x + far_number(a, s);
     for (int t0 = 0; t0 < sinks; t0 += kFarSinks) {
       float k[kFarSinks][V], v[kFarSinks][V], dk[kFarSinks][V] = {}, dv[kFarSinks][V] = {};
       bool kept[kFarSinks];
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(256, 2) attn_far_kernel(const AttnArgs a, cons
           }
         }
         __syncthreads();
-        float* dst = far_slot(a, g, blockIdx.x + far_number(a, s), hk, t0 + t);
+        float* dst = far_slot(a, g, slot, hk, t0 + t);
         for (int e = tid; e < 2 * a.dim; e += 256) {
           float x = 0.f;
 #pragma unroll

@@ -19,7 +19,7 @@
 namespace ocnn {
 namespace {
 
-constexpr int kNormThreads = 256, kNormVectors = 4;
+constexpr int kNormThreads = 256;
 
 struct NormArgs {
   const void *x, *r, *w, *gy, *gs;

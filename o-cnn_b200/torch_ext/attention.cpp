@@ -56,11 +56,12 @@ void once_only(const char* who) {
 
 // Nor do forward-mode derivatives pass through them, and neither a tracer nor a torch.func transform would see what they do.
 void plain_call(std::initializer_list<Tensor> tensors, const char* who) {
+  constexpr c10::DispatchKeySet transforms = c10::DispatchKeySet(c10::DispatchKey::FuncTorchBatched) |
+                                             c10::DispatchKeySet(c10::DispatchKey::FuncTorchGradWrapper);
   TORCH_CHECK(!torch::jit::tracer::isTracing(), who, ": it cannot be traced (torch.jit.trace)");
   for (const Tensor& t : tensors) {
     if (!t.defined()) continue;
-    TORCH_CHECK(!t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper})),
-                who, ": it cannot be transformed (torch.func)");
+    TORCH_CHECK(!t.key_set().has_any(transforms), who, ": it cannot be transformed (torch.func)");
     TORCH_CHECK(!t._fw_grad(0).defined(), who, ": it has no forward-mode derivative");
   }
 }
