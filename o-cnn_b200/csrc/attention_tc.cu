@@ -271,8 +271,9 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
       uint32_t phase = 0;
       bool alive = mbar_wait(smem_u32(qfull), 0, abort_flag, p.status, kErrAttnQ);
       auto scores = [&](int s) {
-        // (the place's last P has to be through)
-        if (scored >= NB) alive = mbar_wait(smem_u32(&pvdone[t]), (scored - NB) & 1, abort_flag, p.status, kErrAttnO);
+        // The place's last P has to be through.  (The last product that was issued is waited for: without a gap it is that one,
+        // and behind blocks that this tile passes over an older one may be two phases back, where its parity would be wrong.)
+        if (scored >= NB) alive = mbar_wait(smem_u32(&pvdone[t]), (n - 1) & 1, abort_flag, p.status, kErrAttnO);
         if (!alive) return;
         tc_fence_after();
         if (leader) {

@@ -116,6 +116,20 @@ def test_a_step_that_overflows_is_not_slow(what):
   assert times[1] <= 10 * times[0], times
 
 
+# ---- blocks that one of two tiles passes over ---------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', [BF16, F16])
+@pytest.mark.parametrize('heads', [1, 2, 4])
+@pytest.mark.parametrize('masked', [None, 0.5])
+def test_first_nodes_around_the_border_of_two_tiles(dtype, heads, masked):
+  """Heads of 128: two tiles of 128 rows share their blocks of keys.  The sequence's first nodes lie on both sides of the shared
+  windows' begin, two blocks that the second tile needs before it passes over some."""
+  border = 256 // heads
+  for start in range(border - 40, border, 3):
+    for window in (1, 7, 30):
+      compare([start, 2 * border], heads, 1, 128, dtype, window, 33, True, masked=masked, seed=start)
+      compare([start, 2 * border], heads, 1, 104, dtype, window, 64, False, masked=masked, seed=start)
+
+
 # ---- weak keys in float16 ---------------------------------------------------------------------------------------------
 def weak_keys(n, dim, least):
   """One strong key of value 1 and n - 1 about 2^-25 as strong of value 16: keys, values, the output, and how far it may be off
