@@ -683,7 +683,8 @@ int ocnn_add_rms_norm_backward(const void* x_dev, int64_t x_row, const void* res
 /* Attention over a window of a sequence's nodes and its first `sinks` ones.  Node i sees key j of its sequence when
  *   causal:  j <= i and (i - j < window or j - start < sinks);   else:  |i - j| < window or j - start < sinks
  * (window 0: every key) and mask[j] != 0 (mask NULL: all).  out_i = sum_j softmax_j(scale * q_i . k_j) v_j, zeros for a
- * node that sees nothing and for nodes outside of every sequence.  q: heads, k and v: kv_heads (a divisor of heads),
+ * node that sees nothing and for nodes outside of every sequence; hidden values may be anything, visible ones that are no
+ * numbers go where they are seen, and scores of -inf alone are NaN.  q: heads, k and v: kv_heads (a divisor of heads),
  * dim up to 128, sinks up to 64.  out: contiguous; lse: what the backward pass needs of
  * this one, or NULL: ocnn_octree_attention_saved_bytes for [heads][n] fp32 and, of 16-bit data, what rounding took from out.
  * The backward pass takes the same structure, out and lse of the forward pass and the gradient of out; dq, dk, dv:

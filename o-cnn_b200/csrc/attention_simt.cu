@@ -12,7 +12,7 @@ constexpr int kPad = 4;                       // a row of DP + 4 floats: 16 rows
 // Bound: instruction issue (fp32 products have no tensor pipe of their accuracy here) and, between a tile's barriers, the
 // latency of its loads, which other thread blocks cover: of up to 32 channels three per SM (80 registers), of 64 two.
 // Blocks of 16 columns that none of a warp's eight rows sees are left out.  Forward and gradients of 20 k nodes, 4 heads of
-// 24, window 64: 325 us (88 + 108 + 132 in the kernels); two blocks per SM and every column of a tile computed: 380.
+// 24, window 64: 316 us (90 + 110 + 134 one by one from cold caches); two blocks per SM and every column of a tile computed: 380.
 template <int DP> constexpr int kPerSm = DP == 32 ? 3 : DP == 64 ? 2 : 1;
 
 // Rows of a [n, heads, dim] tensor as floats, zeros for row < 0 and behind dim.  `index` gives the row for 0 .. kB - 1.

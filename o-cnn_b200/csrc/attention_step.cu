@@ -13,7 +13,7 @@
 //   16-bit caches: every warp copies its rows, 16 at a time, into a ring of its own (cp.async, one row after the other:
 //   rolled caches and the new row need no case of their own) and multiplies them with mma.sync, 16 query heads at a time.
 //   On the CUDA cores, a product and a shuffle per value for each query head, 64 sequences of 4100 rows, 16 heads over 4
-//   of 128, took 510 us, with a bulk copy per row (about 65 cycles each, one after the other) 302 us, now 120.
+//   of 128, took 510 us, with a bulk copy per row (about 65 cycles each, one after the other) 302 us, now 119.
 //   fp32 caches: a warp reads whole rows, 16 bytes a lane, on the CUDA cores.
 #include <cooperative_groups.h>
 
@@ -547,7 +547,8 @@ extern "C" int ocnn_octree_attention_step(const ocnn_attention_cache* c, const v
   a.sinks = window == 0 ? 0 : sinks;
   a.rolls = window > 0 && (long long)window + sinks <= c->capacity;
   a.scale_log2 = scale * 1.4426950408889634f;
-  // CTAs per sequence and key head: until the GPU has four per SM, as long as each still has 64 rows to read.
+  // CTAs per sequence and key head, doubled until the grid has four per SM, as long as each still has 64 rows to read.  (At 128
+  // channels three fit an SM: the 64 sequences above are 1024 CTAs on 444 places, 2.3 rounds.  More parts took 122 us.)
   const bool f32 = c->dtype == OCNN_F32;
   const long long pairs = (long long)a.batch * a.kv_heads;
   const long long most = a.rolls ? (long long)window + sinks : c->capacity;

@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(FwdShape<DP, W, BN, NB>::kThreads, CTAS)
         }
         if (i < a.n) store_row<HALF>(dst, d, a.dim, p.wide, x);
       }
-      if (p.lse != nullptr) {                  // (a loop of its own: in the one above, a pass without it took 235 us, not 233)
+      if (p.lse != nullptr) {                  // (a loop of its own: in the one above, a pass without it took 1 % longer)
         T* rest = attn_rest<T>(a, p.lse) + ((long long)i * a.heads + h) * a.dim;
 #pragma unroll 1
         for (int d = 0; d < a.dim; d += 16) {
@@ -402,7 +402,7 @@ int fwd_launch(AttnFwdArgs& p, cudaStream_t st) {
 template <bool HALF>
 int fwd_by_width(AttnFwdArgs& p, cudaStream_t st) {
   // Up to 64 channels a tile's tensor memory is a quarter of the SM's with one place for scores, and three CTAs share an SM:
-  // 60 k nodes, 8 heads of 32, window 256: 159 us; with two places and two CTAs 178.  At 128 channels there is room for two
+  // 60 k nodes, 8 heads of 32, window 256: 161 us; with two places and two CTAs 178.  At 128 channels there is room for two
   // tiles, which share their copies of K and V and have two places each.
   if (p.a.dim <= 32) return fwd_launch<32, 1, 64, 1, HALF, 3>(p, st);
   if (p.a.dim <= 64) return fwd_launch<64, 1, 64, 1, HALF, 3>(p, st);
