@@ -51,8 +51,8 @@ bool all_on_boundary(const ocnn_attention* a, int elements) {
          on_boundary(a->v_dev, a->v_stride, a->dim, elements, size);
 }
 
-// 16-bit rows in whole pieces of 16 bytes, at strides that a tensor map takes (positive, below 2^40 bytes; nodes are held to
-// 2^31, which no tensor that fits the GPU exceeds), and a positive scale (a tile's maximum is taken before it).
+// 16-bit rows in whole pieces of 16 bytes, at strides that a tensor map takes (positive, below 2^40 bytes; nodes up to 2^31
+// bytes apart, others run on the CUDA cores), and a positive scale (a tile's maximum is taken before it).
 bool map_strides(const int64_t stride[2], int n, int heads) {
   return (n == 1 || (stride[0] > 0 && stride[0] < (1 << 30))) && (heads == 1 || (stride[1] > 0 && stride[1] < (1LL << 38)));
 }

@@ -7,8 +7,9 @@
 // with 128 threads per tile, one row each, between the two products.  m is the row's reference: its running maximum, but
 // moved only when a block exceeds it by more than 8 (any reference gives the same quotient as long as nothing overflows,
 // and 2^8 is far from that), so O is hardly ever scaled.  P is rounded to the data's type, which is what the product takes;
-// its sum is of the unrounded values.  float16 holds nothing below 2^-24: there p is kept at 2^7 p, 2^15 at most (of 10^5 keys at
-// 2^-25 of the strongest, 0.3 % of their values would be lost otherwise).  Scores have two places, so that a block's are ready when its rows come to it.
+// its sum is of the unrounded values.  float16 holds nothing below 2^-24: there p is kept at 2^7 p, 2^15 at most (10^5 keys at
+// 2^-25 of the strongest would add nothing otherwise, 0.3 % of their values).  Scores have two places, so that a block's are
+// ready when its rows come to it.
 //
 // Roles: 4 W warps of rows, W warps that issue products (one thread of each), one warp that brings Q and the blocks of K
 // and V by TMA into a ring of slots (and clears the rows that the mask hides: see clear_rows).
